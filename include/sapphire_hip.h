@@ -208,6 +208,25 @@ size_t sapphire_sample_workspace_bytes(int n, int batch);
 int sapphire_sample_dev(float *logits, int n, int batch, int ld, float temperature, const float *draws_dev,
                         int *tokens_dev, void *workspace, void *stream);
 
+/* ---- beam search ----
+ * The next beams of each of `requests` requests of `beams` beams (rows r * beams + b): over all
+ * beams b and tokens v < n,
+ *   score(b, v) = scores[b] + logits[b][v] - log sum exp logits[b]
+ * and the `beams` best go on, best first: by the score in 64 bits, of equal ones the lowest b, then
+ * the larger logit, then the lowest v. scores_out is rounded to fp32. A row with done != 0 has
+ * ended: its one continuation is end_token at its score unchanged. Tokens of score -inf (a logit of
+ * -inf or NaN; every token of a row whose score is not finite or that has a logit of +inf) are taken
+ * only when fewer than `beams` others are left. tokens[i], parents[i] (the row it continues, r * beams + b) and done_out[i] (its
+ * parent's done, or token == end_token) describe row i's new beam. done and done_out may both be
+ * NULL (no row has ended); an end_token outside [0, n) never matches, and a done row then has
+ * no continuation. logits: rows of stride ld >= n, left as they are. scores_out may be scores, done_out
+ * may be done. workspace: sapphire_beam_workspace_bytes() bytes of device memory, 16-byte aligned;
+ * calls sharing one must be ordered. 1 <= beams <= 16, beams <= n <= 2^21. */
+size_t sapphire_beam_workspace_bytes(int n, int requests, int beams);
+int sapphire_beam_select_dev(const float *logits, int ld, int n, int requests, int beams, const float *scores,
+                             const int *done, int end_token, float *scores_out, int *tokens, int *parents,
+                             int *done_out, void *workspace, void *stream);
+
 /* ---- device copies of tensor_t weights ----
  * The device-resident copy kernel_gemv keeps for a 2-D weight tensor (Q4_0/Q8_0 in the
  * PACKED layout, F32/BF16 as is), created on first use; *layout receives its layout.
@@ -222,6 +241,52 @@ int sapphire_rmsnorm_dev(float *out, const float *in, const float *w, float eps,
 /* Half-split rotation of n_heads consecutive heads at position pos (rope.c:99-117). */
 int sapphire_rope_apply_dev(float *x, int n_heads, int head_dim, int pos,
                             const float *cos_table, const float *sin_table, void *stream);
+
+/* Rows of heads: element d of head h of token t is data[t * token_stride + h * head_stride + d], of
+ * dtype SAPPHIRE_F32, _BF16 or _F16 and aligned to its size. Strides are in elements; for rows that a
+ * call writes, no two elements may coincide ([tokens][heads][head_dim], [heads][tokens][head_dim]
+ * and slices of either, as the q, k and v heads of a fused projection, are all right). */
+typedef struct {
+    void *data;
+    int dtype;
+    int tokens, heads, head_dim;
+    long long token_stride, head_stride;
+} sapphire_rows_t;
+
+/* Rotary positions of many rows, each at its own position (rope.c:99-117 and, in pairs,
+ * positional_encoding.c:95-99, without their tables): the first rotary_dim dims of every head of
+ * token t turn by positions[t] * freqs[i] for pair i < rotary_dim / 2, which is dims (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) when interleaved:
+ *   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c, s = magnitude * (cos, sin) of the angle.
+ * The angle is formed and reduced in 64 bits, so far positions lose nothing; positions may be
+ * negative. The remaining dims are copied. freqs: rotary_dim / 2 doubles in device memory
+ * (sapphire_rope_frequencies). y is x itself (same data, strides and type) or does not overlap it;
+ * both have one type. rotary_dim: even, 2 .. head_dim; head_dim at most 1024. */
+typedef struct {
+    const double *freqs;
+    int rotary_dim;
+    int interleaved;
+    float magnitude;
+} sapphire_rope_t;
+int sapphire_rope_rows_dev(const sapphire_rows_t *x, const sapphire_rows_t *y, const int *positions,
+                           const sapphire_rope_t *rope, void *stream);
+
+/* The frequencies of rotary_dim / 2 pairs into a host array, f_i = base^(-2i / rotary_dim), changed
+ * for contexts `factor` times longer than the model was trained on:
+ *   SAPPHIRE_ROPE_PLAIN   as they are (the other arguments are not looked at)
+ *   SAPPHIRE_ROPE_LINEAR  f_i / factor (positions interpolated)
+ *   SAPPHIRE_ROPE_BASE    base * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair turns
+ *                         `factor` times slower, the fastest as before (rotary_dim > 2)
+ *   SAPPHIRE_ROPE_PARTS   by the turns t_i = trained * f_i / 2 pi that a pair makes over the trained
+ *                         context: t_i <= low: f_i / factor; t_i >= high: f_i; between, the blend
+ *                         f_i ((1 - g) / factor + g), g = (t_i - low) / (high - low)
+ * magnitude (may be NULL) receives 1, for PARTS 0.1 ln(factor) + 1 (what the published method
+ * scales both vectors by; a model that wants none passes 1 in sapphire_rope_t). base > 0,
+ * factor >= 1, trained > 0, 0 <= low < high. 0 / -1; no device work. */
+enum { SAPPHIRE_ROPE_PLAIN = 0, SAPPHIRE_ROPE_LINEAR = 1, SAPPHIRE_ROPE_BASE = 2, SAPPHIRE_ROPE_PARTS = 3 };
+int sapphire_rope_frequencies(double *freqs, float *magnitude, int rotary_dim, double base, int scaling,
+                              double factor, double trained, double low, double high);
+
 /* gate[i] = gelu(gate[i]) * up[i] (transformer.c:150-157, activations.c:64-82). */
 int sapphire_gelu_mul_dev(float *gate, const float *up, int n, void *stream);
 /* Residual pattern n = rmsnorm_delta(h, w); resid += n; h = resid

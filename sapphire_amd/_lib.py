@@ -1,4 +1,4 @@
-"""ctypes prototypes of libsapphire_hip.so (include/kernels.h, tensor.h, sapphire_hip.h)."""
+"""ctypes prototypes of libsapphire_hip.so (include/kernels.h, tensor.h, sapphire_hip.h, paged.h)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -21,6 +21,33 @@ class GemmInput(C.Structure):
 class GemmOutput(C.Structure):
     """sapphire_gemm_output_t (include/sapphire_hip.h)."""
     _fields_ = [("y", C.c_void_p), ("ldy", C.c_int), ("parts", C.c_void_p), ("geglu", C.c_int), ("y_blocked", C.c_int)]
+
+
+class RowsC(C.Structure):
+    """sapphire_rows_t (include/sapphire_hip.h)."""
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("tokens", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int),
+                ("token_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
+class RopeC(C.Structure):
+    """sapphire_rope_t (include/sapphire_hip.h)."""
+    _fields_ = [("freqs", C.c_void_p), ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("magnitude", C.c_float)]
+
+
+class PagedCacheC(C.Structure):
+    """sapphire_paged_cache_t (include/paged.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("layers", C.c_int), ("pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class PageTableC(C.Structure):
+    """sapphire_page_table_t (include/paged.h)."""
+    _fields_ = [("pages", C.c_void_p), ("rows", C.c_int), ("ld", C.c_int)]
+
+
+class AttentionC(C.Structure):
+    """sapphire_attention_t (include/paged.h)."""
+    _fields_ = [("scale", C.c_float), ("window", C.c_int), ("softcap", C.c_float)]
 
 
 def _proto(lib, name, res, args):
@@ -89,6 +116,17 @@ def load_library(path: str):
     P("sapphire_rope_apply_dev", i32, [vp, i32, i32, i32, vp, vp, vp])
     P("sapphire_gelu_mul_dev", i32, [vp, vp, i32, vp])
     P("sapphire_norm_residual_dev", i32, [vp, vp, vp, f32, i32, vp])
+    P("sapphire_rope_rows_dev", i32, [vp, vp, vp, vp, vp])
+    P("sapphire_rope_frequencies", i32, [vp, C.POINTER(f32), i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double])
+    P("sapphire_beam_workspace_bytes", sz, [i32, i32, i32])
+    P("sapphire_beam_select_dev", i32, [vp, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp])
+    # paged.h
+    P("sapphire_paged_cache_bytes", sz, [vp])
+    P("sapphire_paged_write_dev", i32, [vp, i32, vp, vp, vp, vp, vp, vp])
+    P("sapphire_paged_read_dev", i32, [vp, i32, vp, vp, vp, vp, vp, vp])
+    P("sapphire_paged_attention_workspace_bytes", sz, [vp, i32, i32, i32])
+    P("sapphire_paged_attention_dev", i32, [vp, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp])
+    P("sapphire_paged_reorder_dev", i32, [vp, vp, vp, vp, vp, vp, vp, vp])
     P("sapphire_tensor_invalidate", i32, [vp])
     P("sapphire_tensor_device_data", vp, [vp, C.POINTER(i32), vp])
     # tensor.h

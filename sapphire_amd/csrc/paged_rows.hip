@@ -1,0 +1,343 @@
+// paged_rows.hip - rows into the paged cache and out of it, and the cache's part of a beam step.
+//
+// Eight dims of a row are one lane's work and four lanes make a quant block, as in the weight
+// quantizer (quantize.hip), whose arithmetic this is: Q8_0: d = max|x| / 127, q = roundf(x * (1 / d));
+// Q4_0: d = m / -8 with m the first x of largest |x|, q = min(15, trunc(x * (1 / d) + 8.5)); every
+// product, sum and quotient rounded on its own. A block with a NaN or an infinity gets the scale NaN.
+#include <algorithm>
+
+#include "internal.h"
+#include "lanes.h"
+#include "paged_dev.h"
+
+namespace sapphire {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+// over the four lanes of a quad (quad_perm [1,0,3,2], then [2,3,0,1])
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, dpp_u32<0xB1>(v));
+    return max(v, dpp_u32<0x4E>(v));
+}
+__device__ __forceinline__ uint32_t quad_min(uint32_t v) {
+    v = min(v, dpp_u32<0xB1>(v));
+    return min(v, dpp_u32<0x4E>(v));
+}
+
+// The quad's block: its scale and this lane's eight codes (Q8_0 -127 .. 127, Q4_0 0 .. 15).
+template <int CT>
+__device__ __forceinline__ float quantize8(const float (&x)[8], int lq, int (&q)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = quad_max(top);                               // of the magnitudes' bits: NaN above infinity
+    if (top >= 0x7f800000u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = CT == DT_Q8_0 ? 0 : 8;
+        return __uint_as_float(0x7fc00000u);
+    }
+    float d;
+    if constexpr (CT == DT_Q8_0) {
+        d = __fdiv_rn(__uint_as_float(top), 127.0f);
+    } else {
+        uint32_t first = ~0u;                          // (index, sign) of the first element of that magnitude
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const uint32_t u = __float_as_uint(x[i]);
+            if ((u & 0x7fffffffu) == top) first = (uint32_t)(lq * 8 + i) * 2 + (u >> 31);
+        }
+        first = quad_min(first);
+        d = __fmul_rn(__uint_as_float(top), (first & 1) ? 0.125f : -0.125f);
+    }
+    const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+    // a subnormal d has an infinite id: its products saturate, 0 * inf counts as zero
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = __fmul_rn(x[i], id);
+        if constexpr (CT == DT_Q8_0) {
+            // adding the float below 1/2 and truncating rounds halves away from zero, the rest to nearest
+            const float w = v != v ? 0.0f : fminf(fmaxf(v, -127.0f), 127.0f);
+            q[i] = (int)__fadd_rn(w, copysignf(0x1.fffffep-2f, w));
+        } else {
+            const float w = __fadd_rn(v, 8.5f);
+            q[i] = w != w ? 8 : (int)fminf(fmaxf(w, 0.0f), 15.0f);
+        }
+    }
+    return d;
+}
+
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)(d & 255) << 24;
+}
+
+// Dims d .. d + 7 of position p into a tile (V: the V tile). The four lanes of a quad hold one block.
+template <int CT, int HD, bool V>
+__device__ __forceinline__ void store_codes(uint8_t *tile, uint32_t ps, uint32_t p, uint32_t d, const float (&x)[8]) {
+    using T = Tile<CT, HD>;
+    if constexpr (!T::kQuant) {
+        if constexpr (CT == DT_F32) {
+            uint8_t *a = V ? tile + p * T::ROW + d * 4 : tile + T::k_code(p, d);
+            uint8_t *b = V ? a + 16 : tile + T::k_code(p, d + 4);
+            *reinterpret_cast<pf4 *>(a) = pf4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<pf4 *>(b) = pf4{x[4], x[5], x[6], x[7]};
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = to_16(CT, x[2 * i]) | to_16(CT, x[2 * i + 1]) << 16;
+            if constexpr (V && HD == 64) {
+                *reinterpret_cast<pu2 *>(tile + T::v_run(p, d / 4)) = pu2{w[0], w[1]};
+                *reinterpret_cast<pu2 *>(tile + T::v_run(p, d / 4 + 1)) = pu2{w[2], w[3]};
+            } else {
+                *reinterpret_cast<pu4 *>(tile + (V ? p * T::ROW + d * 2 : T::k_code(p, d))) = pu4{w[0], w[1], w[2], w[3]};
+            }
+        }
+    } else {
+        const int lq = (d >> 3) & 3;
+        int q[8];
+        const float scale = quantize8<CT>(x, lq, q);
+        if constexpr (CT == DT_Q8_0) {
+            const uint32_t lo = bytes4(q[0], q[1], q[2], q[3]), hi = bytes4(q[4], q[5], q[6], q[7]);
+            if constexpr (V && HD == 64) {
+                *reinterpret_cast<uint32_t *>(tile + T::v_run(p, d / 4)) = lo;
+                *reinterpret_cast<uint32_t *>(tile + T::v_run(p, d / 4 + 1)) = hi;
+            } else {
+                uint8_t *o = tile + (V ? T::v_run(p, d / T::RUN) + d % T::RUN : T::k_code(p, d));
+                *reinterpret_cast<pu2 *>(o) = pu2{lo, hi};
+            }
+        } else if constexpr (!V) {
+            // two's complement nibbles: code - 8 is code ^ 8 in four bits
+            *reinterpret_cast<uint32_t *>(tile + T::k_code(p, d)) =
+                (bytes4(q[0], q[1], q[2], q[3]) | bytes4(q[4], q[5], q[6], q[7]) << 4) ^ 0x88888888u;
+        } else if constexpr (HD == 256) {
+            // a run is two lanes' dims: the even lane's in the low nibbles
+            const uint32_t a = bytes4(q[0], q[1], q[2], q[3]), b = bytes4(q[4], q[5], q[6], q[7]);
+            const uint32_t pa = dpp_u32<0xB1>(a), pb = dpp_u32<0xB1>(b);
+            *reinterpret_cast<uint32_t *>(tile + T::v_run(p, d / 16) + (lq & 1) * 4) = lq & 1 ? pb | b << 4 : a | pa << 4;
+        } else if constexpr (HD == 128) {
+            *reinterpret_cast<uint32_t *>(tile + T::v_run(p, d / 8)) =
+                bytes4(q[0], q[1], q[2], q[3]) | bytes4(q[4], q[5], q[6], q[7]) << 4;
+        } else {
+            *reinterpret_cast<uint16_t *>(tile + T::v_run(p, d / 4)) = (uint16_t)(bytes4(q[0], q[1], 0, 0) | bytes4(q[2], q[3], 0, 0) << 4);
+            *reinterpret_cast<uint16_t *>(tile + T::v_run(p, d / 4 + 1)) = (uint16_t)(bytes4(q[4], q[5], 0, 0) | bytes4(q[6], q[7], 0, 0) << 4);
+        }
+        if (lq == 0) *reinterpret_cast<float *>(tile + (V ? T::v_scale(ps, p, d / 32) : T::k_scale(ps, p, d / 32))) = scale;
+    }
+}
+
+template <int CT, int HD, bool V>
+__device__ __forceinline__ void load_codes(const uint8_t *tile, uint32_t ps, uint32_t p, uint32_t d, float (&x)[8]) {
+    using T = Tile<CT, HD>;
+    if constexpr (CT == DT_F32) {
+        const uint8_t *a = V ? tile + p * T::ROW + d * 4 : tile + T::k_code(p, d);
+        const uint8_t *b = V ? a + 16 : tile + T::k_code(p, d + 4);
+        const pf4 u = *reinterpret_cast<const pf4 *>(a), w = *reinterpret_cast<const pf4 *>(b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = u[i];
+            x[4 + i] = w[i];
+        }
+    } else if constexpr (!T::kQuant) {
+        pu4 w;
+        if constexpr (V && HD == 64) {
+            const pu2 a = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 4));
+            const pu2 b = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 4 + 1));
+            w = pu4{a.x, a.y, b.x, b.y};
+        } else {
+            w = *reinterpret_cast<const pu4 *>(tile + (V ? p * T::ROW + d * 2 : T::k_code(p, d)));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = from_16(CT, w[i] & 0xffffu);
+            x[2 * i + 1] = from_16(CT, w[i] >> 16);
+        }
+    } else {
+        const float scale = *reinterpret_cast<const float *>(tile + (V ? T::v_scale(ps, p, d / 32) : T::k_scale(ps, p, d / 32)));
+        int q[8];
+        if constexpr (CT == DT_Q8_0) {
+            uint32_t lo, hi;
+            if constexpr (V && HD == 64) {
+                lo = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 4));
+                hi = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 4 + 1));
+            } else {
+                const pu2 w = *reinterpret_cast<const pu2 *>(tile + (V ? T::v_run(p, d / T::RUN) + d % T::RUN : T::k_code(p, d)));
+                lo = w.x;
+                hi = w.y;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[i] = (int8_t)(lo >> (8 * i));
+                q[4 + i] = (int8_t)(hi >> (8 * i));
+            }
+        } else {
+            uint32_t lo, hi;                           // codes 0..3 and 4..7, one nibble per byte
+            if constexpr (!V) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + T::k_code(p, d)) ^ 0x88888888u;
+                lo = w & 0x0f0f0f0fu;
+                hi = w >> 4 & 0x0f0f0f0fu;
+            } else if constexpr (HD == 256) {
+                const pu2 w = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 16));
+                const uint32_t sh = d & 8 ? 4 : 0;
+                lo = w.x >> sh & 0x0f0f0f0fu;
+                hi = w.y >> sh & 0x0f0f0f0fu;
+            } else if constexpr (HD == 128) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 8));
+                lo = w & 0x0f0f0f0fu;
+                hi = w >> 4 & 0x0f0f0f0fu;
+            } else {
+                const uint32_t a = *reinterpret_cast<const uint16_t *>(tile + T::v_run(p, d / 4));
+                const uint32_t b = *reinterpret_cast<const uint16_t *>(tile + T::v_run(p, d / 4 + 1));
+                lo = (a & 0x0f0fu) | (a >> 4 & 0x0f0fu) << 16;
+                hi = (b & 0x0f0fu) | (b >> 4 & 0x0f0fu) << 16;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[i] = (int)(lo >> (8 * i) & 15u) - 8;
+                q[4 + i] = (int)(hi >> (8 * i) & 15u) - 8;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)q[i], scale);
+    }
+}
+
+// grid (units / kThreads, 2): K, then V. A unit is eight dims of a (token, head).
+template <int CT, int HD>
+__global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedCache c, Rows k, Rows v, PageTable tab,
+                                                               const int *__restrict__ seqs,
+                                                               const int *__restrict__ positions, bool kw, bool vw) {
+    constexpr int U = HD / 8;
+    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    const uint64_t row = i / U;
+    const int t = (int)(row / (uint32_t)c.nkv), h = (int)(row % (uint32_t)c.nkv), d = (int)(i % U) * 8;
+    int page, off;
+    if (t >= k.tokens || !paged_place(c, tab, seqs, positions, t, page, off)) return;
+    const size_t at = ((size_t)page * c.nkv + h) * c.tile_bytes;
+    float x[8];
+    if (blockIdx.y == 0) {
+        load8(k.dtype, kw, k.p, (int64_t)t * k.ts + (int64_t)h * k.hs + d, x);
+        store_codes<CT, HD, false>(c.k + at, c.page_size, off, d, x);
+    } else {
+        load8(v.dtype, vw, v.p, (int64_t)t * v.ts + (int64_t)h * v.hs + d, x);
+        store_codes<CT, HD, true>(c.v + at, c.page_size, off, d, x);
+    }
+}
+
+template <int CT, int HD>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedCache c, Rows k, Rows v, PageTable tab,
+                                                              const int *__restrict__ seqs,
+                                                              const int *__restrict__ positions, bool kw, bool vw) {
+    constexpr int U = HD / 8;
+    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    const uint64_t row = i / U;
+    const int t = (int)(row / (uint32_t)c.nkv), h = (int)(row % (uint32_t)c.nkv), d = (int)(i % U) * 8;
+    if (t >= k.tokens) return;
+    int page, off;
+    const bool there = paged_place(c, tab, seqs, positions, t, page, off);
+    const size_t at = there ? ((size_t)page * c.nkv + h) * c.tile_bytes : 0;
+    float x[8] = {};
+    if (blockIdx.y == 0) {
+        if (there) load_codes<CT, HD, false>(c.k + at, c.page_size, off, d, x);
+        store8(k.dtype, kw, k.p, (int64_t)t * k.ts + (int64_t)h * k.hs + d, x);
+    } else {
+        if (there) load_codes<CT, HD, true>(c.v + at, c.page_size, off, d, x);
+        store8(v.dtype, vw, v.p, (int64_t)t * v.ts + (int64_t)h * v.hs + d, x);
+    }
+}
+
+// grid (rows, 2 * layers * heads): one tile's written part to the spare page; the workgroups of
+// blockIdx.y 0 also write their row of the table. code_row, scale_row: bytes of a position's codes
+// and scales; both parts of 16 positions are contiguous in K and V tiles alike.
+__global__ __launch_bounds__(kThreads) void paged_reorder_kernel(PagedCache c, PageTable tab, const int *__restrict__ parents,
+                                                                 const int *__restrict__ lengths,
+                                                                 const int *__restrict__ spare, int *__restrict__ table_out,
+                                                                 int *__restrict__ lengths_out, int code_row, int scale_row) {
+    const int b = blockIdx.x, p = parents[b];
+    const bool has = p >= 0 && p < tab.rows;
+    const int64_t most = (int64_t)tab.ld * c.page_size;
+    const int n = has ? (int)min((int64_t)max(lengths[p], 0), most) : 0;
+    const int full = n / c.page_size, rem = n - full * c.page_size;
+    const int *from = tab.pages + (size_t)(has ? p : 0) * tab.ld;
+    const int dst = rem ? spare[b] : -1, src = rem ? from[full] : -1;
+    const bool copy = dst >= 0 && dst < c.pages && src >= 0 && src < c.pages;
+    if (blockIdx.y == 0) {
+        for (int i = threadIdx.x; i < tab.ld; i += kThreads)
+            table_out[(size_t)b * tab.ld + i] = i < full ? from[i] : i == full && copy ? dst : -1;
+        if (threadIdx.x == 0) lengths_out[b] = n;
+    }
+    if (!copy) return;
+    const int which = blockIdx.y & 1, lh = blockIdx.y >> 1, layer = lh / c.nkv, h = lh - layer * c.nkv;
+    uint8_t *pool = (which ? c.v : c.k) + (size_t)layer * c.layer_bytes;
+    const uint8_t *s = pool + ((size_t)src * c.nkv + h) * c.tile_bytes;
+    uint8_t *o = pool + ((size_t)dst * c.nkv + h) * c.tile_bytes;
+    const int held = (rem + 15) / 16 * 16;
+    auto copy16 = [&](uint32_t at, uint32_t bytes) {
+        constexpr int U = 4;                           // loads in flight per thread
+        const pu4 *sp = reinterpret_cast<const pu4 *>(s + at);
+        pu4 *op = reinterpret_cast<pu4 *>(o + at);
+        const uint32_t m = bytes / 16;
+        for (uint32_t i = threadIdx.x; i < m; i += U * kThreads) {
+            pu4 w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = sp[min(i + u * kThreads, m - 1)];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * kThreads < m) op[i + u * kThreads] = w[u];
+        }
+    };
+    copy16(0, (uint32_t)held * code_row);
+    if (scale_row) copy16((uint32_t)c.page_size * code_row, (uint32_t)held * scale_row);
+}
+
+}  // namespace
+
+#define SPH_PAGED(CALL)                                              \
+    switch (c.dtype) {                                               \
+        case DT_F32: SPH_PAGED_HD(CALL, DT_F32) break;               \
+        case DT_BF16: SPH_PAGED_HD(CALL, DT_BF16) break;             \
+        case DT_F16: SPH_PAGED_HD(CALL, DT_F16) break;               \
+        case DT_Q8_0: SPH_PAGED_HD(CALL, DT_Q8_0) break;             \
+        default: SPH_PAGED_HD(CALL, DT_Q4_0) break;                  \
+    }
+#define SPH_PAGED_HD(CALL, CT)                                       \
+    if (c.hd == 64) CALL(CT, 64);                                    \
+    else if (c.hd == 128) CALL(CT, 128);                             \
+    else CALL(CT, 256);
+
+int launch_paged_write(const PagedCache &c, const Rows &k, const Rows &v, const PageTable &t, const int *seqs,
+                       const int *positions, hipStream_t s) {
+    const int64_t units = (int64_t)k.tokens * c.nkv * (c.hd / 8);
+    const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2), block(kThreads);
+#define SPH_CALL(CT, HD) \
+    hipLaunchKernelGGL((paged_write_kernel<CT, HD>), grid, block, 0, s, c, k, v, t, seqs, positions, rows_wide(k), rows_wide(v))
+    SPH_PAGED(SPH_CALL)
+#undef SPH_CALL
+    return hip_ok(hipGetLastError(), "paged write launch") ? 0 : -1;
+}
+
+int launch_paged_read(const PagedCache &c, const Rows &k, const Rows &v, const PageTable &t, const int *seqs,
+                      const int *positions, hipStream_t s) {
+    const int64_t units = (int64_t)k.tokens * c.nkv * (c.hd / 8);
+    const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2), block(kThreads);
+#define SPH_CALL(CT, HD) \
+    hipLaunchKernelGGL((paged_read_kernel<CT, HD>), grid, block, 0, s, c, k, v, t, seqs, positions, rows_wide(k), rows_wide(v))
+    SPH_PAGED(SPH_CALL)
+#undef SPH_CALL
+    return hip_ok(hipGetLastError(), "paged read launch") ? 0 : -1;
+}
+
+int launch_paged_reorder(const PagedCache &c, const PageTable &t, const int *parents, const int *lengths, const int *spare,
+                         int *table_out, int *lengths_out, hipStream_t s) {
+    const bool quant = is_quant(c.dtype);
+    const int code_row = c.dtype == DT_F32 ? 4 * c.hd : c.dtype == DT_Q8_0 ? c.hd : c.dtype == DT_Q4_0 ? c.hd / 2 : 2 * c.hd;
+    hipLaunchKernelGGL(paged_reorder_kernel, dim3(t.rows, 2 * c.layers * c.nkv), dim3(kThreads), 0, s, c, t, parents,
+                       lengths, spare, table_out, lengths_out, code_row, quant ? c.hd / 8 : 0);
+    return hip_ok(hipGetLastError(), "paged reorder launch") ? 0 : -1;
+}
+
+}  // namespace sapphire

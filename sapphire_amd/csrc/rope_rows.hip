@@ -1,0 +1,153 @@
+// rope_rows.hip - rotary positions of many rows (rope.c:99-117; in pairs positional_encoding.c:95-99)
+// from frequencies instead of tables.
+//
+// A workgroup takes a few tokens, or some heads of one: it forms the tokens' angles once into LDS (64-bit
+// product and reduction to half a turn, then fp32 sine and cosine), and its threads turn 16 bytes of
+// each half at a time.
+#include <algorithm>
+
+#include "paged_dev.h"
+
+namespace sapphire {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kAngles = 1024;              // (token, pair) angles of a workgroup at most
+
+struct RopeArgs {
+    Rows x, y;
+    const int *positions;
+    const double *freqs;
+    int rot, tok, heads;                   // tokens and heads of a workgroup
+    float magnitude;
+};
+
+// VEC elements of 16 bytes, or single ones.
+template <int DT, bool WIDE>
+struct Piece {
+    static constexpr int N = WIDE ? (DT == DT_F32 ? 4 : 8) : 1;
+    float v[N];
+    __device__ __forceinline__ void load(const uint8_t *p, int64_t at) {
+        if constexpr (DT == DT_F32) {
+            const float *f = reinterpret_cast<const float *>(p) + at;
+            if constexpr (WIDE) {
+                const pf4 w = *reinterpret_cast<const pf4 *>(f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = w[i];
+            } else {
+                v[0] = *f;
+            }
+        } else {
+            const uint16_t *f = reinterpret_cast<const uint16_t *>(p) + at;
+            if constexpr (WIDE) {
+                const pu4 w = *reinterpret_cast<const pu4 *>(f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = from_16(DT, w[i] & 0xffffu);
+                    v[2 * i + 1] = from_16(DT, w[i] >> 16);
+                }
+            } else {
+                v[0] = from_16(DT, *f);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t *p, int64_t at) const {
+        if constexpr (DT == DT_F32) {
+            float *f = reinterpret_cast<float *>(p) + at;
+            if constexpr (WIDE) *reinterpret_cast<pf4 *>(f) = pf4{v[0], v[1], v[2], v[3]};
+            else *f = v[0];
+        } else {
+            uint16_t *f = reinterpret_cast<uint16_t *>(p) + at;
+            if constexpr (WIDE) {
+                pu4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = to_16(DT, v[2 * i]) | to_16(DT, v[2 * i + 1]) << 16;
+                *reinterpret_cast<pu4 *>(f) = w;
+            } else {
+                *f = (uint16_t)to_16(DT, v[0]);
+            }
+        }
+    }
+};
+
+// y0 = x0 c - x1 s, y1 = x1 c + x0 s
+__device__ __forceinline__ void turn(float &a, float &b, float2 cs) {
+    const float x0 = a, x1 = b;
+    a = __builtin_fmaf(x0, cs.x, -__fmul_rn(x1, cs.y));
+    b = __builtin_fmaf(x1, cs.x, __fmul_rn(x0, cs.y));
+}
+
+// grid (token groups, head groups)
+template <int DT, bool PAIRS, bool WIDE>
+__global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a) {
+    using P = Piece<DT, WIDE>;
+    __shared__ float2 cs[kAngles];
+    const int half = a.rot / 2, t0 = blockIdx.x * a.tok, nt = min(a.tok, a.x.tokens - t0);
+    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
+        const int t = i / half, p = i - t * half;
+        const double turns = (double)a.positions[t0 + t] * a.freqs[p] * 0.15915494309189533577;
+        const float th = (float)((turns - __builtin_rint(turns)) * 6.2831853071795864769);
+        float s, c;
+        sincosf(th, &s, &c);
+        cs[i] = make_float2(__fmul_rn(c, a.magnitude), __fmul_rn(s, a.magnitude));
+    }
+    __syncthreads();
+    const int h0 = blockIdx.y * a.heads, nh = min(a.heads, a.x.heads - h0);
+    const bool same = a.x.p == a.y.p;      // the remaining dims are there already
+    // units of a head: its turning pieces, then the copied ones
+    const int turning = PAIRS ? (WIDE ? a.rot / P::N : half) : half / P::N;
+    const int units = turning + (same ? 0 : (a.x.hd - a.rot) / P::N), per = nh * units;
+    for (int i = threadIdx.x; i < nt * per; i += kThreads) {
+        const int t = i / per, hu = i - t * per, h = hu / units, u = hu - h * units;
+        const int64_t xi = (int64_t)(t0 + t) * a.x.ts + (int64_t)(h0 + h) * a.x.hs;
+        const int64_t yi = (int64_t)(t0 + t) * a.y.ts + (int64_t)(h0 + h) * a.y.hs;
+        const float2 *w = cs + t * half;
+        P p, q;
+        if (u >= turning) {
+            const int d = a.rot + (u - turning) * P::N;
+            p.load(a.x.p, xi + d);
+            p.store(a.y.p, yi + d);
+        } else if constexpr (PAIRS && WIDE) {
+            const int d = u * P::N;
+            p.load(a.x.p, xi + d);
+#pragma unroll
+            for (int e = 0; e < P::N / 2; ++e) turn(p.v[2 * e], p.v[2 * e + 1], w[d / 2 + e]);
+            p.store(a.y.p, yi + d);
+        } else {
+            const int d = u * P::N, d0 = PAIRS ? 2 * d : d, d1 = PAIRS ? 2 * d + 1 : d + half;
+            p.load(a.x.p, xi + d0);
+            q.load(a.x.p, xi + d1);
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) turn(p.v[e], q.v[e], w[d + e]);
+            p.store(a.y.p, yi + d0);
+            q.store(a.y.p, yi + d1);
+        }
+    }
+}
+
+}  // namespace
+
+int launch_rope_rows(const Rows &x, const Rows &y, const int *positions, const double *freqs, int rot, bool interleaved,
+                     float magnitude, hipStream_t s) {
+    RopeArgs a{x, y, positions, freqs, rot, 1, x.heads, magnitude};
+    const int vec = x.dtype == DT_F32 ? 4 : 8;
+    const bool wide = rows_wide(x) && rows_wide(y) && x.hd % vec == 0 && (interleaved ? rot : rot / 2) % vec == 0;
+    // About four workgroups per CU where the rows suffice, of one to eight 16-byte pieces per thread
+    // (single elements: as many as the threads take in turn): several tokens, or some heads of one.
+    const int64_t units = std::max(1, x.hd / (wide ? 2 * vec : 2)), all = (int64_t)x.tokens * x.heads * units;
+    const int64_t want = std::min<int64_t>(8 * kThreads, std::max<int64_t>(kThreads, all / 1024));
+    if (x.heads * units >= want) {
+        a.heads = (int)std::max<int64_t>(1, want / units);
+    } else {
+        a.tok = (int)std::max<int64_t>(1, std::min<int64_t>(want / (x.heads * units), kAngles / (rot / 2)));
+    }
+    const dim3 grid((unsigned)((x.tokens + a.tok - 1) / a.tok), (unsigned)((x.heads + a.heads - 1) / a.heads)), block(kThreads);
+#define SPH_ROPE(DT, PAIRS, WIDE) \
+    if (x.dtype == DT && interleaved == PAIRS && wide == WIDE) hipLaunchKernelGGL((rope_rows_kernel<DT, PAIRS, WIDE>), grid, block, 0, s, a);
+#define SPH_ROPE_DT(DT) SPH_ROPE(DT, false, false) SPH_ROPE(DT, false, true) SPH_ROPE(DT, true, false) SPH_ROPE(DT, true, true)
+    SPH_ROPE_DT(DT_F32) SPH_ROPE_DT(DT_BF16) SPH_ROPE_DT(DT_F16)
+    return hip_ok(hipGetLastError(), "rope rows launch") ? 0 : -1;
+}
+
+}  // namespace sapphire

@@ -1,0 +1,101 @@
+"""Beam search's selection against every candidate formed and sorted in 64 bits."""
+import numpy as np
+import pytest
+
+from tests import paged_ref as ref
+from tests.test_paged_gpu import dev, sync
+
+pytestmark = pytest.mark.gpu
+
+
+def select(logits, ld, score, done, R, W, end, in_place=False):
+    from sapphire_amd import paged
+    from sapphire_amd.device import DeviceArray
+    n = logits.shape[1]
+    wide = np.full((R * W, ld), 1e30, np.float32)  # what lies between the rows does not count
+    wide[:, :n] = logits
+    dl, ds, dd = dev(wide), dev(score), None if done is None else dev(done)
+    so = ds if in_place else DeviceArray.empty(R * W)
+    to, po, eo = (DeviceArray.empty(R * W, np.int32) for _ in range(3))
+    eo = None if done is None else dd if in_place else eo
+    ws = DeviceArray(paged.beam_workspace_bytes(n, R, W))
+    paged.beam_select(dl, ld, n, R, W, ds, so, to, po, ws, done=dd, done_out=eo, end_token=end)
+    sync()
+    np.testing.assert_array_equal(dl.numpy(), wide)
+    return so.numpy(), to.numpy(), po.numpy(), None if eo is None else eo.numpy()
+
+
+def check(logits, score, done, R, W, end, ld=None, in_place=False):
+    got = select(logits, ld or logits.shape[1], score, done, R, W, end, in_place)
+    want = ref.beams64(logits, score, np.zeros(R * W, int) if done is None else done, R, W, end)
+    for name, g, w in zip(("tokens", "parents", "done"), got[1:], want[1:]):
+        if g is not None:
+            np.testing.assert_array_equal(g, w, err_msg=name)
+    fin = np.isfinite(want[0])
+    np.testing.assert_array_equal(np.isfinite(got[0]), fin)
+    # the normaliser is a sum of fp32 exponentials (2^-22 each, relative) in 64-bit and fp32 steps of at most 64
+    size = np.abs(np.where(np.isfinite(logits), logits, 0)).max()
+    tol = 2.0**-22 * 80 + 2.0**-23 * size * 4 + 2.0**-24 * np.abs(want[0][fin])
+    assert (np.abs(got[0][fin] - want[0][fin]) <= tol).all()
+
+
+@pytest.mark.parametrize("R,W,n,ld", [(1, 1, 1, 1), (1, 4, 4, 7), (1, 16, 16, 16), (3, 5, 63, 65), (2, 4, 2047, 2050), (2, 3, 2049, 2049), (8, 8, 5000, 5003),
+                                      (1, 16, 100001, 100001), (1, 2, 262144, 262144), (70, 3, 300, 300)])
+def test_beams(hip, R, W, n, ld):
+    rng = np.random.default_rng(n)
+    logits = (rng.normal(size=(R * W, n)) * 3).astype(np.float32)
+    score = -np.abs(rng.normal(size=R * W) * 4).astype(np.float32)
+    check(logits, score, None, R, W, -1, ld)
+    done = (rng.random(R * W) < 0.3).astype(np.int32) * 5
+    check(logits, score, done, R, W, min(1, n - 1), ld)
+    check(logits, score, done, R, W, n - 1, ld, in_place=True)
+    check(logits, score, np.ones(R * W, np.int32), R, W, 0, ld)
+
+
+def test_first_step(hip):
+    """All beams but the first at -inf: the first row's best tokens; and with fewer tokens above -inf than beams."""
+    rng = np.random.default_rng(1)
+    R, W, n = 2, 4, 3000
+    logits = rng.normal(size=(R * W, n)).astype(np.float32)
+    score = np.tile([0, -np.inf, -np.inf, -np.inf], R).astype(np.float32)
+    check(logits, score, None, R, W, -1)
+    logits[0, :] = -np.inf
+    logits[0, [5, 2999]] = [1.0, 2.0]
+    logits[4, 7:] = np.nan
+    logits[4, :7] = -np.inf
+    check(logits, score, None, R, W, -1)
+    check(logits, score, np.array([1, 0, 0, 0, 0, 1, 0, 0], np.int32), R, W, 2)
+
+
+def test_ties_masks_and_specials(hip):
+    rng = np.random.default_rng(2)
+    R, W, n = 3, 4, 5000
+    logits = np.round(rng.normal(size=(R * W, n))).astype(np.float32)         # many equal ones
+    logits[logits == 0] = np.where(rng.random((logits == 0).sum()) < 0.5, -0.0, 0.0)
+    score = np.zeros(R * W, np.float32)
+    logits[4:8] = logits[4]                                                     # beams that are alike
+    check(logits, score, None, R, W, -1)
+    logits[rng.random(logits.shape) < 0.5] = -np.inf
+    logits[rng.random(logits.shape) < 0.1] = np.nan
+    check(logits, score, None, R, W, -1)
+    logits[0, 77] = np.inf
+    logits[9] = -np.inf
+    score[2], score[6], score[10] = np.nan, -np.inf, np.inf
+    check(logits, score, None, R, W, -1)
+    check(logits, score, (np.arange(12) % 3 == 0).astype(np.int32), R, W, 4999)
+    check(logits, score, (np.arange(12) % 3 == 0).astype(np.int32), R, W, 5000)
+    check(logits, score, np.ones(12, np.int32), R, W, -3)
+
+
+@pytest.mark.parametrize("down", [False, True])
+def test_sorted_logits(hip, down):
+    """Rising logits, where every element enters the wave's list, and falling ones."""
+    n = 40000
+    x = np.linspace(-5, 5, n, dtype=np.float32)[::-1 if down else 1]
+    check(np.stack([x, x - 1, x + 1, x]).astype(np.float32), np.array([-1, -1, -2, -1.5], np.float32), None, 1, 4, -1)
+
+
+def test_far_logits(hip):
+    """Magnitudes whose exponentials overflow or vanish."""
+    x = np.array([[3e38, 2.9e38, -3e38, 0, 1], [-3e38, -3e38, -2e38, -2e38, -1e38], [88, 89, 90, 91, 1000], [0, 0, 0, 0, 0]], np.float32)
+    check(x, np.array([0, 0, 0, 0], np.float32), None, 1, 4, -1)

@@ -1,0 +1,579 @@
+"""The paged cache on the GPU against plain numpy: rows in and out (bytes and values), attention of one new token,
+reordering, and a beam-search decode through all of it."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import paged_ref as ref
+from tests.paged_ref import BF16, F16, F32, Q4_0, Q8_0
+
+pytestmark = pytest.mark.gpu
+CACHES = [F32, BF16, F16, Q8_0, Q4_0]
+
+
+def dev(a):
+    from sapphire_amd.device import DeviceArray
+    return DeviceArray.from_numpy(np.ascontiguousarray(a))
+
+
+def sync():
+    from sapphire_amd import load
+    assert load().sapphire_synchronize() == 0
+
+
+class Cache:
+    """A cache on the device with its byte-for-byte double on the host."""
+
+    def __init__(self, dtype, layers, pages, ps, nkv, hd, fill=0xff):
+        from sapphire_amd.paged import PagedCache
+        self.dtype, self.ps, self.nkv, self.hd = dtype, ps, nkv, hd
+        self.pool = {w: ref.Pool(w, dtype, layers, pages, ps, nkv, hd, fill) for w in "kv"}
+        self.on = {w: dev(self.pool[w].a) for w in "kv"}
+        self.c = PagedCache(dtype, layers, pages, ps, nkv, hd, k=self.on["k"].ptr, v=self.on["v"].ptr)
+        assert self.c.nbytes == self.pool["k"].a.nbytes
+
+    def upload(self):
+        for w in "kv":
+            self.on[w].upload(self.pool[w].a)
+
+    def fill(self, layer, table, seq, k, v):
+        """Host side only: rows [positions][heads][hd] of sequence `seq`."""
+        for p in range(len(k)):
+            page = table[seq, p // self.ps]
+            if page >= 0:
+                self.pool["k"].put(layer, page, p % self.ps, k[p])
+                self.pool["v"].put(layer, page, p % self.ps, v[p])
+
+
+def tables(rng, lens, ps, extra=3, ld_extra=1):
+    """A table with its pages in no order, -1 behind each row's, and the number of pages."""
+    need = [-(-max(n, 0) // ps) for n in lens]
+    order = rng.permutation(sum(need) + extra)
+    t, at = np.full((len(lens), max(need) + ld_extra), -1, np.int32), 0
+    for r, k in enumerate(need):
+        t[r, :k] = order[at:at + k]
+        at += k
+    return t, len(order)
+
+
+def device_rows(x, dtype, order="thd", pad=0, shift=0):
+    """(rows, buffer, view of a host copy) of fp32 x [tokens][heads][hd] in a layout: tokens or heads outermost, `pad`
+    elements between rows of the outer dim, the data `shift` elements into the buffer."""
+    from sapphire_amd.paged import Rows
+    t, h, hd = x.shape
+    ts, hs = (h * hd + pad, hd) if order == "thd" else (hd, t * hd + pad)
+    n = shift + (t - 1) * ts + (h - 1) * hs + hd
+    host = np.full(n + 5, 7, ref.np_type(dtype))
+    view = np.lib.stride_tricks.as_strided(host[shift:], x.shape, tuple(s * host.itemsize for s in (ts, hs, 1)))
+    view[...] = ref.to_type(dtype, x)
+    d = dev(host)
+    return Rows(d.ptr + shift * host.itemsize, dtype, t, h, hd, ts, hs), d, host, view
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("io,order,pad,shift", [(F32, "thd", 0, 0), (BF16, "thd", 192, 64), (F16, "htd", 8, 8), (F32, "htd", 1, 3), (BF16, "thd", 3, 1)],
+                         ids=["f32", "bf16_slice", "f16_heads_outer", "f32_odd", "bf16_odd"])
+def test_write_and_read(hip, cache, hd, io, order, pad, shift):
+    """Every byte of both pools after a write: the rows' where they belong, the rest as it was; then the rows read back,
+    each the value that the cache holds rounded once to the rows' type: exactly equal. Padding, rows and pages that do
+    not exist are left out and read as zeros."""
+    rng = np.random.default_rng(hd * 10 + cache)
+    nkv, ps, layers = 3, 48, 2
+    lens = [100, 1, 0, 47, 49]
+    table, pages = tables(rng, lens, ps)
+    table[4, 1] = pages + 5                        # a page that does not exist
+    seqs, pos = zip(*[(s, p) for s, n in enumerate(lens) for p in rng.permutation(n)[:40]])
+    seqs, pos = list(seqs) + [0, 0, 9, -1, 1], list(pos) + [-1, 100 * ps, 0, 0, ps]      # none of these exist
+    t = len(seqs)
+    x = {w: (rng.normal(size=(t, nkv, hd)) * 2).astype(np.float32) for w in "kv"}
+    c = Cache(cache, layers, pages, ps, nkv, hd)
+    rk, rv = device_rows(x["k"], io, order, pad, shift), device_rows(x["v"], io, order, pad, shift)
+    from sapphire_amd.paged import PageTable
+    dt, ds, dp = dev(table), dev(np.array(seqs, np.int32)), dev(np.array(pos, np.int32))
+    pt = PageTable(dt, *table.shape)
+    c.c.write(1, rk[0], rv[0], pt, dp, seqs=ds)
+    sync()
+    there, want = [], {w: np.zeros((t, nkv, hd), np.float32) for w in "kv"}
+    for i, (s, p) in enumerate(zip(seqs, pos)):
+        ok = 0 <= s < len(lens) and 0 <= p < table.shape[1] * ps and 0 <= table[s, p // ps] < pages
+        there.append(ok)
+        for w, r in (("k", rk), ("v", rv)):
+            if ok:
+                row = ref.from_type(io, r[3][i])
+                c.pool[w].put(1, table[s, p // ps], p % ps, row)
+                want[w][i] = ref.stored(cache, row)
+    assert 0 < sum(there) < t
+    for w in "kv":
+        np.testing.assert_array_equal(c.on[w].numpy(), c.pool[w].a, err_msg=w)
+    ok_, ov_ = device_rows(np.ones((t, nkv, hd), np.float32), io, order, pad, shift), device_rows(np.ones((t, nkv, hd), np.float32), io, order, pad, shift)
+    c.c.read(1, ok_[0], ov_[0], pt, dp, seqs=ds)
+    sync()
+    for w, r in (("k", ok_), ("v", ov_)):
+        r[3][...] = ref.to_type(io, want[w])       # the host copy with the rows in place: padding included
+        np.testing.assert_array_equal(r[1].numpy(), r[2], err_msg=w)
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+def test_write_special_values(hip, cache):
+    """Zeros of both signs, ties of the largest magnitude, subnormal blocks, halves between codes, NaN and infinities."""
+    hd, ps, t = 64, 16, 12
+    x = np.zeros((t, 1, hd), np.float32)
+    x[0, 0, ::2] = -0.0
+    x[1, 0, 5], x[1, 0, 9] = -3.0, 3.0
+    x[2, 0, 5], x[2, 0, 9] = 3.0, -3.0
+    x[3, 0] = np.float32(1e-41) * np.arange(hd)
+    x[4, 0, :32] = np.arange(32) * 0.5 * 127 / 127
+    x[4, 0, 0] = 127.0
+    x[5, 0] = np.where(np.arange(hd) % 2, 1.5, -2.5)
+    x[5, 0, 3] = 127.0
+    x[6, 0, 7] = np.nan
+    x[7, 0, 40] = np.inf
+    x[8, 0, 1] = -np.inf
+    x[9, 0] = 3e38
+    x[9, 0, 2] = -3e38
+    x[10, 0] = np.float32(1.4e-45)
+    x[11, 0] = 65519.0
+    c = Cache(cache, 1, 1, ps, 1, hd)
+    from sapphire_amd.paged import PageTable
+    dt, dp, ds = dev(np.zeros((1, 1), np.int32)), dev(np.arange(t, dtype=np.int32)), dev(np.zeros(t, np.int32))
+    rk, rv = device_rows(x, F32), device_rows(-x, F32)
+    c.c.write(0, rk[0], rv[0], PageTable(dt, 1, 1), dp, seqs=ds)
+    ok_, ov_ = device_rows(np.ones_like(x), F32), device_rows(np.ones_like(x), F32)
+    c.c.read(0, ok_[0], ov_[0], PageTable(dt, 1, 1), dp, seqs=ds)
+    sync()
+    for w, r, s in (("k", ok_, x), ("v", ov_, -x)):
+        got = r[1].numpy()[:t * hd].reshape(t, hd)
+        np.testing.assert_array_equal(got, ref.stored(cache, s)[:, 0], err_msg=w)
+        if cache in (Q8_0, Q4_0):
+            assert np.isnan(got[6, :32]).all() and np.isnan(got[7, 32:]).all() and np.isfinite(got[7, :32]).all() and np.isnan(got[8, :32]).all()
+
+
+def attend_case(rng, cache, io, hd, nkv, heads, ps, lens, window=0, softcap=0.0, layers=1, layer=0, peak=2.0, max_length=None,
+                broken=(), order="thd", pad=0, lse=True, stream=None, n_given=None):
+    """Runs one call and compares it with 64 bits; returns (out, lse) as read."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, layers, pages, ps, nkv, hd)   # 0xff bytes: NaN wherever nothing is written, scales included
+    ks, vs = [], []
+    for s, n in enumerate(lens):
+        k, v = (rng.normal(size=(n, nkv, hd)).astype(np.float32) for _ in range(2))
+        ks.append(ref.stored(cache, k))
+        vs.append(ref.stored(cache, v))
+        c.fill(layer, table, s, k, v)
+    c.upload()
+    for s, i in broken:
+        table[s, i] = pages + i if i % 2 else -7
+    q = (rng.normal(size=(len(lens), heads, hd)) * peak).astype(np.float32)
+    rq, ro = device_rows(q, io, order, pad), device_rows(q * 0 + 3, io, order, pad)
+    qs = ref.from_type(io, rq[3])
+    top = max_length or max(1, max(lens))
+    dt, dl = dev(table), dev(np.array(lens if n_given is None else n_given, np.int32))
+    dlse = dev(np.full((len(lens) + 1, heads), 5, np.float32))
+    ws = DeviceArray(max(1, c.c.attention_workspace_bytes(len(lens), heads, top)))
+    scale = 1.0 / np.sqrt(hd)
+    c.c.attention(layer, rq[0], ro[0], PageTable(dt, *table.shape), dl, top, scale, window=window, softcap=softcap,
+                  lse=dlse if lse else None, workspace=ws, stream=stream)
+    sync()
+    host = ro[2].copy()
+    raw = ro[1].numpy()
+    ro[2][...] = raw
+    got, glse = ref.from_type(io, ro[3].copy()).astype(np.float64), dlse.numpy()
+    ro[2][...] = host
+    ro[3][...] = 0
+    mask = np.ones(raw.shape, bool)
+    host = np.ones_like(ro[2])
+    np.lib.stride_tricks.as_strided(mask[:], q.shape, tuple(s // host.itemsize for s in ro[3].strides))[...] = False
+    assert (raw[mask] == 7).all(), "elements between the rows were written"
+    assert (glse[-1] == 5).all()
+    rounded = io != F32
+    for s, n in enumerate(lens):
+        keep = np.ones(n, bool)
+        lo = max(0, n - window) if window > 0 else 0
+        keep[:lo] = False
+        for bs, i in broken:
+            if bs == s:
+                keep[i * ps:(i + 1) * ps] = False
+        out, l, size, mean = ref.attention64(qs[s], ks[s][keep], vs[s][keep], scale, 0, softcap)
+        tol, ltol = ref.attention_bound(io, rounded, hd, n, out, l, size, mean, softcap)
+        worst = np.max(np.abs(got[s] - out) / tol)
+        assert worst <= 1, (s, n, worst)
+        if lse:
+            dead = np.isneginf(l)
+            assert np.array_equal(np.isneginf(glse[s]), dead)
+            assert (np.abs(glse[s][~dead] - l[~dead]) <= ltol[~dead]).all(), (s, n)
+            assert (got[s][dead] == 0).all()
+    if not lse:
+        assert (glse == 5).all()
+    return got, glse
+
+
+IO = [(F32, F32), (BF16, F32), (F16, F32), (Q8_0, F32), (Q4_0, F32), (BF16, BF16), (F16, F16), (Q8_0, BF16), (Q8_0, F16), (Q4_0, BF16), (Q4_0, F16)]
+IDS = [f"{ref.NAME[a]}-{ref.NAME[b]}" for a, b in IO]
+LENS = [0, 1, 15, 16, 17, 63, 64, 65, 130, 511]
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+@pytest.mark.parametrize("hd,nkv,heads,ps", [(64, 1, 4, 16), (128, 3, 3, 48), (256, 1, 4, 64), (128, 2, 16, 32), (64, 2, 34, 16), (256, 2, 10, 48)])
+def test_attention(hip, cache, io, hd, nkv, heads, ps):
+    """Lengths around the tiles and pages, NaN behind every sequence's last position, head groups of 1 to 17."""
+    attend_case(np.random.default_rng(hd + heads), cache, io, hd, nkv, heads, ps, LENS)
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+def test_attention_pieces(hip, cache, io):
+    """Few sequences, cut into pieces and joined: short ones beside one of several thousand positions."""
+    rng = np.random.default_rng(7)
+    attend_case(rng, cache, io, 128, 1, 4, 64, [3001, 5, 0, 1024])
+    attend_case(rng, cache, io, 256, 1, 4, 16, [1025], layers=2, layer=1)
+    attend_case(rng, cache, io, 64, 2, 6, 1024, [2049, 2047], order="htd", pad=5)
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+@pytest.mark.parametrize("window,softcap", [(1, 0.0), (16, 0.0), (100, 0.0), (512, 30.0), (0, 5.0)])
+def test_attention_window_and_cap(hip, cache, io, window, softcap):
+    attend_case(np.random.default_rng(window), cache, io, 128, 2, 8, 48, [1, 16, 99, 100, 101, 700], window=window, softcap=softcap, peak=4.0)
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+def test_attention_pages_that_do_not_exist(hip, cache):
+    attend_case(np.random.default_rng(3), cache, F32, 64, 1, 4, 16, [40, 16, 100, 700], broken=[(0, 1), (1, 0), (2, 0), (2, 6), (3, 5), (3, 43)])
+
+
+def test_attention_lengths_are_clamped(hip):
+    rng = np.random.default_rng(4)
+    attend_case(rng, F32, F32, 64, 1, 2, 16, [0, 50, 20], n_given=[-5, 1000, 20], max_length=50, lse=False)
+    attend_case(rng, Q8_0, F32, 64, 1, 2, 16, [0, 50, 20], n_given=[-2**31, 2**31 - 1, 20], max_length=50)
+
+
+@pytest.mark.parametrize("cache", [F32, Q8_0], ids=ref.NAME.get)
+def test_attention_of_peaked_and_flat_scores(hip, cache):
+    """Scores of hundreds (one weight carries all) and of zero (all are equal)."""
+    rng = np.random.default_rng(5)
+    attend_case(rng, cache, F32, 128, 1, 8, 32, [500, 33], peak=100.0)
+    attend_case(rng, cache, F32, 128, 1, 8, 32, [500, 33], peak=0.0)
+
+
+@pytest.mark.parametrize("io", [F32, BF16, F16], ids=ref.NAME.get)
+def test_attention_infinite_and_nan_scores(hip, io):
+    """-inf scores weigh nothing (a row of them only gives 0 and -inf, whatever V holds there); NaN and +inf reach the
+    outputs of their heads and sequences only."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(6)
+    hd, ps, heads = 64, 16, 2
+    for n in (40, 700):
+        table, pages = tables(rng, [n] * 5, ps)
+        c = Cache(io, 1, pages, ps, 1, hd)
+        k, v = (rng.normal(size=(5, n, 1, hd)).astype(np.float32) for _ in range(2))
+        k[..., 0] = 1.0
+        k[0, 3:20, 0, 0] = -np.inf             # some positions weigh nothing
+        k[1, :, 0, 0] = -np.inf                # all of them
+        v[1, :, 0, :] = np.nan
+        k[2, 7, 0, 5] = np.nan
+        k[3, n - 1, 0, 0] = np.inf
+        for s in range(5):
+            c.fill(0, table, s, k[s], v[s])
+        c.upload()
+        q = rng.normal(size=(5, heads, hd)).astype(np.float32)
+        q[..., 0] = 1.0
+        rq, ro = device_rows(q, io), device_rows(q * 0, io)
+        dt, dl, dlse = dev(table), dev(np.full(5, n, np.int32)), DeviceArray.empty((5, heads))
+        ws = DeviceArray(max(1, c.c.attention_workspace_bytes(5, heads, n)))
+        c.c.attention(0, rq[0], ro[0], PageTable(dt, *table.shape), dl, n, 0.125, lse=dlse, workspace=ws)
+        sync()
+        got = ref.from_type(io, ro[1].numpy()[:5 * heads * hd]).reshape(5, heads, hd)
+        lse = dlse.numpy()
+        assert np.isnan(got[2]).all() and np.isnan(got[3]).all() and np.isnan(lse[2]).all() and np.isnan(lse[3]).all()
+        assert (got[1] == 0).all() and np.isneginf(lse[1]).all()
+        for s in (0, 4):
+            out, l, size, mean = ref.attention64(ref.from_type(io, rq[3])[s], np.where(np.isneginf(k[s]), -1e30, ref.stored(io, k[s])), ref.stored(io, v[s]), 0.125)
+            _, _, size, _ = ref.attention64(ref.from_type(io, rq[3])[s], np.where(np.isneginf(k[s]), 0, ref.stored(io, k[s])), ref.stored(io, v[s]), 0.125)
+            tol, ltol = ref.attention_bound(io, io != F32, hd, n, out, l, size, mean)
+            assert (np.abs(got[s] - out) <= tol).all() and (np.abs(lse[s] - l) <= ltol).all()
+
+
+def test_pages_past_four_gigabytes(hip):
+    """Rows written, read and attended to in the last pages of pools of more than 2^32 bytes."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PagedCache, PageTable
+    hd, ps, pages = 256, 64, 70000
+    c = PagedCache(F32, 1, pages, ps, 1, hd)
+    assert c.nbytes > 2**32
+    rng = np.random.default_rng(8)
+    n = 100
+    table = np.array([[pages - 1, pages - 3]], np.int32)
+    k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+    rk, rv = device_rows(k, F32), device_rows(v, F32)
+    dt, dp, ds = dev(table), dev(np.arange(n, dtype=np.int32)), dev(np.zeros(n, np.int32))
+    c.write(0, rk[0], rv[0], PageTable(dt, 1, 2), dp, seqs=ds)
+    ok_, ov_ = device_rows(k * 0, F32), device_rows(v * 0, F32)
+    c.read(0, ok_[0], ov_[0], PageTable(dt, 1, 2), dp, seqs=ds)
+    q = rng.normal(size=(1, 2, hd)).astype(np.float32)
+    rq, ro = device_rows(q, F32), device_rows(q * 0, F32)
+    dl = dev(np.array([n], np.int32))
+    ws = DeviceArray(max(1, c.attention_workspace_bytes(1, 2, n)))
+    c.attention(0, rq[0], ro[0], PageTable(dt, 1, 2), dl, n, 1 / 16, workspace=ws)
+    sync()
+    np.testing.assert_array_equal(ok_[1].numpy(), rk[2])
+    np.testing.assert_array_equal(ov_[1].numpy(), rv[2])
+    out, l, size, mean = ref.attention64(q[0], k, v, 1 / 16)
+    tol, _ = ref.attention_bound(F32, False, hd, n, out, l, size, mean)
+    assert (np.abs(ro[1].numpy()[:2 * hd].reshape(2, hd) - out) <= tol).all()
+    for d in (c.k, c.v):
+        d.free()
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+@pytest.mark.parametrize("hd,nkv,ps", [(64, 2, 16), (128, 1, 48), (256, 1, 64)])
+def test_reorder(hip, cache, hd, nkv, ps):
+    """Tables, lengths and every byte of both pools; parents used several times and not at all, a parent and a spare page
+    that do not exist, full and empty rows, lengths out of range."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(ps)
+    ld, layers = 4, 3
+    lens = np.array([0, 1, 17, ps, ps + 15, 2 * ps + 16, 4 * ps, 3 * ps + 1, -4, 100 * ps], np.int32)
+    rows = len(lens)
+    pages = rows * ld + rows + 2
+    order = rng.permutation(pages).astype(np.int32)
+    table, spare = order[:rows * ld].reshape(rows, ld).copy(), order[rows * ld:rows * ld + rows].copy()
+    parents = np.array([4, 4, 2, 5, 7, 1, 9, 0, 12, 8], np.int32)
+    spare[4] = pages                           # row 4 continues row 7, partly filled
+    c = Cache(cache, layers, pages, ps, nkv, hd)
+    for w in "kv":
+        c.pool[w].a[...] = rng.integers(0, 256, c.pool[w].a.shape, np.uint8)
+    c.upload()
+    d = [dev(a) for a in (table, parents, lens, spare)]
+    to, lo = DeviceArray.empty((rows, ld), np.int32), DeviceArray.empty(rows, np.int32)
+    c.c.reorder(PageTable(d[0], rows, ld), d[1], d[2], d[3], PageTable(to, rows, ld), lo)
+    sync()
+    want_t, want_l = np.full((rows, ld), -1, np.int32), np.zeros(rows, np.int32)
+    for b, p in enumerate(parents):
+        if not 0 <= p < rows:
+            continue
+        n = int(np.clip(lens[p], 0, ld * ps))
+        want_l[b] = n
+        full, rem = divmod(n, ps)
+        want_t[b, :full] = table[p, :full]
+        if rem and 0 <= spare[b] < pages:
+            want_t[b, full] = spare[b]
+            held = -(-rem // 16) * 16
+            for w in "kv":
+                code = c.pool[w].code
+                a = c.pool[w].a
+                a[:, spare[b], :, :held * code] = a[:, table[p, full], :, :held * code]
+                per = (c.pool[w].tile - ps * code) // ps
+                a[:, spare[b], :, ps * code:ps * code + held * per] = a[:, table[p, full], :, ps * code:ps * code + held * per]
+    np.testing.assert_array_equal(to.numpy(), want_t)
+    np.testing.assert_array_equal(lo.numpy(), want_l)
+    for w in "kv":
+        np.testing.assert_array_equal(c.on[w].numpy(), c.pool[w].a)
+
+
+class Graph:
+    """What `work(stream)` enqueues, captured on a stream of its own through the HIP runtime that the library uses."""
+
+    def __init__(self, work):
+        path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+        self.rt, self.stream, self.graph, self.exec = C.CDLL(path), C.c_void_p(), C.c_void_p(), C.c_void_p()
+        self.ok(self.rt.hipStreamCreateWithFlags(C.byref(self.stream), 1))
+        self.ok(self.rt.hipStreamBeginCapture(self.stream, 2))
+        work(self.stream)
+        self.ok(self.rt.hipStreamEndCapture(self.stream, C.byref(self.graph)))
+        self.ok(self.rt.hipGraphInstantiate(C.byref(self.exec), self.graph, None, None, C.c_size_t(0)))
+
+    @staticmethod
+    def ok(rc):
+        assert rc == 0, rc
+
+    def replay(self):
+        self.ok(self.rt.hipGraphLaunch(self.exec, self.stream))
+
+    def close(self):
+        self.ok(self.rt.hipStreamSynchronize(self.stream))
+        self.ok(self.rt.hipGraphExecDestroy(self.exec))
+        self.ok(self.rt.hipGraphDestroy(self.graph))
+        self.ok(self.rt.hipStreamDestroy(self.stream))
+
+
+@pytest.mark.parametrize("cache,io", [(F32, F32), (Q8_0, F32), (BF16, BF16)], ids=["f32", "q8_0", "bf16"])
+def test_captured_step(hip, cache, io):
+    """A step (rotate, write, attend, select, reorder) captured into a graph and replayed as the lengths grow, against the
+    same calls made eagerly on a second cache between the replays: the same bits."""
+    from sapphire_amd import paged
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PagedCache, PageTable, Rows
+    rng = np.random.default_rng(9)
+    b, heads, nkv, hd, ps, ld, n = 3, 4, 1, 64, 16, 20, 900
+    order = rng.permutation(b * ld + b).astype(np.int32)
+    table, spare = dev(order[:b * ld].reshape(b, ld)), dev(order[b * ld:])
+    pos = np.array([0, 30, 7], np.int32)
+    dpos, dlen = dev(pos), dev(pos + 1)
+    freqs = dev(paged.rope_frequencies(hd, 1e4)[0])
+    H, es = heads + 2 * nkv, 4 if io == F32 else 2
+    qkv, logits, score = DeviceArray(b * H * hd * es), DeviceArray(b * n * 4), DeviceArray(4 * b)
+
+    class Side:
+        def __init__(self):
+            self.c = PagedCache(cache, 1, b * ld + b, ps, nkv, hd)
+            self.out, self.turned = DeviceArray.empty(b * heads * hd * es, np.uint8), DeviceArray(b * (heads + nkv) * hd * es)
+            self.lse, self.table = DeviceArray.empty((b, heads)), DeviceArray.empty((b, ld), np.int32)
+            self.ws, self.bws = (DeviceArray(max(1, x)) for x in (self.c.attention_workspace_bytes(b, heads, ld * ps),
+                                                                    paged.beam_workspace_bytes(n, 1, b)))
+            self.new = [DeviceArray.empty(b), *(DeviceArray.empty(b, np.int32) for _ in range(3))]
+            for d in (self.c.k, self.c.v, self.out, self.lse, self.table, *self.new):
+                d.zero()
+
+        def step(self, stream):
+            c, pt = self.c, PageTable(table, b, ld)
+            def rows(d, first, count, width):
+                return Rows(d.ptr + first * hd * es, io, b, count, hd, width * hd, hd)
+            paged.rope(rows(qkv, 0, heads + nkv, H), rows(self.turned, 0, heads + nkv, heads + nkv), dpos, freqs, hd, stream=stream)
+            c.write(0, rows(self.turned, heads, nkv, heads + nkv), rows(qkv, heads + nkv, nkv, H), pt, dpos, stream=stream)
+            c.attention(0, rows(self.turned, 0, heads, heads + nkv), rows(self.out, 0, heads, heads), pt, dlen, ld * ps, 0.125,
+                        lse=self.lse, workspace=self.ws, stream=stream)
+            paged.beam_select(logits, n, n, 1, b, score, self.new[0], self.new[1], self.new[2], self.bws, stream=stream)
+            c.reorder(pt, self.new[2], dlen, spare, PageTable(self.table, b, ld), self.new[3], stream=stream)
+
+        def results(self):
+            return [d.numpy() for d in (self.out, self.lse, self.table, *self.new, self.c.k, self.c.v)]
+
+    def renew():
+        qkv.upload(ref.to_type(io, rng.normal(size=(b, H, hd)).astype(np.float32)))
+        logits.upload(rng.normal(size=(b, n)).astype(np.float32))
+        score.upload(-np.abs(rng.normal(size=b)).astype(np.float32))
+    replayed, eager = Side(), Side()
+    renew()
+    graph = Graph(replayed.step)
+    for k in range(40):
+        graph.replay()
+        eager.step(None)
+        sync()
+        for i, (x, y) in enumerate(zip(replayed.results(), eager.results())):
+            np.testing.assert_array_equal(x, y, err_msg=f"replay {k}, result {i}")
+        assert np.isfinite(replayed.lse.numpy()).all()
+        pos = pos + 5
+        dpos.upload(pos)
+        dlen.upload(pos + 1)
+        renew()
+    graph.close()
+
+
+def test_streams(hip):
+    """The same call on a stream of its own, beside another on the null stream with its own workspace."""
+    from sapphire_amd import load
+    L = load()
+    s = L.sapphire_stream_create()
+    rng = np.random.default_rng(10)
+    attend_case(rng, F32, F32, 128, 1, 4, 32, [900, 40], stream=s)
+    attend_case(rng, Q4_0, F32, 128, 1, 4, 32, [900, 40], stream=s)
+    assert L.sapphire_stream_synchronize(s) == 0 and L.sapphire_stream_destroy(s) == 0
+
+
+def test_results_do_not_depend_on_the_batch(hip):
+    """A sequence's bits beside others equal its bits in another place with other neighbours (same max_length and batch)."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(11)
+    hd, ps, heads = 128, 32, 4
+    lens = [700, 90, 33, 1]
+    table, pages = tables(rng, lens, ps)
+    c = Cache(Q8_0, 1, pages, ps, 1, hd)
+    for s, n in enumerate(lens):
+        c.fill(0, table, s, rng.normal(size=(n, 1, hd)).astype(np.float32), rng.normal(size=(n, 1, hd)).astype(np.float32))
+    c.upload()
+    q = rng.normal(size=(4, heads, hd)).astype(np.float32)
+    got = []
+    for order in ([0, 1, 2, 3], [3, 2, 1, 0], [1, 1, 0, 0]):
+        rq, ro = device_rows(q[order], F32), device_rows(q * 0, F32)
+        dt, dl = dev(table[order]), dev(np.array(lens, np.int32)[order])
+        ws = DeviceArray(max(1, c.c.attention_workspace_bytes(4, heads, 700)))
+        c.c.attention(0, rq[0], ro[0], PageTable(dt, *table.shape), dl, 700, 0.1, workspace=ws)
+        sync()
+        o = ro[1].numpy()[:q.size].reshape(q.shape)
+        got.append({s: o[i] for i, s in enumerate(order)})
+    for g in got[1:]:
+        for s in g:
+            np.testing.assert_array_equal(g[s], got[0][s])
+
+
+@pytest.mark.parametrize("cache", [F32, Q8_0, Q4_0], ids=ref.NAME.get)
+def test_beam_search_decode(hip, cache):
+    """Fourteen steps of beam search (two requests of three beams, two layers) through rotary rows, cache writes,
+    attention, selection and reordering, as a server runs them, against histories kept per beam in 64 bits."""
+    from sapphire_amd import paged
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable, Rows
+    rng = np.random.default_rng(12)
+    R, W, L, heads, nkv, hd, ps, vocab, steps, end = 2, 3, 2, 4, 1, 64, 16, 50, 22, 1
+    B, H = R * W, heads + 2 * nkv
+    emb = rng.normal(size=(vocab, L, H, hd)).astype(np.float32)
+    head = (rng.normal(size=(L * heads * hd, vocab)) * 0.3).astype(np.float32)
+    freqs, _ = paged.rope_frequencies(hd, 1e4)
+    ld = -(-steps // ps) + 1
+    pages = 4 * B * ld
+    c = Cache(cache, L, pages, ps, nkv, hd)
+    free = list(rng.permutation(pages).astype(np.int32))
+    table, spare = np.full((B, ld), -1, np.int32), np.array([free.pop() for _ in range(B)], np.int32)
+    lens = np.zeros(B, np.int32)
+    tok = rng.integers(2, vocab, R).repeat(W)
+    score, done = np.tile([0, -np.inf, -np.inf], R).astype(np.float32), np.zeros(B, np.int32)
+    hist = [[[] for _ in range(L)] for _ in range(B)]           # (k, v) as stored
+    score64 = score.astype(np.float64)
+    dfreqs = dev(freqs)
+    ws = DeviceArray(max(1, c.c.attention_workspace_bytes(B, heads, ld * ps)))
+    bws = DeviceArray(paged.beam_workspace_bytes(vocab, R, W))
+    for step in range(steps):
+        for b in range(B):                                     # a page for the new position where one begins
+            if lens[b] % ps == 0:
+                table[b, lens[b] // ps] = free.pop()
+        dt, dpos, dlen = dev(table), dev(lens), dev(lens + 1)
+        pt = PageTable(dt, B, ld)
+        outs, outs64 = [], []
+        for l in range(L):
+            x = emb[tok, l]
+            dx, dy = dev(x), DeviceArray.empty((B, heads + nkv, hd))
+            do = DeviceArray.empty((B, heads, hd))
+            rows = lambda d, first, n, width: Rows(d.ptr + 4 * first * hd, F32, B, n, hd, width * hd, hd)      # noqa: E731
+            paged.rope(rows(dx, 0, heads + nkv, H), rows(dy, 0, heads + nkv, heads + nkv), dpos, dfreqs, hd)
+            c.c.write(l, rows(dy, heads, nkv, heads + nkv), rows(dx, heads + nkv, nkv, H), pt, dpos)
+            c.c.attention(l, rows(dy, 0, heads, heads + nkv), rows(do, 0, heads, heads), pt, dlen, ld * ps, 0.125, workspace=ws)
+            sync()
+            turned = dy.numpy()
+            want = ref.rope64(x[:, :heads + nkv], lens, freqs, hd, False, 1.0)
+            assert np.abs(turned - want).max() <= 2.0**-21 * np.abs(x).max()
+            outs.append(do.numpy())
+            o64 = np.zeros((B, heads, hd))
+            for b in range(B):
+                hist[b][l].append((ref.stored(cache, turned[b, heads:]), ref.stored(cache, x[b, heads + nkv:])))
+                k, v = (np.stack([e[i] for e in hist[b][l]]) for i in (0, 1))
+                o64[b], l64, size, mean = ref.attention64(turned[b, :heads], k, v, 0.125)
+                tol, _ = ref.attention_bound(F32, False, hd, len(k), o64[b], l64, size, mean)
+                assert (np.abs(outs[-1][b] - o64[b]) <= tol).all(), (step, l, b)
+            outs64.append(o64)
+        logits = (np.stack(outs, 1).reshape(B, -1) @ head).astype(np.float32)
+        dl, ds, dd = dev(logits), dev(score), dev(done)
+        so, to, po, eo = DeviceArray.empty(B), *(DeviceArray.empty(B, np.int32) for _ in range(3))
+        paged.beam_select(dl, vocab, vocab, R, W, ds, so, to, po, bws, done=dd, done_out=eo, end_token=end)
+        t2, l2, dsp = DeviceArray.empty((B, ld), np.int32), DeviceArray.empty(B, np.int32), dev(spare)
+        dn = dev(lens + 1)
+        c.c.reorder(pt, po, dn, dsp, PageTable(t2, B, ld), l2)
+        sync()
+        ws_, wt, wp, wd = ref.beams64(logits, score, done, R, W, end)
+        np.testing.assert_array_equal(to.numpy(), wt)
+        np.testing.assert_array_equal(po.numpy(), wp)
+        np.testing.assert_array_equal(eo.numpy(), wd)
+        assert np.abs(so.numpy() - ws_)[np.isfinite(ws_)].max() <= 1e-5 * np.abs(ws_[np.isfinite(ws_)]).max()
+        parents = po.numpy()
+        hist = [[list(hist[p][l]) for l in range(L)] for p in parents]
+        old = table[:, lens[0] // ps].copy()
+        lens = l2.numpy()
+        assert (lens == step + 1).all()
+        table = t2.numpy()
+        if (step + 1) % ps:
+            spare = old                                        # the pages copied from are the next spares
+        tok, score, done = to.numpy(), so.numpy(), eo.numpy()
+    assert len(set(parents)) < B or done.any()                 # beams were dropped along the way
