@@ -14,8 +14,13 @@ LIB_PATH = os.path.join(HERE, "libsapphire_hip.so")
 
 __all__ = ["LIB_PATH", "load"]
 
+_loaded = None
+
 
 def load():
     """Load libsapphire_hip.so (ctypes.CDLL with prototypes); raises if missing."""
-    from ._lib import load_library
-    return load_library(LIB_PATH)
+    global _loaded
+    if _loaded is None:
+        from ._lib import load_library
+        _loaded = load_library(LIB_PATH)
+    return _loaded
