@@ -21,12 +21,13 @@ constexpr int kCols = 16;                  // query heads of a workgroup
 constexpr int kPos = 16;                   // positions of a tile
 constexpr int kMaxPieces = 256;
 constexpr int kPieceUnit = 64;             // a piece is a multiple of so many positions
-constexpr int kWantGroups = 1024;          // workgroups that fill the chip (four per CU)
+constexpr int kFullGroups = 1024, kWantGroups = 4096;      // workgroups that are left as they are; that cut sequences make
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 struct AttnArgs {
     PagedAttn a;
     int n_heads, group, col_tiles, piece, pieces;
+    uint32_t page_magic;                   // i / (page_size / 16) is its high product with i < 2^26 (0: page_size is 16)
     float *part;                           // [pieces][batch][n_heads][hd], unnormalised O
     float2 *ms;                            // [pieces][batch][n_heads]: maximum (log2 units), sum
 };
@@ -54,10 +55,9 @@ struct Raw {
                 w[j] = *reinterpret_cast<const pu4 *>(tile + T::k_code(off, 0) + (uint32_t)((j * 4 + m) * 16 + c) * 16);
         }
         if constexpr (T::kQuant) {
-            // of position 4m + c % 4: the score product leaves a lane positions 4m .. 4m + 3, its quad has their scales
 #pragma unroll
             for (int b = 0; b < T::NB; b += 2) {
-                const float2 v = *reinterpret_cast<const float2 *>(tile + T::k_scale(ps, off + 4 * m + (c & 3), b));
+                const float2 v = *reinterpret_cast<const float2 *>(tile + T::k_scale(ps, off + c, b));
                 s[b] = v.x;
                 s[b + 1] = v.y;
             }
@@ -87,25 +87,48 @@ struct Raw {
             for (int u = 0; u < N; ++u) w[u] = *reinterpret_cast<const pu4 *>(tile + T::v_run(off + 4 * m + u * T::P, c));
         }
         if constexpr (T::kQuant) {
-            const pf4 v = *reinterpret_cast<const pf4 *>(tile + T::v_scale(ps, off + 4 * m, c * DPL / 32));
+            // of the blocks that column c of the weighted sum stands for
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] = v[r];
+            for (int i = 0; i < (T::NB + 3) / 4; ++i) {
+                const pf4 v = *reinterpret_cast<const pf4 *>(tile + T::v_scale(ps, off + 4 * m, 4 * i + (c & 3) % T::NB));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[4 * i + r] = v[r];
+            }
         }
     }
-    // The operand of block j: its codes (Q4_0: times 16) in element order.
+    // Quantized types. The score product's operand of block j: its codes (Q4_0: times 16) in element order.
     __device__ __forceinline__ pu2 k_codes(int j) const {
         if constexpr (CT == DT_Q8_0) return pu2{w[j / 2][j % 2 * 2], w[j / 2][j % 2 * 2 + 1]};
         const uint32_t v = w[j / T::G][j % T::G];
         return pu2{v << 4 & 0xf0f0f0f0u, v & 0xf0f0f0f0u};
     }
-    // Position 4m + r without effect: zeros, or a scale of 0.
-    __device__ __forceinline__ void clear_v(int r) {
-        if constexpr (T::kQuant) {
-            s[r] = 0.f;
+    // V's codes as signed bytes (Q4_0: times 16), word i: position r's DPL bytes start at byte r * DPL; Q4_0: the low
+    // nibbles' bytes of all positions, then the high ones'.
+    static constexpr int VW = DPL;
+    __device__ __forceinline__ void v_bytes(uint32_t (&q)[VW]) const {
+        if constexpr (CT == DT_Q8_0) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) q[i] = w[i / 4][i % 4];
         } else {
 #pragma unroll
-            for (int i = r * N; i < (r + 1) * N; ++i) w[i / 4][i % 4] = 0;     // N words per position
+            for (int i = 0; i < VW / 2; ++i) {
+                const uint32_t v = w[i / 4][i % 4] ^ 0x88888888u;
+                q[i] = v << 4 & 0xf0f0f0f0u;
+                q[VW / 2 + i] = v & 0xf0f0f0f0u;
+                // (the compiler would rather extract nibbles one by one)
+                asm("" : "+v"(q[i]), "+v"(q[VW / 2 + i]));
+            }
         }
+    }
+    // Element x of position 4m + r of them.
+    static __device__ __forceinline__ float v_byte(const uint32_t (&q)[VW], int r, int x) {
+        const int R = CT == DT_Q8_0 ? DPL : DPL / 2, i = (x / R) * (4 * R) + r * R + x % R;
+        return (float)(int8_t)(q[i / 4] >> (8 * (i % 4)));
+    }
+    // Float types: position 4m + r as it is, or zeros.
+    __device__ __forceinline__ void keep_v(int r, bool on) {
+#pragma unroll
+        for (int i = r * N; i < (r + 1) * N; ++i) w[i / 4][i % 4] = on ? w[i / 4][i % 4] : 0u;     // N words per position
     }
     // 16-bit types: elements x and x + 1 of position 4m + r.
     __device__ __forceinline__ uint32_t v_pair(int r, int x) const {
@@ -116,25 +139,28 @@ struct Raw {
     static __device__ __forceinline__ int v_dim(int x, int c) { return x / W * 16 * W + c * W + x % W; }
     __device__ __forceinline__ float v_at(int r, int x) const {
         if constexpr (CT == DT_F32) return __uint_as_float(w[r * (N / 4) + x / 4][x % 4]);
-        else if constexpr (!T::kQuant) {
-            // words of two elements: DPL / 2 per position, in order
-            const int i = r * (DPL / 2) + x / 2;
-            const uint32_t v = w[i / 4][i % 4];
-            if constexpr (CT == DT_BF16) return __uint_as_float(x & 1 ? v & 0xffff0000u : v << 16);
-            else return from_f16(x & 1 ? v >> 16 : v & 0xffffu);
-        } else if constexpr (CT == DT_Q8_0) {
-            const int i = r * (DPL / 4) + x / 4;
-            return __fmul_rn((float)(int8_t)(w[i / 4][i % 4] >> (8 * (x & 3))), s[r]);
-        } else {
-            const int R = DPL / 2, byte = r * R + x % R;       // R bytes per position
-            const uint32_t q = w[byte / 16][byte / 4 % 4] >> (8 * (byte % 4) + (x / R) * 4) & 15u;
-            return __fmul_rn((float)((int)q - 8), s[r]);
-        }
+        // words of two elements: DPL / 2 per position, in order
+        const uint32_t v = v_pair(r, x);
+        if constexpr (CT == DT_BF16) return __uint_as_float(x & 1 ? v & 0xffff0000u : v << 16);
+        else return from_f16(x & 1 ? v >> 16 : v & 0xffffu);
     }
 };
 
 __device__ __forceinline__ float load1(int dtype, const uint8_t *p, int64_t i) {
     return dtype == DT_F32 ? reinterpret_cast<const float *>(p)[i] : from_16(dtype, reinterpret_cast<const uint16_t *>(p)[i]);
+}
+template <int N>
+__device__ __forceinline__ void load_some(int dtype, const uint8_t *p, int64_t i, float (&x)[N]) {
+    if (dtype == DT_F32) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = reinterpret_cast<const float *>(p)[i + e];
+    } else {
+        uint16_t w[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = reinterpret_cast<const uint16_t *>(p)[i + e];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = from_16(dtype, w[e]);
+    }
 }
 __device__ __forceinline__ void store1(int dtype, uint8_t *p, int64_t i, float v) {
     if (dtype == DT_F32) reinterpret_cast<float *>(p)[i] = v;
@@ -143,188 +169,138 @@ __device__ __forceinline__ void store1(int dtype, uint8_t *p, int64_t i, float v
 
 __device__ __forceinline__ float lse_of(float mx, float sum) { return sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2; }
 
-// How scores and weighted sums are formed.
-//   kExact  fp32 rows over a float cache: v_mfma_f32_16x16x4_f32 on the elements as fp32.
-//   kHalf   16-bit rows over a cache of their type: 16x16x32 products of the elements as they are; the
-//           weights are rounded to that type, and V's 16-bit words are transposed in pairs on the way.
-//   kDigits a quantized cache: the codes as they are against q in four signed 8-bit digits (q rounded to
-//           2^-31 of the head's largest element), exact 32-bit sums per block, one fma with the block's
-//           scale. A head takes four columns, one per digit; NT sets of columns share the codes. The
-//           weighted sum is kExact's, codes times scale as fp32.
-enum Path { kExact = 0, kHalf = 1, kDigits = 2 };
 constexpr float kLazy = 8.0f;              // log2 units that a score may exceed the running maximum by
 
-typedef short ps8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pb8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
 typedef int pi4 __attribute__((ext_vector_type(4)));
 
 template <int CT>
 __device__ __forceinline__ pf4 mfma16(pu4 a, pu4 b, pf4 c) {
-    if constexpr (CT == DT_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8, a), __builtin_bit_cast(pb8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, a), __builtin_bit_cast(ph8, b), c, 0, 0, 0);
+    if constexpr (CT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, a), __builtin_bit_cast(ph8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8, a), __builtin_bit_cast(pb8, b), c, 0, 0, 0);
 }
 
-// Sum over each quad of lanes, in every lane of it.
-__device__ __forceinline__ float quad_sum(float v) {
-    v += lanes::dpp_mov<0xB1>(v);
-    return v + lanes::dpp_mov<0x4E>(v);
-}
-// Lane R of each quad, in every lane of it.
-template <int R>
-__device__ __forceinline__ float quad_lane(float v) {
-    return lanes::dpp_mov<R * 0x55>(v);
-}
+// A workgroup's part of the call: a piece of one sequence, for one K/V head's query heads h0 .. h0 + heads - 1,
+// and its walk over the pages, HALVES tiles of 16 positions at a time.
+template <int HALVES>
+struct Walk {
+    int b, hk, h0, heads, ps, start, lo, hi, last;
+    size_t slot0, head_at, page_bytes;
+    const __attribute__((address_space(4))) int *row;          // constant: page numbers come by scalar loads
+    size_t at[HALVES];                     // a tile's page: its bytes' start
+    uint32_t off[HALVES];                  // and its position in it
+    bool there[HALVES];
 
+    __device__ __forceinline__ Walk(const AttnArgs &g, int per_group) {
+        const PagedAttn &a = g.a;
+        b = blockIdx.z;
+        hk = blockIdx.y / g.col_tiles;
+        const int ct = blockIdx.y - hk * g.col_tiles;
+        h0 = hk * g.group + ct * per_group;
+        heads = min(per_group, g.group - ct * per_group);
+        ps = a.c.page_size;
+        const int n = min(max(a.lengths[b], 0), a.max_length);
+        start = a.window > 0 && n > a.window ? n - a.window : 0;
+        lo = (start & ~(kPos - 1)) + blockIdx.x * g.piece;
+        hi = min(n, lo + g.piece);
+        last = hi > lo ? (hi - 1) & ~(kPos - 1) : 0;           // the piece's last tile
+        slot0 = ((size_t)blockIdx.x * gridDim.z + b) * g.n_heads + h0;
+        head_at = (size_t)hk * a.c.tile_bytes;
+        page_bytes = (size_t)a.c.nkv * a.c.tile_bytes;
+        row = (const __attribute__((address_space(4))) int *)(a.table.pages + (size_t)b * a.table.ld);
+    }
+    // nothing to do: the first piece says so to the join
+    __device__ __forceinline__ bool empty(const AttnArgs &g) const {
+        if (lo < hi || g.pieces == 1) return false;
+        if (blockIdx.x == 0 && (int)threadIdx.x < heads) g.ms[slot0 + threadIdx.x] = make_float2(-INFINITY, 0.f);
+        return true;
+    }
+    // tiles t and on; past the end: the last one again
+    __device__ __forceinline__ void seek(const AttnArgs &g, int t) {
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) {
+            const uint32_t t16 = (uint32_t)min(t + u * kPos, last) / kPos, i = g.page_magic ? __umulhi(t16, g.page_magic) : t16;
+            off[u] = t16 * kPos - i * (uint32_t)ps;
+            const int page = row[__builtin_amdgcn_readfirstlane((int)i)];
+            there[u] = page >= 0 && page < g.a.c.pages;
+            at[u] = (there[u] ? (size_t)page : 0) * page_bytes + head_at;
+        }
+    }
+    __device__ __forceinline__ bool whole(int t) const {       // every position of the step counts
+        bool all = t >= start && t + HALVES * kPos <= hi;
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) all &= there[u];
+        return all;
+    }
+};
+
+__device__ __forceinline__ float capped(float x, float cap) { return __fmul_rn(cap, tanhf(__fdiv_rn(x, cap))); }
+
+// Rows over a float cache. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
+// cache of their type: 16x16x32 products of the elements as they are; the weights are rounded to that type
+// (half a step, what the outputs are rounded by too), and V's 16-bit words are transposed in pairs on the way.
 // grid (pieces, K/V heads x column tiles, sequences).
-template <int CT, int HD, int PATH, int NT>
+template <int CT, int HD, bool HALF>
 __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
-    using T = Tile<CT, HD>;
     constexpr int LD = HD + 4, DPL = R::DPL;
-    constexpr int HEADS = PATH == kDigits ? 4 * NT : kCols;    // of a workgroup
-    constexpr int HALVES = PATH == kHalf ? 2 : 1;              // 16-position tiles of a step
-    constexpr int STEP = kWaves * HALVES * kPos;
+    constexpr int HALVES = HALF ? 2 : 1, STEP = kWaves * HALVES * kPos;
     __shared__ __attribute__((aligned(16))) float buf[2 * kCols * LD];     // q, later the waves' O
     __shared__ float wm[kWaves][kCols], wsum[kWaves][kCols];
-    __shared__ int shift[kCols];                               // kDigits: q * 2^shift are the digits' integers
     const PagedAttn &a = g.a;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, m = lane >> 4;
-    const int b = blockIdx.z, hk = blockIdx.y / g.col_tiles, ct = blockIdx.y - hk * g.col_tiles;
-    const int h0 = hk * g.group + ct * HEADS, heads = min(HEADS, g.group - ct * HEADS);
-    // the head of column c (kDigits: of the four lanes of a head's digits the first NT take a set's each)
-    const int hc = PATH == kDigits ? (c >> 2) * NT + min(c & 3, NT - 1) : c;
-    const bool owner = hc < heads && (PATH != kDigits || (c & 3) < NT);
-    const int ps = a.c.page_size;
-    const int n = min(max(a.lengths[b], 0), a.max_length);
-    const int start = a.window > 0 && n > a.window ? n - a.window : 0;
-    const int lo = (start & ~(kPos - 1)) + blockIdx.x * g.piece, hi = min(n, lo + g.piece);
-    const size_t slot0 = ((size_t)blockIdx.x * gridDim.z + b) * g.n_heads + h0;
-    if (lo >= hi && g.pieces > 1) {
-        if (blockIdx.x == 0 && tid < heads) g.ms[slot0 + tid] = make_float2(-INFINITY, 0.f);
-        return;
-    }
-    // A step's tiles: page and offset run along with the position.
-    const int *row = a.table.pages + (size_t)b * a.table.ld;
-    const size_t head_at = (size_t)hk * a.c.tile_bytes, page_bytes = (size_t)a.c.nkv * a.c.tile_bytes;
-    const int last = hi > lo ? (hi - 1) & ~(kPos - 1) : 0;     // the piece's last tile
-    auto place = [&](int tb, bool &there) -> size_t {          // of a tile: its bytes' start, less the offset's
-        const int page = __builtin_amdgcn_readfirstlane(row[tb / ps]);
-        there = page >= 0 && page < a.c.pages;
-        return (there ? (size_t)page : 0) * page_bytes + head_at;
-    };
+    Walk<HALVES> at(g, kCols);
+    if (at.empty(g)) return;
+    const bool owner = c < at.heads;
     R k[HALVES], v[HALVES];
-    int tb = lo + wid * HALVES * kPos;
-    size_t at[HALVES];
-    bool there[HALVES];
-    auto seek = [&](int t) {
+    auto load_k = [&]() {
 #pragma unroll
-        for (int u = 0; u < HALVES; ++u) at[u] = place(min(t + u * kPos, last), there[u]);
+        for (int u = 0; u < HALVES; ++u) k[u].load_k(a.c.k + at.at[u], at.ps, at.off[u], c, m);
     };
-    auto load_k = [&](int t) {
+    auto load_v = [&]() {
 #pragma unroll
-        for (int u = 0; u < HALVES; ++u) k[u].load_k(a.c.k + at[u], ps, min(t + u * kPos, last) % ps, c, m);
+        for (int u = 0; u < HALVES; ++u) v[u].load_v(a.c.v + at.at[u], at.ps, at.off[u], c, m);
     };
-    auto load_v = [&](int t) {
-#pragma unroll
-        for (int u = 0; u < HALVES; ++u) v[u].load_v(a.c.v + at[u], ps, min(t + u * kPos, last) % ps, c, m);
-    };
-    if (tb < hi) {
-        seek(tb);
-        load_k(tb);
-        load_v(tb);
+    int tb = at.lo + wid * HALVES * kPos;
+    if (tb < at.hi) {
+        at.seek(g, tb);
+        load_k();
+        load_v();
     }
-    // q
-    uint8_t *qb = reinterpret_cast<uint8_t *>(buf);
-    pu4 qh[PATH == kHalf ? HD / 32 : 1];
-    pu2 qd[PATH == kDigits ? NT : 1][PATH == kDigits ? T::NB : 1];
-    const int64_t q_at = (int64_t)b * a.q.ts + (int64_t)h0 * a.q.hs;
-    if constexpr (PATH == kExact) {
+    const int64_t q_at = (int64_t)at.b * a.q.ts + (int64_t)at.h0 * a.q.hs;
+    pu4 qh[HALF ? HD / 32 : 1];
+    if constexpr (!HALF) {
         for (int i = tid; i < kCols * HD; i += kThreads) {
             const int r = i / HD, d = i - r * HD;
-            buf[r * LD + d] = r < heads ? load1(a.q.dtype, a.q.p, q_at + (int64_t)r * a.q.hs + d) : 0.f;
+            buf[r * LD + d] = r < at.heads ? load1(a.q.dtype, a.q.p, q_at + (int64_t)r * a.q.hs + d) : 0.f;
         }
         __syncthreads();
-    } else if constexpr (PATH == kHalf) {
+    } else {
         constexpr int QL = HD + 8;
         uint16_t *qs = reinterpret_cast<uint16_t *>(buf);
         for (int i = tid; i < kCols * HD; i += kThreads) {
             const int r = i / HD, d = i - r * HD;
-            qs[r * QL + d] = r < heads ? reinterpret_cast<const uint16_t *>(a.q.p)[q_at + (int64_t)r * a.q.hs + d] : 0;
+            qs[r * QL + d] = r < at.heads ? reinterpret_cast<const uint16_t *>(a.q.p)[q_at + (int64_t)r * a.q.hs + d] : 0;
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) qh[j] = *reinterpret_cast<const pu4 *>(qs + c * QL + 32 * j + 8 * m);
-    } else {
-        // sixteen threads per head, HD / 16 elements each: the largest magnitude, then the digits, eight
-        // elements (or four) at a time, to where the lanes read them: [set][block][lane][8]
-        const int r = tid >> 4, e0 = (tid & 15) * DPL;
-        constexpr int W = DPL < 8 ? DPL : 8;
-        float x[DPL], top = 0.f;
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < DPL; ++e) {
-            x[e] = r < heads ? load1(a.q.dtype, a.q.p, q_at + (int64_t)r * a.q.hs + e0 + e) : 0.f;
-            odd |= !(fabsf(x[e]) < INFINITY);
-            top = fmaxf(top, fabsf(x[e]));
-        }
-        top = lanes::row16_max(odd ? INFINITY : top);
-        int ex;
-        (void)frexpf(top, &ex);                                // top < 2^ex
-        const int sh = top > 0.f && top < INFINITY ? 30 - ex : 0;
-        if ((tid & 15) == 0) shift[r] = top < INFINITY ? sh : INT_MAX;
-        if (r < HEADS) {
-            const int i = r / NT, t = r - i * NT;
-#pragma unroll
-            for (int w0 = 0; w0 < DPL; w0 += W) {
-                const int d = e0 + w0, blk = d >> 5, mm = (d >> 3) & 3;
-                uint32_t dig[4][2] = {};
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    int X = top < INFINITY ? (int)rintf(ldexpf(x[w0 + e], sh)) : 0;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int dg = (int8_t)X;
-                        dig[q][e >> 2] |= (uint32_t)(dg & 255) << (8 * (e & 3));
-                        X = (X - dg) >> 8;
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint8_t *o = qb + (((size_t)t * T::NB + blk) * kWave + mm * 16 + 4 * i + q) * 8 + (d & 7);
-                    if constexpr (W == 8) *reinterpret_cast<pu2 *>(o) = pu2{dig[q][0], dig[q][1]};
-                    else *reinterpret_cast<uint32_t *>(o) = dig[q][0];
-                }
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < T::NB; ++j) qd[t][j] = *reinterpret_cast<const pu2 *>(qb + ((size_t)(t * T::NB + j) * kWave + lane) * 8);
     }
     pf4 o[DPL];                                        // o[x][r']: dim v_dim(x, 4m + r') of column c
 #pragma unroll
     for (int x = 0; x < DPL; ++x) o[x] = pf4{0.f, 0.f, 0.f, 0.f};
     // scores in log2 units: without a cap in one product
     const float cap = a.softcap, sl2 = cap > 0.f ? a.scale : __fmul_rn(a.scale, kLog2e);
-    float digits[PATH == kDigits ? NT : 1];
-    if constexpr (PATH == kDigits) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int s = shift[(c >> 2) * NT + t];
-            digits[t] = s == INT_MAX ? NAN : ldexpf(CT == DT_Q4_0 ? 0.0625f : 1.0f, 8 * (c & 3) - s);
-        }
-    }
     float mx = -INFINITY, sum = 0.f;                   // sum: this lane's positions only
-    for (; tb < hi; tb += STEP) {
-        const int tn = tb + STEP;
+    for (; tb < at.hi; tb += STEP) {
+        const bool all = at.whole(tb);
         bool here[HALVES];
 #pragma unroll
-        for (int u = 0; u < HALVES; ++u) here[u] = there[u];
+        for (int u = 0; u < HALVES; ++u) here[u] = at.there[u];
         pf4 s4[HALVES];
-        if constexpr (PATH == kExact) {
+        if constexpr (!HALF) {
             pf4 st[4] = {};
 #pragma unroll
             for (int j = 0; j < R::N; ++j)
@@ -336,65 +312,33 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                         st[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0].k_at(j, e0 + e), qv[e], st[e], 0, 0, 0);
                 }
             s4[0] = (st[0] + st[1]) + (st[2] + st[3]);
-        } else if constexpr (PATH == kHalf) {
+        } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s4[u] = pf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) s4[u] = mfma16<CT>(k[u].w[j], qh[j], s4[u]);
             }
-        } else {
-            pf4 st[NT] = {};
-#pragma unroll
-            for (int j = 0; j < T::NB; ++j) {
-                pu2 kb = k[0].k_codes(j);
-                const float sc[4] = {quad_lane<0>(k[0].s[j]), quad_lane<1>(k[0].s[j]), quad_lane<2>(k[0].s[j]), quad_lane<3>(k[0].s[j])};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const pi4 d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, kb), __builtin_bit_cast(long, qd[t][j]),
-                                                                        pi4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) st[t][r] = __builtin_fmaf((float)d[r], sc[r], st[t][r]);
-                }
-            }
-            // the digits of a head lie in a quad; each lane keeps its own head's score
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float own = quad_sum(__fmul_rn(st[0][r], digits[0]));
-#pragma unroll
-                for (int t = 1; t < NT; ++t) {
-                    const float other = quad_sum(__fmul_rn(st[t][r], digits[t]));
-                    own = (c & 3) >= t ? other : own;
-                }
-                s4[0][r] = own;
-            }
         }
-        seek(tn);                                      // past the end: the last tile again
-        load_k(tn);
+        at.seek(g, tb + STEP);
+        load_k();
         float p[HALVES][4], ref = -INFINITY;
 #pragma unroll
         for (int u = 0; u < HALVES; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = __fmul_rn(s4[u][r], sl2);
-                if (cap > 0.f) x = __fmul_rn(__fmul_rn(cap, tanhf(__fdiv_rn(x, cap))), kLog2e);
-                p[u][r] = x;
+                p[u][r] = __fmul_rn(s4[u][r], sl2);
+                if (cap > 0.f) p[u][r] = __fmul_rn(capped(p[u][r], cap), kLog2e);
             }
-        // the piece's first and last tiles, and pages that do not exist: positions that do not count
-        bool all = tb >= start && tb + HALVES * kPos <= hi;
-#pragma unroll
-        for (int u = 0; u < HALVES; ++u) all &= here[u];
-        if (!all) {
+        if (!all) {                                    // a piece's end, or a page that does not exist
 #pragma unroll
             for (int u = 0; u < HALVES; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int t = tb + u * kPos + 4 * m + r;
-                    if (!here[u] || t < start || t >= hi) {
-                        p[u][r] = -INFINITY;
-                        // its weight is 0, and 0 times a NaN there would be NaN
-                        v[u].clear_v(r);
-                    }
+                    const bool on = here[u] && t >= at.start && t < at.hi;
+                    p[u][r] = on ? p[u][r] : -INFINITY;
+                    v[u].keep_v(r, on);                // its weight is 0, and 0 times a NaN there would be NaN
                 }
         }
 #pragma unroll
@@ -417,7 +361,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                 p[u][r] = __builtin_amdgcn_exp2f(p[u][r] - from);
                 sum = __fadd_rn(sum, p[u][r]);
             }
-        if constexpr (PATH == kHalf) {
+        if constexpr (HALF) {
             // contraction index 8m + 4u + r is position 4m + r of half u
             pu4 pw;
 #pragma unroll
@@ -444,7 +388,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
                 for (int x = 0; x < DPL; ++x) o[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0].v_at(r, x), p[0][r], o[x], 0, 0, 0);
         }
-        load_v(tn);
+        load_v();
     }
     sum += __shfl_xor(sum, 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
@@ -488,18 +432,300 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     if (wid != 0 || !owner) return;
     if (g.pieces == 1) {
         const float inv = tot == 0.f ? 0.f : __fdiv_rn(1.0f, tot);
-        const int64_t out_at = (int64_t)b * a.out.ts + (int64_t)(h0 + hc) * a.out.hs;
+        const int64_t out_at = (int64_t)at.b * a.out.ts + (int64_t)(at.h0 + c) * a.out.hs;
 #pragma unroll
         for (int x = 0; x < DPL; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) store1(a.out.dtype, a.out.p, out_at + R::v_dim(x, 4 * m + r), __fmul_rn(o[x][r], inv));
-        if (a.lse && m == 0) a.lse[(size_t)b * g.n_heads + h0 + hc] = lse_of(top, tot);
+        if (a.lse && m == 0) a.lse[(size_t)at.b * g.n_heads + at.h0 + c] = lse_of(top, tot);
     } else {
 #pragma unroll
         for (int x = 0; x < DPL; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) g.part[(slot0 + hc) * HD + R::v_dim(x, 4 * m + r)] = o[x][r];
-        if (m == 0) g.ms[slot0 + hc] = make_float2(top, tot);
+            for (int r = 0; r < 4; ++r) g.part[(at.slot0 + c) * HD + R::v_dim(x, 4 * m + r)] = o[x][r];
+        if (m == 0) g.ms[at.slot0 + c] = make_float2(top, tot);
+    }
+}
+
+// Rows over a quantized cache, 4 NT query heads. K's codes meet q as they are: q is rounded to 2^-31 of its head's
+// largest element and split into four signed 8-bit digits, a head's digits are four rows of the 16x16x32 product, and
+// a lane's four sums, exact in 32 bits, are one head's digits of one position: put together and times the block's
+// scale one fma. The weights go through LDS to the other operand's order. There a column stands for a head and one
+// of four blocks of V (head_dim 256: the contraction runs over both halves of the blocks, each half's codes beside
+// zeros for the other half's rows), and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
+// sums only those of a column's own block are meant. TERMS: bf16 terms of that product, 3 for all its 24 bits;
+// 1 where rows are bf16 (half a step of the outputs' type).
+template <int CT, int HD, int NT, int TERMS>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && CT == DT_Q4_0) ? 4 : NT == 1 ? 3 : 2) void paged_attn_digits_kernel(AttnArgs g) {
+    using R = Raw<CT, HD>;
+    using T = Tile<CT, HD>;
+    constexpr int LD = HD + 4, DPL = R::DPL, HEADS = 4 * NT, SETS = (T::NB + 3) / 4, HALVES = 2 / SETS, STEP = kWaves * HALVES * kPos;
+    constexpr int kQ = NT * T::NB * kWave * 8, kP = kWaves * HALVES * NT * kWave * 4, kO = kWaves * HEADS * LD * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kQ + kP > kO ? kQ + kP : kO];   // digits, weights; later the waves' O
+    __shared__ float wm[kWaves][HEADS], wsum[kWaves][HEADS];
+    __shared__ int shift[kCols];                       // q * 2^shift are the digits' integers
+    const PagedAttn &a = g.a;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int c = lane & 15, m = lane >> 4;
+    Walk<HALVES> at(g, HEADS);
+    if (at.empty(g)) return;
+    R k[HALVES], v[HALVES];
+    auto load_k = [&]() {
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) k[u].load_k(a.c.k + at.at[u], at.ps, at.off[u], c, m);
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) v[u].load_v(a.c.v + at.at[u], at.ps, at.off[u], c, m);
+    };
+    int tb = at.lo + wid * HALVES * kPos;
+    if (tb < at.hi) {
+        at.seek(g, tb);
+        load_k();
+        load_v();
+    }
+    {
+        // sixteen threads per head, HD / 16 elements each: the largest magnitude, then the digits, eight
+        // elements (or four) at a time, to where the lanes read them: [set][block][lane][8]
+        const int r = tid >> 4, e0 = (tid & 15) * DPL;
+        constexpr int W = DPL < 8 ? DPL : 8;
+        const int64_t q_at = (int64_t)at.b * a.q.ts + (int64_t)(at.h0 + r) * a.q.hs + e0;
+        float x[DPL], top = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) x[e] = 0.f;
+        if (r < at.heads) load_some<DPL>(a.q.dtype, a.q.p, q_at, x);
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) {
+            odd |= !(fabsf(x[e]) < INFINITY);
+            top = fmaxf(top, fabsf(x[e]));
+        }
+        top = lanes::row16_max(odd ? INFINITY : top);
+        int ex;
+        (void)frexpf(top, &ex);                        // top < 2^ex
+        const int sh = top > 0.f && top < INFINITY ? 30 - ex : 0;
+        if ((tid & 15) == 0) shift[r] = top < INFINITY ? sh : INT_MAX;
+        if (r < HEADS) {
+#pragma unroll
+            for (int w0 = 0; w0 < DPL; w0 += W) {
+                const int d = e0 + w0, blk = d >> 5, mm = (d >> 3) & 3;
+                uint32_t dig[4][2] = {};
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    int X = top < INFINITY ? (int)rintf(ldexpf(x[w0 + e], sh)) : 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int dg = (int8_t)X;
+                        dig[q][e >> 2] |= (uint32_t)(dg & 255) << (8 * (e & 3));
+                        X = (X - dg) >> 8;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint8_t *o = lds + (((r >> 2) * T::NB + blk) * kWave + mm * 16 + 4 * (r & 3) + q) * 8 + (d & 7);
+                    if constexpr (W == 8) *reinterpret_cast<pu2 *>(o) = pu2{dig[q][0], dig[q][1]};
+                    else *reinterpret_cast<uint32_t *>(o) = dig[q][0];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    pu2 qd[NT][T::NB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) qd[t][j] = *reinterpret_cast<const pu2 *>(lds + ((t * T::NB + j) * kWave + lane) * 8);
+    // from the digits' integers to scores in log2 units (or to what the cap takes); lane (c, m): head 4t + m
+    const float cap = a.softcap;
+    float unit[NT], mx[NT], sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int s = shift[4 * t + m];
+        unit[t] = s == INT_MAX ? NAN : ldexpf(cap > 0.f ? a.scale : __fmul_rn(a.scale, kLog2e), -s - (CT == DT_Q4_0 ? 4 : 0));
+        mx[t] = -INFINITY;
+        sum[t] = 0.f;                                  // this lane's position of every tile
+    }
+    pf4 o[NT][DPL];                                    // o[t][x][r']: dim (4m + r') * DPL + x, column c
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < DPL; ++x) o[t][x] = pf4{0.f, 0.f, 0.f, 0.f};
+    float *pw = reinterpret_cast<float *>(lds + kQ) + wid * HALVES * NT * kWave;
+    for (; tb < at.hi; tb += STEP) {
+        const bool all = at.whole(tb);
+        bool here[HALVES];
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) here[u] = at.there[u];
+        float sc[HALVES][NT] = {};
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                const pu2 kb = k[u].k_codes(j);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const pi4 d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, qd[t][j]), __builtin_bit_cast(long, kb),
+                                                                        pi4{0, 0, 0, 0}, 0, 0, 0);
+                    // below 2^28: 32 products of 2^14, times 2^8
+                    const float low = (float)(d[1] * 256 + d[0]), high = (float)(d[3] * 256 + d[2]);
+                    sc[u][t] = __builtin_fmaf(__builtin_fmaf(high, 65536.0f, low), k[u].s[j], sc[u][t]);
+                }
+            }
+            // (the sums of a few blocks at a time: all of them at once would not fit the registers)
+            if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        at.seek(g, tb + STEP);
+        load_k();
+        float ref[NT];
+        bool far = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                sc[u][t] = __fmul_rn(sc[u][t], unit[t]);
+                if (cap > 0.f) sc[u][t] = __fmul_rn(capped(sc[u][t], cap), kLog2e);
+            }
+        }
+        if (!all) {                                    // a piece's end, or a page that does not exist
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                // [from, to): what counts of the tile
+                const int from = here[u] ? at.start - tb - u * kPos : kPos, to = at.hi - tb - u * kPos;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) sc[u][t] = c >= from && c < to ? sc[u][t] : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4 * SETS; ++i) {   // a weight of 0 times a scale of NaN there would be NaN
+                    const int at_r = 4 * m + i % 4;
+                    v[u].s[i] = at_r >= from && at_r < to ? v[u].s[i] : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            ref[t] = fmaxf(sc[0][t], sc[HALVES - 1][t]);
+            far |= ref[t] > mx[t] + kLazy;
+        }
+        // The maximum moves, with O and the sums, only for a score far above it: weights up to 2^kLazy do no harm.
+        if (__any(far)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float mn = fmaxf(mx[t], lanes::row16_max(ref[t])), f = mx[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx[t] - mn);
+                mx[t] = mn;
+                sum[t] = __fmul_rn(sum[t], f);
+                const float fc = __shfl(f, (c >> 2) * 16, kWave);          // of the column's head
+#pragma unroll
+                for (int x = 0; x < DPL; ++x) o[t][x] *= fc;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float from = mx[t] == -INFINITY ? 0.f : mx[t];           // nothing above -inf yet: all weights 0
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                const float p = __builtin_amdgcn_exp2f(sc[u][t] - from);
+                sum[t] = __fadd_rn(sum[t], p);
+                pw[(u * NT + t) * kWave + lane] = p;
+            }
+        }
+        // a wave's LDS accesses stay in order; the compiler is told
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        // contraction index 8m + 4i + r is position 4m + r of tile i, or of the tile and set i of blocks
+        pu4 w[NT][TERMS];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                const pf4 p = *reinterpret_cast<const pf4 *>(pw + (u * NT + t) * kWave + (c >> 2) * 16 + 4 * m);
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) {
+                    float x[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = __fmul_rn(p[r], v[u].s[4 * s + r]);
+#pragma unroll
+                    for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float &x0 = x[2 * i], &x1 = x[2 * i + 1];
+                            if constexpr (TERMS == 1) {
+                                w[t][q][2 * (u + s) + i] = to_bf16(x0) | to_bf16(x1) << 16;
+                            } else {                   // the upper half of the word, and what it leaves
+                                w[t][q][2 * (u + s) + i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+                                x0 = __fsub_rn(x0, __uint_as_float(__float_as_uint(x0) & 0xffff0000u));
+                                x1 = __fsub_rn(x1, __uint_as_float(__float_as_uint(x1) & 0xffff0000u));
+                            }
+                        }
+                }
+            }
+        uint32_t vb[HALVES][R::VW];
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) v[u].v_bytes(vb[u]);
+#pragma unroll
+        for (int x = 0; x < DPL; ++x) {
+            pu4 code;                                  // exact in bf16
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t two = __builtin_amdgcn_perm(__float_as_uint(R::v_byte(vb[u], 2 * i + 1, x)), __float_as_uint(R::v_byte(vb[u], 2 * i, x)), 0x07060302u);
+                    if constexpr (SETS == 1) {
+                        code[2 * u + i] = two;
+                    } else {                           // row c is a dim of block c / 2
+                        code[i] = c < 8 ? two : 0u;
+                        code[2 + i] = c < 8 ? 0u : two;
+                    }
+                }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int q = 0; q < TERMS; ++q) o[t][x] = mfma16<DT_BF16>(code, w[t][q], o[t][x]);
+            // (one dim's codes at a time: all of them at once would not fit the registers)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load_v();
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        sum[t] = lanes::row16_sum(sum[t]);
+        if (c == 0) {
+            wm[wid][4 * t + m] = mx[t];
+            wsum[wid][4 * t + m] = sum[t];
+        }
+    }
+    __syncthreads();                                   // every wave is past its digits and weights
+    float *buf = reinterpret_cast<float *>(lds);       // the waves' O: [wave][head][LD]
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            // rows 4m + r of the column's own block
+            const int blk = (4 * m + r) * DPL / 32;
+            if (blk % 4 != (c & 3)) continue;
+#pragma unroll
+            for (int x = 0; x < DPL; ++x) buf[(wid * HEADS + 4 * t + (c >> 2)) * LD + (4 * m + r) * DPL + x] = __fmul_rn(o[t][x][r], CT == DT_Q4_0 ? 0.0625f : 1.0f);
+        }
+    __syncthreads();
+    for (int i = tid; i < at.heads * HD; i += kThreads) {
+        const int r = i / HD, d = i - r * HD;
+        float top = wm[0][r], tot = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wm[w][r]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float s = wsum[w][r];
+            if (s == 0.f) continue;                    // no positions, or scores of -inf only
+            const float f = __builtin_amdgcn_exp2f(wm[w][r] - top);
+            tot = __builtin_fmaf(s, f, tot);
+            x = __builtin_fmaf(buf[(w * HEADS + r) * LD + d], f, x);
+        }
+        if (g.pieces == 1) {
+            store1(a.out.dtype, a.out.p, (int64_t)at.b * a.out.ts + (int64_t)(at.h0 + r) * a.out.hs + d, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
+            if (a.lse && d == 0) a.lse[(size_t)at.b * g.n_heads + at.h0 + r] = lse_of(top, tot);
+        } else {
+            g.part[(at.slot0 + r) * HD + d] = x;
+            if (d == 0) g.ms[at.slot0 + r] = make_float2(top, tot);
+        }
     }
 }
 
@@ -564,11 +790,11 @@ struct Plan {
 Plan plan_of(int dtype, int nkv, int batch, int n_heads, int max_length, int window) {
     Plan p;
     const int group = n_heads / nkv;
-    p.col_heads = !is_quant(dtype) ? kCols : group <= 4 ? 4 : group <= 8 ? 8 : 16;
+    p.col_heads = !is_quant(dtype) ? kCols : group <= 4 ? 4 : 8;
     p.col_tiles = (group + p.col_heads - 1) / p.col_heads;
     const int64_t groups = (int64_t)batch * nkv * p.col_tiles;
     const int64_t len = (window > 0 && window < max_length - kPos ? window + kPos : max_length);
-    p.want = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPieces, kWantGroups / groups));
+    p.want = groups >= kFullGroups ? 1 : (int)std::min<int64_t>(kMaxPieces, kWantGroups / groups);
     p.piece = (int)(((len + p.want - 1) / p.want + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
     p.pieces = (int)((len + p.piece - 1) / p.piece);
     return p;
@@ -593,18 +819,22 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.col_tiles = p.col_tiles;
     g.piece = p.piece;
     g.pieces = p.pieces;
+    // ceil(2^32 / d), d <= 64: off by less than d / 2^32 relative to 1 / d, and i * d < 2^32
+    const uint64_t d = a.c.page_size / kPos;
+    g.page_magic = d == 1 ? 0 : (uint32_t)(((1ull << 32) + d - 1) / d);
     g.part = reinterpret_cast<float *>(a.ws);
     g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);
-    const bool half = a.q.dtype != DT_F32;
-#define SPH_ATTN(COND, CT, HD, PATH, NT) \
-    if (a.c.dtype == CT && a.c.hd == HD && (COND)) hipLaunchKernelGGL((paged_attn_kernel<CT, HD, PATH, NT>), grid, block, 0, s, g);
-#define SPH_ATTN_16(CT, HD) SPH_ATTN(!half, CT, HD, kExact, 1) SPH_ATTN(half, CT, HD, kHalf, 1)
-#define SPH_ATTN_Q(CT, HD)                                                          \
-    SPH_ATTN(p.col_heads == 4, CT, HD, kDigits, 1) SPH_ATTN(p.col_heads == 8, CT, HD, kDigits, 2) \
-    SPH_ATTN(p.col_heads == 16, CT, HD, kDigits, 4)
-#define SPH_ATTN_HD(HD) \
-    SPH_ATTN(true, DT_F32, HD, kExact, 1) SPH_ATTN_16(DT_BF16, HD) SPH_ATTN_16(DT_F16, HD) SPH_ATTN_Q(DT_Q8_0, HD) SPH_ATTN_Q(DT_Q4_0, HD)
+    const bool half = a.q.dtype != DT_F32, short_terms = a.q.dtype == DT_BF16, few = p.col_heads == 4;
+#define SPH_FLOAT(CT, HD, HALF) \
+    if (a.c.dtype == CT && a.c.hd == HD && half == HALF) hipLaunchKernelGGL((paged_attn_kernel<CT, HD, HALF>), grid, block, 0, s, g);
+#define SPH_DIGITS(CT, HD, NT, TERMS)                                                             \
+    if (a.c.dtype == CT && a.c.hd == HD && few == (NT == 1) && short_terms == (TERMS == 1))       \
+        hipLaunchKernelGGL((paged_attn_digits_kernel<CT, HD, NT, TERMS>), grid, block, 0, s, g);
+#define SPH_QUANT(CT, HD) SPH_DIGITS(CT, HD, 1, 1) SPH_DIGITS(CT, HD, 1, 3) SPH_DIGITS(CT, HD, 2, 1) SPH_DIGITS(CT, HD, 2, 3)
+#define SPH_ATTN_HD(HD)                                                                           \
+    SPH_FLOAT(DT_F32, HD, false) SPH_FLOAT(DT_BF16, HD, false) SPH_FLOAT(DT_BF16, HD, true)       \
+    SPH_FLOAT(DT_F16, HD, false) SPH_FLOAT(DT_F16, HD, true) SPH_QUANT(DT_Q8_0, HD) SPH_QUANT(DT_Q4_0, HD)
     SPH_ATTN_HD(64) SPH_ATTN_HD(128) SPH_ATTN_HD(256)
     if (!hip_ok(hipGetLastError(), "paged attention launch")) return -1;
     if (p.pieces > 1) {
