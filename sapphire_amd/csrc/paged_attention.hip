@@ -21,7 +21,7 @@ constexpr int kCols = 16;                  // query heads of a workgroup
 constexpr int kPos = 16;                   // positions of a tile
 constexpr int kMaxPieces = 256;
 constexpr int kPieceUnit = 64;             // a piece is a multiple of so many positions
-constexpr int kFullGroups = 1024, kWantGroups = 4096;      // workgroups that are left as they are; that cut sequences make
+constexpr int kFullGroups = 1024, kWantGroups = 2048;      // workgroups that are left as they are; that cut sequences make
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 struct AttnArgs {
@@ -108,7 +108,10 @@ struct Raw {
     __device__ __forceinline__ void v_bytes(uint32_t (&q)[VW]) const {
         if constexpr (CT == DT_Q8_0) {
 #pragma unroll
-            for (int i = 0; i < VW; ++i) q[i] = w[i / 4][i % 4];
+            for (int i = 0; i < VW; ++i) {
+                q[i] = w[i / 4][i % 4];
+                asm("" : "+v"(q[i]));
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < VW / 2; ++i) {
@@ -237,6 +240,170 @@ struct Walk {
 
 __device__ __forceinline__ float capped(float x, float cap) { return __fmul_rn(cap, tanhf(__fdiv_rn(x, cap))); }
 
+// The waves' O ([wave][head][HD + 4], unnormalised) and (maximum, sum) of each head: to out, or to the piece's part.
+template <int HD, int HEADS>
+__device__ __forceinline__ void finish(const AttnArgs &g, int b, int h0, int heads, size_t slot0, const float *o,
+                                       const float (&wm)[kWaves][HEADS], const float (&wsum)[kWaves][HEADS]) {
+    constexpr int LD = HD + 4;
+    const PagedAttn &a = g.a;
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * HD; i += kThreads) {
+        const int r = i / HD, d = i - r * HD;
+        float top = wm[0][r], tot = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wm[w][r]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            // a wave without positions, or with scores of -inf only, has sum 0; its factor must not be NaN
+            const float s = wsum[w][r], f = s == 0.f ? 0.f : __builtin_amdgcn_exp2f(wm[w][r] - top);
+            tot = __builtin_fmaf(s, f, tot);
+            x = __builtin_fmaf(o[(w * HEADS + r) * LD + d], f, x);
+        }
+        if (g.pieces == 1) {
+            store1(a.out.dtype, a.out.p, (int64_t)b * a.out.ts + (int64_t)(h0 + r) * a.out.hs + d, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
+            if (a.lse && d == 0) a.lse[(size_t)b * g.n_heads + h0 + r] = lse_of(top, tot);
+        } else {
+            g.part[(slot0 + r) * HD + d] = x;
+            if (d == 0) g.ms[slot0 + r] = make_float2(top, tot);
+        }
+    }
+}
+
+// Thread (r, i), r = tid / 16: q's elements HD / 16 * i and on of head h0 + r, zeros past the heads.
+template <int N>
+__device__ __forceinline__ void load_q(const Rows &q, int b, int h0, int heads, float (&x)[N]) {
+    const int r = threadIdx.x >> 4;
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = 0.f;
+    if (r < heads) load_some<N>(q.dtype, q.p, (int64_t)b * q.ts + (int64_t)(h0 + r) * q.hs + (threadIdx.x & 15) * N, x);
+}
+
+// fp32 rows over a float cache, at most four query heads of a K/V head. v_mfma_f32_4x4x1_16b_f32 is sixteen products of
+// four rows and four columns: block (m, c / 4) multiplies the positions 4 (c / 4) .. + 3 of dim chunk m with the heads,
+// and for the weighted sum the dims of lanes 4 (c / 4) .. + 3 at position 4m + r. Every column is used, where
+// 16x16x4 would leave twelve of sixteen idle: a quarter of its cycles.
+template <int CT, int HD>
+__global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_few_kernel(AttnArgs g) {
+    using R = Raw<CT, HD>;
+    constexpr int LD = HD + 4, DPL = R::DPL, HEADS = 4, STEP = kWaves * kPos;
+    __shared__ __attribute__((aligned(16))) float buf[kWaves * HEADS * LD];    // q, later the waves' O
+    __shared__ float wm[kWaves][HEADS], wsum[kWaves][HEADS];
+    const PagedAttn &a = g.a;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int c = lane & 15, m = lane >> 4;
+    Walk<1> at(g, HEADS);
+    if (at.empty(g)) return;
+    float qx[DPL];
+    load_q<DPL>(a.q, at.b, at.h0, at.heads, qx);
+    R k, v;
+    int tb = at.lo + wid * kPos;
+    if (tb < at.hi) {
+        at.seek(g, tb);
+        k.load_k(a.c.k + at.at[0], at.ps, at.off[0], c, m);
+        v.load_v(a.c.v + at.at[0], at.ps, at.off[0], c, m);
+    }
+    if (tid < 16 * HEADS) {
+#pragma unroll
+        for (int e = 0; e < DPL; e += 4) *reinterpret_cast<pf4 *>(buf + (tid >> 4) * LD + (tid & 15) * DPL + e) = pf4{qx[e], qx[e + 1], qx[e + 2], qx[e + 3]};
+    }
+    __syncthreads();
+    pf4 o[DPL];                                        // o[x][i]: dim v_dim(x, 4 (c / 4) + i) of head c % 4, positions of m only
+#pragma unroll
+    for (int x = 0; x < DPL; ++x) o[x] = pf4{0.f, 0.f, 0.f, 0.f};
+    // scores in log2 units: without a cap in one product
+    const float cap = a.softcap, sl2 = cap > 0.f ? a.scale : __fmul_rn(a.scale, kLog2e);
+    float mx = -INFINITY, sum = 0.f;                   // sum: this lane's positions only
+    for (; tb < at.hi; tb += STEP) {
+        const bool all = at.whole(tb), here = at.there[0];
+        pf4 st[4] = {};
+#pragma unroll
+        for (int j = 0; j < R::N; ++j)
+#pragma unroll
+            for (int e0 = 0; e0 < R::KE; e0 += 4) {
+                const pf4 qv = *reinterpret_cast<const pf4 *>(buf + (c & 3) * LD + R::k_dim(j, m, e0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st[e] = __builtin_amdgcn_mfma_f32_4x4x1f32(k.k_at(j, e0 + e), qv[e], st[e], 0, 0, 0);
+                if ((j * (R::KE / 4) + e0 / 4) % 4 == 3) __builtin_amdgcn_sched_barrier(0);    // (few words at a time: registers)
+            }
+        at.seek(g, tb + STEP);
+        k.load_k(a.c.k + at.at[0], at.ps, at.off[0], c, m);
+        // the four chunks' sums, then positions 4 (c / 4) + r of head c % 4
+        const pf4 s4 = (st[0] + st[1]) + (st[2] + st[3]);
+        float p[4], ref;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = s4[r];
+            x += __shfl_xor(x, 16, kWave);
+            x += __shfl_xor(x, 32, kWave);
+            p[r] = __fmul_rn(x, sl2);
+            if (cap > 0.f) p[r] = __fmul_rn(capped(p[r], cap), kLog2e);
+        }
+        if (!all) {                                    // a piece's end, or a page that does not exist
+            // [from, to): what counts of the tile
+            const int from = here ? at.start - tb : kPos, to = at.hi - tb;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = (c >> 2) * 4 + r, tv = 4 * m + r;
+                p[r] = t >= from && t < to ? p[r] : -INFINITY;
+                v.keep_v(r, tv >= from && tv < to);    // its weight is 0, and 0 times a NaN there would be NaN
+            }
+        }
+        ref = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+        // The maximum moves, with O and the sums, only for a score far above it: weights up to 2^kLazy do no harm.
+        if (__any(ref > mx + kLazy)) {
+            ref = fmaxf(ref, __shfl_xor(ref, 4, kWave));
+            ref = fmaxf(ref, __shfl_xor(ref, 8, kWave));
+            const float mn = fmaxf(mx, ref), f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+            mx = mn;
+            sum = __fmul_rn(sum, f);
+#pragma unroll
+            for (int x = 0; x < DPL; ++x) o[x] *= f;
+        }
+        const float from = mx == -INFINITY ? 0.f : mx; // nothing above -inf yet: all weights 0
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(p[r] - from);
+            sum = __fadd_rn(sum, p[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = __shfl(p[r], (m << 2) | (c & 3), kWave);     // of position 4m + r
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < DPL; ++x) o[x] = __builtin_amdgcn_mfma_f32_4x4x1f32(v.v_at(r, x), p[r], o[x], 0, 0, 0);
+        v.load_v(a.c.v + at.at[0], at.ps, at.off[0], c, m);
+    }
+    sum += __shfl_xor(sum, 4, kWave);
+    sum += __shfl_xor(sum, 8, kWave);
+    if (lane < HEADS) {
+        wm[wid][lane] = mx;
+        wsum[wid][lane] = sum;
+    }
+    // The sums over m, each lane left with a quarter of the dims: x = m * DPL / 4 and on. A swap puts two words'
+    // lower halves (rows of 16 lanes: even rows) into one and their upper halves into the other.
+    constexpr int H = DPL / 2, Q = DPL / 4;
+#pragma unroll
+    for (int x = 0; x < H; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[x][i]), __float_as_uint(o[x + H][i]), false, false);
+            o[x][i] = __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        }
+#pragma unroll
+    for (int x = 0; x < Q; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[x][i]), __float_as_uint(o[x + Q][i]), false, false);
+            o[x][i] = __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        }
+    __syncthreads();                                   // every wave is past its reads of q
+#pragma unroll
+    for (int x = 0; x < Q; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) buf[(wid * HEADS + (c & 3)) * LD + R::v_dim(m * Q + x, (c >> 2) * 4 + i)] = o[x][i];
+    finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
+}
+
 // Rows over a float cache. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
 // cache of their type: 16x16x32 products of the elements as they are; the weights are rounded to that type
 // (half a step, what the outputs are rounded by too), and V's 16-bit words are transposed in pairs on the way.
@@ -254,6 +421,8 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     Walk<HALVES> at(g, kCols);
     if (at.empty(g)) return;
     const bool owner = c < at.heads;
+    float qx[DPL];
+    load_q<DPL>(a.q, at.b, at.h0, at.heads, qx);
     R k[HALVES], v[HALVES];
     auto load_k = [&]() {
 #pragma unroll
@@ -269,24 +438,24 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
         load_k();
         load_v();
     }
-    const int64_t q_at = (int64_t)at.b * a.q.ts + (int64_t)at.h0 * a.q.hs;
     pu4 qh[HALF ? HD / 32 : 1];
-    if constexpr (!HALF) {
-        for (int i = tid; i < kCols * HD; i += kThreads) {
-            const int r = i / HD, d = i - r * HD;
-            buf[r * LD + d] = r < at.heads ? load1(a.q.dtype, a.q.p, q_at + (int64_t)r * a.q.hs + d) : 0.f;
-        }
-        __syncthreads();
-    } else {
-        constexpr int QL = HD + 8;
-        uint16_t *qs = reinterpret_cast<uint16_t *>(buf);
-        for (int i = tid; i < kCols * HD; i += kThreads) {
-            const int r = i / HD, d = i - r * HD;
-            qs[r * QL + d] = r < at.heads ? reinterpret_cast<const uint16_t *>(a.q.p)[q_at + (int64_t)r * a.q.hs + d] : 0;
-        }
-        __syncthreads();
+    {
+        const int r = tid >> 4, e0 = (tid & 15) * DPL;
+        if constexpr (!HALF) {
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) qh[j] = *reinterpret_cast<const pu4 *>(qs + c * QL + 32 * j + 8 * m);
+            for (int e = 0; e < DPL; e += 4) *reinterpret_cast<pf4 *>(buf + r * LD + e0 + e) = pf4{qx[e], qx[e + 1], qx[e + 2], qx[e + 3]};
+            __syncthreads();
+        } else {
+            constexpr int QL = HD + 8;
+            uint16_t *qs = reinterpret_cast<uint16_t *>(buf);
+#pragma unroll
+            for (int e = 0; e < DPL; e += 4)           // (they were of that type: nothing is rounded)
+                *reinterpret_cast<pu2 *>(qs + r * QL + e0 + e) =
+                    pu2{to_16(CT, qx[e]) | to_16(CT, qx[e + 1]) << 16, to_16(CT, qx[e + 2]) | to_16(CT, qx[e + 3]) << 16};
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) qh[j] = *reinterpret_cast<const pu4 *>(qs + c * QL + 32 * j + 8 * m);
+        }
     }
     pf4 o[DPL];                                        // o[x][r']: dim v_dim(x, 4m + r') of column c
 #pragma unroll
@@ -310,6 +479,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         st[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0].k_at(j, e0 + e), qv[e], st[e], 0, 0, 0);
+                    if ((j * (R::KE / 4) + e0 / 4) % 4 == 3) __builtin_amdgcn_sched_barrier(0);    // (few words at a time: registers)
                 }
             s4[0] = (st[0] + st[1]) + (st[2] + st[3]);
         } else {
@@ -381,6 +551,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                     }
                 o[x] = mfma16<CT>(even, pw, o[x]);
                 o[x + 1] = mfma16<CT>(odd, pw, o[x + 1]);
+                if (HD == 256) __builtin_amdgcn_sched_barrier(0);      // (few words at a time: registers)
             }
         } else {
 #pragma unroll
@@ -469,6 +640,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
     const int c = lane & 15, m = lane >> 4;
     Walk<HALVES> at(g, HEADS);
     if (at.empty(g)) return;
+    float x[DPL];
+    load_q<DPL>(a.q, at.b, at.h0, at.heads, x);
     R k[HALVES], v[HALVES];
     auto load_k = [&]() {
 #pragma unroll
@@ -489,12 +662,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
         // elements (or four) at a time, to where the lanes read them: [set][block][lane][8]
         const int r = tid >> 4, e0 = (tid & 15) * DPL;
         constexpr int W = DPL < 8 ? DPL : 8;
-        const int64_t q_at = (int64_t)at.b * a.q.ts + (int64_t)(at.h0 + r) * a.q.hs + e0;
-        float x[DPL], top = 0.f;
+        float top = 0.f;
         bool odd = false;
-#pragma unroll
-        for (int e = 0; e < DPL; ++e) x[e] = 0.f;
-        if (r < at.heads) load_some<DPL>(a.q.dtype, a.q.p, q_at, x);
 #pragma unroll
         for (int e = 0; e < DPL; ++e) {
             odd |= !(fabsf(x[e]) < INFINITY);
@@ -662,25 +831,30 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
 #pragma unroll
         for (int u = 0; u < HALVES; ++u) v[u].v_bytes(vb[u]);
 #pragma unroll
-        for (int x = 0; x < DPL; ++x) {
-            pu4 code;                                  // exact in bf16
+        for (int x0 = 0; x0 < DPL; x0 += 2) {
+            pu4 code[2];                               // exact in bf16
 #pragma unroll
-            for (int u = 0; u < HALVES; ++u)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t two = __builtin_amdgcn_perm(__float_as_uint(R::v_byte(vb[u], 2 * i + 1, x)), __float_as_uint(R::v_byte(vb[u], 2 * i, x)), 0x07060302u);
-                    if constexpr (SETS == 1) {
-                        code[2 * u + i] = two;
-                    } else {                           // row c is a dim of block c / 2
-                        code[i] = c < 8 ? two : 0u;
-                        code[2 + i] = c < 8 ? 0u : two;
+                for (int u = 0; u < HALVES; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t two = __builtin_amdgcn_perm(__float_as_uint(R::v_byte(vb[u], 2 * i + 1, x0 + e)),
+                                                                   __float_as_uint(R::v_byte(vb[u], 2 * i, x0 + e)), 0x07060302u);
+                        if constexpr (SETS == 1) {
+                            code[e][2 * u + i] = two;
+                        } else {                       // row c is a dim of block c / 2
+                            code[e][i] = c < 8 ? two : 0u;
+                            code[e][2 + i] = c < 8 ? 0u : two;
+                        }
                     }
-                }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-                for (int q = 0; q < TERMS; ++q) o[t][x] = mfma16<DT_BF16>(code, w[t][q], o[t][x]);
-            // (one dim's codes at a time: all of them at once would not fit the registers)
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) o[t][x0 + e] = mfma16<DT_BF16>(code[e], w[t][q], o[t][x0 + e]);
+            // (two dims' codes at a time: all of them at once would not fit the registers)
             __builtin_amdgcn_sched_barrier(0);
         }
         load_v();
@@ -705,28 +879,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
 #pragma unroll
             for (int x = 0; x < DPL; ++x) buf[(wid * HEADS + 4 * t + (c >> 2)) * LD + (4 * m + r) * DPL + x] = __fmul_rn(o[t][x][r], CT == DT_Q4_0 ? 0.0625f : 1.0f);
         }
-    __syncthreads();
-    for (int i = tid; i < at.heads * HD; i += kThreads) {
-        const int r = i / HD, d = i - r * HD;
-        float top = wm[0][r], tot = 0.f, x = 0.f;
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wm[w][r]);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float s = wsum[w][r];
-            if (s == 0.f) continue;                    // no positions, or scores of -inf only
-            const float f = __builtin_amdgcn_exp2f(wm[w][r] - top);
-            tot = __builtin_fmaf(s, f, tot);
-            x = __builtin_fmaf(buf[(w * HEADS + r) * LD + d], f, x);
-        }
-        if (g.pieces == 1) {
-            store1(a.out.dtype, a.out.p, (int64_t)at.b * a.out.ts + (int64_t)(at.h0 + r) * a.out.hs + d, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
-            if (a.lse && d == 0) a.lse[(size_t)at.b * g.n_heads + at.h0 + r] = lse_of(top, tot);
-        } else {
-            g.part[(at.slot0 + r) * HD + d] = x;
-            if (d == 0) g.ms[at.slot0 + r] = make_float2(top, tot);
-        }
-    }
+    finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
 // grid (heads, sequences): the pieces of one head. A wave takes every fourth piece, HD / 64 dims per lane.
@@ -787,10 +940,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
 struct Plan {
     int col_heads, col_tiles, want, piece, pieces;
 };
-Plan plan_of(int dtype, int nkv, int batch, int n_heads, int max_length, int window) {
+Plan plan_of(int dtype, bool half, int nkv, int batch, int n_heads, int max_length, int window) {
     Plan p;
     const int group = n_heads / nkv;
-    p.col_heads = !is_quant(dtype) ? kCols : group <= 4 ? 4 : 8;
+    p.col_heads = !is_quant(dtype) ? (!half && group <= 4 ? 4 : kCols) : group <= 4 ? 4 : 8;
     p.col_tiles = (group + p.col_heads - 1) / p.col_heads;
     const int64_t groups = (int64_t)batch * nkv * p.col_tiles;
     const int64_t len = (window > 0 && window < max_length - kPos ? window + kPos : max_length);
@@ -806,7 +959,7 @@ size_t part_bytes(int hd, int batch, int n_heads, int pieces) { return (size_t)p
 
 // For any window: a plan has at most as many pieces as it may want, and as the positions have units.
 size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length) {
-    const int pieces = std::min(plan_of(dtype, nkv, batch, n_heads, max_length, 0).want, (max_length + kPieceUnit - 1) / kPieceUnit);
+    const int pieces = std::min(plan_of(dtype, false, nkv, batch, n_heads, max_length, 0).want, (max_length + kPieceUnit - 1) / kPieceUnit);
     return pieces == 1 ? 0 : part_bytes(hd, batch, n_heads, pieces) + (size_t)pieces * batch * n_heads * sizeof(float2);
 }
 
@@ -815,7 +968,8 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.a = a;
     g.n_heads = a.q.heads;
     g.group = g.n_heads / a.c.nkv;
-    const Plan p = plan_of(a.c.dtype, a.c.nkv, a.q.tokens, g.n_heads, a.max_length, a.window);
+    const bool half = a.q.dtype != DT_F32;
+    const Plan p = plan_of(a.c.dtype, half, a.c.nkv, a.q.tokens, g.n_heads, a.max_length, a.window);
     g.col_tiles = p.col_tiles;
     g.piece = p.piece;
     g.pieces = p.pieces;
@@ -825,14 +979,17 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.part = reinterpret_cast<float *>(a.ws);
     g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);
-    const bool half = a.q.dtype != DT_F32, short_terms = a.q.dtype == DT_BF16, few = p.col_heads == 4;
+    const bool short_terms = a.q.dtype == DT_BF16, few = p.col_heads == 4;
 #define SPH_FLOAT(CT, HD, HALF) \
-    if (a.c.dtype == CT && a.c.hd == HD && half == HALF) hipLaunchKernelGGL((paged_attn_kernel<CT, HD, HALF>), grid, block, 0, s, g);
+    if (a.c.dtype == CT && a.c.hd == HD && half == HALF && !few) hipLaunchKernelGGL((paged_attn_kernel<CT, HD, HALF>), grid, block, 0, s, g);
+#define SPH_FEW(CT, HD) \
+    if (a.c.dtype == CT && a.c.hd == HD && few) hipLaunchKernelGGL((paged_attn_few_kernel<CT, HD>), grid, block, 0, s, g);
 #define SPH_DIGITS(CT, HD, NT, TERMS)                                                             \
     if (a.c.dtype == CT && a.c.hd == HD && few == (NT == 1) && short_terms == (TERMS == 1))       \
         hipLaunchKernelGGL((paged_attn_digits_kernel<CT, HD, NT, TERMS>), grid, block, 0, s, g);
 #define SPH_QUANT(CT, HD) SPH_DIGITS(CT, HD, 1, 1) SPH_DIGITS(CT, HD, 1, 3) SPH_DIGITS(CT, HD, 2, 1) SPH_DIGITS(CT, HD, 2, 3)
 #define SPH_ATTN_HD(HD)                                                                           \
+    SPH_FEW(DT_F32, HD) SPH_FEW(DT_BF16, HD) SPH_FEW(DT_F16, HD)                                  \
     SPH_FLOAT(DT_F32, HD, false) SPH_FLOAT(DT_BF16, HD, false) SPH_FLOAT(DT_BF16, HD, true)       \
     SPH_FLOAT(DT_F16, HD, false) SPH_FLOAT(DT_F16, HD, true) SPH_QUANT(DT_Q8_0, HD) SPH_QUANT(DT_Q4_0, HD)
     SPH_ATTN_HD(64) SPH_ATTN_HD(128) SPH_ATTN_HD(256)
