@@ -1,8 +1,7 @@
 // beam.hip - beam search's selection: one pass over the logits, then one workgroup per request.
 //
 // Within a row the order of the scores is the order of the logits, so the pass needs no normaliser: each
-// wave keeps its best W (logit, index) keys in its first lanes, sorted, and only elements above the W-th
-// touch them; beside that it sums exp. The rows' lists and normalisers meet in the second launch, where
+// wave keeps its best W (logit, index) keys, and beside that it sums exp. The rows' lists and normalisers meet in the second launch, where
 // the scores of the W x W candidates left are formed and compared in 64 bits.
 #include <algorithm>
 
@@ -19,9 +18,9 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 256, kWave = 64, kWaves = kThreads / kWave;
 constexpr int kMaxBeams = 16;
-constexpr int kStep = 8;                   // loads in flight per lane
+constexpr int kStep = 8, kBatch = 4;       // logits of a lane, two times four consecutive ones; times as many at once
 constexpr int kChunkMin = 2048;            // logits of a workgroup at least
-constexpr int kWantGroups = 1024;
+constexpr int kWantGroups = 2048;
 
 // Larger logits, then lower indices, have larger keys; NaN counts as -inf, -0 as 0. Never 0.
 __device__ __forceinline__ u64 key_of(float x, uint32_t i) {
@@ -35,139 +34,258 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
 
-// The `w` largest keys seen by a wave, in its lanes 0 .. w - 1, largest first (0: none yet).
+// The `w` largest keys that a wave has seen. Keys above the w-th (`last`) gather in 64 words of LDS; when they would
+// not fit, and at the end, each one's place is the number of larger ones, and the first w stay.
 struct Best {
-    u64 key = 0, last = 0;                 // this lane's, the w-th
-    // every lane offers one key (0: none)
-    __device__ __forceinline__ void offer(u64 k, int w) {
+    u64 *buf;
+    int w, count = 0;
+    u64 last = 0;                          // 0: fewer than w so far
+
+    __device__ __forceinline__ Best(u64 *lds, int beams) : buf(lds), w(beams) {}
+    // a wave's LDS accesses stay in order; the compiler is told
+    static __device__ __forceinline__ void handover() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ void sort() {
         const int lane = threadIdx.x & (kWave - 1);
+        handover();
+        const u64 k = lane < count ? buf[lane] : 0;
+        int place = 0;
+        for (int j = 0; j < count; j += 4)             // (lanes from count on hold 0)
+            place += (u64_lane(k, j) > k) + (u64_lane(k, j + 1) > k) + (u64_lane(k, j + 2) > k) + (u64_lane(k, j + 3) > k);
+        handover();
+        if (lane < count && place < w) buf[place] = k;
+        count = min(count, w);
+        const u64 mask = __ballot(k != 0 && place == w - 1);
+        last = mask ? u64_lane(k, __builtin_ctzll(mask)) : 0;
+        handover();
+    }
+    // every lane offers one key (0: none)
+    __device__ __forceinline__ void offer(u64 k) {
         u64 mask = __ballot(k > last);
-        while (mask) {
-            const u64 top = u64_lane(k, __builtin_ctzll(mask));
-            const int at = __popcll(__ballot(lane < w && key > top));
-            const u64 up = __shfl_up(key, 1, kWave);
-            key = lane < at ? key : lane == at ? top : up;
-            last = u64_lane(key, w - 1);
-            mask &= mask - 1;
-            mask &= __ballot(k > last);
+        if (count + __popcll(mask) > kWave) {
+            sort();
+            mask = __ballot(k > last);
+            if (count + __popcll(mask) > kWave) {      // up to w held and 64 offered: in two halves
+                const bool low = (threadIdx.x & (kWave - 1)) < kWave / 2;
+                put(low ? k : 0, __ballot(low && k > last));
+                sort();
+                k = low ? 0 : k;
+                mask = __ballot(k > last);
+            }
         }
+        put(k, mask);
+    }
+    __device__ __forceinline__ void put(u64 k, u64 mask) {
+        const int lane = threadIdx.x & (kWave - 1);
+        if (mask >> lane & 1) buf[count + __popcll(mask & ((1ull << lane) - 1))] = k;
+        count += __popcll(mask);
     }
 };
 
-// grid (chunks, rows): keys[row][chunk][beams] largest first, norm[row][chunk] = (max, sum exp(x - max)).
-// Rows that have ended, and dead ones, need neither.
-__global__ __launch_bounds__(kThreads) void beam_rows_kernel(const float *__restrict__ logits, int ld, int n, int beams,
+__device__ __forceinline__ double wave_sum(double s) {
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    return s;
+}
+
+// Part of a row's normaliser: its largest logit and the sum of exp(x - max).
+struct Norm {
+    double sum;
+    float max;
+};
+
+// exp(x - m) for x <= m (NaN where both are infinite, 0 for a NaN x). log2 e in two floats: the rounding of one would
+// be off the same way in every term, where the others' roundings even out over a row.
+__device__ __forceinline__ float exp_of(float x, float m) {
+    constexpr float hi = 0x1.715476p+0f, lo = 0x1.4ae0cp-26f;
+    const float d = __fsub_rn(fmaxf(x, m - 150.0f), m);
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi, __fmul_rn(d, lo)));
+}
+
+// A value that at least w of the wave's 64 reach: the least of the maxima of (at least) w groups of lanes.
+__device__ __forceinline__ float reached_by(float t, int w) {
+    t = fmaxf(t, lanes::dpp_mov<0xB1>(t));
+    t = fmaxf(t, lanes::dpp_mov<0x4E>(t));             // of four lanes
+    if (w <= 8) t = fmaxf(t, lanes::dpp_mov<0x141>(t));
+    if (w <= 4) t = fmaxf(t, lanes::dpp_mov<0x140>(t));
+    return -lanes::wave_max(-t);
+}
+
+// grid (chunks, rows): keys[row][place][chunk], norm[row][chunk]. Rows that have ended, and dead ones, need neither.
+// A wave holds BATCH x 512 logits in its registers, eight of 512 in a lane, and has as many more on their way (BATCH
+// 1 for chunks of no more than that per wave: a quarter of the code to fetch). Only those that reach a value that W of
+// them do are looked at as keys.
+template <int BATCH>
+__global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__restrict__ logits, int ld, int n, int beams,
                                                              const float *__restrict__ scores, const int *__restrict__ done,
-                                                             int chunk, u64 *__restrict__ keys, float2 *__restrict__ norm) {
-    __shared__ u64 all[kWaves * kMaxBeams];
-    __shared__ float2 part[kWaves];
-    const int row = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+                                                             int chunk, u64 *__restrict__ keys, Norm *__restrict__ norm) {
+    __shared__ u64 lists[kWaves][kWave];
+    __shared__ Norm part[kWaves];
+    const int row = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if ((done && done[row] != 0) || !(fabsf(scores[row]) < INFINITY)) return;
     const float *x = logits + (size_t)row * ld;
     const int lo = blockIdx.x * chunk, hi = min(n, lo + chunk);
-    Best best;
-    float mx = -INFINITY, sum = 0.f;
-    for (int i0 = lo + wid * kStep * kWave; i0 < hi; i0 += kWaves * kStep * kWave) {
-        float v[kStep];
+    Best best(lists[wid], beams);
+    float mx = -INFINITY;
+    double sum = 0.0;
+    constexpr int kSpan = kStep * kWave, kAll = kWaves * BATCH * kSpan;
+    auto spot = [](int u) { return (u >> 2) * (4 * kWave) + (u & 3); };       // of a lane's u-th logit, from its first
+    auto load = [&](float (&v)[BATCH][kStep], int i0) {
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) v[u] = x[min(i0 + u * kWave + lane, hi - 1)];
-        float top = -INFINITY;
+        for (int g = 0; g < BATCH; ++g) {
+            const int first = i0 + g * kWaves * kSpan, at = first + lane * 4;
+            if (first + kSpan <= hi) {                                 // rows start anywhere
+                __builtin_memcpy(v[g], x + at, 16);
+                __builtin_memcpy(v[g] + 4, x + at + 4 * kWave, 16);
+            } else if (first < hi) {
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {
-            if (i0 + u * kWave + lane >= hi || v[u] != v[u]) v[u] = -INFINITY;
-            top = fmaxf(top, v[u]);
+                for (int u = 0; u < kStep; ++u) v[g][u] = x[min(at + spot(u), hi - 1)];
+            }
         }
-        const float m = fmaxf(mx, top);
-        if (m > -INFINITY) {
-            sum *= __expf(mx - m);
+    };
+    float v[BATCH][kStep];
+    int i0 = lo + wid * kSpan;
+    if (i0 < hi) load(v, i0);
+    while (i0 < hi) {
+        float next[BATCH][kStep];                                      // on its way during this batch's work
+        if (i0 + kAll < hi) load(next, i0 + kAll);
+        float most[BATCH], top = -INFINITY;                            // (a maximum with a NaN is the other one)
 #pragma unroll
-            for (int u = 0; u < kStep; ++u) sum += __expf(v[u] - m);
-            mx = m;
-        }
+        for (int g = 0; g < BATCH; ++g) {
+            const int first = i0 + g * kWaves * kSpan, at = first + lane * 4;
+            if (first + kSpan > hi) {
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {
-            const int i = i0 + u * kWave + lane;
-            best.offer(i < hi ? key_of(v[u], (uint32_t)i) : 0, beams);
+                for (int u = 0; u < kStep; ++u) v[g][u] = at + spot(u) < hi ? v[g][u] : -INFINITY;
+            }
+            most[g] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kStep; u += 2) most[g] = fmaxf(most[g], fmaxf(v[g][u], v[g][u + 1]));
+            top = fmaxf(top, most[g]);
         }
+        const float m = fmaxf(mx, top), from = m > -INFINITY ? m : 0.f;
+        sum *= (double)exp_of(mx, from);                               // 0 before the first
+        mx = m;
+        float floor = key_value(best.last);
+        if (best.last == 0) floor = reached_by(top, beams);
+        uint64_t reach = 0;
+#pragma unroll
+        for (int g = 0; g < BATCH; ++g) {
+            const int first = i0 + g * kWaves * kSpan, at = first + lane * 4;
+            if (first >= hi) continue;
+            float e[kStep];
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) e[u] = exp_of(v[g][u], from);
+            sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+            if (__any(most[g] >= floor)) {
+#pragma unroll
+                for (int u = 0; u < kStep; ++u) reach |= (uint64_t)(!(v[g][u] < floor) && at + spot(u) < hi) << (g * kStep + u);
+            }
+        }
+        while (__any(reach != 0)) {
+            const int bit = reach ? __builtin_ctzll(reach) : 0, at = i0 + bit / kStep * kWaves * kSpan + lane * 4 + spot(bit % kStep);
+            float mine = v[0][0];
+#pragma unroll
+            for (int i = 1; i < BATCH * kStep; ++i) mine = bit == i ? v[i / kStep][i % kStep] : mine;
+            best.offer(reach ? key_of(mine, (uint32_t)at) : 0);
+            reach &= reach - 1;
+        }
+        best.sort();
+        i0 += kAll;
+#pragma unroll
+        for (int g = 0; g < BATCH; ++g)
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) v[g][u] = next[g][u];
     }
     const float wm = lanes::wave_max(mx);
-    const float ws = lanes::wave_sum(mx > -INFINITY ? sum * __expf(mx - wm) : 0.f);
-    if (lane < beams) all[wid * beams + lane] = best.key;
-    if (lane == 0) part[wid] = make_float2(wm, ws);
+    const double ws = wave_sum(mx > -INFINITY ? sum * (double)exp_of(mx, wm) : 0.0);
+    if (lane >= best.count && lane < beams) lists[wid][lane] = 0;
+    if (lane == 0) part[wid] = Norm{ws, wm};
     __syncthreads();
     if (wid != 0) return;
-    Best merged;                                       // of the waves' lists, a key per lane
-    merged.offer(lane < kWaves * beams ? all[lane] : 0, beams);
-    if (lane < beams) keys[((size_t)row * gridDim.x + blockIdx.x) * beams + lane] = merged.key;
+    // of the waves' lists, a key per lane, the first `beams` (0 where there are fewer)
+    const u64 k = lane < kWaves * beams ? lists[lane / beams][lane % beams] : 0;
+    int place = 0;
+    for (int j = 0; j < kWaves * beams; j += 4)        // (lanes from there on hold 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u64 other = u64_lane(k, j + i);
+            place += other > k || (other == k && j + i < lane);
+        }
+    if (lane < kWaves * beams && place < beams) keys[((size_t)row * beams + place) * gridDim.x + blockIdx.x] = k;
     if (lane == 0) {
-        float m = -INFINITY, s = 0.f;
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, part[w].x);
+        float m = -INFINITY;
+        double s = 0.0;
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, part[w].max);
         for (int w = 0; w < kWaves; ++w)
-            if (part[w].x > -INFINITY) s += part[w].y * __expf(part[w].x - m);
-        norm[(size_t)row * gridDim.x + blockIdx.x] = make_float2(m, s);
+            if (part[w].max > -INFINITY) s += part[w].sum * (double)exp_of(part[w].max, m);
+        norm[(size_t)row * gridDim.x + blockIdx.x] = Norm{s, m};
     }
 }
 
-// grid (requests)
-__global__ __launch_bounds__(kThreads) void beam_pick_kernel(int n, int beams, int chunks, const float *scores,
-                                                             const int *done, int end_token,
-                                                             const u64 *__restrict__ keys, const float2 *__restrict__ norm,
-                                                             float *scores_out, int *__restrict__ tokens,
-                                                             int *__restrict__ parents, int *done_out) {
+// grid (requests), a wave per beam
+__global__ __launch_bounds__(kMaxBeams *kWave) void beam_pick_kernel(int n, int beams, int chunks, const float *scores,
+                                                                     const int *done, int end_token,
+                                                                     const u64 *__restrict__ keys,
+                                                                     const Norm *__restrict__ norm, float *scores_out,
+                                                                     int *__restrict__ tokens, int *__restrict__ parents,
+                                                                     int *done_out) {
+    __shared__ u64 lists[kMaxBeams][kWave];
     __shared__ double score[kMaxBeams * kMaxBeams];
     __shared__ int token[kMaxBeams * kMaxBeams], ended[kMaxBeams];
-    const int r0 = blockIdx.x * beams, lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
-    for (int b = wid; b < beams; b += kWaves) {
-        const int row = r0 + b;
-        const float cum = scores[row];
-        const bool over = done && done[row] != 0;
-        bool dead = !(fabsf(cum) < INFINITY) || (over && (end_token < 0 || end_token >= n));
-        Best best;
-        double lse = 0.0;
-        if (!dead && !over) {
-            const float2 *nr = norm + (size_t)row * chunks;
-            float m = -INFINITY;
-            for (int i = lane; i < chunks; i += kWave) m = fmaxf(m, nr[i].x);
-            m = lanes::wave_max(m);
-            double s = 0.0;
-            for (int i = lane; i < chunks; i += kWave)
-                if (nr[i].x > -INFINITY) s += (double)nr[i].y * (double)__expf(nr[i].x - m);
-#pragma unroll
-            for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-            lse = (double)m + log(s);
-            dead = !(fabs(lse) < (double)INFINITY);    // a logit of +inf, or none above -inf
-            const u64 *kr = keys + (size_t)row * chunks * beams;
-            for (int i0 = 0; i0 < chunks * beams; i0 += kWave) best.offer(i0 + lane < chunks * beams ? kr[i0 + lane] : 0, beams);
+    const int r0 = blockIdx.x * beams, lane = threadIdx.x & (kWave - 1), b = threadIdx.x / kWave, row = r0 + b;
+    const float cum = scores[row];
+    const bool over = done && done[row] != 0;
+    bool dead = !(fabsf(cum) < INFINITY) || (over && (end_token < 0 || end_token >= n));
+    Best best(lists[b], beams);
+    u64 mine = 0;
+    double lse = 0.0;
+    if (!dead && !over) {
+        const u64 *kr = keys + (size_t)row * chunks * beams;
+        const Norm *nr = norm + (size_t)row * chunks;
+        const Norm first = nr[min(lane, chunks - 1)];          // (on its way beside the keys)
+        for (int i0 = 0; i0 < chunks * beams; i0 += kWave) best.offer(i0 + lane < chunks * beams ? kr[i0 + lane] : 0);
+        best.sort();
+        mine = lane < beams ? lists[b][lane] : 0;
+        const float m = key_value(u64_lane(mine, 0));  // the largest logit
+        double s = lane < chunks && first.max > -INFINITY ? first.sum * (double)exp_of(first.max, m) : 0.0;
+        for (int i = lane + kWave; i < chunks; i += kWave)
+            if (nr[i].max > -INFINITY) s += nr[i].sum * (double)exp_of(nr[i].max, m);
+        lse = (double)m + log(wave_sum(s));
+        dead = !(fabs(lse) < (double)INFINITY);        // a logit of +inf, or none above -inf
+    }
+    if (lane < beams) {
+        double sc = -(double)INFINITY;
+        int tok = lane;                                // what a row of -inf offers
+        if (!dead && over) {
+            tok = lane == 0 ? end_token : lane - 1 + (lane - 1 >= end_token);
+            if (lane == 0) sc = (double)cum;
+        } else if (!dead) {
+            sc = (double)cum + ((double)key_value(mine) - lse);
+            tok = (int)key_index(mine);
         }
-        if (lane < beams) {
-            double sc = -(double)INFINITY;
-            int tok = lane;                            // what a row of -inf offers
-            if (!dead && over) {
-                tok = lane == 0 ? end_token : lane - 1 + (lane - 1 >= end_token);
-                if (lane == 0) sc = (double)cum;
-            } else if (!dead) {
-                sc = (double)cum + ((double)key_value(best.key) - lse);
-                tok = (int)key_index(best.key);
-            }
-            score[b * beams + lane] = sc;
-            token[b * beams + lane] = tok;
-            if (lane == 0) ended[b] = over;
-        }
+        score[b * beams + lane] = sc;
+        token[b * beams + lane] = tok;
+        if (lane == 0) ended[b] = over;
     }
     __syncthreads();
-    // each candidate's place is the number of better ones; of equal scores the lower row, then the
-    // row's own order, goes first
-    const int i = threadIdx.x, all = beams * beams;
+    // Each candidate's place is the number of better ones; of equal scores the lower row, then the row's own order,
+    // goes first. Four threads count for one candidate (64 beams threads are at least 4 beams^2).
+    const int i = threadIdx.x >> 2, all = beams * beams;
     if (i >= all) return;
     const double sc = score[i];
     int place = 0;
-    for (int j = 0; j < all; ++j) place += score[j] > sc || (score[j] == sc && j < i);
-    if (place >= beams) return;
-    const int b = i / beams;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < all; j += 4) place += score[j] > sc || (score[j] == sc && j < i);
+    place += __builtin_amdgcn_update_dpp(0, place, 0xB1, 0xF, 0xF, false);
+    place += __builtin_amdgcn_update_dpp(0, place, 0x4E, 0xF, 0xF, false);
+    if (place >= beams || (threadIdx.x & 3) != 0) return;
+    const int from = i / beams;
     scores_out[r0 + place] = (float)sc;
     tokens[r0 + place] = token[i];
-    parents[r0 + place] = r0 + b;
-    if (done_out) done_out[r0 + place] = ended[b] || token[i] == end_token;
+    parents[r0 + place] = r0 + from;
+    if (done_out) done_out[r0 + place] = ended[from] || token[i] == end_token;
 }
 
 int chunks_of(int n, int rows) {
@@ -179,7 +297,7 @@ int chunk_of(int n, int chunks) { return (n + chunks - 1) / chunks; }
 }  // namespace
 
 size_t beam_workspace_bytes(int n, int rows, int beams) {
-    return (size_t)rows * chunks_of(n, rows) * (beams * sizeof(u64) + sizeof(float2));
+    return (size_t)rows * chunks_of(n, rows) * (beams * sizeof(u64) + sizeof(Norm));
 }
 
 int launch_beam_select(const float *logits, int ld, int n, int requests, int beams, const float *scores, const int *done,
@@ -187,11 +305,14 @@ int launch_beam_select(const float *logits, int ld, int n, int requests, int bea
                        hipStream_t s) {
     const int rows = requests * beams, chunks = chunks_of(n, rows);
     u64 *keys = static_cast<u64 *>(ws);
-    float2 *norm = reinterpret_cast<float2 *>(keys + (size_t)rows * chunks * beams);
-    hipLaunchKernelGGL(beam_rows_kernel, dim3(chunks, rows), dim3(kThreads), 0, s, logits, ld, n, beams, scores, done,
-                       chunk_of(n, chunks), keys, norm);
+    Norm *norm = reinterpret_cast<Norm *>(keys + (size_t)rows * chunks * beams);
+    const int chunk = chunk_of(n, chunks);
+    if (chunk <= kWaves * kStep * kWave)
+        hipLaunchKernelGGL((beam_rows_kernel<1>), dim3(chunks, rows), dim3(kThreads), 0, s, logits, ld, n, beams, scores, done, chunk, keys, norm);
+    else
+        hipLaunchKernelGGL((beam_rows_kernel<kBatch>), dim3(chunks, rows), dim3(kThreads), 0, s, logits, ld, n, beams, scores, done, chunk, keys, norm);
     if (!hip_ok(hipGetLastError(), "beam rows launch")) return -1;
-    hipLaunchKernelGGL(beam_pick_kernel, dim3(requests), dim3(kThreads), 0, s, n, beams, chunks, scores, done, end_token,
+    hipLaunchKernelGGL(beam_pick_kernel, dim3(requests), dim3(beams * kWave), 0, s, n, beams, chunks, scores, done, end_token,
                        keys, norm, scores_out, tokens, parents, done_out);
     return hip_ok(hipGetLastError(), "beam pick launch") ? 0 : -1;
 }

@@ -451,7 +451,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
             for (int e = 0; e < DPL; e += 4)           // (they were of that type: nothing is rounded)
                 *reinterpret_cast<pu2 *>(qs + r * QL + e0 + e) =
-                    pu2{to_16(CT, qx[e]) | to_16(CT, qx[e + 1]) << 16, to_16(CT, qx[e + 2]) | to_16(CT, qx[e + 3]) << 16};
+                    pu2{pack_16(CT, qx[e], qx[e + 1]), pack_16(CT, qx[e + 2], qx[e + 3])};
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) qh[j] = *reinterpret_cast<const pu4 *>(qs + c * QL + 32 * j + 8 * m);
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) pw[2 * u + i] = to_16(CT, p[u][2 * i]) | to_16(CT, p[u][2 * i + 1]) << 16;
+                for (int i = 0; i < 2; ++i) pw[2 * u + i] = pack_16(CT, p[u][2 * i], p[u][2 * i + 1]);
 #pragma unroll
             for (int x = 0; x < DPL; x += 2) {
                 pu4 even, odd;
@@ -818,7 +818,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
                         for (int i = 0; i < 2; ++i) {
                             float &x0 = x[2 * i], &x1 = x[2 * i + 1];
                             if constexpr (TERMS == 1) {
-                                w[t][q][2 * (u + s) + i] = to_bf16(x0) | to_bf16(x1) << 16;
+                                w[t][q][2 * (u + s) + i] = pack_16(DT_BF16, x0, x1);
                             } else {                   // the upper half of the word, and what it leaves
                                 w[t][q][2 * (u + s) + i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
                                 x0 = __fsub_rn(x0, __uint_as_float(__float_as_uint(x0) & 0xffff0000u));

@@ -82,6 +82,14 @@ __device__ __forceinline__ uint32_t to_bf16(float v) {
 }
 __device__ __forceinline__ uint32_t to_f16(float v) { return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v); }
 __device__ __forceinline__ uint32_t to_16(int dtype, float v) { return dtype == DT_BF16 ? to_bf16(v) : to_f16(v); }
+// two values in one word, the first in its lower half
+typedef float pf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pb2 __attribute__((ext_vector_type(2)));
+typedef _Float16 ph2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_16(int dtype, float a, float b) {
+    const pf2 v = {a, b};
+    return dtype == DT_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pb2)) : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ph2));
+}
 __device__ __forceinline__ float from_16(int dtype, uint32_t b) { return dtype == DT_BF16 ? from_bf16(b) : from_f16(b); }
 
 __device__ __forceinline__ void load8(int dtype, bool wide, const uint8_t *base, int64_t at, float (&x)[8]) {
@@ -129,14 +137,14 @@ __device__ __forceinline__ void store8(int dtype, bool wide, uint8_t *base, int6
         }
     } else {
         uint16_t *p = reinterpret_cast<uint16_t *>(base) + at;
-        uint32_t w[8];
+        pu4 w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = to_16(dtype, x[i]);
+        for (int i = 0; i < 4; ++i) w[i] = pack_16(dtype, x[2 * i], x[2 * i + 1]);
         if (wide) {
-            *reinterpret_cast<pu4 *>(p) = pu4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
+            *reinterpret_cast<pu4 *>(p) = w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = (uint16_t)w[i];
+            for (int i = 0; i < 8; ++i) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
         }
     }
 }

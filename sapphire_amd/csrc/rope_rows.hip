@@ -62,7 +62,7 @@ struct Piece {
             if constexpr (WIDE) {
                 pu4 w;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = to_16(DT, v[2 * i]) | to_16(DT, v[2 * i + 1]) << 16;
+                for (int i = 0; i < 4; ++i) w[i] = pack_16(DT, v[2 * i], v[2 * i + 1]);
                 *reinterpret_cast<pu4 *>(f) = w;
             } else {
                 *f = (uint16_t)to_16(DT, v[0]);
@@ -95,33 +95,50 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a) {
     __syncthreads();
     const int h0 = blockIdx.y * a.heads, nh = min(a.heads, a.x.heads - h0);
     const bool same = a.x.p == a.y.p;      // the remaining dims are there already
-    // units of a head: its turning pieces, then the copied ones
+    // units of a head: its turning pieces, then the copied ones. A thread keeps its unit and steps over the heads and
+    // tokens, `across` at a time.
     const int turning = PAIRS ? (WIDE ? a.rot / P::N : half) : half / P::N;
-    const int units = turning + (same ? 0 : (a.x.hd - a.rot) / P::N), per = nh * units;
-    for (int i = threadIdx.x; i < nt * per; i += kThreads) {
-        const int t = i / per, hu = i - t * per, h = hu / units, u = hu - h * units;
-        const int64_t xi = (int64_t)(t0 + t) * a.x.ts + (int64_t)(h0 + h) * a.x.hs;
-        const int64_t yi = (int64_t)(t0 + t) * a.y.ts + (int64_t)(h0 + h) * a.y.hs;
-        const float2 *w = cs + t * half;
-        P p, q;
-        if (u >= turning) {
-            const int d = a.rot + (u - turning) * P::N;
-            p.load(a.x.p, xi + d);
-            p.store(a.y.p, yi + d);
-        } else if constexpr (PAIRS && WIDE) {
-            const int d = u * P::N;
-            p.load(a.x.p, xi + d);
+    const int units = turning + (same ? 0 : (a.x.hd - a.rot) / P::N), across = max(1, kThreads / units);
+    const int row = threadIdx.x / units;
+    for (int u = threadIdx.x - row * units; row < across && u < units; u += kThreads) {
+        int t = 0, h = row;
+        while (h >= nh) {
+            h -= nh;
+            ++t;
+        }
+        int64_t xi = (int64_t)(t0 + t) * a.x.ts + (int64_t)(h0 + h) * a.x.hs;
+        int64_t yi = (int64_t)(t0 + t) * a.y.ts + (int64_t)(h0 + h) * a.y.hs;
+        while (t < nt) {
+            const float2 *w = cs + t * half;
+            P p, q;
+            if (u >= turning) {
+                const int d = a.rot + (u - turning) * P::N;
+                p.load(a.x.p, xi + d);
+                p.store(a.y.p, yi + d);
+            } else if constexpr (PAIRS && WIDE) {
+                const int d = u * P::N;
+                p.load(a.x.p, xi + d);
 #pragma unroll
-            for (int e = 0; e < P::N / 2; ++e) turn(p.v[2 * e], p.v[2 * e + 1], w[d / 2 + e]);
-            p.store(a.y.p, yi + d);
-        } else {
-            const int d = u * P::N, d0 = PAIRS ? 2 * d : d, d1 = PAIRS ? 2 * d + 1 : d + half;
-            p.load(a.x.p, xi + d0);
-            q.load(a.x.p, xi + d1);
+                for (int e = 0; e < P::N / 2; ++e) turn(p.v[2 * e], p.v[2 * e + 1], w[d / 2 + e]);
+                p.store(a.y.p, yi + d);
+            } else {
+                const int d = u * P::N, d0 = PAIRS ? 2 * d : d, d1 = PAIRS ? 2 * d + 1 : d + half;
+                p.load(a.x.p, xi + d0);
+                q.load(a.x.p, xi + d1);
 #pragma unroll
-            for (int e = 0; e < P::N; ++e) turn(p.v[e], q.v[e], w[d + e]);
-            p.store(a.y.p, yi + d0);
-            q.store(a.y.p, yi + d1);
+                for (int e = 0; e < P::N; ++e) turn(p.v[e], q.v[e], w[d + e]);
+                p.store(a.y.p, yi + d0);
+                q.store(a.y.p, yi + d1);
+            }
+            h += across;
+            xi += across * a.x.hs;
+            yi += across * a.y.hs;
+            while (h >= nh) {
+                h -= nh;
+                ++t;
+                xi += a.x.ts - nh * a.x.hs;
+                yi += a.y.ts - nh * a.y.hs;
+            }
         }
     }
 }
