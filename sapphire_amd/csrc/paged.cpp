@@ -132,7 +132,7 @@ bool move_ok(const sapphire_paged_cache_t *c, int layer, const sapphire_rows_t *
     }
     if (!positions) { set_error("paged cache: no positions"); return false; }
     if (!seqs && k->tokens > t->rows) { set_error("paged cache: %d tokens for %d table rows", k->tokens, t->rows); return false; }
-    if ((int64_t)k->tokens * c->n_kv_heads * (c->head_dim / 8) > kMaxUnits) { set_error("paged cache: too many rows in one call"); return false; }
+    if (((int64_t)k->tokens + 15) * c->n_kv_heads * (c->head_dim / 8) > kMaxUnits) { set_error("paged cache: too many rows in one call"); return false; }
     return true;
 }
 

@@ -60,10 +60,10 @@ __device__ __forceinline__ bool paged_place(const PagedCache &c, const PageTable
                                             const int *__restrict__ positions, int t, int &page, int &off) {
     const int row = seqs ? seqs[t] : t, pos = positions[t];
     if (row < 0 || row >= tab.rows || pos < 0) return false;
-    const int i = pos / c.page_size;
-    if (i >= tab.ld) return false;
+    const uint32_t i = (uint32_t)pos / (uint32_t)c.page_size;
+    if (i >= (uint32_t)tab.ld) return false;
     page = tab.pages[(size_t)row * tab.ld + i];
-    off = pos - i * c.page_size;
+    off = pos - (int)i * c.page_size;
     return page >= 0 && page < c.pages;
 }
 

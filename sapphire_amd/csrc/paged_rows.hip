@@ -5,6 +5,7 @@
 // Q4_0: d = m / -8 with m the first x of largest |x|, q = min(15, trunc(x * (1 / d) + 8.5)); every
 // product, sum and quotient rounded on its own. A block with a NaN or an infinity gets the scale NaN.
 #include <algorithm>
+#include <climits>
 
 #include "internal.h"
 #include "lanes.h"
@@ -25,49 +26,72 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     v = max(v, dpp_u32<0xB1>(v));
     return max(v, dpp_u32<0x4E>(v));
 }
+__device__ __forceinline__ int quad_max(int v) {
+    v = max(v, (int)dpp_u32<0xB1>((uint32_t)v));
+    return max(v, (int)dpp_u32<0x4E>((uint32_t)v));
+}
 __device__ __forceinline__ uint32_t quad_min(uint32_t v) {
     v = min(v, dpp_u32<0xB1>(v));
     return min(v, dpp_u32<0x4E>(v));
 }
 
-// The quad's block: its scale and this lane's eight codes (Q8_0 -127 .. 127, Q4_0 0 .. 15).
+// The quad's block: its scale and this lane's eight codes (Q8_0 -127 .. 127, Q4_0 0 .. 15). As signed integers the
+// words' largest is the largest positive element (NaN above infinity), as unsigned ones the negative element of
+// largest magnitude.
 template <int CT>
 __device__ __forceinline__ float quantize8(const float (&x)[8], int lq, int (&q)[8]) {
-    uint32_t top = 0;
+    int up = INT_MIN;
+    uint32_t down = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = quad_max(top);                               // of the magnitudes' bits: NaN above infinity
-    if (top >= 0x7f800000u) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = CT == DT_Q8_0 ? 0 : 8;
-        return __uint_as_float(0x7fc00000u);
+    for (int i = 0; i < 8; i += 2) {
+        up = max(up, max((int)__float_as_uint(x[i]), (int)__float_as_uint(x[i + 1])));
+        down = max(down, max(__float_as_uint(x[i]), __float_as_uint(x[i + 1])));
     }
+    up = max(quad_max(up), 0);
+    down = quad_max(down);
+    down = down & 0x80000000u ? down & 0x7fffffffu : 0u;
+    const uint32_t top = max((uint32_t)up, down);
+    const bool bad = top >= 0x7f800000u;
     float d;
     if constexpr (CT == DT_Q8_0) {
         d = __fdiv_rn(__uint_as_float(top), 127.0f);
     } else {
-        uint32_t first = ~0u;                          // (index, sign) of the first element of that magnitude
+        bool minus = down > (uint32_t)up;
+        if (__any(down == (uint32_t)up)) {             // both signs have that magnitude: the first element's counts
+            uint32_t first = ~0u;
 #pragma unroll
-        for (int i = 7; i >= 0; --i) {
-            const uint32_t u = __float_as_uint(x[i]);
-            if ((u & 0x7fffffffu) == top) first = (uint32_t)(lq * 8 + i) * 2 + (u >> 31);
+            for (int i = 7; i >= 0; --i) {
+                const uint32_t u = __float_as_uint(x[i]);
+                if ((u & 0x7fffffffu) == top) first = (uint32_t)(lq * 8 + i) * 2 + (u >> 31);
+            }
+            first = quad_min(first);
+            minus = first & 1;
         }
-        first = quad_min(first);
-        d = __fmul_rn(__uint_as_float(top), (first & 1) ? 0.125f : -0.125f);
+        d = __fmul_rn(__uint_as_float(top), minus ? 0.125f : -0.125f);
     }
     const float id = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-    // a subnormal d has an infinite id: its products saturate, 0 * inf counts as zero
+    // Adding the float below 1/2 and truncating rounds halves away from zero, the rest to nearest. Magnitudes stay
+    // within the codes (Q4_0: but for the one of the other sign, 16).
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float v = __fmul_rn(x[i], id);
-        if constexpr (CT == DT_Q8_0) {
-            // adding the float below 1/2 and truncating rounds halves away from zero, the rest to nearest
-            const float w = v != v ? 0.0f : fminf(fmaxf(v, -127.0f), 127.0f);
-            q[i] = (int)__fadd_rn(w, copysignf(0x1.fffffep-2f, w));
-        } else {
-            const float w = __fadd_rn(v, 8.5f);
-            q[i] = w != w ? 8 : (int)fminf(fmaxf(w, 0.0f), 15.0f);
+        if constexpr (CT == DT_Q8_0) q[i] = (int)__fadd_rn(v, copysignf(0x1.fffffep-2f, v));
+        else q[i] = (int)fminf(__fadd_rn(v, 8.5f), 15.0f);
+    }
+    // a subnormal d has an infinite id: its products saturate, 0 * inf counts as zero
+    if (__any(bad || fabsf(id) == INFINITY)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = __fmul_rn(x[i], id);
+            if constexpr (CT == DT_Q8_0) {
+                const float w = v != v ? 0.0f : fminf(fmaxf(v, -127.0f), 127.0f);
+                q[i] = bad ? 0 : (int)__fadd_rn(w, copysignf(0x1.fffffep-2f, w));
+            } else {
+                const float w = __fadd_rn(v, 8.5f);
+                q[i] = bad || w != w ? 8 : (int)fminf(fmaxf(w, 0.0f), 15.0f);
+            }
         }
+        if (bad) d = __uint_as_float(0x7fc00000u);
     }
     return d;
 }
@@ -89,7 +113,7 @@ __device__ __forceinline__ void store_codes(uint8_t *tile, uint32_t ps, uint32_t
         } else {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = to_16(CT, x[2 * i]) | to_16(CT, x[2 * i + 1]) << 16;
+            for (int i = 0; i < 4; ++i) w[i] = pack_16(CT, x[2 * i], x[2 * i + 1]);
             if constexpr (V && HD == 64) {
                 *reinterpret_cast<pu2 *>(tile + T::v_run(p, d / 4)) = pu2{w[0], w[1]};
                 *reinterpret_cast<pu2 *>(tile + T::v_run(p, d / 4 + 1)) = pu2{w[2], w[3]};
@@ -158,7 +182,6 @@ __device__ __forceinline__ void load_codes(const uint8_t *tile, uint32_t ps, uin
         }
     } else {
         const float scale = *reinterpret_cast<const float *>(tile + (V ? T::v_scale(ps, p, d / 32) : T::k_scale(ps, p, d / 32)));
-        int q[8];
         if constexpr (CT == DT_Q8_0) {
             uint32_t lo, hi;
             if constexpr (V && HD == 64) {
@@ -171,8 +194,8 @@ __device__ __forceinline__ void load_codes(const uint8_t *tile, uint32_t ps, uin
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                q[i] = (int8_t)(lo >> (8 * i));
-                q[4 + i] = (int8_t)(hi >> (8 * i));
+                x[i] = __fmul_rn((float)(int8_t)(lo >> (8 * i)), scale);
+                x[4 + i] = __fmul_rn((float)(int8_t)(hi >> (8 * i)), scale);
             }
         } else {
             uint32_t lo, hi;                           // codes 0..3 and 4..7, one nibble per byte
@@ -195,59 +218,65 @@ __device__ __forceinline__ void load_codes(const uint8_t *tile, uint32_t ps, uin
                 lo = (a & 0x0f0fu) | (a >> 4 & 0x0f0fu) << 16;
                 hi = (b & 0x0f0fu) | (b >> 4 & 0x0f0fu) << 16;
             }
+            asm("" : "+v"(lo), "+v"(hi));              // (the compiler would rather extract nibbles one by one)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                q[i] = (int)(lo >> (8 * i) & 15u) - 8;
-                q[4 + i] = (int)(hi >> (8 * i) & 15u) - 8;
+                x[i] = __fmul_rn(__fsub_rn((float)(lo >> (8 * i) & 255u), 8.0f), scale);
+                x[4 + i] = __fmul_rn(__fsub_rn((float)(hi >> (8 * i) & 255u), 8.0f), scale);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)q[i], scale);
     }
 }
 
-// grid (units / kThreads, 2): K, then V. A unit is eight dims of a (token, head).
+// A thread's eight dims: the workgroups take the heads' rows sixteen tokens at a time, so that those of a prompt, which go
+// to sixteen positions of a tile, leave whole lines to one L2 (an L2 each would write its part of every line).
+struct Unit {
+    int t, h, d;
+};
+template <int HD>
+__device__ __forceinline__ Unit unit_of(int nkv) {
+    constexpr int U = HD / 8, kRows = kThreads / U;            // 32, 16 or 8 rows of a workgroup
+    const uint32_t row = blockIdx.x * kRows + threadIdx.x / U, g = __builtin_amdgcn_readfirstlane(row >> 4);     // one per wave
+    return Unit{(int)(g / (uint32_t)nkv * 16 + (row & 15)), (int)(g % (uint32_t)nkv), (int)(threadIdx.x % U) * 8};
+}
+int64_t row_groups(const Rows &r, int nkv, int hd) {
+    const int rows = kThreads / (hd / 8);
+    return ((int64_t)(r.tokens + 15) / 16 * 16 * nkv + rows - 1) / rows;
+}
+
+// grid (row_groups). A thread takes its unit of K and of V: one look at the table, both loads under way together.
 template <int CT, int HD>
 __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedCache c, Rows k, Rows v, PageTable tab,
                                                                const int *__restrict__ seqs,
                                                                const int *__restrict__ positions, bool kw, bool vw) {
-    constexpr int U = HD / 8;
-    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    const uint64_t row = i / U;
-    const int t = (int)(row / (uint32_t)c.nkv), h = (int)(row % (uint32_t)c.nkv), d = (int)(i % U) * 8;
+    const Unit u = unit_of<HD>(c.nkv);
+    if (u.t >= k.tokens) return;
+    float x[8], y[8];
+    load8(k.dtype, kw, k.p, (int64_t)u.t * k.ts + (int64_t)u.h * k.hs + u.d, x);
+    load8(v.dtype, vw, v.p, (int64_t)u.t * v.ts + (int64_t)u.h * v.hs + u.d, y);
     int page, off;
-    if (t >= k.tokens || !paged_place(c, tab, seqs, positions, t, page, off)) return;
-    const size_t at = ((size_t)page * c.nkv + h) * c.tile_bytes;
-    float x[8];
-    if (blockIdx.y == 0) {
-        load8(k.dtype, kw, k.p, (int64_t)t * k.ts + (int64_t)h * k.hs + d, x);
-        store_codes<CT, HD, false>(c.k + at, c.page_size, off, d, x);
-    } else {
-        load8(v.dtype, vw, v.p, (int64_t)t * v.ts + (int64_t)h * v.hs + d, x);
-        store_codes<CT, HD, true>(c.v + at, c.page_size, off, d, x);
-    }
+    if (!paged_place(c, tab, seqs, positions, u.t, page, off)) return;
+    const size_t at = ((size_t)page * c.nkv + u.h) * c.tile_bytes;
+    store_codes<CT, HD, false>(c.k + at, c.page_size, off, u.d, x);
+    store_codes<CT, HD, true>(c.v + at, c.page_size, off, u.d, y);
 }
 
 template <int CT, int HD>
 __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedCache c, Rows k, Rows v, PageTable tab,
                                                               const int *__restrict__ seqs,
                                                               const int *__restrict__ positions, bool kw, bool vw) {
-    constexpr int U = HD / 8;
-    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    const uint64_t row = i / U;
-    const int t = (int)(row / (uint32_t)c.nkv), h = (int)(row % (uint32_t)c.nkv), d = (int)(i % U) * 8;
-    if (t >= k.tokens) return;
+    const Unit u = unit_of<HD>(c.nkv);
+    if (u.t >= k.tokens) return;
     int page, off;
-    const bool there = paged_place(c, tab, seqs, positions, t, page, off);
-    const size_t at = there ? ((size_t)page * c.nkv + h) * c.tile_bytes : 0;
-    float x[8] = {};
-    if (blockIdx.y == 0) {
-        if (there) load_codes<CT, HD, false>(c.k + at, c.page_size, off, d, x);
-        store8(k.dtype, kw, k.p, (int64_t)t * k.ts + (int64_t)h * k.hs + d, x);
-    } else {
-        if (there) load_codes<CT, HD, true>(c.v + at, c.page_size, off, d, x);
-        store8(v.dtype, vw, v.p, (int64_t)t * v.ts + (int64_t)h * v.hs + d, x);
+    const bool there = paged_place(c, tab, seqs, positions, u.t, page, off);
+    float x[8] = {}, y[8] = {};
+    if (there) {
+        const size_t at = ((size_t)page * c.nkv + u.h) * c.tile_bytes;
+        load_codes<CT, HD, false>(c.k + at, c.page_size, off, u.d, x);
+        load_codes<CT, HD, true>(c.v + at, c.page_size, off, u.d, y);
     }
+    store8(k.dtype, kw, k.p, (int64_t)u.t * k.ts + (int64_t)u.h * k.hs + u.d, x);
+    store8(v.dtype, vw, v.p, (int64_t)u.t * v.ts + (int64_t)u.h * v.hs + u.d, y);
 }
 
 // grid (rows, 2 * layers * heads): one tile's written part to the spare page; the workgroups of
@@ -311,8 +340,7 @@ __global__ __launch_bounds__(kThreads) void paged_reorder_kernel(PagedCache c, P
 
 int launch_paged_write(const PagedCache &c, const Rows &k, const Rows &v, const PageTable &t, const int *seqs,
                        const int *positions, hipStream_t s) {
-    const int64_t units = (int64_t)k.tokens * c.nkv * (c.hd / 8);
-    const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2), block(kThreads);
+    const dim3 grid((unsigned)row_groups(k, c.nkv, c.hd)), block(kThreads);
 #define SPH_CALL(CT, HD) \
     hipLaunchKernelGGL((paged_write_kernel<CT, HD>), grid, block, 0, s, c, k, v, t, seqs, positions, rows_wide(k), rows_wide(v))
     SPH_PAGED(SPH_CALL)
@@ -322,8 +350,7 @@ int launch_paged_write(const PagedCache &c, const Rows &k, const Rows &v, const 
 
 int launch_paged_read(const PagedCache &c, const Rows &k, const Rows &v, const PageTable &t, const int *seqs,
                       const int *positions, hipStream_t s) {
-    const int64_t units = (int64_t)k.tokens * c.nkv * (c.hd / 8);
-    const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2), block(kThreads);
+    const dim3 grid((unsigned)row_groups(k, c.nkv, c.hd)), block(kThreads);
 #define SPH_CALL(CT, HD) \
     hipLaunchKernelGGL((paged_read_kernel<CT, HD>), grid, block, 0, s, c, k, v, t, seqs, positions, rows_wide(k), rows_wide(v))
     SPH_PAGED(SPH_CALL)
