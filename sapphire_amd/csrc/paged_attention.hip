@@ -413,14 +413,13 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     using R = Raw<CT, HD>;
     constexpr int LD = HD + 4, DPL = R::DPL;
     constexpr int HALVES = HALF ? 2 : 1, STEP = kWaves * HALVES * kPos;
-    __shared__ __attribute__((aligned(16))) float buf[2 * kCols * LD];     // q, later the waves' O
+    __shared__ __attribute__((aligned(16))) float buf[kWaves * kCols * LD];        // q, later the waves' O
     __shared__ float wm[kWaves][kCols], wsum[kWaves][kCols];
     const PagedAttn &a = g.a;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, m = lane >> 4;
     Walk<HALVES> at(g, kCols);
     if (at.empty(g)) return;
-    const bool owner = c < at.heads;
     float qx[DPL];
     load_q<DPL>(a.q, at.b, at.h0, at.heads, qx);
     R k[HALVES], v[HALVES];
@@ -568,54 +567,13 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
         wsum[wid][c] = sum;
     }
     __syncthreads();                                   // every wave is past its reads of q
-    float top = wm[0][c];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wm[w][c]);
-    // a wave without positions, or with scores of -inf only, has sum 0; its factor must not be NaN
-    const float fw = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(mx - top);
-    float tot = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-        if (wsum[w][c] != 0.f) tot += __fmul_rn(wsum[w][c], __builtin_amdgcn_exp2f(wm[w][c] - top));
-#pragma unroll
-    for (int x = 0; x < DPL; ++x)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[x][r] = sum == 0.f ? 0.f : __fmul_rn(o[x][r], fw);
-    // two waves at a time leave their O, the two before add theirs to it
-#pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
-        float *mine = buf + ((wid & (half - 1)) * kCols + c) * LD;
-        if (wid >= half && wid < 2 * half && owner) {
-#pragma unroll
-            for (int x = 0; x < DPL; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mine[R::v_dim(x, 4 * m + r)] = o[x][r];
-        }
-        __syncthreads();
-        if (wid < half && owner) {
-#pragma unroll
-            for (int x = 0; x < DPL; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[x][r] = __fadd_rn(o[x][r], mine[R::v_dim(x, 4 * m + r)]);
-        }
-        __syncthreads();
-    }
-    if (wid != 0 || !owner) return;
-    if (g.pieces == 1) {
-        const float inv = tot == 0.f ? 0.f : __fdiv_rn(1.0f, tot);
-        const int64_t out_at = (int64_t)at.b * a.out.ts + (int64_t)(at.h0 + c) * a.out.hs;
+    if (c < at.heads) {
 #pragma unroll
         for (int x = 0; x < DPL; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) store1(a.out.dtype, a.out.p, out_at + R::v_dim(x, 4 * m + r), __fmul_rn(o[x][r], inv));
-        if (a.lse && m == 0) a.lse[(size_t)at.b * g.n_heads + at.h0 + c] = lse_of(top, tot);
-    } else {
-#pragma unroll
-        for (int x = 0; x < DPL; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) g.part[(at.slot0 + c) * HD + R::v_dim(x, 4 * m + r)] = o[x][r];
-        if (m == 0) g.ms[at.slot0 + c] = make_float2(top, tot);
+            for (int r = 0; r < 4; ++r) buf[(wid * kCols + c) * LD + R::v_dim(x, 4 * m + r)] = o[x][r];
     }
+    finish<HD, kCols>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
 // Rows over a quantized cache, 4 NT query heads. K's codes meet q as they are: q is rounded to 2^-31 of its head's
