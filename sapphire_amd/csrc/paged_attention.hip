@@ -657,11 +657,16 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
         }
     }
     __syncthreads();
-    pu2 qd[NT][T::NB];
+    // the digits in registers, or where O takes most of those, read from LDS as they are used
+    constexpr bool kHold = NT == 1 || HD == 64;
+    pu2 held[kHold ? NT : 1][kHold ? T::NB : 1];
+    auto digits = [&](int t, int j) { return *reinterpret_cast<const pu2 *>(lds + ((t * T::NB + j) * kWave + lane) * 8); };
+    if constexpr (kHold) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < T::NB; ++j) qd[t][j] = *reinterpret_cast<const pu2 *>(lds + ((t * T::NB + j) * kWave + lane) * 8);
+            for (int j = 0; j < T::NB; ++j) held[t][j] = digits(t, j);
+    }
     // from the digits' integers to scores in log2 units (or to what the cap takes); lane (c, m): head 4t + m
     const float cap = a.softcap;
     float unit[NT], mx[NT], sum[NT];
@@ -691,7 +696,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
                 const pu2 kb = k[u].k_codes(j);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const pi4 d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, qd[t][j]), __builtin_bit_cast(long, kb),
+                    pu2 qd;
+                    if constexpr (kHold) qd = held[t][j];
+                    else qd = digits(t, j);
+                    const pi4 d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, qd), __builtin_bit_cast(long, kb),
                                                                         pi4{0, 0, 0, 0}, 0, 0, 0);
                     // below 2^28: 32 products of 2^14, times 2^8
                     const float low = (float)(d[1] * 256 + d[0]), high = (float)(d[3] * 256 + d[2]);
