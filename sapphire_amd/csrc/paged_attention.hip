@@ -27,6 +27,7 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 struct AttnArgs {
     PagedAttn a;
     int n_heads, group, col_tiles, piece, pieces;
+    bool ordered;                          // longest sequences first
     uint32_t page_magic;                   // i / (page_size / 16) is its high product with i < 2^26 (0: page_size is 16)
     float *part;                           // [pieces][batch][n_heads][hd], unnormalised O
     float2 *ms;                            // [pieces][batch][n_heads]: maximum (log2 units), sum
@@ -184,6 +185,46 @@ __device__ __forceinline__ pf4 mfma16(pu4 a, pu4 b, pf4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8, a), __builtin_bit_cast(pb8, b), c, 0, 0, 0);
 }
 
+// The sequence that workgroups z take when the longest go first, by eighths of max_length (in order within one): where
+// whole sequences are a workgroup's work, a long one started late would run alone at the end. The same in every
+// workgroup. masks: 64 words of LDS per 512 sequences.
+constexpr int kOrdered = 1024, kClasses = 8;
+__device__ __forceinline__ int nth_longest(const int *__restrict__ lengths, int batch, int max_length, int z,
+                                           unsigned long long *masks) {
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, chunks = (batch + kWave - 1) / kWave;
+    const float scale = (float)kClasses / (float)max_length;
+    for (int q = wid; q < chunks; q += kWaves) {
+        const int b = q * kWave + lane, n = b < batch ? min(max(lengths[b], 0), max_length) : 0;
+        const int cls = b < batch ? kClasses - 1 - min(kClasses - 1, (int)((float)n * scale)) : -1;
+#pragma unroll
+        for (int k = 0; k < kClasses; ++k) {
+            const unsigned long long mask = __ballot(cls == k);
+            if (lane == 0) masks[k * chunks + q] = mask;
+        }
+    }
+    __syncthreads();
+    // entries in order, 64 at a time: the one whose running count passes z
+    for (int e0 = 0; e0 < kClasses * chunks; e0 += kWave) {
+        const unsigned long long mask = e0 + lane < kClasses * chunks ? masks[e0 + lane] : 0;
+        const int mine = __popcll(mask);
+        int upto = mine;
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) {
+            const int below = __shfl_up(upto, off, kWave);
+            upto += lane >= off ? below : 0;
+        }
+        const unsigned long long past = __ballot(upto > z);
+        if (past) {
+            const int e = __builtin_ctzll(past), left = z - __shfl(upto - mine, e, kWave);
+            const unsigned long long m = lanes::u64_lane(mask, e);
+            const unsigned long long at = __ballot((m >> lane & 1) && __popcll(m & ((1ull << lane) - 1)) == left);
+            return (e0 + e) % chunks * kWave + __builtin_ctzll(at);
+        }
+        z -= __shfl(upto, kWave - 1, kWave);
+    }
+    return 0;                                          // (not reached: every sequence is in a class)
+}
+
 // A workgroup's part of the call: a piece of one sequence, for one K/V head's query heads h0 .. h0 + heads - 1,
 // and its walk over the pages, HALVES tiles of 16 positions at a time.
 template <int HALVES>
@@ -198,6 +239,10 @@ struct Walk {
     __device__ __forceinline__ Walk(const AttnArgs &g, int per_group) {
         const PagedAttn &a = g.a;
         b = blockIdx.z;
+        if (g.ordered) {
+            __shared__ unsigned long long masks[kOrdered / kWave * kClasses];
+            b = __builtin_amdgcn_readfirstlane(nth_longest(a.lengths, gridDim.z, a.max_length, b, masks));
+        }
         hk = blockIdx.y / g.col_tiles;
         const int ct = blockIdx.y - hk * g.col_tiles;
         h0 = hk * g.group + ct * per_group;
@@ -905,13 +950,14 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
 // at least.
 struct Plan {
     int col_heads, col_tiles, want, piece, pieces;
+    int64_t groups;
 };
 Plan plan_of(int dtype, bool half, int nkv, int batch, int n_heads, int max_length, int window) {
     Plan p;
     const int group = n_heads / nkv;
     p.col_heads = !is_quant(dtype) ? (!half && group <= 4 ? 4 : kCols) : group <= 4 ? 4 : 8;
     p.col_tiles = (group + p.col_heads - 1) / p.col_heads;
-    const int64_t groups = (int64_t)batch * nkv * p.col_tiles;
+    const int64_t groups = p.groups = (int64_t)batch * nkv * p.col_tiles;
     const int64_t len = (window > 0 && window < max_length - kPos ? window + kPos : max_length);
     p.want = groups >= kFullGroups ? 1 : (int)std::min<int64_t>(kMaxPieces, kWantGroups / groups);
     p.piece = (int)(((len + p.want - 1) / p.want + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
@@ -939,6 +985,7 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.col_tiles = p.col_tiles;
     g.piece = p.piece;
     g.pieces = p.pieces;
+    g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kFullGroups;
     // ceil(2^32 / d), d <= 64: off by less than d / 2^32 relative to 1 / d, and i * d < 2^32
     const uint64_t d = a.c.page_size / kPos;
     g.page_magic = d == 1 ? 0 : (uint32_t)(((1ull << 32) + d - 1) / d);

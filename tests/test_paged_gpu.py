@@ -242,6 +242,19 @@ def test_attention_pages_that_do_not_exist(hip, cache):
     attend_case(np.random.default_rng(3), cache, F32, 64, 1, 4, 16, [40, 16, 100, 700], broken=[(0, 1), (1, 0), (2, 0), (2, 6), (3, 5), (3, 43)])
 
 
+@pytest.mark.parametrize("cache,io,batch,nkv", [(BF16, BF16, 257, 4), (Q4_0, F32, 1024, 1), (F32, F32, 1100, 1), (Q8_0, BF16, 64, 17), (F16, F32, 520, 2)],
+                         ids=["257x4", "1024", "1100", "64x17", "520x2"])
+def test_attention_of_many_sequences(hip, cache, io, batch, nkv):
+    """Enough whole sequences to fill the chip, which the workgroups take by length: every one, empty ones and lengths out
+    of range among them, gets its own output."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(0, 80, batch)]
+    lens[3], lens[7] = 0, 80
+    given = np.array(lens)
+    given[3], given[7] = -7, 10**9
+    attend_case(rng, cache, io, 64, nkv, nkv * 2, 16, lens, n_given=given, max_length=80)
+
+
 def test_attention_lengths_are_clamped(hip):
     rng = np.random.default_rng(4)
     attend_case(rng, F32, F32, 64, 1, 2, 16, [0, 50, 20], n_given=[-5, 1000, 20], max_length=50, lse=False)
