@@ -85,11 +85,13 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * positions. lengths outside [0, max_length] are taken as its nearest end; max_length is at most
  * table->ld * page_size. A sequence of length 0 gets out = 0 and lse = -inf, and so does one whose
  * scores are all -inf or whose pages do not exist. A NaN or +inf score makes the head's outputs NaN.
- * What lies behind a sequence's last position, NaN included, does not count.
+ * What lies behind a sequence's last position, NaN included, does not count. Over a quantized cache a
+ * NaN or an infinity in q makes its head's outputs NaN. (Weights reach 2^8 before they are scaled:
+ * values of V above 2^119 can overflow the sums.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the
- * same type or a quantized one. out is rounded once, at the end; over a 16-bit cache with 16-bit rows
- * and over quantized ones with 16-bit rows the weights exp(s_p - max s) are rounded to that type
- * before they meet V. lse: [tokens][n_heads] fp32, or NULL. Long sequences are cut into pieces that
+ * same type or a quantized one. out is rounded once, at the end; with 16-bit rows over a cache of their
+ * type, and with BF16 rows over a quantized one, the weights exp(s_p - max s) are rounded to that type
+ * before they meet V (as much as the outputs are). lse: [tokens][n_heads] fp32, or NULL. Long sequences are cut into pieces that
  * run side by side and are joined by a second launch; the results do not depend on which workgroup
  * runs when, nor on what the other sequences hold.
  * workspace: sapphire_paged_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is

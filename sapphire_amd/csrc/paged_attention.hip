@@ -457,6 +457,9 @@ template <int CT, int HD, bool HALF>
 __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
     constexpr int LD = HD + 4, DPL = R::DPL;
+    // fp16 weights: mx is held this much below the maximum, so that weights of down to 2^-21 of the largest stay normal
+    // (2^(kLift + kLazy) is in range)
+    constexpr float kLift = HALF && CT == DT_F16 ? 7.0f : 0.0f;
     constexpr int HALVES = HALF ? 2 : 1, STEP = kWaves * HALVES * kPos;
     __shared__ __attribute__((aligned(16))) float buf[kWaves * kCols * LD];        // q, later the waves' O
     __shared__ float wm[kWaves][kCols], wsum[kWaves][kCols];
@@ -558,10 +561,10 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
         for (int u = 0; u < HALVES; ++u) ref = fmaxf(ref, fmaxf(fmaxf(p[u][0], p[u][1]), fmaxf(p[u][2], p[u][3])));
         // The maximum moves, with O and the sums, only for a score far above it: weights up to 2^kLazy do no harm.
-        if (__any(ref > mx + kLazy)) {
+        if (__any(ref > mx + kLift + kLazy)) {
             ref = fmaxf(ref, __shfl_xor(ref, 16, kWave));
             ref = fmaxf(ref, __shfl_xor(ref, 32, kWave));
-            const float mn = fmaxf(mx, ref), f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
+            const float mn = fmaxf(mx, ref - kLift), f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
             mx = mn;
             sum = __fmul_rn(sum, f);
 #pragma unroll

@@ -308,6 +308,32 @@ def test_attention_infinite_and_nan_scores(hip, io):
             assert (np.abs(got[s] - out) <= tol).all() and (np.abs(lse[s] - l) <= ltol).all()
 
 
+@pytest.mark.parametrize("io", [F32, BF16, F16], ids=ref.NAME.get)
+def test_attention_of_many_small_weights(hip, io):
+    """One position outweighs each of 2^17 - 1 others by 2^25: together they weigh 2^-8, which is the output (its value is
+    0, theirs 1)."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PagedCache, PageTable
+    hd, ps, n = 64, 256, 1 << 17
+    c = PagedCache(io, 1, n // ps, ps, 1, hd)
+    k, v = np.zeros((n, 1, hd), np.float32), np.ones((n, 1, hd), np.float32)
+    k[0, 0, 0], v[0] = 25 * np.log(2), 0
+    rk, rv = device_rows(k, io), device_rows(v, io)
+    q = np.zeros((1, 1, hd), np.float32)
+    q[0, 0, 0] = 1
+    rq, ro = device_rows(q, io), device_rows(q, io)
+    dt, dp, ds = dev(np.arange(n // ps, dtype=np.int32)[None]), dev(np.arange(n, dtype=np.int32)), dev(np.zeros(n, np.int32))
+    pt = PageTable(dt, 1, n // ps)
+    c.write(0, rk[0], rv[0], pt, dp, seqs=ds)
+    ws = DeviceArray(max(1, c.attention_workspace_bytes(1, 1, n)))
+    c.attention(0, rq[0], ro[0], pt, dev(np.array([n], np.int32)), n, 1.0, workspace=ws)
+    sync()
+    got = ref.from_type(io, ro[1].numpy()[:hd]).astype(np.float64)
+    out, l, size, mean = ref.attention64(q[0], ref.from_type(io, rk[3]), v, 1.0)
+    tol, _ = ref.attention_bound(io, io != F32, hd, n, out, l, size, mean)
+    assert (np.abs(got - out[0]) <= np.minimum(tol[0], out[0] / 50)).all()
+
+
 def test_pages_past_four_gigabytes(hip):
     """Rows written, read and attended to in the last pages of pools of more than 2^32 bytes."""
     from sapphire_amd.device import DeviceArray
