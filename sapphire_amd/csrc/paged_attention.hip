@@ -450,8 +450,8 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 }
 
 // Rows over a float cache. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
-// cache of their type: 16x16x32 products of the elements as they are; the weights are rounded to that type
-// (half a step, what the outputs are rounded by too), and V's 16-bit words are transposed in pairs on the way.
+// cache of their type: 16x16x32 products of the elements as they are; the weights come in two terms of that type (one
+// would be off by as much as the outputs' own rounding), and V's 16-bit words are transposed in pairs on the way.
 // grid (pieces, K/V heads x column tiles, sequences).
 template <int CT, int HD, bool HALF>
 __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(AttnArgs g) {
@@ -580,11 +580,16 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
             }
         if constexpr (HALF) {
             // contraction index 8m + 4u + r is position 4m + r of half u
-            pu4 pw;
+            pu4 pw, rest;                              // the weights in that type, and what that leaves of them
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) pw[2 * u + i] = pack_16(CT, p[u][2 * i], p[u][2 * i + 1]);
+                for (int i = 0; i < 2; ++i) {
+                    const float p0 = p[u][2 * i], p1 = p[u][2 * i + 1];
+                    const uint32_t w = pack_16(CT, p0, p1);
+                    pw[2 * u + i] = w;
+                    rest[2 * u + i] = pack_16(CT, __fsub_rn(p0, from_16(CT, w & 0xffffu)), __fsub_rn(p1, from_16(CT, w >> 16)));
+                }
 #pragma unroll
             for (int x = 0; x < DPL; x += 2) {
                 pu4 even, odd;
@@ -598,6 +603,8 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                     }
                 o[x] = mfma16<CT>(even, pw, o[x]);
                 o[x + 1] = mfma16<CT>(odd, pw, o[x + 1]);
+                o[x] = mfma16<CT>(even, rest, o[x]);
+                o[x + 1] = mfma16<CT>(odd, rest, o[x + 1]);
                 if (HD == 256) __builtin_amdgcn_sched_barrier(0);      // (few words at a time: registers)
             }
         } else {
@@ -631,7 +638,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 // of four blocks of V (head_dim 256: the contraction runs over both halves of the blocks, each half's codes beside
 // zeros for the other half's rows), and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
 // sums only those of a column's own block are meant. TERMS: bf16 terms of that product, 3 for all its 24 bits;
-// 1 where rows are bf16 (half a step of the outputs' type).
+// 2 where rows are bf16 (its rounding is then 2^-7 of the outputs').
 template <int CT, int HD, int NT, int TERMS>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && CT == DT_Q4_0) ? 4 : NT == 1 ? 3 : 2) void paged_attn_digits_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
@@ -831,13 +838,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             float &x0 = x[2 * i], &x1 = x[2 * i + 1];
-                            if constexpr (TERMS == 1) {
-                                w[t][q][2 * (u + s) + i] = pack_16(DT_BF16, x0, x1);
-                            } else {                   // the upper half of the word, and what it leaves
-                                w[t][q][2 * (u + s) + i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
-                                x0 = __fsub_rn(x0, __uint_as_float(__float_as_uint(x0) & 0xffff0000u));
-                                x1 = __fsub_rn(x1, __uint_as_float(__float_as_uint(x1) & 0xffff0000u));
-                            }
+                            // the upper half of the word, and what it leaves
+                            w[t][q][2 * (u + s) + i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+                            x0 = __fsub_rn(x0, __uint_as_float(__float_as_uint(x0) & 0xffff0000u));
+                            x1 = __fsub_rn(x1, __uint_as_float(__float_as_uint(x1) & 0xffff0000u));
                         }
                 }
             }
@@ -1001,9 +1005,9 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
 #define SPH_FEW(CT, HD) \
     if (a.c.dtype == CT && a.c.hd == HD && few) hipLaunchKernelGGL((paged_attn_few_kernel<CT, HD>), grid, block, 0, s, g);
 #define SPH_DIGITS(CT, HD, NT, TERMS)                                                             \
-    if (a.c.dtype == CT && a.c.hd == HD && few == (NT == 1) && short_terms == (TERMS == 1))       \
+    if (a.c.dtype == CT && a.c.hd == HD && few == (NT == 1) && short_terms == (TERMS == 2))       \
         hipLaunchKernelGGL((paged_attn_digits_kernel<CT, HD, NT, TERMS>), grid, block, 0, s, g);
-#define SPH_QUANT(CT, HD) SPH_DIGITS(CT, HD, 1, 1) SPH_DIGITS(CT, HD, 1, 3) SPH_DIGITS(CT, HD, 2, 1) SPH_DIGITS(CT, HD, 2, 3)
+#define SPH_QUANT(CT, HD) SPH_DIGITS(CT, HD, 1, 2) SPH_DIGITS(CT, HD, 1, 3) SPH_DIGITS(CT, HD, 2, 2) SPH_DIGITS(CT, HD, 2, 3)
 #define SPH_ATTN_HD(HD)                                                                           \
     SPH_FEW(DT_F32, HD) SPH_FEW(DT_BF16, HD) SPH_FEW(DT_F16, HD)                                  \
     SPH_FLOAT(DT_F32, HD, false) SPH_FLOAT(DT_BF16, HD, false) SPH_FLOAT(DT_BF16, HD, true)       \
