@@ -225,6 +225,15 @@ __device__ __forceinline__ int nth_longest(const int *__restrict__ lengths, int 
     return 0;                                          // (not reached: every sequence is in a class)
 }
 
+// The same over 16 positions: two words a lane.
+typedef short ps4 __attribute__((ext_vector_type(4)));
+typedef _Float16 ph4 __attribute__((ext_vector_type(4)));
+template <int CT>
+__device__ __forceinline__ pf4 mfma8(pu2 a, pu2 b, pf4 c) {
+    if constexpr (CT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(ph4, a), __builtin_bit_cast(ph4, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ps4, a), __builtin_bit_cast(ps4, b), c, 0, 0, 0);
+}
+
 // A workgroup's part of the call: a piece of one sequence, for one K/V head's query heads h0 .. h0 + heads - 1,
 // and its walk over the pages, HALVES tiles of 16 positions at a time.
 template <int HALVES>
@@ -450,7 +459,8 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 }
 
 // Rows over a float cache. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
-// cache of their type: 16x16x32 products of the elements as they are; the weights come in two terms of that type (one
+// cache of their type: 16x16x32 products of the elements as they are, of two tiles for the weighted sum (of one where
+// two do not fit the registers, 16x16x16); the weights come in two terms of that type (one
 // would be off by as much as the outputs' own rounding), and V's 16-bit words are transposed in pairs on the way.
 // grid (pieces, K/V heads x column tiles, sequences).
 template <int CT, int HD, bool HALF>
@@ -460,7 +470,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     // fp16 weights: mx is held this much below the maximum, so that weights of down to 2^-21 of the largest stay normal
     // (2^(kLift + kLazy) is in range)
     constexpr float kLift = HALF && CT == DT_F16 ? 7.0f : 0.0f;
-    constexpr int HALVES = HALF ? 2 : 1, STEP = kWaves * HALVES * kPos;
+    constexpr int HALVES = HALF && HD < 256 ? 2 : 1, STEP = kWaves * HALVES * kPos;
     __shared__ __attribute__((aligned(16))) float buf[kWaves * kCols * LD];        // q, later the waves' O
     __shared__ float wm[kWaves][kCols], wsum[kWaves][kCols];
     const PagedAttn &a = g.a;
@@ -531,7 +541,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
             s4[0] = (st[0] + st[1]) + (st[2] + st[3]);
         } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < HALVES; ++u) {
                 s4[u] = pf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) s4[u] = mfma16<CT>(k[u].w[j], qh[j], s4[u]);
@@ -579,10 +589,10 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                 sum = __fadd_rn(sum, p[u][r]);
             }
         if constexpr (HALF) {
-            // contraction index 8m + 4u + r is position 4m + r of half u
-            pu4 pw, rest;                              // the weights in that type, and what that leaves of them
+            // contraction index 4 HALVES m + 4u + r is position 4m + r of half u
+            uint32_t pw[2 * HALVES], rest[2 * HALVES]; // the weights in that type, and what that leaves of them
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < HALVES; ++u)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float p0 = p[u][2 * i], p1 = p[u][2 * i + 1];
@@ -592,20 +602,24 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
                 }
 #pragma unroll
             for (int x = 0; x < DPL; x += 2) {
-                pu4 even, odd;
+                uint32_t even[2 * HALVES], odd[2 * HALVES];
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < HALVES; ++u)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t w0 = v[u].v_pair(2 * i, x), w1 = v[u].v_pair(2 * i + 1, x);
                         even[2 * u + i] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
                         odd[2 * u + i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
                     }
-                o[x] = mfma16<CT>(even, pw, o[x]);
-                o[x + 1] = mfma16<CT>(odd, pw, o[x + 1]);
-                o[x] = mfma16<CT>(even, rest, o[x]);
-                o[x + 1] = mfma16<CT>(odd, rest, o[x + 1]);
-                if (HD == 256) __builtin_amdgcn_sched_barrier(0);      // (few words at a time: registers)
+                auto product = [](const uint32_t (&a)[2 * HALVES], const uint32_t (&b)[2 * HALVES], pf4 c) {
+                    if constexpr (HALVES == 2) return mfma16<CT>(pu4{a[0], a[1], a[2], a[3]}, pu4{b[0], b[1], b[2], b[3]}, c);
+                    else return mfma8<CT>(pu2{a[0], a[1]}, pu2{b[0], b[1]}, c);
+                };
+                o[x] = product(even, pw, o[x]);
+                o[x + 1] = product(odd, pw, o[x + 1]);
+                o[x] = product(even, rest, o[x]);
+                o[x + 1] = product(odd, rest, o[x + 1]);
+                if (HD == 256 && x % 4 == 2) __builtin_amdgcn_sched_barrier(0);        // (few words at a time: registers)
             }
         } else {
 #pragma unroll
