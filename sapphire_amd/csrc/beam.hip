@@ -245,7 +245,15 @@ __global__ __launch_bounds__(kMaxBeams *kWave) void beam_pick_kernel(int n, int 
         const u64 *kr = keys + (size_t)row * chunks * beams;
         const Norm *nr = norm + (size_t)row * chunks;
         const Norm first = nr[min(lane, chunks - 1)];          // (on its way beside the keys)
-        for (int i0 = 0; i0 < chunks * beams; i0 += kWave) best.offer(i0 + lane < chunks * beams ? kr[i0 + lane] : 0);
+        for (int i0 = 0; i0 < chunks * beams; i0 += 4 * kWave) {
+            u64 k[4];                                  // (on their way together)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = kr[min(i0 + j * kWave + lane, chunks * beams - 1)];
+            for (int j = 0; j < 4; ++j) {
+                const u64 mine = j == 0 ? k[0] : j == 1 ? k[1] : j == 2 ? k[2] : k[3];
+                best.offer(i0 + j * kWave + lane < chunks * beams ? mine : 0);
+            }
+        }
         best.sort();
         mine = lane < beams ? lists[b][lane] : 0;
         const float m = key_value(u64_lane(mine, 0));  // the largest logit

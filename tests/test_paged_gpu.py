@@ -334,6 +334,40 @@ def test_attention_of_many_small_weights(hip, io):
     assert (np.abs(got - out[0]) <= np.minimum(tol[0], out[0] / 50)).all()
 
 
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+@pytest.mark.parametrize("heads", [4, 7])
+def test_attention_of_extreme_queries(hip, cache, heads):
+    """Rows of zeros, of 1e-30 and of 1e30 (under scales that bring their scores back), one element a million times the
+    others; a NaN makes its own head NaN and no other."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(13)
+    hd, ps, n = 128, 16, 200
+    table, pages = tables(rng, [n], ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+    c.fill(0, table, 0, k, v)
+    c.upload()
+    ks, vs = ref.stored(cache, k), ref.stored(cache, v)
+    dt, dl, ws = dev(table), dev(np.array([n], np.int32)), DeviceArray(max(1, c.c.attention_workspace_bytes(1, heads, n)))
+    for size in (0.0, 1e-30, 1.0, 1e30):
+        q = (rng.normal(size=(1, heads, hd)) * size).astype(np.float32)
+        if size == 1.0:
+            q[0, 1, 77] = 1e6
+            q[0, 2, 5] = np.nan
+        scale = 0.1 / size if size else 0.1
+        rq, ro = device_rows(q, F32), device_rows(np.ones_like(q), F32)
+        c.c.attention(0, rq[0], ro[0], PageTable(dt, *table.shape), dl, n, scale, workspace=ws)
+        sync()
+        got = ro[1].numpy()[:heads * hd].reshape(heads, hd)
+        if size == 1.0:
+            assert np.isnan(got[2]).all()
+            got, q = np.delete(got, 2, 0), np.delete(q, 2, 1)
+        out, l, big, mean = ref.attention64(q[0], ks, vs, float(np.float32(scale)))
+        tol, _ = ref.attention_bound(F32, False, hd, n, out, l, big, mean)
+        assert (np.abs(got - out) <= tol).all(), size
+
+
 def test_pages_past_four_gigabytes(hip):
     """Rows written, read and attended to in the last pages of pools of more than 2^32 bytes."""
     from sapphire_amd.device import DeviceArray
