@@ -546,6 +546,64 @@ def test_streams(hip):
     assert L.sapphire_stream_synchronize(s) == 0 and L.sapphire_stream_destroy(s) == 0
 
 
+def test_two_streams_at_once(hip):
+    """Calls on two streams, each with its own workspace and outputs, over one cache: the bits of calls one after the other."""
+    from sapphire_amd import load
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    L = load()
+    rng = np.random.default_rng(14)
+    hd, ps, heads, lens = 128, 32, 4, [1500, 700, 90]
+    table, pages = tables(rng, lens, ps)
+    c = Cache(Q8_0, 1, pages, ps, 1, hd)
+    for s, n in enumerate(lens):
+        c.fill(0, table, s, rng.normal(size=(n, 1, hd)).astype(np.float32), rng.normal(size=(n, 1, hd)).astype(np.float32))
+    c.upload()
+    dt, dl = dev(table), dev(np.array(lens, np.int32))
+    streams = [L.sapphire_stream_create() for _ in range(2)]
+    qs = [device_rows(rng.normal(size=(3, heads, hd)).astype(np.float32), F32) for _ in range(20)]
+    ws = [DeviceArray(c.c.attention_workspace_bytes(3, heads, 1500)) for _ in range(2)]
+    outs = [[device_rows(np.zeros((3, heads, hd), np.float32), F32) for _ in qs] for _ in range(2)]
+    for side in range(2):
+        for i, q in enumerate(qs):
+            c.c.attention(0, q[0], outs[side][i][0], PageTable(dt, *table.shape), dl, 1500, 0.1, workspace=ws[i % 2 if side else 0],
+                          stream=streams[i % 2] if side else None)
+        sync()
+    for a, b in zip(*outs):
+        np.testing.assert_array_equal(a[1].numpy(), b[1].numpy())
+    for s in streams:
+        L.sapphire_stream_destroy(s)
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=ref.NAME.get)
+def test_write_to_one_place_twice(hip, cache):
+    """Which of two rows for one place is kept is open; every other byte is as it should be."""
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(15)
+    hd, ps, t = 128, 16, 40
+    c = Cache(cache, 1, 3, ps, 2, hd)
+    pos = np.arange(t, dtype=np.int32)
+    pos[[7, 21]] = 30
+    x = {w: rng.normal(size=(t, 2, hd)).astype(np.float32) for w in "kv"}
+    rk, rv = device_rows(x["k"], F32), device_rows(x["v"], F32)
+    dt, ds = dev(np.array([[2, 0, 1]], np.int32)), dev(np.zeros(t, np.int32))
+    c.c.write(0, rk[0], rv[0], PageTable(dt, 1, 3), dev(pos), seqs=ds)
+    sync()
+    for w in "kv":
+        got, spare = c.on[w].numpy(), ref.Pool(w, cache, 1, 3, ps, 2, hd)
+        for p, page in ((q, [2, 0, 1][q // ps]) for q in range(3 * ps)):
+            rows = np.flatnonzero(pos == p)
+            if p == 30:                        # taken over as it is: what remains to be compared is the rest
+                at, _ = spare._at(p % ps)
+                for h in range(2):
+                    a = np.unique(np.concatenate([np.ravel(at[:, None] + np.arange({F32: 4, BF16: 2, F16: 2}.get(cache, 1))),
+                                                  np.ravel(spare._scale_at(p % ps)[:, None] + np.arange(4)) if cache in (Q8_0, Q4_0) else at[:0]]))
+                    c.pool[w].a[0, page, h, a] = got[0, page, h, a]
+            elif len(rows):
+                c.pool[w].put(0, page, p % ps, x[w][rows[0]])
+        np.testing.assert_array_equal(got, c.pool[w].a, err_msg=w)
+
+
 def test_results_do_not_depend_on_the_batch(hip):
     """A sequence's bits beside others equal its bits in another place with other neighbours (same max_length and batch)."""
     from sapphire_amd.device import DeviceArray
