@@ -87,12 +87,13 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * scores are all -inf or whose pages do not exist. A NaN or +inf score makes the head's outputs NaN.
  * What lies behind a sequence's last position, NaN included, does not count. Over a quantized cache a
  * NaN or an infinity in q makes its head's outputs NaN. (Weights reach 2^8 before they are scaled:
- * values of V above 2^119 can overflow the sums.)
+ * values of V above 2^119 can overflow the sums; over a quantized cache so can K above 2^86.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the
- * same type or a quantized one. out is rounded once, at the end; with 16-bit rows the weights exp(s_p -
- * max s) meet V with 16 bits or more. lse: [tokens][n_heads] fp32, or NULL. Long sequences are cut into pieces that
- * run side by side and are joined by a second launch; the results do not depend on which workgroup
- * runs when, nor on what the other sequences hold.
+ * same type or a quantized one. out is q itself (same data and strides) or shares no element with it.
+ * out is rounded once, at the end; with 16-bit rows the weights exp(s_p - max s) meet V with 16 bits
+ * or more. lse: [tokens][n_heads] fp32, or NULL. Long sequences are cut into pieces that run side by
+ * side and are joined by a second launch; the results do not depend on which workgroup runs when, nor
+ * on what the other sequences hold.
  * workspace: sapphire_paged_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is
  * 0); calls that share one must be ordered on one stream. */
 typedef struct {

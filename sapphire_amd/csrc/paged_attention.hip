@@ -150,9 +150,6 @@ struct Raw {
     }
 };
 
-__device__ __forceinline__ float load1(int dtype, const uint8_t *p, int64_t i) {
-    return dtype == DT_F32 ? reinterpret_cast<const float *>(p)[i] : from_16(dtype, reinterpret_cast<const uint16_t *>(p)[i]);
-}
 template <int N>
 __device__ __forceinline__ void load_some(int dtype, const uint8_t *p, int64_t i, float (&x)[N]) {
     if (dtype == DT_F32) {

@@ -546,6 +546,29 @@ def test_streams(hip):
     assert L.sapphire_stream_synchronize(s) == 0 and L.sapphire_stream_destroy(s) == 0
 
 
+@pytest.mark.parametrize("cache,io,heads", [(F32, F32, 4), (F32, F32, 20), (F16, F16, 3), (Q8_0, BF16, 12)], ids=["few", "f32", "f16", "q8_0"])
+@pytest.mark.parametrize("lens", [[40, 3], [3000, 200]], ids=["one", "pieces"])
+def test_attention_in_place(hip, cache, io, heads, lens):
+    """out is q itself: the bits of the call with an out of its own."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(16)
+    hd, ps = 64, 16
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    for s, n in enumerate(lens):
+        c.fill(0, table, s, rng.normal(size=(n, 1, hd)).astype(np.float32), rng.normal(size=(n, 1, hd)).astype(np.float32))
+    c.upload()
+    q = device_rows(rng.normal(size=(2, heads, hd)).astype(np.float32), io)
+    out = device_rows(np.zeros((2, heads, hd), np.float32), io)
+    dt, dl = dev(table), dev(np.array(lens, np.int32))
+    ws = DeviceArray(max(16, c.c.attention_workspace_bytes(2, heads, max(lens))))
+    for o in (out, q):
+        c.c.attention(0, q[0], o[0], PageTable(dt, *table.shape), dl, max(lens), 0.2, workspace=ws)
+    sync()
+    np.testing.assert_array_equal(out[1].numpy(), q[1].numpy())
+
+
 def test_two_streams_at_once(hip):
     """Calls on two streams, each with its own workspace and outputs, over one cache: the bits of calls one after the other."""
     from sapphire_amd import load
