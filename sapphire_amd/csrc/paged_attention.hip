@@ -28,6 +28,7 @@ struct AttnArgs {
     PagedAttn a;
     int n_heads, group, col_tiles, piece, pieces;
     bool ordered;                          // longest sequences first
+    bool wide;                             // out's data and strides are multiples of 16 bytes
     uint32_t page_magic;                   // i / (page_size / 16) is its high product with i < 2^26 (0: page_size is 16)
     float *part;                           // [pieces][batch][n_heads][hd], unnormalised O
     float2 *ms;                            // [pieces][batch][n_heads]: maximum (log2 units), sum
@@ -168,6 +169,18 @@ __device__ __forceinline__ void store1(int dtype, uint8_t *p, int64_t i, float v
     else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)to_16(dtype, v);
 }
 
+// Four elements; `wide`: out's data and strides are multiples of 16 bytes.
+__device__ __forceinline__ void store4(int dtype, bool wide, uint8_t *p, int64_t i, pf4 x) {
+    if (!wide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store1(dtype, p, i + e, x[e]);
+    } else if (dtype == DT_F32) {
+        *reinterpret_cast<pf4 *>(p + i * 4) = x;
+    } else {
+        *reinterpret_cast<pu2 *>(p + i * 2) = pu2{pack_16(dtype, x[0], x[1]), pack_16(dtype, x[2], x[3])};
+    }
+}
+
 __device__ __forceinline__ float lse_of(float mx, float sum) { return sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2; }
 
 constexpr float kLazy = 8.0f;              // log2 units that a score may exceed the running maximum by
@@ -291,30 +304,36 @@ struct Walk {
 
 __device__ __forceinline__ float capped(float x, float cap) { return __fmul_rn(cap, tanhf(__fdiv_rn(x, cap))); }
 
-// The waves' O ([wave][head][HD + 4], unnormalised) and (maximum, sum) of each head: to out, or to the piece's part.
+// The waves' O ([wave][head][HD + 4], unnormalised) and (maximum, sum) of each head: to out, or to the piece's part. A
+// thread takes four dims.
 template <int HD, int HEADS>
 __device__ __forceinline__ void finish(const AttnArgs &g, int b, int h0, int heads, size_t slot0, const float *o,
                                        const float (&wm)[kWaves][HEADS], const float (&wsum)[kWaves][HEADS]) {
     constexpr int LD = HD + 4;
     const PagedAttn &a = g.a;
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * HD; i += kThreads) {
-        const int r = i / HD, d = i - r * HD;
-        float top = wm[0][r], tot = 0.f, x = 0.f;
+    for (int i = threadIdx.x; i < heads * (HD / 4); i += kThreads) {
+        const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+        float top = wm[0][r], tot = 0.f;
+        pf4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) top = fmaxf(top, wm[w][r]);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             // a wave without positions, or with scores of -inf only, has sum 0; its factor must not be NaN
             const float s = wsum[w][r], f = s == 0.f ? 0.f : __builtin_amdgcn_exp2f(wm[w][r] - top);
+            const pf4 ow = *reinterpret_cast<const pf4 *>(o + (w * HEADS + r) * LD + d);
             tot = __builtin_fmaf(s, f, tot);
-            x = __builtin_fmaf(o[(w * HEADS + r) * LD + d], f, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(ow[e], f, x[e]);
         }
         if (g.pieces == 1) {
-            store1(a.out.dtype, a.out.p, (int64_t)b * a.out.ts + (int64_t)(h0 + r) * a.out.hs + d, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = tot == 0.f ? 0.f : __fdiv_rn(x[e], tot);
+            store4(a.out.dtype, g.wide, a.out.p, (int64_t)b * a.out.ts + (int64_t)(h0 + r) * a.out.hs + d, x);
             if (a.lse && d == 0) a.lse[(size_t)b * g.n_heads + h0 + r] = lse_of(top, tot);
         } else {
-            g.part[(slot0 + r) * HD + d] = x;
+            *reinterpret_cast<pf4 *>(g.part + (slot0 + r) * HD + d) = x;
             if (d == 0) g.ms[slot0 + r] = make_float2(top, tot);
         }
     }
@@ -911,54 +930,80 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
     finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
-// grid (heads, sequences): the pieces of one head. A wave takes every fourth piece, HD / 64 dims per lane.
+// grid (heads, sequences): the pieces of one head. Every wave has all pieces' weights, one or more per lane, and adds
+// every fourth piece, HD / 64 dims per lane. All first loads start before the length is known: the slots of all pieces
+// are in the workspace.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
-    constexpr int D = HD / kWave, U = 8;               // U: loads in flight
-    __shared__ float part[kWaves][HD], ws[kWaves];
+    constexpr int D = HD / kWave, U = 8, Q = kMaxPieces / kWave;       // U: loads in flight
+    __shared__ float part[kWaves][HD];
     const PagedAttn &a = g.a;
-    const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+    const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const size_t stride = (size_t)gridDim.y * g.n_heads, slot = (size_t)b * g.n_heads + h;
+    float2 ms[Q];
+    ms[0] = g.ms[slot + min(lane, g.pieces - 1) * stride];
+    float v[U][D];
+    auto load = [&](int i0, int last) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[u][d] = g.part[(slot + min(i0 + u * kWaves, last) * stride) * HD + lane * D + d];
+    };
+    load(wid, g.pieces - 1);
     const int n = min(max(a.lengths[b], 0), a.max_length);
     const int start = a.window > 0 && n > a.window ? n - a.window : 0;
     const int used = max(1, (n - (start & ~(kPos - 1)) + g.piece - 1) / g.piece);
-    // every wave finds the maximum, then adds its own pieces
-    float top = -INFINITY;
-    for (int i = lane; i < used; i += kWave) top = fmaxf(top, g.ms[slot + i * stride].x);
+    float top = lane < used ? ms[0].x : -INFINITY;
+#pragma unroll
+    for (int q = 1; q < Q; ++q) {
+        if (q * kWave >= used) break;
+        ms[q] = g.ms[slot + min(lane + q * kWave, used - 1) * stride];
+        top = fmaxf(top, ms[q].x);
+    }
     top = lanes::wave_max(top);
-    float o[D] = {}, sum = 0.f;
-    for (int i0 = wid; i0 < used; i0 += kWaves * U) {
-        float2 ms[U];
-        float v[U][D];
+    float f[Q], tot = 0.f;
+    unsigned long long mask[Q];                        // pieces that count: an empty one has written no O
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        f[q] = 0.f;
+        mask[q] = 0;
+        if (q * kWave >= used) continue;
+        // a sum of NaN has a weight of NaN, whatever its maximum
+        const bool on = lane + q * kWave < used && ms[q].y != 0.f;
+        f[q] = !on ? 0.f : ms[q].y != ms[q].y ? ms[q].y : __builtin_amdgcn_exp2f(ms[q].x - top);
+        tot = __builtin_fmaf(on ? ms[q].y : 0.f, f[q], tot);
+        mask[q] = __ballot(on);
+    }
+    tot = lanes::wave_sum(tot);
+    float o[D] = {};
+    for (int i0 = wid; i0 < used;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const size_t at = slot + (size_t)min(i0 + u * kWaves, used - 1) * stride;
-            ms[u] = g.ms[at];
+            const int i = i0 + u * kWaves;
+            if (i >= used) break;
+            float fi = 0.f;
+            bool on = false;
 #pragma unroll
-            for (int d = 0; d < D; ++d) v[u][d] = g.part[at * HD + lane * D + d];
+            for (int q = 0; q < Q; ++q)
+                if (i / kWave == q) {
+                    fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[q]), i % kWave));
+                    on = mask[q] >> i % kWave & 1;
+                }
+            if (!on) continue;
+#pragma unroll
+            for (int d = 0; d < D; ++d) o[d] = __builtin_fmaf(fi, v[u][d], o[d]);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // an empty piece has written no O; a sum of NaN has a weight of NaN, whatever its maximum
-            if (i0 + u * kWaves >= used || ms[u].y == 0.f) continue;
-            const float f = ms[u].y != ms[u].y ? ms[u].y : __builtin_amdgcn_exp2f(ms[u].x - top);
-            sum = __builtin_fmaf(f, ms[u].y, sum);
-#pragma unroll
-            for (int d = 0; d < D; ++d) o[d] = __builtin_fmaf(f, v[u][d], o[d]);
-        }
+        i0 += kWaves * U;
+        if (i0 < used) load(i0, used - 1);
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) part[wid][lane * D + d] = o[d];
-    if (lane == 0) ws[wid] = sum;
     __syncthreads();
     const int t = threadIdx.x;
     if (t >= HD) return;
-    float x = 0.f, tot = 0.f;
+    float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        x += part[w][t];
-        tot += ws[w];
-    }
+    for (int w = 0; w < kWaves; ++w) x += part[w][t];
     store1(a.out.dtype, a.out.p, (int64_t)b * a.out.ts + (int64_t)h * a.out.hs + t, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
     if (a.lse && t == 0) a.lse[slot] = lse_of(top, tot);
 }
@@ -1003,6 +1048,7 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.col_tiles = p.col_tiles;
     g.piece = p.piece;
     g.pieces = p.pieces;
+    g.wide = rows_wide(a.out);
     g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kFullGroups;
     // ceil(2^32 / d), d <= 64: off by less than d / 2^32 relative to 1 / d, and i * d < 2^32
     const uint64_t d = a.c.page_size / kPos;
