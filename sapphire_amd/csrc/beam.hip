@@ -34,6 +34,21 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
 
+// How many of the first `n` keys of `list` (16-byte aligned, zeros up to the next multiple of eight) are larger than k.
+// All lanes read the same words, which costs the LDS one read each.
+__device__ __forceinline__ int larger_than(u64 k, const u64 *list, int n) {
+    typedef u64 two __attribute__((ext_vector_type(2)));
+    int c = 0;
+    for (int j = 0; j < n; j += 8) {
+        two o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const two *>(list + j + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += (o[i].x > k) + (o[i].y > k);
+    }
+    return c;
+}
+
 // The `w` largest keys that a wave has seen. Keys above the w-th (`last`) gather in 64 words of LDS; when they would
 // not fit, and at the end, each one's place is the number of larger ones, and the first w stay.
 struct Best {
@@ -51,9 +66,9 @@ struct Best {
         const int lane = threadIdx.x & (kWave - 1);
         handover();
         const u64 k = lane < count ? buf[lane] : 0;
-        int place = 0;
-        for (int j = 0; j < count; j += 4)             // (lanes from count on hold 0)
-            place += (u64_lane(k, j) > k) + (u64_lane(k, j + 1) > k) + (u64_lane(k, j + 2) > k) + (u64_lane(k, j + 3) > k);
+        if (lane >= count) buf[lane] = 0;
+        handover();
+        const int place = larger_than(k, buf, count);
         handover();
         if (lane < count && place < w) buf[place] = k;
         count = min(count, w);
@@ -84,10 +99,22 @@ struct Best {
     }
 };
 
+// Over the wave, the same in every lane: rows of 16 lanes, then the four rows.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const u64 u = __builtin_bit_cast(u64, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (u64)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum(double s) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-    return s;
+    s += dpp_f64<0xB1>(s);
+    s += dpp_f64<0x4E>(s);
+    s += dpp_f64<0x141>(s);
+    s += dpp_f64<0x140>(s);
+    const u64 u = __builtin_bit_cast(u64, s);
+    auto of = [&](int l) { return __builtin_bit_cast(double, u64_lane(u, l)); };
+    return (of(0) + of(16)) + (of(32) + of(48));
 }
 
 // Part of a row's normaliser: its largest logit and the sum of exp(x - max).
@@ -121,7 +148,7 @@ template <int BATCH>
 __global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__restrict__ logits, int ld, int n, int beams,
                                                              const float *__restrict__ scores, const int *__restrict__ done,
                                                              int chunk, u64 *__restrict__ keys, Norm *__restrict__ norm) {
-    __shared__ u64 lists[kWaves][kWave];
+    __shared__ __attribute__((aligned(16))) u64 lists[kWaves][kWave], all[kWave];
     __shared__ Norm part[kWaves];
     const int row = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if ((done && done[row] != 0) || !(fabsf(scores[row]) < INFINITY)) return;
@@ -169,10 +196,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__r
         mx = m;
         float floor = key_value(best.last);
         if (best.last == 0) floor = reached_by(top, beams);
-        uint64_t reach = 0;
+        uint32_t reach = 0;                                            // bit 8 g + u
 #pragma unroll
         for (int g = 0; g < BATCH; ++g) {
-            const int first = i0 + g * kWaves * kSpan, at = first + lane * 4;
+            const int first = i0 + g * kWaves * kSpan;
             if (first >= hi) continue;
             float e[kStep];
 #pragma unroll
@@ -180,15 +207,27 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__r
             sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
             if (__any(most[g] >= floor)) {
 #pragma unroll
-                for (int u = 0; u < kStep; ++u) reach |= (uint64_t)(!(v[g][u] < floor) && at + spot(u) < hi) << (g * kStep + u);
+                for (int u = 0; u < kStep; ++u) reach |= v[g][u] < floor ? 0u : 1u << (g * kStep + u);
+            }
+        }
+        if (i0 + kAll > hi) {                          // past the end: no keys
+#pragma unroll 1
+            for (int g = 0; g < BATCH; ++g) {
+                const int left = hi - (i0 + g * kWaves * kSpan + lane * 4);
+                const uint32_t one = (1u << min(max(left, 0), 4)) - 1, two = (1u << min(max(left - 4 * kWave, 0), 4)) - 1;
+                reach &= ~((~(one | two << 4) & 255u) << (g * kStep));
             }
         }
         while (__any(reach != 0)) {
-            const int bit = reach ? __builtin_ctzll(reach) : 0, at = i0 + bit / kStep * kWaves * kSpan + lane * 4 + spot(bit % kStep);
-            float mine = v[0][0];
+            const int bit = reach ? __builtin_ctz(reach) : 0, at = i0 + bit / kStep * kWaves * kSpan + lane * 4 + spot(bit % kStep);
+            float pick[BATCH * kStep];                                 // v[bit], a bit of its number at a time
 #pragma unroll
-            for (int i = 1; i < BATCH * kStep; ++i) mine = bit == i ? v[i / kStep][i % kStep] : mine;
-            best.offer(reach ? key_of(mine, (uint32_t)at) : 0);
+            for (int i = 0; i < BATCH * kStep; ++i) pick[i] = v[i / kStep][i % kStep];
+#pragma unroll
+            for (int b = 0; (1 << b) < BATCH * kStep; ++b)
+#pragma unroll
+                for (int i = 0; i < (BATCH * kStep) >> (b + 1); ++i) pick[i] = bit >> b & 1 ? pick[2 * i + 1] : pick[2 * i];
+            best.offer(reach ? key_of(pick[0], (uint32_t)at) : 0);
             reach &= reach - 1;
         }
         best.sort();
@@ -200,24 +239,23 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__r
     }
     const float wm = lanes::wave_max(mx);
     const double ws = wave_sum(mx > -INFINITY ? sum * (double)exp_of(mx, wm) : 0.0);
-    if (lane >= best.count && lane < beams) lists[wid][lane] = 0;
+    // the waves' lists one behind the other, zeros where there are fewer and up to a multiple of eight
+    if (lane < beams) all[wid * beams + lane] = lane < best.count ? lists[wid][lane] : 0;
+    if (wid == kWaves - 1 && kWaves * beams + lane < (kWaves * beams + 7) / 8 * 8) all[kWaves * beams + lane] = 0;
     if (lane == 0) part[wid] = Norm{ws, wm};
     __syncthreads();
     if (wid != 0) return;
-    // of the waves' lists, a key per lane, the first `beams` (0 where there are fewer)
-    const u64 k = lane < kWaves * beams ? lists[lane / beams][lane % beams] : 0;
-    int place = 0;
-    for (int j = 0; j < kWaves * beams; j += 4)        // (lanes from there on hold 0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u64 other = u64_lane(k, j + i);
-            place += other > k || (other == k && j + i < lane);
-        }
-    if (lane < kWaves * beams && place < beams) keys[((size_t)row * beams + place) * gridDim.x + blockIdx.x] = k;
+    const u64 k = lane < kWaves * beams ? all[lane] : 0;
+    const int place = larger_than(k, all, kWaves * beams), held = __popcll(__ballot(k != 0));
+    u64 *out = keys + (size_t)row * beams * gridDim.x + blockIdx.x;
+    if (k != 0 && place < beams) out[(size_t)place * gridDim.x] = k;
+    if (lane >= held && lane < beams) out[(size_t)lane * gridDim.x] = 0;
     if (lane == 0) {
         float m = -INFINITY;
         double s = 0.0;
+#pragma unroll
         for (int w = 0; w < kWaves; ++w) m = fmaxf(m, part[w].max);
+#pragma unroll
         for (int w = 0; w < kWaves; ++w)
             if (part[w].max > -INFINITY) s += part[w].sum * (double)exp_of(part[w].max, m);
         norm[(size_t)row * gridDim.x + blockIdx.x] = Norm{s, m};
@@ -231,7 +269,7 @@ __global__ __launch_bounds__(kMaxBeams *kWave) void beam_pick_kernel(int n, int 
                                                                      const Norm *__restrict__ norm, float *scores_out,
                                                                      int *__restrict__ tokens, int *__restrict__ parents,
                                                                      int *done_out) {
-    __shared__ u64 lists[kMaxBeams][kWave];
+    __shared__ __attribute__((aligned(16))) u64 lists[kMaxBeams][kWave];
     __shared__ double score[kMaxBeams * kMaxBeams];
     __shared__ int token[kMaxBeams * kMaxBeams], ended[kMaxBeams];
     const int r0 = blockIdx.x * beams, lane = threadIdx.x & (kWave - 1), b = threadIdx.x / kWave, row = r0 + b;
