@@ -206,8 +206,10 @@ __global__ __launch_bounds__(kThreads, 4) void beam_rows_kernel(const float *__r
             for (int u = 0; u < kStep; ++u) e[u] = exp_of(v[g][u], from);
             sum += (double)(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
             if (__any(most[g] >= floor)) {
+                uint32_t byte = 0;
 #pragma unroll
-                for (int u = 0; u < kStep; ++u) reach |= v[g][u] < floor ? 0u : 1u << (g * kStep + u);
+                for (int u = 0; u < kStep; ++u) byte |= v[g][u] < floor ? 0u : 1u << u;
+                reach |= byte << (g * kStep);
             }
         }
         if (i0 + kAll > hi) {                          // past the end: no keys
