@@ -106,6 +106,7 @@ bool cache_ok(const sapphire_paged_cache_t *c, int layer, PagedCache &o) {
     o.page_size = c->page_size;
     o.nkv = c->n_kv_heads;
     o.hd = c->head_dim;
+    set_page_division(o);
     o.tile_bytes = (uint32_t)(c->page_size * row_bytes(c->dtype, c->head_dim));
     o.layer_bytes = (size_t)c->pages * c->n_kv_heads * o.tile_bytes;
     const size_t at = layer > 0 ? (size_t)layer * o.layer_bytes : 0;

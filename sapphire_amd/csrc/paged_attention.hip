@@ -29,7 +29,6 @@ struct AttnArgs {
     int n_heads, group, col_tiles, piece, pieces;
     bool ordered;                          // longest sequences first
     bool wide;                             // out's data and strides are multiples of 16 bytes
-    uint32_t page_magic;                   // i / (page_size / 16) is its high product with i < 2^26 (0: page_size is 16)
     float *part;                           // [pieces][batch][n_heads][hd], unnormalised O
     float2 *ms;                            // [pieces][batch][n_heads]: maximum (log2 units), sum
 };
@@ -287,7 +286,7 @@ struct Walk {
     __device__ __forceinline__ void seek(const AttnArgs &g, int t) {
 #pragma unroll
         for (int u = 0; u < HALVES; ++u) {
-            const uint32_t t16 = (uint32_t)min(t + u * kPos, last) / kPos, i = g.page_magic ? __umulhi(t16, g.page_magic) : t16;
+            const uint32_t t16 = (uint32_t)min(t + u * kPos, last) / kPos, i = page_of(g.a.c, t16);
             off[u] = t16 * kPos - i * (uint32_t)ps;
             const int page = row[__builtin_amdgcn_readfirstlane((int)i)];
             there[u] = page >= 0 && page < g.a.c.pages;
@@ -1050,9 +1049,6 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.pieces = p.pieces;
     g.wide = rows_wide(a.out);
     g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kFullGroups;
-    // ceil(2^32 / d), d <= 64: off by less than d / 2^32 relative to 1 / d, and i * d < 2^32
-    const uint64_t d = a.c.page_size / kPos;
-    g.page_magic = d == 1 ? 0 : (uint32_t)(((1ull << 32) + d - 1) / d);
     g.part = reinterpret_cast<float *>(a.ws);
     g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);

@@ -15,6 +15,7 @@ struct PagedCache {
     uint8_t *k = nullptr, *v = nullptr;    // the layer's pools (all layers' for the reorder)
     int dtype = 0, layers = 0, pages = 0, page_size = 0, nkv = 0, hd = 0;
     uint32_t tile_bytes = 0;               // one page of one head
+    uint32_t page_mul = 0, page_shift = 0; // see page_of
     size_t layer_bytes = 0;
 };
 struct Rows {
@@ -55,20 +56,33 @@ struct Tile {
     static constexpr uint32_t bytes(int ps) { return (uint32_t)ps * (ROW + (kQuant ? NB * 4 : 0)); }
 };
 
-// Where token t goes: its page and position in it, or false.
-__device__ __forceinline__ bool paged_place(const PagedCache &c, const PageTable &tab, const int *__restrict__ seqs,
-                                            const int *__restrict__ positions, int t, int &page, int &off) {
-    const int row = seqs ? seqs[t] : t, pos = positions[t];
+// The page of a row that 16 positions belong to, t16 / d with d = page_size / 16 (at most 64) and t16 < 2^27: a power of two
+// by a shift, others by the high product with ceil(2^33 / d) < 2^32, which is off by less than 2^6 / 2^33 relative to 1 / d:
+// t16 times that is less than 1 / d.
+inline void set_page_division(PagedCache &c) {
+    const uint32_t d = (uint32_t)c.page_size / 16;
+    if ((d & (d - 1)) == 0) {
+        c.page_mul = 0;
+        c.page_shift = (uint32_t)__builtin_ctz(d);
+    } else {
+        c.page_mul = (uint32_t)((((uint64_t)1 << 33) + d - 1) / d);
+        c.page_shift = 1;
+    }
+}
+__device__ __forceinline__ uint32_t page_of(const PagedCache &c, uint32_t t16) {
+    return (c.page_mul ? __umulhi(t16, c.page_mul) : t16) >> c.page_shift;
+}
+
+// Where position pos of a table row lies: its page and the position in it, or false.
+__device__ __forceinline__ bool paged_place(const PagedCache &c, const PageTable &tab, int row, int pos, int &page, int &off) {
     if (row < 0 || row >= tab.rows || pos < 0) return false;
-    const uint32_t i = (uint32_t)pos / (uint32_t)c.page_size;
+    const uint32_t i = page_of(c, (uint32_t)pos >> 4);
     if (i >= (uint32_t)tab.ld) return false;
     page = tab.pages[(size_t)row * tab.ld + i];
-    off = pos - (int)i * c.page_size;
+    off = pos - (int)(i * (uint32_t)c.page_size);
     return page >= 0 && page < c.pages;
 }
 
-// Eight consecutive elements of a row as fp32, and back (rounded to nearest even). `wide`: the rows'
-// data and strides are multiples of 16 bytes.
 typedef float pf4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu4 __attribute__((ext_vector_type(4)));
 typedef uint32_t pu2 __attribute__((ext_vector_type(2)));
@@ -92,36 +106,47 @@ __device__ __forceinline__ uint32_t pack_16(int dtype, float a, float b) {
 }
 __device__ __forceinline__ float from_16(int dtype, uint32_t b) { return dtype == DT_BF16 ? from_bf16(b) : from_f16(b); }
 
-__device__ __forceinline__ void load8(int dtype, bool wide, const uint8_t *base, int64_t at, float (&x)[8]) {
+// Eight consecutive elements of a row as they are, and as fp32. `wide`: the rows' data and strides are multiples of 16
+// bytes. (Loading and converting are apart, so that several rows' loads are under way together.)
+struct Raw8 {
+    pu4 a, b;                              // b: fp32's second half
+};
+__device__ __forceinline__ void load8(int dtype, bool wide, const uint8_t *base, int64_t at, Raw8 &r) {
     if (dtype == DT_F32) {
-        const float *p = reinterpret_cast<const float *>(base) + at;
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(base) + at;
         if (wide) {
-            const pf4 a = *reinterpret_cast<const pf4 *>(p), b = *reinterpret_cast<const pf4 *>(p + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = a[i];
-                x[4 + i] = b[i];
-            }
+            r.a = *reinterpret_cast<const pu4 *>(p);
+            r.b = *reinterpret_cast<const pu4 *>(p + 4);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p[i];
+            for (int i = 0; i < 4; ++i) {
+                r.a[i] = p[i];
+                r.b[i] = p[4 + i];
+            }
         }
     } else {
         const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + at;
-        uint32_t w[8];
         if (wide) {
-            const pu4 a = *reinterpret_cast<const pu4 *>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[2 * i] = a[i] & 0xffffu;
-                w[2 * i + 1] = a[i] >> 16;
-            }
+            r.a = *reinterpret_cast<const pu4 *>(p);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = p[i];
+            for (int i = 0; i < 4; ++i) r.a[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
         }
+    }
+}
+__device__ __forceinline__ void values8(int dtype, const Raw8 &r, float (&x)[8]) {
+    if (dtype == DT_F32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = from_16(dtype, w[i]);
+        for (int i = 0; i < 4; ++i) {
+            x[i] = __uint_as_float(r.a[i]);
+            x[4 + i] = __uint_as_float(r.b[i]);
+        }
+    } else if (dtype == DT_BF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i & 1 ? r.a[i / 2] & 0xffff0000u : r.a[i / 2] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = from_f16(i & 1 ? r.a[i / 2] >> 16 : r.a[i / 2] & 0xffffu);
     }
 }
 
@@ -138,8 +163,13 @@ __device__ __forceinline__ void store8(int dtype, bool wide, uint8_t *base, int6
     } else {
         uint16_t *p = reinterpret_cast<uint16_t *>(base) + at;
         pu4 w;
+        if (dtype == DT_BF16) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack_16(dtype, x[2 * i], x[2 * i + 1]);
+            for (int i = 0; i < 4; ++i) w[i] = pack_16(DT_BF16, x[2 * i], x[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_16(DT_F16, x[2 * i], x[2 * i + 1]);
+        }
         if (wide) {
             *reinterpret_cast<pu4 *>(p) = w;
         } else {

@@ -96,8 +96,10 @@ __device__ __forceinline__ float quantize8(const float (&x)[8], int lq, int (&q)
     return d;
 }
 
+// The four low bytes.
 __device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)(d & 255) << 24;
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x0c0c0400u), lo, 0x05040100u);
 }
 
 // Dims d .. d + 7 of position p into a tile (V: the V tile). The four lanes of a quad hold one block.
@@ -251,13 +253,17 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedCache c, Row
                                                                const int *__restrict__ positions, bool kw, bool vw) {
     const Unit u = unit_of<HD>(c.nkv);
     if (u.t >= k.tokens) return;
-    float x[8], y[8];
-    load8(k.dtype, kw, k.p, (int64_t)u.t * k.ts + (int64_t)u.h * k.hs + u.d, x);
-    load8(v.dtype, vw, v.p, (int64_t)u.t * v.ts + (int64_t)u.h * v.hs + u.d, y);
+    const int row = seqs ? seqs[u.t] : u.t, pos = positions[u.t];
+    Raw8 rk, rv;
+    load8(k.dtype, kw, k.p, (int64_t)u.t * k.ts + (int64_t)u.h * k.hs + u.d, rk);
+    load8(v.dtype, vw, v.p, (int64_t)u.t * v.ts + (int64_t)u.h * v.hs + u.d, rv);
     int page, off;
-    if (!paged_place(c, tab, seqs, positions, u.t, page, off)) return;
+    if (!paged_place(c, tab, row, pos, page, off)) return;
     const size_t at = ((size_t)page * c.nkv + u.h) * c.tile_bytes;
+    float x[8], y[8];
+    values8(k.dtype, rk, x);
     store_codes<CT, HD, false>(c.k + at, c.page_size, off, u.d, x);
+    values8(v.dtype, rv, y);
     store_codes<CT, HD, true>(c.v + at, c.page_size, off, u.d, y);
 }
 
@@ -268,7 +274,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(PagedCache c, Rows
     const Unit u = unit_of<HD>(c.nkv);
     if (u.t >= k.tokens) return;
     int page, off;
-    const bool there = paged_place(c, tab, seqs, positions, u.t, page, off);
+    const bool there = paged_place(c, tab, seqs ? seqs[u.t] : u.t, positions[u.t], page, off);
     float x[8] = {}, y[8] = {};
     if (there) {
         const size_t at = ((size_t)page * c.nkv + u.h) * c.tile_bytes;
