@@ -82,17 +82,10 @@ __device__ __forceinline__ void turn(float &a, float &b, float2 cs) {
 template <int DT, bool PAIRS, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a) {
     using P = Piece<DT, WIDE>;
+    constexpr bool ONE = PAIRS && WIDE;    // a piece holds both of a pair
+    constexpr int U = 2;                   // pieces (or pairs of them) of a thread on their way together
     __shared__ float2 cs[kAngles];
     const int half = a.rot / 2, t0 = blockIdx.x * a.tok, nt = min(a.tok, a.x.tokens - t0);
-    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
-        const int t = i / half, p = i - t * half;
-        const double turns = (double)a.positions[t0 + t] * a.freqs[p] * 0.15915494309189533577;
-        const float th = (float)((turns - __builtin_rint(turns)) * 6.2831853071795864769);
-        float s, c;
-        sincosf(th, &s, &c);
-        cs[i] = make_float2(__fmul_rn(c, a.magnitude), __fmul_rn(s, a.magnitude));
-    }
-    __syncthreads();
     const int h0 = blockIdx.y * a.heads, nh = min(a.heads, a.x.heads - h0);
     const bool same = a.x.p == a.y.p;      // the remaining dims are there already
     // units of a head: its turning pieces, then the copied ones. A thread keeps its unit and steps over the heads and
@@ -100,36 +93,38 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a) {
     const int turning = PAIRS ? (WIDE ? a.rot / P::N : half) : half / P::N;
     const int units = turning + (same ? 0 : (a.x.hd - a.rot) / P::N), across = max(1, kThreads / units);
     const int row = threadIdx.x / units;
-    for (int u = threadIdx.x - row * units; row < across && u < units; u += kThreads) {
-        int t = 0, h = row;
+    int unit = row < across ? (int)threadIdx.x - row * units : units, t, h;
+    int64_t xi, yi;
+    P p[U], q[ONE ? 1 : U];
+    int of[U];                             // a piece's token, nt where there is none
+    int64_t at[U];
+    // a unit's first and second dims, and of a pair's second one
+    auto dims = [&](int &d0, int &d1) {
+        const int d = unit * P::N;
+        d0 = unit >= turning ? a.rot + (unit - turning) * P::N : ONE || !PAIRS ? d : 2 * d;
+        d1 = PAIRS ? 2 * d + 1 : d + half;
+    };
+    auto start = [&]() {
+        t = 0;
+        h = row;
         while (h >= nh) {
             h -= nh;
             ++t;
         }
-        int64_t xi = (int64_t)(t0 + t) * a.x.ts + (int64_t)(h0 + h) * a.x.hs;
-        int64_t yi = (int64_t)(t0 + t) * a.y.ts + (int64_t)(h0 + h) * a.y.hs;
-        while (t < nt) {
-            const float2 *w = cs + t * half;
-            P p, q;
-            if (u >= turning) {
-                const int d = a.rot + (u - turning) * P::N;
-                p.load(a.x.p, xi + d);
-                p.store(a.y.p, yi + d);
-            } else if constexpr (PAIRS && WIDE) {
-                const int d = u * P::N;
-                p.load(a.x.p, xi + d);
+        xi = (int64_t)(t0 + t) * a.x.ts + (int64_t)(h0 + h) * a.x.hs;
+        yi = (int64_t)(t0 + t) * a.y.ts + (int64_t)(h0 + h) * a.y.hs;
+    };
+    auto fetch = [&]() {
+        int d0, d1;
+        dims(d0, d1);
 #pragma unroll
-                for (int e = 0; e < P::N / 2; ++e) turn(p.v[2 * e], p.v[2 * e + 1], w[d / 2 + e]);
-                p.store(a.y.p, yi + d);
-            } else {
-                const int d = u * P::N, d0 = PAIRS ? 2 * d : d, d1 = PAIRS ? 2 * d + 1 : d + half;
-                p.load(a.x.p, xi + d0);
-                q.load(a.x.p, xi + d1);
-#pragma unroll
-                for (int e = 0; e < P::N; ++e) turn(p.v[e], q.v[e], w[d + e]);
-                p.store(a.y.p, yi + d0);
-                q.store(a.y.p, yi + d1);
-            }
+        for (int i = 0; i < U; ++i) {
+            of[i] = min(t, nt);
+            at[i] = yi;
+            if (t >= nt) continue;
+            p[i].load(a.x.p, xi + d0);
+            if constexpr (!ONE)
+                if (unit < turning) q[i].load(a.x.p, xi + d1);
             h += across;
             xi += across * a.x.hs;
             yi += across * a.y.hs;
@@ -140,6 +135,44 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(RopeArgs a) {
                 yi += a.y.ts - nh * a.y.hs;
             }
         }
+    };
+    if (unit < units) {
+        start();
+        fetch();
+    }
+    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
+        const int k = i / half, j = i - k * half;
+        const double turns = (double)a.positions[t0 + k] * a.freqs[j] * 0.15915494309189533577;
+        const float th = (float)((turns - __builtin_rint(turns)) * 6.2831853071795864769);
+        float s, c;
+        sincosf(th, &s, &c);
+        cs[i] = make_float2(__fmul_rn(c, a.magnitude), __fmul_rn(s, a.magnitude));
+    }
+    __syncthreads();
+    while (unit < units) {
+        int d0, d1;
+        dims(d0, d1);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (of[i] >= nt) continue;
+            const float2 *w = cs + of[i] * half;
+            if (unit < turning) {
+                if constexpr (ONE) {
+#pragma unroll
+                    for (int e = 0; e < P::N / 2; ++e) turn(p[i].v[2 * e], p[i].v[2 * e + 1], w[d0 / 2 + e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < P::N; ++e) turn(p[i].v[e], q[i].v[e], w[unit * P::N + e]);
+                    q[i].store(a.y.p, at[i] + d1);
+                }
+            }
+            p[i].store(a.y.p, at[i] + d0);
+        }
+        if (t >= nt) {                     // the next unit, of heads of more than kThreads
+            unit += kThreads;
+            if (unit < units) start();
+        }
+        if (unit < units) fetch();
     }
 }
 
@@ -150,10 +183,10 @@ int launch_rope_rows(const Rows &x, const Rows &y, const int *positions, const d
     RopeArgs a{x, y, positions, freqs, rot, 1, x.heads, magnitude};
     const int vec = x.dtype == DT_F32 ? 4 : 8;
     const bool wide = rows_wide(x) && rows_wide(y) && x.hd % vec == 0 && (interleaved ? rot : rot / 2) % vec == 0;
-    // About four workgroups per CU where the rows suffice, of one to eight 16-byte pieces per thread
+    // About four workgroups per CU where the rows suffice, of one to sixteen 16-byte pieces per thread
     // (single elements: as many as the threads take in turn): several tokens, or some heads of one.
     const int64_t units = std::max(1, x.hd / (wide ? 2 * vec : 2)), all = (int64_t)x.tokens * x.heads * units;
-    const int64_t want = std::min<int64_t>(8 * kThreads, std::max<int64_t>(kThreads, all / 1024));
+    const int64_t want = std::min<int64_t>(16 * kThreads, std::max<int64_t>(kThreads, all / 1024));
     if (x.heads * units >= want) {
         a.heads = (int)std::max<int64_t>(1, want / units);
     } else {
