@@ -350,7 +350,8 @@ __device__ __forceinline__ void load_q(const Rows &q, int b, int h0, int heads, 
 // fp32 rows over a float cache, at most four query heads of a K/V head. v_mfma_f32_4x4x1_16b_f32 is sixteen products of
 // four rows and four columns: block (m, c / 4) multiplies the positions 4 (c / 4) .. + 3 of dim chunk m with the heads,
 // and for the weighted sum the dims of lanes 4 (c / 4) .. + 3 at position 4m + r. Every column is used, where
-// 16x16x4 would leave twelve of sixteen idle: a quarter of its cycles.
+// 16x16x4 would leave twelve of sixteen idle: a quarter of its cycles. (Eight heads as two sets of four gained 1 to 4 %
+// over 16x16x4: not kept.)
 template <int CT, int HD>
 __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_few_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
@@ -382,6 +383,16 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     // scores in log2 units: without a cap in one product
     const float cap = a.softcap, sl2 = cap > 0.f ? a.scale : __fmul_rn(a.scale, kLog2e);
     float mx = -INFINITY, sum = 0.f;                   // sum: this lane's positions only
+    // A swap puts two words' lower halves (rows of 16 lanes: even rows) into one and their upper halves into the other:
+    // both words' sums over two m, each left in its half of the lanes.
+    auto halves = [](float x, float y) {
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        return __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    };
+    auto rows = [](float x, float y) {
+        const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+        return __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    };
     for (; tb < at.hi; tb += STEP) {
         const bool all = at.whole(tb), here = at.there[0];
         pf4 st[4] = {};
@@ -396,32 +407,22 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
             }
         at.seek(g, tb + STEP);
         k.load_k(a.c.k + at.at[0], at.ps, at.off[0], c, m);
-        // the four chunks' sums, then positions 4 (c / 4) + r of head c % 4
+        // the four chunks' sums: lane (c, m) is left with position 4 (c / 4) + m of head c % 4
         const pf4 s4 = (st[0] + st[1]) + (st[2] + st[3]);
-        float p[4], ref;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float x = s4[r];
-            x += __shfl_xor(x, 16, kWave);
-            x += __shfl_xor(x, 32, kWave);
-            p[r] = __fmul_rn(x, sl2);
-            if (cap > 0.f) p[r] = __fmul_rn(capped(p[r], cap), kLog2e);
-        }
+        float p = __fmul_rn(rows(halves(s4[0], s4[2]), halves(s4[1], s4[3])), sl2);
+        if (cap > 0.f) p = __fmul_rn(capped(p, cap), kLog2e);
         if (!all) {                                    // a piece's end, or a page that does not exist
             // [from, to): what counts of the tile
-            const int from = here ? at.start - tb : kPos, to = at.hi - tb;
+            const int from = here ? at.start - tb : kPos, to = at.hi - tb, pos = (c >> 2) * 4 + m;
+            p = pos >= from && pos < to ? p : -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = (c >> 2) * 4 + r, tv = 4 * m + r;
-                p[r] = t >= from && t < to ? p[r] : -INFINITY;
-                v.keep_v(r, tv >= from && tv < to);    // its weight is 0, and 0 times a NaN there would be NaN
-            }
+            for (int r = 0; r < 4; ++r) v.keep_v(r, 4 * m + r >= from && 4 * m + r < to);      // its weight is 0, and 0 times a NaN there would be NaN
         }
-        ref = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
         // The maximum moves, with O and the sums, only for a score far above it: weights up to 2^kLazy do no harm.
-        if (__any(ref > mx + kLazy)) {
-            ref = fmaxf(ref, __shfl_xor(ref, 4, kWave));
-            ref = fmaxf(ref, __shfl_xor(ref, 8, kWave));
+        if (__any(p > mx + kLazy)) {
+            float ref = p;
+#pragma unroll
+            for (int off = 4; off < kWave; off *= 2) ref = fmaxf(ref, __shfl_xor(ref, off, kWave));
             const float mn = fmaxf(mx, ref), f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mn);
             mx = mn;
             sum = __fmul_rn(sum, f);
@@ -429,42 +430,32 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
             for (int x = 0; x < DPL; ++x) o[x] *= f;
         }
         const float from = mx == -INFINITY ? 0.f : mx; // nothing above -inf yet: all weights 0
+        p = __builtin_amdgcn_exp2f(p - from);
+        sum = __fadd_rn(sum, p);
+        float w[4];                                    // of position 4m + r
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(p[r] - from);
-            sum = __fadd_rn(sum, p[r]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = __shfl(p[r], (m << 2) | (c & 3), kWave);     // of position 4m + r
+        for (int r = 0; r < 4; ++r) w[r] = __shfl(p, (r << 4) | (m << 2) | (c & 3), kWave);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int x = 0; x < DPL; ++x) o[x] = __builtin_amdgcn_mfma_f32_4x4x1f32(v.v_at(r, x), p[r], o[x], 0, 0, 0);
+            for (int x = 0; x < DPL; ++x) o[x] = __builtin_amdgcn_mfma_f32_4x4x1f32(v.v_at(r, x), w[r], o[x], 0, 0, 0);
         v.load_v(a.c.v + at.at[0], at.ps, at.off[0], c, m);
     }
-    sum += __shfl_xor(sum, 4, kWave);
-    sum += __shfl_xor(sum, 8, kWave);
+#pragma unroll
+    for (int off = 4; off < kWave; off *= 2) sum += __shfl_xor(sum, off, kWave);
     if (lane < HEADS) {
         wm[wid][lane] = mx;
         wsum[wid][lane] = sum;
     }
-    // The sums over m, each lane left with a quarter of the dims: x = m * DPL / 4 and on. A swap puts two words'
-    // lower halves (rows of 16 lanes: even rows) into one and their upper halves into the other.
+    // O's sums over m, each lane left with a quarter of the dims: x = m * DPL / 4 and on
     constexpr int H = DPL / 2, Q = DPL / 4;
 #pragma unroll
-    for (int x = 0; x < H; ++x)
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[x][i]), __float_as_uint(o[x + H][i]), false, false);
-            o[x][i] = __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
-        }
+        for (int x = 0; x < H; ++x) o[x][i] = halves(o[x][i], o[x + H][i]);
 #pragma unroll
-    for (int x = 0; x < Q; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[x][i]), __float_as_uint(o[x + Q][i]), false, false);
-            o[x][i] = __fadd_rn(__uint_as_float(w[0]), __uint_as_float(w[1]));
-        }
+        for (int x = 0; x < Q; ++x) o[x][i] = rows(o[x][i], o[x + Q][i]);
+    }
     __syncthreads();                                   // every wave is past its reads of q
 #pragma unroll
     for (int x = 0; x < Q; ++x)
@@ -1052,13 +1043,14 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.part = reinterpret_cast<float *>(a.ws);
     g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);
-    const bool short_terms = a.q.dtype == DT_BF16, few = p.col_heads == 4;
-#define SPH_FLOAT(CT, HD, HALF) \
-    if (a.c.dtype == CT && a.c.hd == HD && half == HALF && !few) hipLaunchKernelGGL((paged_attn_kernel<CT, HD, HALF>), grid, block, 0, s, g);
+    const bool short_terms = a.q.dtype == DT_BF16;
+#define SPH_FLOAT(CT, HD, HALF)                                                                    \
+    if (a.c.dtype == CT && a.c.hd == HD && half == HALF && p.col_heads == kCols)                  \
+        hipLaunchKernelGGL((paged_attn_kernel<CT, HD, HALF>), grid, block, 0, s, g);
 #define SPH_FEW(CT, HD) \
-    if (a.c.dtype == CT && a.c.hd == HD && few) hipLaunchKernelGGL((paged_attn_few_kernel<CT, HD>), grid, block, 0, s, g);
+    if (a.c.dtype == CT && a.c.hd == HD && p.col_heads == 4) hipLaunchKernelGGL((paged_attn_few_kernel<CT, HD>), grid, block, 0, s, g);
 #define SPH_DIGITS(CT, HD, NT, TERMS)                                                             \
-    if (a.c.dtype == CT && a.c.hd == HD && few == (NT == 1) && short_terms == (TERMS == 2))       \
+    if (a.c.dtype == CT && a.c.hd == HD && p.col_heads == 4 * NT && short_terms == (TERMS == 2))  \
         hipLaunchKernelGGL((paged_attn_digits_kernel<CT, HD, NT, TERMS>), grid, block, 0, s, g);
 #define SPH_QUANT(CT, HD) SPH_DIGITS(CT, HD, 1, 2) SPH_DIGITS(CT, HD, 1, 3) SPH_DIGITS(CT, HD, 2, 2) SPH_DIGITS(CT, HD, 2, 3)
 #define SPH_ATTN_HD(HD)                                                                           \
