@@ -1,8 +1,13 @@
 // beam.hip - beam search's selection: one pass over the logits, then one workgroup per request.
 //
 // Within a row the order of the scores is the order of the logits, so the pass needs no normaliser: each
-// wave keeps its best W (logit, index) keys, and beside that it sums exp. The rows' lists and normalisers meet in the second launch, where
-// the scores of the W x W candidates left are formed and compared in 64 bits.
+// wave keeps its best W (logit, index) keys, and beside that it sums exp. The rows' lists and normalisers
+// meet in the second launch, where the scores of the W x W candidates left are formed and compared in 64 bits.
+//
+// 64 rows of 262144 logits, a quarter of them ended (50 MB read): the pass 16.8 us (3.0 TB/s), the second launch 5.1. The
+// pass is bound by the vector units: nine operations and an exp per logit are half of its time, and the rest is the
+// latency of first loads, lists and joins, which at a copy's rate would be 10 us for the bytes. Four rows of 4096: 4.7 and
+// 2.9 us, launches and latency.
 #include <algorithm>
 
 #include "internal.h"

@@ -1,10 +1,23 @@
 // paged_attention.hip - attention of one new token per sequence over the paged cache.
 //
-// Scores and the weighted sum run on the fp32 matrix cores as in the prompt's attention
-// (prefill.hip): S^T = K q^T with the query heads of a K/V head as columns leaves lane (c, m) head c's
-// scores of positions 4m .. 4m + 3, which is the B operand of O^T = V^T P^T. One pass over K and V with
-// a running maximum and sum per column; a sequence's positions are cut into pieces that workgroups take
-// side by side, and a second launch joins the pieces' (maximum, sum, O).
+// With scores s_p in log2 units, out = sum 2^(s_p - m) v_p / sum 2^(s_p - m) in one pass over K and V: a wave takes a
+// tile of 16 positions (or two), forms the scores on the matrix cores with the query heads of a K/V head as columns,
+// keeps a running maximum m and sum per column, and adds the weighted V on the matrix cores. Nothing is staged in LDS:
+// the cache's tiles are in operand order, so that a wave's loads are whole KiB and land in the registers that the
+// products read; the next tile's K is under way during the softmax and V's product, its V during the next scores.
+//
+// The bytes of K and V bound it, each read once by one workgroup for all heads of its K/V head (sixteen at most, over
+// quantized caches eight). A sequence is cut into pieces of a fixed number of positions that workgroups take side by
+// side, and a second launch joins their (maximum, sum, O); where whole sequences fill the chip they are not cut and the
+// longest go first. The products' forms:
+//   float cache, fp32 rows, up to 4 heads   4x4x1 fp32: its four columns are the heads
+//   float cache, fp32 rows, more            16x16x4 fp32
+//   float cache, 16-bit rows                16x16x32 of their type, the weights in two terms of it
+//   quantized cache                         K's codes in 8-bit products with q's digits, V's codes as bf16
+//
+// Whole calls over 400 MB of K and V, sequences of 2000 positions, head_dim 64 to 256: up to four heads per K/V head
+// 74-107 us (3.8-5.3 TB/s; a large copy moves 4.9), eight heads 78-102 us over float caches, 84-118 over Q8_0, 107-170
+// over Q4_0, whose conversions keep the vector units as busy as the bytes keep the memory.
 #include <algorithm>
 #include <climits>
 
@@ -464,10 +477,13 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
-// Rows over a float cache. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
+// Rows over a float cache: S^T = K q^T leaves lane (c, m) head c's scores of positions 4m .. 4m + 3, which is the B operand
+// of O^T = V^T P^T. fp32 rows: v_mfma_f32_16x16x4_f32 on the elements as fp32. 16-bit rows (HALF) over a
 // cache of their type: 16x16x32 products of the elements as they are, of two tiles for the weighted sum (of one where
 // two do not fit the registers, 16x16x16); the weights come in two terms of that type (one
 // would be off by as much as the outputs' own rounding), and V's 16-bit words are transposed in pairs on the way.
+// 250 sequences of up to 2000 positions, 8 K/V heads of 128 dims, bf16 (1.0 GB): 175 us, 5.7 TB/s; two of three cycles wait
+// for memory.
 // grid (pieces, K/V heads x column tiles, sequences).
 template <int CT, int HD, bool HALF>
 __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(AttnArgs g) {
@@ -659,6 +675,9 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 // zeros for the other half's rows), and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
 // sums only those of a column's own block are meant. TERMS: bf16 terms of that product, 3 for all its 24 bits;
 // 2 where rows are bf16 (its rounding is then 2^-7 of the outputs').
+// Three sequences of up to 131072 positions, 32 heads over 8 of 128 dims, Q4_0, fp32 rows (374 MB): 75-80 us, 4.7-5.0 TB/s,
+// of which the vector units are busy for 41 and the matrix cores for 15; sixteen of up to 2048, 4 heads over one of 256, Q8_0
+// (9.7 MB): 8.3 us, a chain as above.
 template <int CT, int HD, int NT, int TERMS>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && CT == DT_Q4_0) ? 4 : NT == 1 ? 3 : 2) void paged_attn_digits_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
@@ -920,7 +939,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
     finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
-// grid (heads, sequences): the pieces of one head. Every wave has all pieces' weights, one or more per lane, and adds
+// grid (heads, sequences): the pieces of one head. 2.2 us for nine pieces of 256 dims, 5.8 for 3 x 32 heads of 85 pieces.
+// Every wave has all pieces' weights, one or more per lane, and adds
 // every fourth piece, HD / 64 dims per lane. All first loads start before the length is known: the slots of all pieces
 // are in the workspace.
 template <int HD>
@@ -998,9 +1018,11 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
     if (a.lse && t == 0) a.lse[slot] = lse_of(top, tot);
 }
 
-// A piece is a fixed number of positions, so that sequences of different lengths make equal work: as
-// many as give kWantGroups workgroups if all sequences were max_length long, a stride of the waves
-// at least.
+// A piece is a fixed number of positions, so that sequences of different lengths make equal work: as many as give
+// kWantGroups workgroups if all sequences were max_length long, a stride of the waves at least. Three sequences of up to
+// 131072 (24 K/V heads) with 1024, 2048, 4096 workgroups wanted: 93, 89, 95 us. 250 sequences of 2000 (2000 K/V heads) take
+// 175 us whole and 226 in pieces, hence kFullGroups; 584 heads are faster cut. (Smaller pieces for sequences of many
+// bytes gained as often as they lost.)
 struct Plan {
     int col_heads, col_tiles, want, piece, pieces;
     int64_t groups;

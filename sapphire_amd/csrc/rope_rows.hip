@@ -3,7 +3,10 @@
 //
 // A workgroup takes a few tokens, or some heads of one: it forms the tokens' angles once into LDS (64-bit
 // product and reduction to half a turn, then fp32 sine and cosine), and its threads turn 16 bytes of
-// each half at a time.
+// each half at a time, two such pieces on their way at once and the first ones while the angles are formed.
+//
+// Bytes bound it: 8192 tokens of 40 heads of 128 dims, bf16, half of them turned (168 MB read and written) take 36.8 us,
+// 4.6 TB/s, a copy's rate; with one piece at a time and none ahead it was 39.5. One token's heads: 2.3 us, a launch.
 #include <algorithm>
 
 #include "paged_dev.h"
