@@ -95,7 +95,8 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * side and are joined by a second launch; the results do not depend on which workgroup runs when, nor
  * on what the other sequences hold.
  * workspace: sapphire_paged_attention_workspace_bytes() bytes, 16-byte aligned (NULL where that is
- * 0); calls that share one must be ordered on one stream. */
+ * 0), which are enough for calls of fewer and shorter sequences too; calls that share one must be
+ * ordered on one stream. */
 typedef struct {
     float scale;
     int window;

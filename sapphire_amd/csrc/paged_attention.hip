@@ -34,7 +34,6 @@ constexpr int kCols = 16;                  // query heads of a workgroup
 constexpr int kPos = 16;                   // positions of a tile
 constexpr int kMaxPieces = 256;
 constexpr int kPieceUnit = 64;             // a piece is a multiple of so many positions
-constexpr int kFullGroups = 1024, kWantGroups = 2048;      // workgroups that are left as they are; that cut sequences make
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 struct AttnArgs {
@@ -1018,24 +1017,42 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
     if (a.lse && t == 0) a.lse[slot] = lse_of(top, tot);
 }
 
-// A piece is a fixed number of positions, so that sequences of different lengths make equal work: as many as give
-// kWantGroups workgroups if all sequences were max_length long, a stride of the waves at least. Three sequences of up to
-// 131072 (24 K/V heads) with 1024, 2048, 4096 workgroups wanted: 93, 89, 95 us. 250 sequences of 2000 (2000 K/V heads) take
-// 175 us whole and 226 in pieces, hence kFullGroups; 584 heads are faster cut. (Smaller pieces for sequences of many
-// bytes gained as often as they lost.)
+// A piece is a fixed number of positions, so that sequences of different lengths make equal work. Sequences of many
+// (sequence, K/V head) pairs are not cut: each start costs about 2 us and the join 2 to 7, and the longest, first to go,
+// end in time where a single workgroup reaches a good part of what its share of the memory's rate is. That takes fewer pairs
+// where it does little but load (16-bit rows over their own type, up to four fp32 heads over fp32) than where it converts;
+// likewise the pieces of others are larger. In us, for pairs x positions, and at a copy's rate for the bytes:
+//   bf16, 4 heads of 128 dims        256 x 2774 (35): whole 39, in 2 to 16 pieces 41-50;    128 x 5548 (38): 42; 41-49
+//   fp32 over Q4_0, 4 x 128          256 x 8877 (35): whole 85, in 4 to 16 pieces 45-65;    512 x 6658 (53): 72; 69-81
+//   fp32 over fp16, 8 x 128          256 x 2774 (35): whole 88, 51-73;                      512 x 2080 (53): 79; 72-102
+// Pieces of 160 KiB and 768 KiB take 0.93 of the time, in the mean over 64 ragged batches, that as many pieces as make 2048
+// workgroups take.
+struct Wanted {
+    int whole, bytes;                      // pairs from which on sequences are not cut; a piece's bytes of K and V
+};
+constexpr Wanted kLoads = {256, 768 << 10}, kConverts = {512, 160 << 10};
+constexpr int kFill = 512;                 // workgroups that smaller pieces are made for
+int pieces_wanted(Wanted w, int64_t groups, int64_t len, int row) {
+    if (groups >= w.whole) return 1;
+    return (int)std::min<int64_t>(kMaxPieces, std::max((len * row + w.bytes - 1) / w.bytes, (kFill + groups - 1) / groups));
+}
+int row_bytes_kv(int dtype, int hd) { return 2 * (dtype == DT_F32 ? 4 * hd : dtype == DT_Q8_0 ? hd * 9 / 8 : dtype == DT_Q4_0 ? hd * 5 / 8 : 2 * hd); }
 struct Plan {
-    int col_heads, col_tiles, want, piece, pieces;
+    int col_heads, col_tiles, piece, pieces;
     int64_t groups;
 };
-Plan plan_of(int dtype, bool half, int nkv, int batch, int n_heads, int max_length, int window) {
+Plan plan_of(int dtype, bool half, int nkv, int hd, int batch, int n_heads, int max_length, int window) {
     Plan p;
     const int group = n_heads / nkv;
-    p.col_heads = !is_quant(dtype) ? (!half && group <= 4 ? 4 : kCols) : group <= 4 ? 4 : 8;
+    // quantized caches: four or eight heads a workgroup; float caches: four for fp32 rows of no more, or sixteen
+    p.col_heads = is_quant(dtype) ? (group <= 4 ? 4 : 8) : !half && group <= 4 ? 4 : kCols;
     p.col_tiles = (group + p.col_heads - 1) / p.col_heads;
-    const int64_t groups = p.groups = (int64_t)batch * nkv * p.col_tiles;
+    p.groups = (int64_t)batch * nkv * p.col_tiles;
+    const bool loads = !is_quant(dtype) && (half || (dtype == DT_F32 && p.col_heads == 4));
+    const int row = row_bytes_kv(dtype, hd);
     const int64_t len = (window > 0 && window < max_length - kPos ? window + kPos : max_length);
-    p.want = groups >= kFullGroups ? 1 : (int)std::min<int64_t>(kMaxPieces, kWantGroups / groups);
-    p.piece = (int)(((len + p.want - 1) / p.want + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
+    const int64_t want = pieces_wanted(loads ? kLoads : kConverts, p.groups, len, row);
+    p.piece = (int)(((len + want - 1) / want + kPieceUnit - 1) / kPieceUnit * kPieceUnit);
     p.pieces = (int)((len + p.piece - 1) / p.piece);
     return p;
 }
@@ -1044,10 +1061,17 @@ size_t part_bytes(int hd, int batch, int n_heads, int pieces) { return (size_t)p
 
 }  // namespace
 
-// For any window: a plan has at most as many pieces as it may want, and as the positions have units.
+// Enough for every call of at most `batch` sequences of at most max_length, whatever its window and type of rows: b
+// sequences that are cut, b k < kConverts.whole, have no more pieces than max(by bytes, kFill / (b k) + 1), all bounds grow
+// with the length, and b times that is at most what the largest such b makes of either term.
 size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length) {
-    const int pieces = std::min(plan_of(dtype, false, nkv, batch, n_heads, max_length, 0).want, (max_length + kPieceUnit - 1) / kPieceUnit);
-    return pieces == 1 ? 0 : part_bytes(hd, batch, n_heads, pieces) + (size_t)pieces * batch * n_heads * sizeof(float2);
+    const int64_t k = plan_of(dtype, false, nkv, hd, 1, n_heads, max_length, 0).groups;
+    const int64_t b = std::min<int64_t>(batch, (kConverts.whole - 1) / k);
+    const int64_t most = std::min<int64_t>(kMaxPieces, ((int64_t)max_length + kPieceUnit - 1) / kPieceUnit);
+    if (b == 0 || most == 1) return 0;
+    const int64_t bytes = ((int64_t)max_length * row_bytes_kv(dtype, hd) + kConverts.bytes - 1) / kConverts.bytes;
+    const int64_t slots = std::max(b * std::min(most, bytes), std::min(b * most, kFill / k + b));
+    return (size_t)slots * n_heads * (hd * sizeof(float) + sizeof(float2));
 }
 
 int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
@@ -1056,12 +1080,12 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     g.n_heads = a.q.heads;
     g.group = g.n_heads / a.c.nkv;
     const bool half = a.q.dtype != DT_F32;
-    const Plan p = plan_of(a.c.dtype, half, a.c.nkv, a.q.tokens, g.n_heads, a.max_length, a.window);
+    const Plan p = plan_of(a.c.dtype, half, a.c.nkv, a.c.hd, a.q.tokens, g.n_heads, a.max_length, a.window);
     g.col_tiles = p.col_tiles;
     g.piece = p.piece;
     g.pieces = p.pieces;
     g.wide = rows_wide(a.out);
-    g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kFullGroups;
+    g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kLoads.whole;
     g.part = reinterpret_cast<float *>(a.ws);
     g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);

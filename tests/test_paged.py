@@ -95,6 +95,16 @@ def test_attention_refused(lib, change):
     assert lib.sapphire_last_error()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, Q8_0, Q4_0], ids=ref.NAME.get)
+@pytest.mark.parametrize("nkv,heads", [(1, 1), (1, 40), (3, 12), (8, 64), (600, 600)])
+def test_workspace_is_enough_for_smaller_calls(lib, dtype, nkv, heads):
+    c = cache(dtype, nkv=nkv, hd=128)
+    need = np.array([[lib.sapphire_paged_attention_workspace_bytes(C.byref(c), b, heads, n) for n in (1, 64, 65, 500, 2000, 9000, 131072, 2**30)]
+                     for b in (1, 2, 3, 20, 63, 64, 65, 170, 171, 511, 512, 4000)], dtype=np.int64)
+    assert (np.diff(need, axis=0) >= 0).all() and (np.diff(need, axis=1) >= 0).all()
+    assert need[0, 0] == 0 and (need[:, -1] > 0).all() == (nkv < 512)
+
+
 def test_reorder_refused(lib):
     c, t, o = cache(), PageTableC(P, 3, 4), PageTableC(2 * P, 3, 4)
     good = [C.byref(c), C.byref(t), 3 * P, 4 * P, 5 * P, C.byref(o), 6 * P, None]

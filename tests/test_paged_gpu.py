@@ -569,6 +569,36 @@ def test_attention_in_place(hip, cache, io, heads, lens):
     np.testing.assert_array_equal(out[1].numpy(), q[1].numpy())
 
 
+@pytest.mark.parametrize("cache,io,heads", [(F32, F32, 4), (BF16, BF16, 8), (F16, F32, 6), (Q8_0, F32, 4), (Q4_0, F16, 8)],
+                         ids=["f32", "bf16", "f16_f32", "q8_0", "q4_0"])
+def test_workspace_of_the_largest_call(hip, cache, io, heads):
+    """One workspace, of the size for the largest batch and length, serves smaller calls: nothing behind it is written, and
+    the outputs are the bits of a call with a workspace of its own."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(17)
+    hd, ps, top = 64, 64, 9000
+    lens = [top, 1, 4500, 700, 8999, 64, 0, 130]
+    table, pages = tables(rng, [top], ps)                      # (all sequences read the same pages)
+    table = np.repeat(table, 520, 0)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    c.fill(0, table, 0, rng.normal(size=(top, 1, hd)).astype(np.float32), rng.normal(size=(top, 1, hd)).astype(np.float32))
+    c.upload()
+    nbytes, guard = c.c.attention_workspace_bytes(520, heads, top), 8 << 20
+    ws = DeviceArray.from_numpy(np.full(nbytes + guard, 0x5a, np.uint8))
+    dt = dev(table)
+    for batch, most in [(1, top), (2, top), (3, 5000), (8, top), (60, 2000), (129, top), (255, 300), (256, top), (511, top), (512, top), (520, top)]:
+        n = np.minimum(np.resize(lens, batch), most).astype(np.int32)
+        q = device_rows(rng.normal(size=(batch, heads, hd)).astype(np.float32), io)
+        dl, outs = dev(n), []
+        for w in (ws, DeviceArray(max(16, c.c.attention_workspace_bytes(batch, heads, most)))):
+            outs.append(device_rows(np.zeros((batch, heads, hd), np.float32), io))
+            c.c.attention(0, q[0], outs[-1][0], PageTable(dt, *table.shape), dl, most, 0.2, workspace=w)
+            sync()
+        np.testing.assert_array_equal(outs[0][1].numpy(), outs[1][1].numpy(), err_msg=f"{batch} {most}")
+        assert (ws.numpy()[nbytes:] == 0x5a).all(), (batch, most)
+
+
 def test_two_streams_at_once(hip):
     """Calls on two streams, each with its own workspace and outputs, over one cache: the bits of calls one after the other."""
     from sapphire_amd import load
