@@ -20,6 +20,7 @@
 // over Q4_0, whose conversions keep the vector units as busy as the bytes keep the memory.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "internal.h"
 #include "lanes.h"
@@ -32,7 +33,7 @@ namespace {
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kCols = 16;                  // query heads of a workgroup
 constexpr int kPos = 16;                   // positions of a tile
-constexpr int kMaxPieces = 256;
+constexpr int kMaxPieces = 256, kManyPieces = 32;          // of a sequence; that sixteen waves join instead of four
 constexpr int kPieceUnit = 64;             // a piece is a multiple of so many positions
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
@@ -938,14 +939,14 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
     finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
-// grid (heads, sequences): the pieces of one head. 2.2 us for nine pieces of 256 dims, 5.8 for 3 x 32 heads of 85 pieces.
-// Every wave has all pieces' weights, one or more per lane, and adds
-// every fourth piece, HD / 64 dims per lane. All first loads start before the length is known: the slots of all pieces
+// grid (heads, sequences): the pieces of one head. Every wave has all pieces' weights, one or more per lane, and adds
+// every W-th piece, HD / 64 dims per lane: four waves 2.2 us for nine pieces of 256 dims; for 128 pieces of 96 heads of 128
+// dims 9.5 us with four waves, 7.1 with sixteen. All first loads start before the length is known: the slots of all pieces
 // are in the workspace.
-template <int HD>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
+template <int HD, int W>
+__global__ __launch_bounds__(W *kWave) void paged_join_kernel(AttnArgs g) {
     constexpr int D = HD / kWave, U = 8, Q = kMaxPieces / kWave;       // U: loads in flight
-    __shared__ float part[kWaves][HD];
+    __shared__ float part[W][HD];
     const PagedAttn &a = g.a;
     const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const size_t stride = (size_t)gridDim.y * g.n_heads, slot = (size_t)b * g.n_heads + h;
@@ -956,7 +957,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int d = 0; d < D; ++d) v[u][d] = g.part[(slot + min(i0 + u * kWaves, last) * stride) * HD + lane * D + d];
+            for (int d = 0; d < D; ++d) v[u][d] = g.part[(slot + min(i0 + u * W, last) * stride) * HD + lane * D + d];
     };
     load(wid, g.pieces - 1);
     const int n = min(max(a.lengths[b], 0), a.max_length);
@@ -988,7 +989,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
     for (int i0 = wid; i0 < used;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kWaves;
+            const int i = i0 + u * W;
             if (i >= used) break;
             float fi = 0.f;
             bool on = false;
@@ -1002,7 +1003,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = __builtin_fmaf(fi, v[u][d], o[d]);
         }
-        i0 += kWaves * U;
+        i0 += W * U;
         if (i0 < used) load(i0, used - 1);
     }
 #pragma unroll
@@ -1012,7 +1013,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
     if (t >= HD) return;
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) x += part[w][t];
+    for (int w = 0; w < W; ++w) x += part[w][t];
     store1(a.out.dtype, a.out.p, (int64_t)b * a.out.ts + (int64_t)h * a.out.hs + t, tot == 0.f ? 0.f : __fdiv_rn(x, tot));
     if (a.lse && t == 0) a.lse[slot] = lse_of(top, tot);
 }
@@ -1025,16 +1026,21 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(AttnArgs g) {
 //   bf16, 4 heads of 128 dims        256 x 2774 (35): whole 39, in 2 to 16 pieces 41-50;    128 x 5548 (38): 42; 41-49
 //   fp32 over Q4_0, 4 x 128          256 x 8877 (35): whole 85, in 4 to 16 pieces 45-65;    512 x 6658 (53): 72; 69-81
 //   fp32 over fp16, 8 x 128          256 x 2774 (35): whole 88, 51-73;                      512 x 2080 (53): 79; 72-102
-// Pieces of 160 KiB and 768 KiB take 0.93 of the time, in the mean over 64 ragged batches, that as many pieces as make 2048
-// workgroups take.
+// Pieces of 160 KiB and 768 KiB, and fewer than that of long sequences, take 0.92 of the time, in the mean over 64 ragged
+// batches of 60 to 1000 MB, that as many pieces as make 2048 workgroups take.
 struct Wanted {
     int whole, bytes;                      // pairs from which on sequences are not cut; a piece's bytes of K and V
 };
 constexpr Wanted kLoads = {256, 768 << 10}, kConverts = {512, 160 << 10};
 constexpr int kFill = 512;                 // workgroups that smaller pieces are made for
+constexpr int64_t kJoined = 48;            // pieces from which on their number grows as the root of the bytes: the join counts
+int pieces_by_bytes(Wanted w, int64_t len, int row) {
+    const int64_t n = (len * row + w.bytes - 1) / w.bytes;
+    return (int)std::min<int64_t>(kMaxPieces, n <= kJoined ? n : (int64_t)std::sqrt((double)(kJoined * n)));
+}
 int pieces_wanted(Wanted w, int64_t groups, int64_t len, int row) {
     if (groups >= w.whole) return 1;
-    return (int)std::min<int64_t>(kMaxPieces, std::max((len * row + w.bytes - 1) / w.bytes, (kFill + groups - 1) / groups));
+    return (int)std::min<int64_t>(kMaxPieces, std::max<int64_t>(pieces_by_bytes(w, len, row), (kFill + groups - 1) / groups));
 }
 int row_bytes_kv(int dtype, int hd) { return 2 * (dtype == DT_F32 ? 4 * hd : dtype == DT_Q8_0 ? hd * 9 / 8 : dtype == DT_Q4_0 ? hd * 5 / 8 : 2 * hd); }
 struct Plan {
@@ -1069,7 +1075,7 @@ size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_he
     const int64_t b = std::min<int64_t>(batch, (kConverts.whole - 1) / k);
     const int64_t most = std::min<int64_t>(kMaxPieces, ((int64_t)max_length + kPieceUnit - 1) / kPieceUnit);
     if (b == 0 || most == 1) return 0;
-    const int64_t bytes = ((int64_t)max_length * row_bytes_kv(dtype, hd) + kConverts.bytes - 1) / kConverts.bytes;
+    const int64_t bytes = pieces_by_bytes(kConverts, max_length, row_bytes_kv(dtype, hd));
     const int64_t slots = std::max(b * std::min(most, bytes), std::min(b * most, kFill / k + b));
     return (size_t)slots * n_heads * (hd * sizeof(float) + sizeof(float2));
 }
@@ -1107,9 +1113,10 @@ int launch_paged_attention(const PagedAttn &a, hipStream_t s) {
     if (!hip_ok(hipGetLastError(), "paged attention launch")) return -1;
     if (p.pieces > 1) {
         const dim3 jg(g.n_heads, a.q.tokens);
-        if (a.c.hd == 64) hipLaunchKernelGGL((paged_join_kernel<64>), jg, block, 0, s, g);
-        else if (a.c.hd == 128) hipLaunchKernelGGL((paged_join_kernel<128>), jg, block, 0, s, g);
-        else hipLaunchKernelGGL((paged_join_kernel<256>), jg, block, 0, s, g);
+#define SPH_JOIN(HD, W) \
+    if (a.c.hd == HD && (p.pieces > kManyPieces) == (W == 16)) hipLaunchKernelGGL((paged_join_kernel<HD, W>), jg, dim3(W * kWave), 0, s, g);
+#define SPH_JOIN_HD(HD) SPH_JOIN(HD, 4) SPH_JOIN(HD, 16)
+        SPH_JOIN_HD(64) SPH_JOIN_HD(128) SPH_JOIN_HD(256)
         if (!hip_ok(hipGetLastError(), "paged attention join launch")) return -1;
     }
     return 0;
