@@ -16,8 +16,8 @@
 //   quantized cache                         K's codes in 8-bit products with q's digits, V's codes as bf16
 //
 // Whole calls over 400 MB of K and V, sequences of 2000 positions, head_dim 64 to 256: up to four heads per K/V head
-// 74-107 us (3.8-5.3 TB/s; a large copy moves 4.9), eight heads 78-102 us over float caches, 84-118 over Q8_0, 107-170
-// over Q4_0, whose conversions keep the vector units as busy as the bytes keep the memory.
+// 72-101 us (4.0-5.5 TB/s; a large copy moves 4.9), eight heads 77-108 us over float caches, 90-118 over Q8_0, 126-170
+// over Q4_0, whose conversions keep the vector units busier than the bytes keep the memory.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -675,9 +675,9 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 // zeros for the other half's rows), and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
 // sums only those of a column's own block are meant. TERMS: bf16 terms of that product, 3 for all its 24 bits;
 // 2 where rows are bf16 (its rounding is then 2^-7 of the outputs').
-// Three sequences of up to 131072 positions, 32 heads over 8 of 128 dims, Q4_0, fp32 rows (374 MB): 75-80 us, 4.7-5.0 TB/s,
+// Three sequences of up to 131072 positions, 32 heads over 8 of 128 dims, Q4_0, fp32 rows (374 MB): 77-83 us, 4.5-4.9 TB/s,
 // of which the vector units are busy for 41 and the matrix cores for 15; sixteen of up to 2048, 4 heads over one of 256, Q8_0
-// (9.7 MB): 8.3 us, a chain as above.
+// (9.7 MB): 8.5 us, a chain as above.
 template <int CT, int HD, int NT, int TERMS>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && CT == DT_Q4_0) ? 4 : NT == 1 ? 3 : 2) void paged_attn_digits_kernel(AttnArgs g) {
     using R = Raw<CT, HD>;
