@@ -231,6 +231,16 @@ def test_attention_pieces(hip, cache, io):
     attend_case(rng, cache, io, 64, 2, 6, 1024, [2049, 2047], order="htd", pad=5)
 
 
+@pytest.mark.parametrize("cache,io", [(F32, F32), (BF16, BF16), (Q8_0, F32), (Q4_0, F16)], ids=["f32", "bf16", "q8_0_f32", "q4_0_f16"])
+def test_attention_of_very_many_pieces(hip, cache, io):
+    """Two hundred pieces and more of one sequence, some of them without a page, beside short sequences; a window that
+    starts inside a piece."""
+    rng = np.random.default_rng(18)
+    attend_case(rng, cache, io, 64, 1, 4, 256, [16500, 7, 0, 9000], broken=[(0, 0), (0, 1), (0, 40), (3, 35)])
+    attend_case(rng, cache, io, 128, 1, 2, 128, [8300, 4097], window=6001)
+    attend_case(rng, cache, io, 256, 1, 5, 64, [4200])
+
+
 @pytest.mark.parametrize("cache,io", IO, ids=IDS)
 @pytest.mark.parametrize("window,softcap", [(1, 0.0), (16, 0.0), (100, 0.0), (512, 30.0), (0, 5.0)])
 def test_attention_window_and_cap(hip, cache, io, window, softcap):
