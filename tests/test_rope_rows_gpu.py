@@ -50,6 +50,32 @@ def test_rope_rows(hip, io, inter, t, h, hd, rot):
         np.testing.assert_array_equal(raw, rx[2], err_msg="elements between the rows, in place")
 
 
+@pytest.mark.parametrize("io", [F32, BF16], ids=ref.NAME.get)
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "pairs"])
+@pytest.mark.parametrize("t,h,hd,rot", [(6001, 7, 128, 64), (5003, 5, 128, 66), (20000, 1, 64, 64), (257, 129, 64, 32)])
+def test_rope_rows_of_long_prompts(hip, io, inter, t, h, hd, rot):
+    """Rows enough that a thread takes many pieces, of several heads and tokens; to other rows and in place."""
+    from sapphire_amd import paged
+    rng = np.random.default_rng(t)
+    x = rng.normal(size=(t, h, hd)).astype(np.float32)
+    pos = rng.integers(0, 1 << 18, t).astype(np.int32)
+    freqs, _ = paged.rope_frequencies(rot, 1e4)
+    dp, df = dev(pos), dev(freqs)
+    rx, ry = device_rows(x, io, "thd", 64, 0), device_rows(x * 0 + 9, io, "htd", 8, 8)
+    for to in (ry, rx):
+        paged.rope(rx[0], to[0], dp, df, rot, interleaved=inter)
+        sync()
+        raw = to[1].numpy()
+        got = np.lib.stride_tricks.as_strided(raw[8 if to is ry else 0:], x.shape, to[3].strides).copy()
+        if to is ry:
+            check(io, x, ref.from_type(io, rx[3]), ref.from_type(io, got), pos, freqs, rot, inter, 1.0)
+            first = got
+        else:
+            np.testing.assert_array_equal(got, first)
+        to[3][...] = got
+        np.testing.assert_array_equal(raw, to[2], err_msg="elements between the rows")
+
+
 def test_rope_rows_agree_with_the_tables(hip, oracle):
     """The half layout over a whole head against the table form at the same position: the tables hold fp32 angles' sines
     (an angle of up to 2047 rounded to 2^-24 of itself and its fp32 frequency's error), so to 4e-4 of the values."""
