@@ -95,6 +95,27 @@ def test_sorted_logits(hip, down):
     check(np.stack([x, x - 1, x + 1, x]).astype(np.float32), np.array([-1, -1, -2, -1.5], np.float32), None, 1, 4, -1)
 
 
+@pytest.mark.parametrize("R,W,n,ld", [(8, 8, 70001, 70003), (4, 16, 131072, 131072), (40, 8, 60000, 60001), (300, 1, 50000, 50000)])
+def test_many_rows_of_a_large_vocabulary(hip, R, W, n, ld):
+    """Rows enough that a workgroup takes thousands of logits, of the largest several batches: random ones, rising and
+    falling ones, few above -inf, equal ones, and NaN of both kinds."""
+    rng = np.random.default_rng(n + W)
+    rows = R * W
+    x = (rng.normal(size=(rows, n)) * 3).astype(np.float32)
+    ramp = np.linspace(-9, 9, n, dtype=np.float32)
+    x[1 % rows::7], x[2 % rows::7] = ramp, ramp[::-1]
+    x[3 % rows::7] = np.round(x[3 % rows::7])
+    few = x[4 % rows::7]
+    few[rng.random(few.shape) < 0.9999] = -np.inf
+    bad = x[5 % rows::7].view(np.uint32)
+    bad[rng.random(bad.shape) < 0.01] = 0x7fc00000             # quiet, signalling, negative
+    bad[rng.random(bad.shape) < 0.01] = 0x7f800001
+    bad[rng.random(bad.shape) < 0.01] = 0xff923456
+    score = -np.abs(rng.normal(size=rows) * 4).astype(np.float32)
+    check(x, score, None, R, W, -1, ld)
+    check(x, score, (rng.random(rows) < 0.2).astype(np.int32), R, W, 5, ld, in_place=True)
+
+
 def test_far_logits(hip):
     """Magnitudes whose exponentials overflow or vanish."""
     x = np.array([[3e38, 2.9e38, -3e38, 0, 1], [-3e38, -3e38, -2e38, -2e38, -1e38], [88, 89, 90, 91, 1000], [0, 0, 0, 0, 0]], np.float32)
