@@ -944,9 +944,9 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
 }
 
 // grid (heads, sequences): the pieces of one head. Every wave has all pieces' weights, one or more per lane, and adds
-// every W-th piece, HD / 64 dims per lane: four waves 2.2 us for nine pieces of 256 dims; for 128 pieces of 96 heads of 128
-// dims 9.5 us with four waves, 7.1 with sixteen. All first loads start before the length is known: the slots of all pieces
-// are in the workspace.
+// every W-th piece, HD / 64 dims per lane. Up to 32 pieces, one trip of four waves: nine pieces of 256 dims 2.7 us (sixteen waves
+// 3.5), 32 of 64 heads 3.6 (4.3); 128 pieces of 96 heads of 128 dims 7.1 with sixteen waves (four 9.5). All first loads start
+// before the length is known: the slots of all pieces are in the workspace.
 template <int HD, int W>
 __global__ __launch_bounds__(W *kWave) void paged_join_kernel(AttnArgs g) {
     constexpr int D = HD / kWave, U = 8, Q = kMaxPieces / kWave;       // U: loads in flight
