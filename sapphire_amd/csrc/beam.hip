@@ -128,11 +128,12 @@ struct Norm {
     float max;
 };
 
-// exp(x - m) for x <= m (NaN where both are infinite, 0 for a NaN x). log2 e in two floats: the rounding of one would
-// be off the same way in every term, where the others' roundings even out over a row.
+// exp(x - m) for x <= m, m above -inf; 0 for a NaN x, and for every x where m is +inf. The difference is taken first: next to
+// an m of 2^32 and more, m - 150 is m. log2 e in two floats: the rounding of one would be off the same way in every term,
+// where the others' roundings even out over a row.
 __device__ __forceinline__ float exp_of(float x, float m) {
     constexpr float hi = 0x1.715476p+0f, lo = 0x1.4ae0cp-26f;
-    const float d = __fsub_rn(fmaxf(x, m - 150.0f), m);
+    const float d = fmaxf(__fsub_rn(x, m), -150.0f);
     return __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi, __fmul_rn(d, lo)));
 }
 
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(kMaxBeams *kWave) void beam_pick_kernel(int n, int 
         for (int i = lane + kWave; i < chunks; i += kWave)
             if (nr[i].max > -INFINITY) s += nr[i].sum * (double)exp_of(nr[i].max, m);
         lse = (double)m + log(wave_sum(s));
-        dead = !(fabs(lse) < (double)INFINITY);        // a logit of +inf, or none above -inf
+        dead = !(fabs(lse) < (double)INFINITY);        // a logit of +inf (inf + log 0), or none above -inf
     }
     if (lane < beams) {
         double sc = -(double)INFINITY;

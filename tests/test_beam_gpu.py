@@ -120,3 +120,38 @@ def test_far_logits(hip):
     """Magnitudes whose exponentials overflow or vanish."""
     x = np.array([[3e38, 2.9e38, -3e38, 0, 1], [-3e38, -3e38, -2e38, -2e38, -1e38], [88, 89, 90, 91, 1000], [0, 0, 0, 0, 0]], np.float32)
     check(x, np.array([0, 0, 0, 0], np.float32), None, 1, 4, -1)
+
+
+FAR = [(4.3e9, 0.0), (1e10, 0.0), (1e10, -np.inf), (1e10, np.nan), (1e12, 9e11), (-1e10, -2e10), (-1e10, -np.inf), (-1e12, np.nan),
+       (float(np.finfo(np.float32).min), -np.inf), (float(np.finfo(np.float32).max), -1e38)]
+
+
+@pytest.mark.parametrize("top,rest", FAR)
+@pytest.mark.parametrize("n", [5000, 100001])
+def test_far_maxima(hip, n, top, rest):
+    """Rows of one logit far from zero, the others far below it: their normaliser is that logit, so the row's best score is
+    its beam's own, ahead of an ended beam at -5 and of an ordinary one at -3.
+
+    A score is off by the normaliser's error, which does not grow with the logits: at most eight exponentials in a row of
+    factors (2^-22 each, and their arguments, ln n in the mean, by 2^-23 of themselves) and sums in fp32 of 2^-22, together below
+    2^-18; by the roundings of m + log s and of x - (m + log s) in 64 bits, here and in the oracle; and by that to fp32."""
+    rng = np.random.default_rng(n)
+    R, W = 3, 3
+    logits = np.full((R * W, n), rest, np.float32)
+    at = [0, n // 2 + 1, n - 1]
+    for r in range(R):
+        logits[r * W, at[r]] = top
+        logits[r * W + 2] = rng.normal(size=n) * 3
+    score = np.tile([0.0, -5.0, -3.0], R).astype(np.float32)
+    done = np.tile([0, 1, 0], R).astype(np.int32)
+    got = select(logits, n, score, done, R, W, 7)
+    want = ref.beams64(logits, score, done, R, W, 7)
+    for g, w in zip(got[1:], want[1:]):
+        np.testing.assert_array_equal(g, w)
+    for r in range(R):
+        assert got[1][r * W] == at[r] and got[2][r * W] == r * W
+    fin = np.isfinite(want[0])
+    tol = 2.0**-18 + 4 * 2.0**-53 * abs(top) + 2.0**-24 * np.abs(want[0][fin])
+    if abs(top) > 2e12:                        # there the oracle's own m + log s is coarse; the best score is 0 all the same
+        np.testing.assert_array_equal(got[0][::W], 0.0)
+    assert (np.abs(got[0][fin] - want[0][fin]) <= tol).all()
