@@ -117,25 +117,47 @@ struct Raw {
         return pu2{v << 4 & 0xf0f0f0f0u, v & 0xf0f0f0f0u};
     }
     // V's codes as signed bytes (Q4_0: times 16), word i: position r's DPL bytes start at byte r * DPL; Q4_0: the low
-    // nibbles' bytes of all positions, then the high ones'.
+    // nibbles' bytes of all positions, then the high ones'. Of two sets of four blocks (head_dim 256) a lane has the first
+    // set's dims in the first half of its elements and the second's in the other: lanes c < 8, which hold the first set, and
+    // c + 8 exchange halves (v_element_dim).
     static constexpr int VW = DPL;
-    __device__ __forceinline__ void v_bytes(uint32_t (&q)[VW]) const {
+    static constexpr bool kTwoSets = T::NB == 8;
+    // a in lanes c < 8 and b of lane c - 8 in the others; or b of lane c + 8 and a (row_ror:8 into half of the banks)
+    static __device__ __forceinline__ uint32_t low_own(uint32_t a, uint32_t b) {
+        return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xF, 0xC, false);
+    }
+    static __device__ __forceinline__ uint32_t high_own(uint32_t a, uint32_t b) {
+        return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xF, 0x3, false);
+    }
+    __device__ __forceinline__ void v_bytes(uint32_t (&q)[VW], int c) const {
         if constexpr (CT == DT_Q8_0) {
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                q[i] = w[i / 4][i % 4];
+                if constexpr (!kTwoSets) q[i] = w[i / 4][i % 4];
+                else q[i] = i % 4 < 2 ? low_own(w[i / 4][i % 4], w[i / 4][i % 4 + 2]) : high_own(w[i / 4][i % 4], w[i / 4][i % 4 - 2]);
                 asm("" : "+v"(q[i]));
             }
         } else {
+            const int up = kTwoSets && c >= 8 ? 0 : 4;
 #pragma unroll
             for (int i = 0; i < VW / 2; ++i) {
                 const uint32_t v = w[i / 4][i % 4] ^ 0x88888888u;
-                q[i] = v << 4 & 0xf0f0f0f0u;
-                q[VW / 2 + i] = v & 0xf0f0f0f0u;
+                if constexpr (!kTwoSets) {
+                    q[i] = v << 4 & 0xf0f0f0f0u;
+                    q[VW / 2 + i] = v & 0xf0f0f0f0u;
+                } else {                               // lanes c < 8 keep and take low nibbles, the others high ones
+                    q[i] = low_own(v, v) << up & 0xf0f0f0f0u;
+                    q[VW / 2 + i] = high_own(v, v) << up & 0xf0f0f0f0u;
+                }
                 // (the compiler would rather extract nibbles one by one)
                 asm("" : "+v"(q[i]), "+v"(q[VW / 2 + i]));
             }
         }
+    }
+    // Dim of lane c's element x of them.
+    static __device__ __forceinline__ int v_element_dim(int x, int c) {
+        if constexpr (kTwoSets) return x / 8 * 128 + (c & 7) * 16 + (c >> 3) * 8 + x % 8;
+        else return c * DPL + x;
     }
     // Element x of position 4m + r of them.
     static __device__ __forceinline__ float v_byte(const uint32_t (&q)[VW], int r, int x) {
@@ -675,9 +697,9 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 // largest element and split into four signed 8-bit digits, a head's digits are four rows of the 16x16x32 product, and
 // a lane's four sums, exact in 32 bits, are one head's digits of one position: put together and times the block's
 // scale one fma. The weights go through LDS to the other operand's order. There a column stands for a head and one
-// of four blocks of V (head_dim 256: the contraction runs over both halves of the blocks, each half's codes beside
-// zeros for the other half's rows), and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
-// sums only those of a column's own block are meant. TERMS: bf16 terms of that product, 3 for all its 24 bits;
+// of four blocks of V, and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
+// sums only those of a column's own block are meant. (head_dim 256 has two sets of four blocks, each with products of its own:
+// in one, zeros would stand beside the other set's weights, and 0 times the scale NaN of a block is NaN in another.) TERMS: bf16 terms of that product, 3 for all its 24 bits;
 // 2 where rows are bf16 (its rounding is then 2^-7 of the outputs').
 // Three sequences of up to 131072 positions, 32 heads over 8 of 128 dims, Q4_0, fp32 rows (374 MB): 77-83 us, 4.5-4.9 TB/s,
 // of which the vector units are busy for 41 and the matrix cores for 15; sixteen of up to 2048, 4 heads over one of 256, Q8_0
@@ -775,7 +797,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
         mx[t] = -INFINITY;
         sum[t] = 0.f;                                  // this lane's position of every tile
     }
-    pf4 o[NT][DPL];                                    // o[t][x][r']: dim (4m + r') * DPL + x, column c
+    pf4 o[NT][DPL];                                    // o[t][x][r']: dim v_element_dim(x, 4m + r'), column c
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -864,7 +886,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
         // a wave's LDS accesses stay in order; the compiler is told
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        // contraction index 8m + 4i + r is position 4m + r of tile i, or of the tile and set i of blocks
+        // contraction index 8m + 4i + r is position 4m + r of tile i; of one tile and two sets, words 2i and 2i + 1 are set i's
         pu4 w[NT][TERMS];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -890,31 +912,32 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
             }
         uint32_t vb[HALVES][R::VW];
 #pragma unroll
-        for (int u = 0; u < HALVES; ++u) v[u].v_bytes(vb[u]);
+        for (int u = 0; u < HALVES; ++u) v[u].v_bytes(vb[u], c);
 #pragma unroll
         for (int x0 = 0; x0 < DPL; x0 += 2) {
-            pu4 code[2];                               // exact in bf16
+            pu4 code[2];                               // exact in bf16 (of one tile: two words)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int u = 0; u < HALVES; ++u)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t two = __builtin_amdgcn_perm(__float_as_uint(R::v_byte(vb[u], 2 * i + 1, x0 + e)),
+                        code[e][2 * u + i] = __builtin_amdgcn_perm(__float_as_uint(R::v_byte(vb[u], 2 * i + 1, x0 + e)),
                                                                    __float_as_uint(R::v_byte(vb[u], 2 * i, x0 + e)), 0x07060302u);
-                        if constexpr (SETS == 1) {
-                            code[e][2 * u + i] = two;
-                        } else {                       // row c is a dim of block c / 2
-                            code[e][i] = c < 8 ? two : 0u;
-                            code[e][2 + i] = c < 8 ? 0u : two;
-                        }
                     }
 #pragma unroll
             for (int q = 0; q < TERMS; ++q)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) o[t][x0 + e] = mfma16<DT_BF16>(code[e], w[t][q], o[t][x0 + e]);
+                    for (int e = 0; e < 2; ++e) {
+                        if constexpr (SETS == 1) {
+                            o[t][x0 + e] = mfma16<DT_BF16>(code[e], w[t][q], o[t][x0 + e]);
+                        } else {
+                            const int set = x0 / 8;
+                            o[t][x0 + e] = mfma8<DT_BF16>(pu2{code[e][0], code[e][1]}, pu2{w[t][q][2 * set], w[t][q][2 * set + 1]}, o[t][x0 + e]);
+                        }
+                    }
             // (two dims' codes at a time: all of them at once would not fit the registers)
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -934,11 +957,11 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            // rows 4m + r of the column's own block
-            const int blk = (4 * m + r) * DPL / 32;
-            if (blk % 4 != (c & 3)) continue;
+            // rows 4m + r of the column's own block (of both sets)
+            if (R::v_element_dim(0, 4 * m + r) / 32 != (c & 3)) continue;
 #pragma unroll
-            for (int x = 0; x < DPL; ++x) buf[(wid * HEADS + 4 * t + (c >> 2)) * LD + (4 * m + r) * DPL + x] = __fmul_rn(o[t][x][r], CT == DT_Q4_0 ? 0.0625f : 1.0f);
+            for (int x = 0; x < DPL; ++x)
+                buf[(wid * HEADS + 4 * t + (c >> 2)) * LD + R::v_element_dim(x, 4 * m + r)] = __fmul_rn(o[t][x][r], CT == DT_Q4_0 ? 0.0625f : 1.0f);
         }
     finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }

@@ -771,3 +771,61 @@ def test_beam_search_decode(hip, cache):
             spare = old                                        # the pages copied from are the next spares
         tok, score, done = to.numpy(), so.numpy(), eo.numpy()
     assert len(set(parents)) < B or done.any()                 # beams were dropped along the way
+
+
+def compare_special(got, lse, q, k, v, scale, io, n, weights=0.0):
+    """Outputs against 64 bits where some are NaN or infinite: these have to be the same, the others within the bound of an fp32
+    evaluation whose weights are off by `weights`, relative."""
+    with np.errstate(all="ignore"):
+        out, l, size, mean = ref.attention64(q, k, v, scale)
+        assert np.array_equal(np.isnan(got), np.isnan(out)), np.argwhere(np.isnan(got) != np.isnan(out))[:4]
+        inf = np.isinf(out)
+        assert np.array_equal(got[inf], out[inf]) and np.array_equal(np.isinf(got), inf)
+        tol, ltol = ref.attention_bound(io, False, q.shape[1], n, out, l, size, mean)
+        tol = tol + 2 * weights * mean
+        fin = np.isfinite(out)
+        assert (np.abs(got - out)[fin] <= tol[fin]).all(), np.nanmax((np.abs(got - out) / tol)[fin])
+        assert (np.abs(lse - l) <= ltol).all()
+
+
+def attend(c, table, lens, q, io, scale, nkv):
+    """(out, lse, q as it was rounded) of one call."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rq, ro = device_rows(q, io), device_rows(q * 0, io)
+    dt, dl, dlse = dev(table), dev(np.array(lens, np.int32)), DeviceArray.empty(q.shape[:2])
+    ws = DeviceArray(max(16, c.c.attention_workspace_bytes(len(lens), q.shape[1], max(lens))))
+    c.c.attention(0, rq[0], ro[0], PageTable(dt, *table.shape), dl, max(lens), scale, lse=dlse, workspace=ws)
+    sync()
+    return ref.from_type(io, ro[1].numpy()[:q.size]).reshape(q.shape).astype(np.float64), dlse.numpy(), ref.from_type(io, rq[3])
+
+
+@pytest.mark.parametrize("cache", [Q8_0, Q4_0], ids=ref.NAME.get)
+@pytest.mark.parametrize("io", [F32, BF16, F16], ids=ref.NAME.get)
+@pytest.mark.parametrize("hd,heads", [(64, 4), (64, 7), (128, 4), (128, 8), (256, 1), (256, 4), (256, 5), (256, 8), (256, 20)])
+def test_attention_nan_blocks_of_v(hip, cache, io, hd, heads):
+    """A NaN or an infinity in a block of V makes that block's dims NaN, in every head that reads it, and no other."""
+    rng = np.random.default_rng(hd + heads)
+    lens, ps = [200, 200, 1500, 37, 40], 48
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    ks, vs = [], []
+    for s, n in enumerate(lens):
+        k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+        if s == 0:
+            v[5, 0, 3] = np.nan
+        elif s == 1:
+            v[77, 0, hd - 1], v[199, 0, hd - 1] = np.inf, np.nan
+        elif s == 2:
+            v[0, 0, 32], v[1499, 0, hd - 40] = -np.inf, np.nan
+        elif s == 3:
+            v[36, 0, ::32] = np.nan            # all of them
+        ks.append(ref.stored(cache, k))
+        vs.append(ref.stored(cache, v))
+        c.fill(0, table, s, k, v)
+    c.upload()
+    got, lse, q = attend(c, table, lens, rng.normal(size=(len(lens), heads, hd)).astype(np.float32), io, 1 / np.sqrt(hd), 1)
+    for s, n in enumerate(lens):
+        assert np.isnan(got[s]).any() == (s < 4)
+        # bf16 rows: the weights' first 16 bits
+        compare_special(got[s], lse[s], q[s], ks[s], vs[s], 1 / np.sqrt(hd), io, n, 2.0**-15 if io == BF16 else 0.0)
