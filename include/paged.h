@@ -85,7 +85,9 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * positions. lengths outside [0, max_length] are taken as its nearest end; max_length is at most
  * table->ld * page_size. A sequence of length 0 gets out = 0 and lse = -inf, and so does one whose
  * scores are all -inf or whose pages do not exist. A NaN or +inf score makes the head's outputs NaN.
- * What lies behind a sequence's last position, NaN included, does not count. Over a quantized cache a
+ * What lies behind a sequence's last position, NaN included, does not count. A NaN in V makes its dim
+ * NaN (over a quantized cache its block's dims), an infinity makes it infinite; NaN where infinities of
+ * both signs meet, or one meets a weight that is 0 in fp32. Over a quantized cache a
  * NaN or an infinity in q makes its head's outputs NaN. (Weights reach 2^8 before they are scaled:
  * values of V above 2^119 can overflow the sums; over a quantized cache so can K above 2^86.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the

@@ -679,6 +679,40 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     }
     sum += __shfl_xor(sum, 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
+    if constexpr (HALF) {
+        // An infinity in V times a term of 0, or times terms of both signs, is NaN. Where O is NaN and the weights are not, the
+        // wave goes over its positions again, with the weights as they are (mx is the last one) on fp32 products.
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < DPL; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) odd |= o[x][r] != o[x][r];
+        if (__any(odd && sum == sum && c < at.heads)) {
+#pragma unroll
+            for (int x = 0; x < DPL; ++x) o[x] = pf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int t0 = at.lo + wid * HALVES * kPos; t0 < at.hi; t0 += STEP)
+#pragma unroll 1
+                for (int t = t0; t < min(t0 + HALVES * kPos, at.hi); t += kPos) {
+                    at.seek(g, t);
+                    k[0].load_k(a.c.k + at.at[0], at.ps, at.off[0], c, m);
+                    v[0].load_v(a.c.v + at.at[0], at.ps, at.off[0], c, m);
+                    pf4 s4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) s4 = mfma16<CT>(k[0].w[j], qh[j], s4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float p = __fmul_rn(s4[r], sl2);
+                        if (cap > 0.f) p = __fmul_rn(capped(p, cap), kLog2e);
+                        const bool on = at.there[0] && t + 4 * m + r >= at.start && t + 4 * m + r < at.hi;
+                        v[0].keep_v(r, on);
+                        p = on ? __builtin_amdgcn_exp2f(p - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+#pragma unroll
+                        for (int x = 0; x < DPL; ++x) o[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0].v_at(r, x), p, o[x], 0, 0, 0);
+                    }
+                }
+        }
+    }
     if (m == 0) {
         wm[wid][c] = mx;
         wsum[wid][c] = sum;

@@ -829,3 +829,34 @@ def test_attention_nan_blocks_of_v(hip, cache, io, hd, heads):
         assert np.isnan(got[s]).any() == (s < 4)
         # bf16 rows: the weights' first 16 bits
         compare_special(got[s], lse[s], q[s], ks[s], vs[s], 1 / np.sqrt(hd), io, n, 2.0**-15 if io == BF16 else 0.0)
+
+
+@pytest.mark.parametrize("cache,io", [(BF16, BF16), (F16, F16), (F32, F32), (BF16, F32), (F16, F32)],
+                         ids=["bf16", "f16", "f32", "bf16-f32", "f16-f32"])
+@pytest.mark.parametrize("hd,heads", [(64, 1), (64, 20), (128, 4), (128, 7), (256, 4), (256, 16)])
+def test_attention_infinite_v(hip, cache, io, hd, heads):
+    """Infinities in V reach their own dim as infinities of their sign, NaN where both signs meet or one is there already."""
+    rng = np.random.default_rng(hd + heads)
+    lens, ps = [200, 33, 1500, 40, 700], 32
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    ks, vs = [], []
+    for s, n in enumerate(lens):
+        k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+        if s == 0:
+            v[5, 0, 3], v[199, 0, hd - 1] = np.inf, -np.inf
+        elif s == 1:
+            v[32, 0, 0], v[31, 0, 0], v[0, 0, 9], v[7, 0, 10] = -np.inf, -np.inf, np.nan, np.inf
+        elif s == 2:
+            v[0, 0, 32], v[1499, 0, 32] = np.inf, -np.inf      # both: NaN
+            v[700:, 0, 33] = np.inf
+        elif s == 3:
+            k[:], v[:, 0, :20] = 0, np.inf                     # all weights alike
+        ks.append(ref.stored(cache, k))
+        vs.append(ref.stored(cache, v))
+        c.fill(0, table, s, k, v)
+    c.upload()
+    got, lse, q = attend(c, table, lens, rng.normal(size=(len(lens), heads, hd)).astype(np.float32), io, 1 / np.sqrt(hd), 1)
+    for s, n in enumerate(lens):
+        assert np.isinf(got[s]).any() == (s < 4)
+        compare_special(got[s], lse[s], q[s], ks[s], vs[s], 1 / np.sqrt(hd), io, n, 2.0**-16 if io != F32 else 0.0)
