@@ -71,7 +71,8 @@ int sapphire_paged_write_dev(const sapphire_paged_cache_t *cache, int layer, con
                              const int *positions, void *stream);
 
 /* The reverse: the rows at those places, as the values they stand for, rounded to the type of k and
- * v. Places that do not exist give zero rows. */
+ * v. Places that do not exist give zero rows. k and v share no element: they lie apart, or are slices
+ * of one buffer, of the same strides (rows between each other with other strides are refused). */
 int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, const sapphire_rows_t *k,
                             const sapphire_rows_t *v, const sapphire_page_table_t *table, const int *seqs,
                             const int *positions, void *stream);
@@ -91,7 +92,8 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * NaN or an infinity in q makes its head's outputs NaN. (Weights reach 2^8 before they are scaled:
  * values of V above 2^119 can overflow the sums; over a quantized cache so can K above 2^86.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the
- * same type or a quantized one. out is q itself (same data and strides) or shares no element with it.
+ * same type or a quantized one. out is q itself (same data and strides) or shares no element with it,
+ * as k and v of a read.
  * out is rounded once, at the end; with 16-bit rows the weights exp(s_p - max s) meet V with 16 bits
  * or more. lse: [tokens][n_heads] fp32, or NULL. Long sequences are cut into pieces that run side by
  * side and are joined by a second launch; the results do not depend on which workgroup runs when, nor

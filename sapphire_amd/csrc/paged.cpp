@@ -1,6 +1,9 @@
 // paged.cpp - the entry points of paged.h, and of sapphire_hip.h's rows of heads and beam search: checks of
 // what can be checked on the host, then the launches.
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <numeric>
 
 #include "../../include/paged.h"
 #include "paged_dev.h"
@@ -58,6 +61,44 @@ bool rows_ok(const sapphire_rows_t *r, const char *what, bool written) {
 bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + nb && y < x + na;
+}
+
+// Whether a and b, of one type, share no element, as far as their strides tell: their spans do not meet; or, as slices of one
+// buffer, they stay in different parts of a period (modulo the period a stride that is a multiple of it does not move; another
+// one adds its whole way to the part); or, of the same strides, no row of b starts within head_dim elements of one of a.
+bool apart(const sapphire_rows_t *a, const sapphire_rows_t *b) {
+    uint64_t na = 0, nb = 0;
+    if (!rows_span(a, na) || !rows_span(b, nb)) return false;
+    if (!overlap(a->data, na, b->data, nb)) return true;
+    const int64_t off = (reinterpret_cast<intptr_t>(b->data) - reinterpret_cast<intptr_t>(a->data)) / (a->dtype == DT_F32 ? 4 : 2);
+    auto differ = [&](int64_t period) {
+        if (period <= 0) return false;
+        auto part = [&](const sapphire_rows_t *r) {            // (below 2^60: rows_span)
+            int64_t n = r->head_dim;
+            if (r->tokens > 1 && r->token_stride % period != 0) n += (int64_t)(r->tokens - 1) * r->token_stride;
+            if (r->heads > 1 && r->head_stride % period != 0) n += (int64_t)(r->heads - 1) * r->head_stride;
+            return n;
+        };
+        const int64_t o = (off % period + period) % period;
+        return part(a) <= o && part(b) <= period - o;
+    };
+    auto step = [](int n, long long stride) { return n > 1 ? (int64_t)stride : 0; };
+    const int64_t ta = step(a->tokens, a->token_stride), tb = step(b->tokens, b->token_stride);
+    const int64_t ha = step(a->heads, a->head_stride), hb = step(b->heads, b->head_stride);
+    if (differ(std::gcd(std::gcd(ta, tb), std::gcd(ha, hb))) || (ta == tb && differ(ta)) || (ha == hb && differ(ha))) return true;
+    if (ta != tb || ha != hb) return false;
+    for (int64_t h = 1 - (int64_t)a->heads; h < b->heads; ++h) {       // b's head less a's; t: b's token less a's
+        const int64_t at = off + h * ha;
+        const int64_t t0 = ta ? -at / ta : 0;                          // (and its neighbours: at + t ta nearest to 0)
+        for (int64_t t = t0 - 1; t <= t0 + 1; ++t)
+            if (t > -(int64_t)a->tokens && t < b->tokens && std::llabs(at + t * ta) < std::max(a->head_dim, b->head_dim)) return false;
+    }
+    return true;
+}
+// The same rows in the same place.
+bool identical(const sapphire_rows_t *a, const sapphire_rows_t *b) {
+    return a->data == b->data && (a->tokens == 1 || a->token_stride == b->token_stride) &&
+           (a->heads == 1 || a->head_stride == b->head_stride);
 }
 
 Rows as_rows(const sapphire_rows_t *r) {
@@ -157,6 +198,7 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *c, int layer, const sa
                             const sapphire_page_table_t *t, const int *seqs, const int *positions, void *stream) {
     PagedCache pc;
     if (!move_ok(c, layer, k, v, t, seqs, positions, true, pc)) return -1;
+    if (!apart(k, v)) { set_error("paged read: k and v overlap"); return -1; }
     return launch_paged_read(pc, as_rows(k), as_rows(v), as_table(t), seqs, positions, as_stream(stream));
 }
 
@@ -191,6 +233,7 @@ int sapphire_paged_attention_dev(const sapphire_paged_cache_t *c, int layer, con
         set_error("paged attention: %d sequences, %d heads, %d table rows", q->tokens, q->heads, t->rows);
         return -1;
     }
+    if (!identical(q, out) && !apart(q, out)) { set_error("paged attention: out overlaps q without being q"); return -1; }
     if (max_length <= 0 || max_length > (int64_t)t->ld * c->page_size || max_length > (1 << 30)) {
         set_error("paged attention: max_length %d with %d pages of %d per row", max_length, t->ld, c->page_size);
         return -1;

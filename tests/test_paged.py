@@ -95,6 +95,34 @@ def test_attention_refused(lib, change):
     assert lib.sapphire_last_error()
 
 
+# (data, token stride, head stride) of three tokens of two heads of 64 dims, in elements from a first one of [256][64]
+OVERLAPS = [((0, 128, 64), (64, 128, 64)), ((0, 128, 64), (128, 128, 64)), ((128, 128, 64), (0, 128, 64)), ((0, 128, 64), (0, 256, 64)),
+            ((0, 128, 64), (0, 256, 128)), ((0, 64, 192), (64, 64, 192)), ((0, 64, 192), (0, 128, 64)), ((0, 256, 64), (127, 256, 64)),
+            ((0, 256, 64), (129, 256, 64)), ((0, 256, 128), (63, 256, 128)), ((0, 256, 128), (256, 256, 128)), ((0, 200, 64), (136, 200, 64)),
+            ((0, 0, 64), (64, 128, 64))]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ref.NAME.get)
+@pytest.mark.parametrize("a,b", OVERLAPS)
+def test_overlapping_rows_refused(lib, dtype, a, b):
+    """Rows that share elements in some other way than being each other: an attention's out with its q, a read's k with its v."""
+    es = 4 if dtype == F32 else 2
+    at = [{(off + t * ts + h * hs + d) for t in range(3) for h in range(2) for d in range(64)} for off, ts, hs in (a, b)]
+    assert at[0] & at[1]
+    c, t = cache(dtype), PageTableC(P, 3, 4)
+    x, y = (rows(dtype=dtype, data=4 * P + es * off, ts=ts, hs=hs) for off, ts, hs in (a, b))
+    assert lib.sapphire_paged_read_dev(C.byref(c), 0, C.byref(x), C.byref(y), C.byref(t), None, P, None) == -1
+    assert lib.sapphire_paged_attention_dev(C.byref(c), 0, C.byref(x), C.byref(y), C.byref(t), P, 128, C.byref(AttentionC(1.0, 0, 0.0)),
+                                            None, P, None) == -1
+    assert b"overlap" in lib.sapphire_last_error()
+
+
+def test_read_refuses_the_same_rows(lib):
+    c, t, r = cache(), PageTableC(P, 3, 4), rows()
+    assert lib.sapphire_paged_read_dev(C.byref(c), 0, C.byref(r), C.byref(r), C.byref(t), None, P, None) == -1
+    assert b"overlap" in lib.sapphire_last_error()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16, Q8_0, Q4_0], ids=ref.NAME.get)
 @pytest.mark.parametrize("nkv,heads", [(1, 1), (1, 40), (3, 12), (8, 64), (600, 600)])
 def test_workspace_is_enough_for_smaller_calls(lib, dtype, nkv, heads):

@@ -860,3 +860,53 @@ def test_attention_infinite_v(hip, cache, io, hd, heads):
     for s, n in enumerate(lens):
         assert np.isinf(got[s]).any() == (s < 4)
         compare_special(got[s], lse[s], q[s], ks[s], vs[s], 1 / np.sqrt(hd), io, n, 2.0**-16 if io != F32 else 0.0)
+
+
+@pytest.mark.parametrize("cache,io", [(F32, F32), (BF16, BF16), (Q4_0, F16)], ids=["f32", "bf16", "q4_0"])
+def test_slices_of_one_buffer(hip, cache, io):
+    """q and out beside each other in every token's row, K and V read to interleaved heads and to the two halves of one row:
+    the bits of calls with buffers of their own, and nothing between them written."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable, Rows
+    rng = np.random.default_rng(19)
+    hd, ps, heads, nkv, b = 64, 16, 4, 2, 3
+    es, lens = 4 if io == F32 else 2, [40, 3, 900]
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, nkv, hd)
+    for s, n in enumerate(lens):
+        c.fill(0, table, s, rng.normal(size=(n, nkv, hd)).astype(np.float32), rng.normal(size=(n, nkv, hd)).astype(np.float32))
+    c.upload()
+    q = ref.to_type(io, rng.normal(size=(b, heads, hd)).astype(np.float32))
+    dt, dl, pos = dev(table), dev(np.array(lens, np.int32)), dev(np.array(lens, np.int32) - 1)
+    pt = PageTable(dt, *table.shape)
+    ws = DeviceArray(max(16, c.c.attention_workspace_bytes(b, heads, max(lens))))
+    dq, out, k, v = dev(q), dev(np.zeros_like(q)), dev(np.zeros_like(q[:, :nkv])), dev(np.zeros_like(q[:, :nkv]))
+    plain = lambda d, h: Rows(d.ptr, io, b, h, hd)                      # noqa: E731
+    c.c.attention(0, plain(dq, heads), plain(out, heads), pt, dl, max(lens), 0.2, workspace=ws)
+    c.c.read(0, plain(k, nkv), plain(v, nkv), pt, pos)
+    sync()
+    want, wk, wv = out.numpy(), k.numpy(), v.numpy()
+    for at in ([0, heads + 1], [heads + 2, 1]):        # q first, out first
+        row = np.full((b, 2 * heads + 3, hd), 7, q.dtype)
+        row[:, at[0]:at[0] + heads] = q
+        d = dev(row)
+        rows = [Rows(d.ptr + es * hd * i, io, b, heads, hd, token_stride=row.shape[1] * hd) for i in at]
+        c.c.attention(0, *rows, pt, dl, max(lens), 0.2, workspace=ws)
+        sync()
+        row[:, at[1]:at[1] + heads] = want
+        np.testing.assert_array_equal(d.numpy(), row)
+    both = np.stack([wk, wv], 2)                       # [tokens][heads][2][hd]
+    for shape, ts, hs, step, ans in ((both.shape, 2 * nkv * hd, 2 * hd, hd, both),
+                                     ((b, 2, nkv, hd), 2 * nkv * hd, hd, nkv * hd, np.stack([wk, wv], 1)),
+                                     ((nkv, b, 2, hd), 2 * hd, 2 * b * hd, hd, both.transpose(1, 0, 2, 3))):
+        d = dev(np.zeros(shape, q.dtype))
+        c.c.read(0, *(Rows(d.ptr + es * step * i, io, b, nkv, hd, ts, hs) for i in (0, 1)), pt, pos)
+        sync()
+        np.testing.assert_array_equal(d.numpy(), ans)
+    hs = 2 * b * hd + hd                               # heads that start in the middle of a token's pair
+    host = np.zeros(nkv * hs, q.dtype)
+    d = dev(host)
+    c.c.read(0, *(Rows(d.ptr + es * hd * i, io, b, nkv, hd, 2 * hd, hs) for i in (0, 1)), pt, pos)
+    sync()
+    host.reshape(nkv, hs)[:, :2 * b * hd] = both.transpose(1, 0, 2, 3).reshape(nkv, -1)
+    np.testing.assert_array_equal(d.numpy(), host)
