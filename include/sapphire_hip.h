@@ -260,8 +260,9 @@ typedef struct {
  *   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c, s = magnitude * (cos, sin) of the angle.
  * The angle is formed and reduced in 64 bits, so far positions lose nothing; positions may be
  * negative. The remaining dims are copied. freqs: rotary_dim / 2 doubles in device memory
- * (sapphire_rope_frequencies). y is x itself (same data, strides and type) or does not overlap it;
- * both have one type. rotary_dim: even, 2 .. head_dim; head_dim at most 1024. */
+ * (sapphire_rope_frequencies). y is x itself (same data, strides and type) or shares no element with
+ * it: it lies apart, or both are slices of one buffer, of the same strides. Both have one type.
+ * rotary_dim: even, 2 .. head_dim; head_dim at most 1024. */
 typedef struct {
     const double *freqs;
     int rotary_dim;

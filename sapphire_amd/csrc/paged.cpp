@@ -288,12 +288,7 @@ int sapphire_rope_rows_dev(const sapphire_rows_t *x, const sapphire_rows_t *y, c
         set_error("rope: x and y must have one type and shape");
         return -1;
     }
-    uint64_t nx = 0, ny = 0;
-    rows_span(x, nx);
-    rows_span(y, ny);
-    const bool same = x->data == y->data && (x->tokens == 1 || x->token_stride == y->token_stride) &&
-                      (x->heads == 1 || x->head_stride == y->head_stride);
-    if (!same && overlap(x->data, nx, y->data, ny)) { set_error("rope: y overlaps x without being x"); return -1; }
+    if (!identical(x, y) && !apart(x, y)) { set_error("rope: y overlaps x without being x"); return -1; }
     return launch_rope_rows(as_rows(x), as_rows(y), positions, rope->freqs, rope->rotary_dim, rope->interleaved != 0,
                             rope->magnitude, as_stream(stream));
 }

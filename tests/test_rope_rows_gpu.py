@@ -103,3 +103,28 @@ def test_rope_rows_undone_by_negative_positions(hip):
     paged.rope(r[0], r[0], dev(-pos), df, 64)
     sync()
     assert np.abs(r[1].numpy()[:x.size].reshape(x.shape) - x).max() <= 2.0**-24 * 32 * np.abs(x).max()
+
+
+@pytest.mark.parametrize("io", [F32, BF16], ids=ref.NAME.get)
+@pytest.mark.parametrize("inter", [False, True], ids=["half", "pairs"])
+@pytest.mark.parametrize("rot", [64, 34])
+def test_rope_rows_between_slices_of_one_buffer(hip, io, inter, rot):
+    """From some heads of every token's row to others, behind them or ahead: the bits of a call with a y of its own, and
+    nothing else written."""
+    from sapphire_amd import paged
+    from sapphire_amd.paged import Rows
+    rng = np.random.default_rng(rot)
+    t, h, hd, H = 37, 3, 64, 8
+    es = 4 if io == F32 else 2
+    x = ref.to_type(io, rng.normal(size=(t, H, hd)).astype(np.float32))
+    dp, df = dev(rng.integers(0, 5000, t).astype(np.int32)), dev(paged.rope_frequencies(rot, 1e4)[0])
+    for src, dst in ((0, 3), (0, 5), (5, 1)):
+        dx, dy = dev(x), dev(x[:, :h] * 0)
+        def rows(d, first, width):
+            return Rows(d.ptr + es * hd * first, io, t, h, hd, token_stride=width * hd)
+        paged.rope(rows(dx, src, H), rows(dy, 0, h), dp, df, rot, interleaved=inter)
+        paged.rope(rows(dx, src, H), rows(dx, dst, H), dp, df, rot, interleaved=inter)
+        sync()
+        want = x.copy()
+        want[:, dst:dst + h] = dy.numpy()
+        np.testing.assert_array_equal(dx.numpy(), want)
