@@ -89,8 +89,10 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * What lies behind a sequence's last position, NaN included, does not count. A NaN in V makes its dim
  * NaN (over a quantized cache its block's dims), an infinity makes it infinite; NaN where infinities of
  * both signs meet, or one meets a weight that is 0 in fp32. Over a quantized cache a
- * NaN or an infinity in q makes its head's outputs NaN. (Weights reach 2^8 before they are scaled:
- * values of V above 2^119 can overflow the sums; over a quantized cache so can K above 2^86.)
+ * NaN or an infinity in q makes its head's outputs NaN. (Sums are of up to 2^8 times the
+ * values before they are scaled: they do not overflow where the largest |V| times the number of
+ * positions is below 2^119, over Q4_0 2^115, nor those of the scores over a quantized cache where |K|
+ * is below 2^85.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the
  * same type or a quantized one. out is q itself (same data and strides) or shares no element with it,
  * as k and v of a read.

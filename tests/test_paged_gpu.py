@@ -910,3 +910,54 @@ def test_slices_of_one_buffer(hip, cache, io):
     sync()
     host.reshape(nkv, hs)[:, :2 * b * hd] = both.transpose(1, 0, 2, 3).reshape(nkv, -1)
     np.testing.assert_array_equal(d.numpy(), host)
+
+
+@pytest.mark.parametrize("cache,io", [(F32, F32), (BF16, F32), (BF16, BF16), (Q8_0, F32), (Q8_0, BF16), (Q4_0, F32), (Q4_0, BF16)],
+                         ids=["f32", "bf16-f32", "bf16", "q8_0", "q8_0-bf16", "q4_0", "q4_0-bf16"])
+@pytest.mark.parametrize("hd,heads", [(64, 4), (128, 8), (256, 4), (256, 8)])
+def test_attention_of_the_largest_values(hip, cache, io, hd, heads):
+    """V just below 2^119 (Q4_0: 2^115) over the number of positions, nearly all of them with weights of almost 2^8: the
+    maximum stays that of the first tiles, which scores up to 8 log2 units above it do not move. Whole sequences, so that
+    every wave's first tiles lie in the first 128 positions."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PageTable
+    rng = np.random.default_rng(hd)
+    n, ps, batch = 2048, 256, 512
+    table = np.repeat(rng.permutation(n // ps).astype(np.int32)[None], batch, 0)
+    c = Cache(cache, 1, n // ps, ps, 1, hd)
+    k, v = np.zeros((n, 1, hd), np.float32), np.empty((n, 1, hd), np.float32)
+    k[128:, 0, 0] = 7.9 * np.log(2)
+    v[...] = 2.0**(119 - 11 - (4 if cache == Q4_0 else 0)) * 0.99
+    v[:, 0, ::3] *= -0.7
+    c.fill(0, table, 0, k, v)
+    c.upload()
+    q = np.zeros((batch, heads, hd), np.float32)
+    q[..., 0] = 1.0
+    rq, ro = device_rows(q, io), device_rows(q, io)
+    dt, dl, dlse = dev(table), dev(np.full(batch, n, np.int32)), DeviceArray.empty((batch, heads))
+    ws = DeviceArray(max(16, c.c.attention_workspace_bytes(batch, heads, n)))
+    c.c.attention(0, rq[0], ro[0], PageTable(dt, *table.shape), dl, n, 1.0, lse=dlse, workspace=ws)
+    sync()
+    got = ref.from_type(io, ro[1].numpy()[:q.size]).reshape(q.shape).astype(np.float64)
+    assert (got == got[:1, :1]).all()
+    compare_special(got[0], dlse.numpy()[0], q[0], ref.stored(cache, k), ref.stored(cache, v), 1.0, io, n,
+                    0.0 if io == F32 else 2.0**-16 if cache == BF16 else 2.0**-15)
+
+
+@pytest.mark.parametrize("cache", CACHES[:2] + CACHES[3:], ids=ref.NAME.get)
+@pytest.mark.parametrize("hd,heads", [(64, 4), (128, 7), (256, 4), (256, 8)])
+def test_attention_of_the_largest_keys(hip, cache, hd, heads):
+    """K just below 2^85 in every dim, under queries of one sign that bring the scores back."""
+    rng = np.random.default_rng(hd)
+    n, ps = 150, 16
+    table, pages = tables(rng, [n], ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    k = np.full((n, 1, hd), 2.0**85 * 0.99, np.float32)
+    k[1::3] *= -1
+    k[2::3, 0, ::2] *= -0.4
+    v = rng.normal(size=(n, 1, hd)).astype(np.float32)
+    c.fill(0, table, 0, k, v)
+    c.upload()
+    q = (rng.uniform(0.5, 1, (1, heads, hd)) * 2.0**-85).astype(np.float32)
+    got, lse, q = attend(c, table, [n], q, F32, 1 / hd, 1)
+    compare_special(got[0], lse[0], q[0], ref.stored(cache, k), ref.stored(cache, v), 1 / hd, F32, n)
