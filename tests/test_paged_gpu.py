@@ -961,3 +961,36 @@ def test_attention_of_the_largest_keys(hip, cache, hd, heads):
     q = (rng.uniform(0.5, 1, (1, heads, hd)) * 2.0**-85).astype(np.float32)
     got, lse, q = attend(c, table, [n], q, F32, 1 / hd, 1)
     compare_special(got[0], lse[0], q[0], ref.stored(cache, k), ref.stored(cache, v), 1 / hd, F32, n)
+
+
+# the weights' bits that meet V: two roundings to the rows' type over a cache of that type (fp16: of 2^-22, and of half the
+# smallest subnormal, 2^-25, for a largest weight of 2^7 at least), over a quantized one the first 16 bits, truncated, for bf16 rows
+# and all 24 otherwise
+WEIGHTS = {(BF16, BF16): 2.0**-16, (F16, F16): 2.0**-21, (Q8_0, BF16): 2.0**-15, (Q4_0, BF16): 2.0**-15}
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+@pytest.mark.parametrize("hd,heads", [(64, 8), (128, 4), (256, 5)])
+def test_attention_weights_keep_their_bits(hip, cache, io, hd, heads):
+    """Sums that nearly cancel show the weights' own rounding, which an output's would hide: half of the positions weigh 1 and
+    have values about 1, the others weigh a third and have values of about -3. Beside them random rows. lse is fp32's."""
+    rng = np.random.default_rng(hd)
+    lens, ps, scale = [300, 300, 77, 1], 48, 1.0 if hd == 64 else 0.5
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    q = rng.normal(size=(len(lens), heads, hd)).astype(np.float32)
+    q[0] = 0
+    q[0, :, 0] = (1 + 0.01 * np.arange(heads)) / scale
+    ks, vs = [], []
+    for s, n in enumerate(lens):
+        k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+        if s == 0:
+            k[:], v[:] = 0, 1
+            k[1::2, 0, 0], v[1::2] = -np.log(3), -np.linspace(2.9, 3.1, hd)
+        ks.append(ref.stored(cache, k))
+        vs.append(ref.stored(cache, v))
+        c.fill(0, table, s, k, v)
+    c.upload()
+    got, lse, q = attend(c, table, lens, q, io, scale, 1)
+    for s, n in enumerate(lens):
+        compare_special(got[s], lse[s], q[s], ks[s], vs[s], scale, io, n, WEIGHTS.get((cache, io), 0.0))
