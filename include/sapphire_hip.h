@@ -213,11 +213,14 @@ int sapphire_sample_dev(float *logits, int n, int batch, int ld, float temperatu
  * beams b and tokens v < n,
  *   score(b, v) = scores[b] + logits[b][v] - log sum exp logits[b]
  * and the `beams` best go on, best first: by the score in 64 bits, of equal ones the lowest b, then
- * the larger logit, then the lowest v. scores_out is rounded to fp32. A row with done != 0 has
- * ended: its one continuation is end_token at its score unchanged. Tokens of score -inf (a logit of
- * -inf or NaN; every token of a row whose score is not finite or that has a logit of +inf) are taken
- * only when fewer than `beams` others are left. tokens[i], parents[i] (the row it continues, r * beams + b) and done_out[i] (its
- * parent's done, or token == end_token) describe row i's new beam. done and done_out may both be
+ * the larger logit, then the lowest v. (log sum exp is of fp32 exponentials, added up in 64 bits, and
+ * off by about 2^-20 at most: candidates of different beams that are closer than that can change
+ * places; those of one beam, or of rows alike, cannot.) scores_out is rounded to fp32. A row with
+ * done != 0 has ended: its one continuation is end_token at its score unchanged. Tokens of score -inf
+ * (a logit of -inf or NaN; every token of a row whose score is not finite or that has a logit of +inf)
+ * are taken only when fewer than `beams` others are left. tokens[i], parents[i] (the row it continues,
+ * r * beams + b) and done_out[i] (its parent's done, or token == end_token) describe row i's new beam.
+ * done and done_out may both be
  * NULL (no row has ended); an end_token outside [0, n) never matches, and a done row then has
  * no continuation. logits: rows of stride ld >= n, left as they are. scores_out may be scores, done_out
  * may be done. workspace: sapphire_beam_workspace_bytes() bytes of device memory, 16-byte aligned;
@@ -258,8 +261,8 @@ typedef struct {
  * token t turn by positions[t] * freqs[i] for pair i < rotary_dim / 2, which is dims (i, i +
  * rotary_dim / 2), or (2i, 2i + 1) when interleaved:
  *   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c, s = magnitude * (cos, sin) of the angle.
- * The angle is formed and reduced in 64 bits, so far positions lose nothing; positions may be
- * negative. The remaining dims are copied. freqs: rotary_dim / 2 doubles in device memory
+ * The angle is formed and reduced in 64 bits, so that positions of millions lose nothing; positions
+ * may be negative. The remaining dims are copied. freqs: rotary_dim / 2 doubles in device memory
  * (sapphire_rope_frequencies). y is x itself (same data, strides and type) or shares no element with
  * it: it lies apart, or both are slices of one buffer, of the same strides. Both have one type.
  * rotary_dim: even, 2 .. head_dim; head_dim at most 1024. */

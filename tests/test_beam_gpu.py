@@ -155,3 +155,24 @@ def test_far_maxima(hip, n, top, rest):
     if abs(top) > 2e12:                        # there the oracle's own m + log s is coarse; the best score is 0 all the same
         np.testing.assert_array_equal(got[0][::W], 0.0)
     assert (np.abs(got[0][fin] - want[0][fin]) <= tol).all()
+
+
+@pytest.mark.parametrize("shift", [0.0, 1000.0, -1e6])
+@pytest.mark.parametrize("R,W,n", [(2, 4, 3000), (1, 16, 100001), (40, 8, 60000), (1, 1, 262144)])
+def test_normaliser(hip, R, W, n, shift):
+    """Scores within the normaliser's error (2^-18: see test_far_maxima; of rows whose maximum moves at a handful of
+    batches), however far the logits are from zero. Those are multiples of 1/8, which a shift leaves as they are; the tokens
+    and parents are compared where no other candidate is that near."""
+    rng = np.random.default_rng(n)
+    rows = R * W
+    x = np.round(rng.normal(size=(rows, n)) * 24).astype(np.float32) / 8 + np.float32(shift)
+    x[0] = np.round(np.linspace(-9, 9, n) * 8).astype(np.float32) / 8 + np.float32(shift)
+    score = -np.abs(rng.normal(size=rows) * 4).astype(np.float32)
+    got = select(x, n, score, None, R, W, -1)
+    want = ref.beams64(x, score, np.zeros(rows, int), R, W, -1)
+    tol = 2.0**-18 + 4 * 2.0**-53 * abs(shift) + 2.0**-24 * np.abs(want[0])
+    assert (np.abs(got[0] - want[0]) <= tol).all()
+    clear = np.array([np.sum(np.abs(want[0] - s) < 1e-5) == 1 for s in want[0]])
+    clear[W - 1::W] = False                    # (the last one's rival may not be among them)
+    np.testing.assert_array_equal(got[1][clear], want[1][clear])
+    np.testing.assert_array_equal(got[2][clear], want[2][clear])
