@@ -350,8 +350,10 @@ int chunk_of(int n, int chunks) { return (n + chunks - 1) / chunks; }
 
 }  // namespace
 
+// Enough for calls of fewer rows too, which have more chunks: rows times chunks is at most kWantGroups, or one chunk each.
 size_t beam_workspace_bytes(int n, int rows, int beams) {
-    return (size_t)rows * chunks_of(n, rows) * (beams * sizeof(u64) + sizeof(Norm));
+    const size_t slots = std::min((size_t)rows * ((n + kChunkMin - 1) / kChunkMin), (size_t)std::max(kWantGroups, rows));
+    return slots * (beams * sizeof(u64) + sizeof(Norm));
 }
 
 int launch_beam_select(const float *logits, int ld, int n, int requests, int beams, const float *scores, const int *done,

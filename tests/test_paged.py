@@ -174,6 +174,18 @@ def test_beam_refused(lib):
     assert lib.sapphire_beam_workspace_bytes(262144, 8, 8) > 0
 
 
+@pytest.mark.parametrize("n", [16, 2048, 2049, 5000, 262144, 2**21])
+def test_beam_workspace_is_enough_for_smaller_calls(lib, n):
+    """More of anything never needs less. What a call uses is a slot of `beams` keys (8 bytes) and a partial sum (16) for each
+    row and chunk of it, min(2048 / rows, n / 2048) chunks, one at least."""
+    need = np.array([[lib.sapphire_beam_workspace_bytes(n, r, w) for w in range(1, 17)] for r in range(1, 700)], dtype=np.int64)
+    assert (np.diff(need, axis=0) >= 0).all() and (np.diff(need, axis=1) >= 0).all()
+    assert lib.sapphire_beam_workspace_bytes(max(16, n - 1), 41, 7) <= lib.sapphire_beam_workspace_bytes(n, 41, 7)
+    rows = np.arange(1, 700)[:, None] * np.arange(1, 17)
+    chunks = np.minimum(np.maximum(1, 2048 // rows), -(-n // 2048))
+    assert (need >= rows * chunks * (8 * np.arange(1, 17) + 16)).all()
+
+
 @pytest.mark.parametrize("rot,base", [(2, 10000.0), (64, 10000.0), (256, 1e6), (18, 500.0)])
 def test_frequencies(rot, base):
     """Each is one pow and at most a few more roundings in 64 bits."""
