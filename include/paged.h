@@ -87,12 +87,11 @@ int sapphire_paged_read_dev(const sapphire_paged_cache_t *cache, int layer, cons
  * table->ld * page_size. A sequence of length 0 gets out = 0 and lse = -inf, and so does one whose
  * scores are all -inf or whose pages do not exist. A NaN or +inf score makes the head's outputs NaN.
  * What lies behind a sequence's last position, NaN included, does not count. A NaN in V makes its dim
- * NaN (over a quantized cache its block's dims), an infinity makes it infinite; NaN where infinities of
- * both signs meet, or one meets a weight that is 0 in fp32. Over a quantized cache a
- * NaN or an infinity in q makes its head's outputs NaN. (Sums are of up to 2^8 times the
- * values before they are scaled: they do not overflow where the largest |V| times the number of
- * positions is below 2^119, over Q4_0 2^115, nor those of the scores over a quantized cache where |K|
- * is below 2^85.)
+ * NaN whatever its weight (over a quantized cache its block's dims), an infinity makes it infinite, or
+ * NaN where infinities of both signs meet or one meets a weight that is 0 in fp32. Over a quantized
+ * cache a NaN or an infinity in q makes its head's outputs NaN. (Sums are of up to 2^8 times the values
+ * before they are scaled: they do not overflow where the largest |V| times the number of positions is
+ * below 2^119, over Q4_0 2^115, nor those of the scores over a quantized cache where |K| is below 2^85.)
  * q and out: q->tokens x n_heads x head_dim, both of one type: F32; or BF16 / F16 over a cache of the
  * same type or a quantized one. out is q itself (same data and strides) or shares no element with it,
  * as k and v of a read.

@@ -1033,15 +1033,15 @@ __global__ __launch_bounds__(W *kWave) void paged_join_kernel(AttnArgs g) {
     }
     top = lanes::wave_max(top);
     float f[Q], tot = 0.f;
-    unsigned long long mask[Q];                        // pieces that count: an empty one has written no O
+    unsigned long long mask[Q];                        // pieces with an O (a sequence of length 0 has none)
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         f[q] = 0.f;
         mask[q] = 0;
         if (q * kWave >= used) continue;
-        // a sum of NaN has a weight of NaN, whatever its maximum
-        const bool on = lane + q * kWave < used && ms[q].y != 0.f;
-        f[q] = !on ? 0.f : ms[q].y != ms[q].y ? ms[q].y : __builtin_amdgcn_exp2f(ms[q].x - top);
+        // a sum of NaN has a weight of NaN, whatever its maximum; one of 0 the weight 0 (its O may be NaN)
+        const bool on = lane + q * kWave < used && n > 0;
+        f[q] = !on || ms[q].y == 0.f ? 0.f : ms[q].y != ms[q].y ? ms[q].y : __builtin_amdgcn_exp2f(ms[q].x - top);
         tot = __builtin_fmaf(on ? ms[q].y : 0.f, f[q], tot);
         mask[q] = __ballot(on);
     }

@@ -994,3 +994,35 @@ def test_attention_weights_keep_their_bits(hip, cache, io, hd, heads):
     got, lse, q = attend(c, table, lens, q, io, scale, 1)
     for s, n in enumerate(lens):
         compare_special(got[s], lse[s], q[s], ks[s], vs[s], scale, io, n, WEIGHTS.get((cache, io), 0.0))
+
+
+@pytest.mark.parametrize("cache,io", [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16)], ids=["f32", "bf16-f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads", [2, 9])
+def test_attention_nan_v_where_scores_are_minus_infinity(hip, cache, io, heads):
+    """A NaN of V makes its dim NaN whatever its weight, in a tile with others as in a wave's or a piece's share in which
+    nothing else weighs; unless no score of the sequence is above -inf."""
+    rng = np.random.default_rng(heads)
+    hd, ps, lens = 64, 32, [40, 700, 3000, 50]
+    table, pages = tables(rng, lens, ps)
+    c = Cache(cache, 1, pages, ps, 1, hd)
+    ks, vs = [], []
+    for s, n in enumerate(lens):
+        k, v = (rng.normal(size=(n, 1, hd)).astype(np.float32) for _ in range(2))
+        k[:n // 2 if s < 3 else n, 0, 0] = -np.inf
+        v[5, 0, 3], v[n // 2 - 1, 0, 60] = np.nan, np.nan
+        ks.append(k)
+        vs.append(ref.stored(cache, v))
+        c.fill(0, table, s, k, v)
+    c.upload()
+    q = rng.normal(size=(len(lens), heads, hd)).astype(np.float32)
+    q[..., 0] = 1.0
+    got, lse, q = attend(c, table, lens, q, io, 0.125, 1)
+    assert (got[3] == 0).all() and np.isneginf(lse[3]).all()
+    for s, n in enumerate(lens[:3]):
+        assert np.isnan(got[s][:, [3, 60]]).all(), s
+        rest = np.arange(hd)[~np.isin(np.arange(hd), [3, 60])]
+        k = ref.stored(cache, ks[s][n // 2:])
+        out, l, size, mean = ref.attention64(q[s], k, vs[s][n // 2:], 0.125)
+        tol, ltol = ref.attention_bound(io, False, hd, n, out, l, size, mean)
+        tol = tol + 2 * WEIGHTS.get((cache, io), 0.0) * mean
+        assert (np.abs(got[s] - out) <= tol)[:, rest].all() and (np.abs(lse[s] - l) <= ltol).all(), s
