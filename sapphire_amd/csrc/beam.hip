@@ -4,10 +4,11 @@
 // wave keeps its best W (logit, index) keys, and beside that it sums exp. The rows' lists and normalisers
 // meet in the second launch, where the scores of the W x W candidates left are formed and compared in 64 bits.
 //
-// 64 rows of 262144 logits, a quarter of them ended (50 MB read): the pass 16.8 us (3.0 TB/s), the second launch 5.1. The
-// pass is bound by the vector units: nine operations and an exp per logit are half of its time, and the rest is the
-// latency of first loads, lists and joins, which at a copy's rate would be 10 us for the bytes. Four rows of 4096: 4.7 and
-// 2.9 us, launches and latency.
+// 64 rows of 262144 logits, a quarter of them ended (50 MB read): the pass 16.3 us (3.1 TB/s), the second launch 5.1. Half
+// of the pass is vector issue, 25 instructions per logit of a lane: about seven make its part of the maximum and the sum, a few
+// compare it, and most look for keys, since a wave of that size has one batch and must find a value that W of it reach, some
+// keys above it and their order for that alone. The rest is the latency of first loads, lists and joins, where a
+// copy's rate would be 10 us for the bytes. Four rows of 4096: 4.8 and 2.9 us, launches and latency.
 #include <algorithm>
 
 #include "internal.h"

@@ -16,8 +16,10 @@
 //   quantized cache                         K's codes in 8-bit products with q's digits, V's codes as bf16
 //
 // Whole calls over 400 MB of K and V, sequences of 2000 positions, head_dim 64 to 256: up to four heads per K/V head
-// 72-101 us (4.0-5.5 TB/s; a large copy moves 4.9), eight heads 77-108 us over float caches, 90-118 over Q8_0, 126-170
-// over Q4_0, whose conversions keep the vector units busier than the bytes keep the memory.
+// 73-103 us (3.9-5.5 TB/s; a large copy moves 4.9), eight heads 78-107 us over float caches, 87-118 over Q8_0, 115-154
+// over Q4_0. There vector and matrix units take turns at two waves per SIMD: of 91 us (100 sequences of up to 2000, 8 K/V heads
+// of 256 dims) 49 are vector issue and 36 matrix cores. Sixteen heads over a quantized cache read and convert K and V twice:
+// 137-255 us.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -229,6 +231,15 @@ __device__ __forceinline__ pf4 mfma16(pu4 a, pu4 b, pf4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8, a), __builtin_bit_cast(pb8, b), c, 0, 0, 0);
 }
 
+// The same over 16 positions: two words a lane.
+typedef short ps4 __attribute__((ext_vector_type(4)));
+typedef _Float16 ph4 __attribute__((ext_vector_type(4)));
+template <int CT>
+__device__ __forceinline__ pf4 mfma8(pu2 a, pu2 b, pf4 c) {
+    if constexpr (CT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(ph4, a), __builtin_bit_cast(ph4, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ps4, a), __builtin_bit_cast(ps4, b), c, 0, 0, 0);
+}
+
 // The sequence that workgroups z take when the longest go first, by eighths of max_length (in order within one): where
 // whole sequences are a workgroup's work, a long one started late would run alone at the end. The same in every
 // workgroup. masks: 64 words of LDS per 512 sequences.
@@ -267,15 +278,6 @@ __device__ __forceinline__ int nth_longest(const int *__restrict__ lengths, int 
         z -= __shfl(upto, kWave - 1, kWave);
     }
     return 0;                                          // (not reached: every sequence is in a class)
-}
-
-// The same over 16 positions: two words a lane.
-typedef short ps4 __attribute__((ext_vector_type(4)));
-typedef _Float16 ph4 __attribute__((ext_vector_type(4)));
-template <int CT>
-__device__ __forceinline__ pf4 mfma8(pu2 a, pu2 b, pf4 c) {
-    if constexpr (CT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(ph4, a), __builtin_bit_cast(ph4, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(ps4, a), __builtin_bit_cast(ps4, b), c, 0, 0, 0);
 }
 
 // A workgroup's part of the call: a piece of one sequence, for one K/V head's query heads h0 .. h0 + heads - 1,
@@ -733,7 +735,8 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 // scale one fma. The weights go through LDS to the other operand's order. There a column stands for a head and one
 // of four blocks of V, and carries weight times that block's scale, so that V's codes come in as small bf16 integers; of the
 // sums only those of a column's own block are meant. (head_dim 256 has two sets of four blocks, each with products of its own:
-// in one, zeros would stand beside the other set's weights, and 0 times the scale NaN of a block is NaN in another.) TERMS: bf16 terms of that product, 3 for all its 24 bits;
+// in one, zeros would stand beside the other set's weights, and 0 times the scale NaN of a block is NaN in another; 100
+// sequences of up to 2000 positions, 64 heads over 8, Q4_0: 91 us, and 95 with the zeros.) TERMS: bf16 terms of that product, 3 for all its 24 bits;
 // 2 where rows are bf16 (its rounding is then 2^-7 of the outputs').
 // Three sequences of up to 131072 positions, 32 heads over 8 of 128 dims, Q4_0, fp32 rows (374 MB): 77-83 us, 4.5-4.9 TB/s,
 // of which the vector units are busy for 41 and the matrix cores for 15; sixteen of up to 2048, 4 heads over one of 256, Q8_0

@@ -7,8 +7,9 @@
 //
 // Bytes bound a prompt's rows, with the vector units close behind: 8192 tokens of 8 heads of 128 dims, bf16 to Q4_0 (K and
 // V, 44 MB), are written in 13.4 us and read back in 10.6 (3.3 and 4.2 TB/s; a large copy moves 4.9), 7 and 6 us of that
-// being instruction issue: a code takes a product, a sum, a minimum and a conversion. A decode step's rows (16 tokens of a
-// head) are one memory latency after another, position -> page -> row: 3.0 and 2.9 us.
+// being instruction issue: an element written takes 17 vector instructions (conversion, the block's largest of both signs,
+// product, sum, minimum, conversion, packing, a share of the loads and addresses), one read 13. A decode step's rows (16
+// tokens of a head) are one memory latency after another, position -> page -> row: 3.0 and 2.9 us.
 #include <algorithm>
 #include <climits>
 

@@ -26,7 +26,7 @@ struct RopeArgs {
     float magnitude;
 };
 
-// VEC elements of 16 bytes, or single ones.
+// N elements: 16 bytes, or a single one.
 template <int DT, bool WIDE>
 struct Piece {
     static constexpr int N = WIDE ? (DT == DT_F32 ? 4 : 8) : 1;
