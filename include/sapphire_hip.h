@@ -220,11 +220,11 @@ int sapphire_sample_dev(float *logits, int n, int batch, int ld, float temperatu
  * (a logit of -inf or NaN; every token of a row whose score is not finite or that has a logit of +inf)
  * are taken only when fewer than `beams` others are left. tokens[i], parents[i] (the row it continues,
  * r * beams + b) and done_out[i] (its parent's done, or token == end_token) describe row i's new beam.
- * done and done_out may both be
- * NULL (no row has ended); an end_token outside [0, n) never matches, and a done row then has
- * no continuation. logits: rows of stride ld >= n, left as they are. scores_out may be scores, done_out
+ * done and done_out may both be NULL (no row has ended); an end_token outside [0, n) never matches,
+ * and a done row then has no continuation. logits: rows of stride ld >= n, left as they are. scores_out may be scores, done_out
  * may be done. workspace: sapphire_beam_workspace_bytes() bytes of device memory, 16-byte aligned,
- * which are enough for calls of fewer requests, beams and tokens too; calls sharing one must be ordered. 1 <= beams <= 16, beams <= n <= 2^21. */
+ * which are enough for calls of fewer requests, beams and tokens too; calls sharing one must be
+ * ordered. 1 <= beams <= 16, beams <= n <= 2^21. */
 size_t sapphire_beam_workspace_bytes(int n, int requests, int beams);
 int sapphire_beam_select_dev(const float *logits, int ld, int n, int requests, int beams, const float *scores,
                              const int *done, int end_token, float *scores_out, int *tokens, int *parents,
