@@ -214,8 +214,9 @@ int sapphire_sample_dev(float *logits, int n, int batch, int ld, float temperatu
  *   score(b, v) = scores[b] + logits[b][v] - log sum exp logits[b]
  * and the `beams` best go on, best first: by the score in 64 bits, of equal ones the lowest b, then
  * the larger logit, then the lowest v. (log sum exp is of fp32 exponentials, added up in 64 bits, and
- * off by about 2^-20 at most: candidates of different beams that are closer than that can change
- * places; those of one beam, or of rows alike, cannot.) scores_out is rounded to fp32. A row with
+ * off by up to about 2^-20, more where a row's maximum rises a hundred times along it: candidates of
+ * different beams that are closer than that can change places; those of one beam, or of rows alike,
+ * cannot.) scores_out is rounded to fp32. A row with
  * done != 0 has ended: its one continuation is end_token at its score unchanged. Tokens of score -inf
  * (a logit of -inf or NaN; every token of a row whose score is not finite or that has a logit of +inf)
  * are taken only when fewer than `beams` others are left. tokens[i], parents[i] (the row it continues,
