@@ -41,7 +41,7 @@ def listed():
         # Three drafted tokens of one sequence over the small test vocabulary: the smallest call.
         {"name": "verify-small", "kind": "verify", "requests": 1, "drafts": 3, "n": 4096, "draft": True, "temperature": 1.0},
         # A batch with five drafts each over the whole Gemma-3 vocabulary, by a draft model of the same one.
-        {"name": "verify-vocab", "kind": "verify", "requests": 16, "drafts": 5, "n": 262144, "draft": True, "temperature": 0.8},
+        {"name": "verify-vocab", "kind": "verify", "requests": 16, "drafts": 5, "n": 262144, "draft": True, "temperature": 0.75},
         # Drafts looked up in the prompt: no probabilities of their own.
         {"name": "verify-lookup", "kind": "verify", "requests": 8, "drafts": 4, "n": 262144, "draft": False, "temperature": 1.0},
         # The forward pass that verifies five drafts of one chat: six rows of the 270M shape over an fp32 cache.
@@ -91,7 +91,7 @@ def draw(rng):
     c = {"kind": kind}
     if kind == "verify":
         d = rng.randint(1, 8)
-        c.update(drafts=d, n=_log_int(rng, 500, 262144), draft=rng.random() < 0.7, temperature=rng.choice([1.0, 0.7, 1.3, 0.0]))
+        c.update(drafts=d, n=_log_int(rng, 500, 262144), draft=rng.random() < 0.7, temperature=rng.choice([1.0, 0.75, 1.25, 0.0]))
         c["requests"] = _log_int(rng, 1, 176 // (2 * d + 1))
     elif kind == "shared":
         h, kv, hd = _heads(rng)
