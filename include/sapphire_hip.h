@@ -231,6 +231,28 @@ int sapphire_beam_select_dev(const float *logits, int ld, int n, int requests, i
                              const int *done, int end_token, float *scores_out, int *tokens, int *parents,
                              int *done_out, void *workspace, void *stream);
 
+/* ---- drafted tokens ----
+ * Which of a request's drafted tokens the target model's probabilities keep, and the token behind them (speculative
+ * decoding). Request r has draft_tokens[r * drafts + i], i < counts[r] (NULL: all `drafts`; taken into
+ * 0 .. drafts), the target's logits before each of them and behind the last, rows r * (drafts + 1) + i of `logits`
+ * (stride ld >= n), and the draft model's, rows r * drafts + i of draft_logits (stride draft_ld >= n), or NULL for drafts
+ * without probabilities, as from a lookup: q is then 1 at the draft. With p = softmax(logits / temperature), q likewise:
+ *   draft x stays while draws[r][i] * q_i(x) < p_i(x); the first one that does not, i = a, ends the drafts
+ *   the next token is the first t with sum_{v <= t} w(v) > draws[r][drafts] * sum w, w = max(p_a - q_a, 0), or p behind
+ *   the last draft or where that is 0 everywhere (the last t with w(t) > 0 if a rounding leaves none)
+ * so that the tokens are distributed as the target's own, whatever the draft model. temperature <= 0: drafts stay
+ * while they are the first of the largest logits of their row, which is the next token too; draft_logits and
+ * draws are not looked at. All in 64 bits. draws: [requests][drafts + 1], taken into 0 .. 1 (NaN: 0). A NaN logit counts as
+ * -inf; where a row's largest is infinite, the entries equal to it share the probability. A drafted token outside
+ * [0, n) does not stay. tokens[r * (drafts + 1) + i]: the drafts that stay, the next token, then -1; accepted[r]: how many
+ * stay. Rows of logits behind counts[r] are not read. Outputs overlap neither each other nor inputs. workspace:
+ * sapphire_verify_workspace_bytes() bytes of device memory, 16-byte aligned, which are enough for smaller calls too;
+ * calls sharing one must be ordered. 1 <= drafts <= 64, 1 <= n <= 2^21, requests * (2 drafts + 1) < 65536. */
+size_t sapphire_verify_workspace_bytes(int n, int requests, int drafts);
+int sapphire_verify_dev(const float *logits, int ld, const float *draft_logits, int draft_ld, int n, int requests,
+                        int drafts, const int *draft_tokens, const int *counts, float temperature, const float *draws,
+                        int *tokens, int *accepted, void *workspace, void *stream);
+
 /* ---- device copies of tensor_t weights ----
  * The device-resident copy kernel_gemv keeps for a 2-D weight tensor (Q4_0/Q8_0 in the
  * PACKED layout, F32/BF16 as is), created on first use; *layout receives its layout.

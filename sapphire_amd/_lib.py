@@ -120,6 +120,8 @@ def load_library(path: str):
     P("sapphire_rope_frequencies", i32, [vp, C.POINTER(f32), i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double])
     P("sapphire_beam_workspace_bytes", sz, [i32, i32, i32])
     P("sapphire_beam_select_dev", i32, [vp, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp])
+    P("sapphire_verify_workspace_bytes", sz, [i32, i32, i32])
+    P("sapphire_verify_dev", i32, [vp, i32, vp, i32, i32, i32, i32, vp, vp, f32, vp, vp, vp, vp, vp])
     # paged.h
     P("sapphire_paged_cache_bytes", sz, [vp])
     P("sapphire_paged_write_dev", i32, [vp, i32, vp, vp, vp, vp, vp, vp])

@@ -345,4 +345,39 @@ int sapphire_beam_select_dev(const float *logits, int ld, int n, int requests, i
                               done_out, workspace, as_stream(stream));
 }
 
+static bool verify_shape_ok(int n, int requests, int drafts) {
+    return drafts >= 1 && drafts <= 64 && n >= 1 && n <= (1 << 21) && requests >= 1 && (int64_t)requests * (2 * drafts + 1) <= kGridYZ;
+}
+
+size_t sapphire_verify_workspace_bytes(int n, int requests, int drafts) {
+    return verify_shape_ok(n, requests, drafts) ? verify_workspace_bytes(n, requests, drafts) : 0;
+}
+
+int sapphire_verify_dev(const float *logits, int ld, const float *draft_logits, int draft_ld, int n, int requests, int drafts,
+                        const int *draft_tokens, const int *counts, float temperature, const float *draws, int *tokens,
+                        int *accepted, void *workspace, void *stream) {
+    if (!logits || ld < n || (draft_logits && draft_ld < n) || !draft_tokens || !tokens || !accepted || !workspace) {
+        set_error("bad verify arguments");
+        return -1;
+    }
+    if (!verify_shape_ok(n, requests, drafts)) {
+        set_error("verify: 1..64 drafts, 1..2^21 logits per row, up to 65535 rows (n %d, %d requests of %d drafts)", n, requests, drafts);
+        return -1;
+    }
+    if (!(std::fabs(temperature) < INFINITY) || (temperature > 0.0f && !draws)) {
+        set_error("verify: temperature %g%s", (double)temperature, draws ? "" : ", no draws");
+        return -1;
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("the verify workspace must be 16-byte aligned"); return -1; }
+    const uint64_t rb = (uint64_t)requests * sizeof(int), db = rb * drafts, tb = rb * (drafts + 1);
+    if (overlap(tokens, tb, accepted, rb) || overlap(tokens, tb, draft_tokens, db) || overlap(accepted, rb, draft_tokens, db) ||
+        (counts && (overlap(tokens, tb, counts, rb) || overlap(accepted, rb, counts, rb))) ||
+        (draws && (overlap(tokens, tb, draws, tb) || overlap(accepted, rb, draws, tb)))) {
+        set_error("verify: outputs overlap inputs or one another");
+        return -1;
+    }
+    return launch_verify(logits, ld, draft_logits, draft_ld, n, requests, drafts, draft_tokens, counts, temperature, draws, tokens,
+                         accepted, workspace, as_stream(stream));
+}
+
 }  // extern "C"

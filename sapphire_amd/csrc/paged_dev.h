@@ -212,5 +212,9 @@ size_t beam_workspace_bytes(int n, int rows, int beams);
 int launch_beam_select(const float *logits, int ld, int n, int requests, int beams, const float *scores, const int *done,
                        int end_token, float *scores_out, int *tokens, int *parents, int *done_out, void *ws,
                        hipStream_t s);
+size_t verify_workspace_bytes(int n, int requests, int drafts);
+int launch_verify(const float *logits, int ld, const float *draft_logits, int draft_ld, int n, int requests, int drafts,
+                  const int *draft_tokens, const int *counts, float temperature, const float *draws, int *tokens, int *accepted,
+                  void *ws, hipStream_t s);
 
 }  // namespace sapphire

@@ -60,6 +60,18 @@ def beam_select(logits, ld, n, requests, beams, scores, scores_out, tokens, pare
         check(-1, "beam select")
 
 
+def verify_workspace_bytes(n, requests, drafts) -> int:
+    return load().sapphire_verify_workspace_bytes(n, requests, drafts)
+
+
+def verify(logits, ld, n, requests, drafts, draft_tokens, draws, tokens, accepted, workspace, draft_logits=None, draft_ld=0, counts=None,
+           temperature=1.0, stream=None) -> None:
+    """How many of each request's drafted tokens stay, and the token behind them."""
+    if load().sapphire_verify_dev(_at(logits), ld, _at(draft_logits), draft_ld, n, requests, drafts, _at(draft_tokens), _at(counts),
+                                  temperature, _at(draws), _at(tokens), _at(accepted), _at(workspace), stream):
+        check(-1, "verify")
+
+
 class PagedCache:
     """Pages of K and V rows of every layer. k and v: device buffers of `nbytes` each; allocated when not given."""
 
