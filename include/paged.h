@@ -114,6 +114,35 @@ int sapphire_paged_attention_dev(const sapphire_paged_cache_t *cache, int layer,
                                  int max_length, const sapphire_attention_t *attention, float *lse, void *workspace,
                                  void *stream);
 
+/* Bounds of K per page, for the choice below: of each dim the lowest and the highest value of the page's written rows, as
+ * 16 bits (F16 over an F16 cache, else BF16; values of other types rounded down and up). bounds: a buffer of
+ * sapphire_paged_bounds_bytes(), 16-byte aligned, [layers][pages][n_kv_heads][2][head_dim], low ones first. A call makes those
+ * of the pages that hold positions start[b] .. lengths[b] - 1 of table row b (every row of the table; start NULL: from 0;
+ * both taken into 0 .. ld * page_size), from all their positions below lengths[b]. So a program calls it after each
+ * sapphire_paged_write_dev, with start = the first position written, and for a page that sapphire_paged_reorder_dev copied.
+ * max_new: at least lengths[b] - start[b]; of more positions the last max_new's pages are made. A NaN in K makes its dim's
+ * bounds NaN. Rows that share a page write the same to it if they are of the same length there; else which is unspecified. */
+size_t sapphire_paged_bounds_bytes(const sapphire_paged_cache_t *cache);
+int sapphire_paged_bounds_dev(const sapphire_paged_cache_t *cache, int layer, void *bounds, const sapphire_page_table_t *table,
+                              const int *start, const int *lengths, int max_new, void *stream);
+
+/* The pages of each sequence and K/V head that its new token attends to. With lo and hi the bounds of a page of row b, its
+ * score is the largest, over the query heads h of the K/V head, of sum_d max(q_hd lo_d, q_hd hi_d): no q . k of the page is
+ * larger (a positive scale is assumed). choice->pages are chosen, all if there are no more: the first `first` and the last `last`
+ * of the ceil(lengths[b] / page_size) pages, and the others by score, in 64 bits, of equal ones the first. A score of NaN, as
+ * from bounds or a q that are not finite, counts as +inf. Pages that do not exist are not chosen.
+ * selected[b][head][0 .. pages): their places in the sequence (page p / page_size of position p), rising, then -1. q: tokens x
+ * n_heads x head_dim as for the attention, of any of the three types. lengths and max_length as there.
+ * first + last <= pages. workspace: sapphire_paged_select_workspace_bytes() bytes, 16-byte aligned, which are enough for
+ * calls of fewer and shorter sequences too; calls that share one must be ordered. */
+typedef struct {
+    int pages, first, last;
+} sapphire_page_choice_t;
+size_t sapphire_paged_select_workspace_bytes(const sapphire_paged_cache_t *cache, int batch, int max_length);
+int sapphire_paged_select_dev(const sapphire_paged_cache_t *cache, int layer, const void *bounds, const sapphire_rows_t *q,
+                              const sapphire_page_table_t *table, const int *lengths, int max_length,
+                              const sapphire_page_choice_t *choice, int *selected, void *workspace, void *stream);
+
 /* After sapphire_beam_select_dev: row b continues row p = parents[b] of `table`, of which lengths[p]
  * positions are written. Row b of table_out gets p's full pages (shared, not copied); a partly
  * filled last page is copied, in every layer and head, to page spare[b], which takes its place: its

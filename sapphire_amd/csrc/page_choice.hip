@@ -1,0 +1,483 @@
+// page_choice.hip - the choice of pages: bounds of K per page, and the pages whose bounds promise the largest scores.
+//
+// With lo <= k <= hi in every dim of a page, q . k <= sum_d max(q_d lo_d, q_d hi_d) for all of its rows, so that pages are
+// ranked without reading them. Borders between chosen and left pages are as close as scores come, so that sums run in 64 bits
+// and ties go by the page's place in the sequence.
+#include <algorithm>
+
+#include "internal.h"
+#include "lanes.h"
+#include "paged_dev.h"
+
+namespace sapphire {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
+
+struct BoundsArgs {
+    PagedCache c;
+    PageTable table;
+    const int *from, *lengths;
+    int slots;                             // pages of a row that the grid has
+    uint16_t *bounds;                      // the layer's: [pages][heads][2][hd]
+};
+
+__device__ __forceinline__ float low_of(float a, float b) { return __builtin_elementwise_minimum(a, b); }      // (NaN stays)
+__device__ __forceinline__ float high_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// fp32 to 16 bits, rounded up or down. The values of a cache of that type stay as they are.
+template <int CT>
+__device__ __forceinline__ uint32_t outward(float x, bool up) {
+    if constexpr (CT == DT_F16) return to_f16(x);
+    if (x != x) return 0x7fc0u;
+    const uint32_t u = __float_as_uint(x);
+    return ((u >> 31 != 0) == up ? u : u + 0xffffu) >> 16;
+}
+
+// The dims of a lane (c, m) of 16 positions of K: values e of piece j, and where they are. (The layout is that of the attention's
+// operands: a lane has position c, so that bounds are the extremes over c.)
+template <int CT, int HD>
+struct Part {
+    using T = Tile<CT, HD>;
+    static constexpr int PARTS = HD > 128 ? 2 : 1;                         // of the dims: the extremes of 128 fit the registers
+    static constexpr int W = CT == DT_F32 ? 4 : 8, N = HD / (4 * W) / PARTS;           // values of a piece, pieces
+    static constexpr int B = CT == DT_Q4_0 ? 4 * T::G : 16;                // bytes of a load
+    static constexpr int L = T::ROW / 4 / B / PARTS, NB = T::NB / PARTS;   // loads, scales
+    uint32_t w[L][B / 4];
+    float s[T::kQuant ? NB : 1];
+
+    __device__ __forceinline__ void load(const uint8_t *tile, uint32_t ps, uint32_t p0, int part, int c, int m) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const uint8_t *p = tile + T::k_code(p0, 0) + (uint32_t)(((part * L + l) * 4 + m) * 16 + c) * B;
+            if constexpr (B == 8) *reinterpret_cast<pu2 *>(w[l]) = *reinterpret_cast<const pu2 *>(p);
+            else *reinterpret_cast<pu4 *>(w[l]) = *reinterpret_cast<const pu4 *>(p);
+        }
+        if constexpr (T::kQuant) {
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                const pf2 v = *reinterpret_cast<const pf2 *>(tile + T::k_scale(ps, p0 + c, part * NB + b));
+                s[b] = v.x;
+                s[b + 1] = v.y;
+            }
+        }
+    }
+    static __device__ __forceinline__ int dim(int j, int m) { return (4 * j + m) * W; }
+    __device__ __forceinline__ float at(int j, int e) const {
+        if constexpr (CT == DT_F32) return __uint_as_float(w[j][e]);
+        else if constexpr (CT == DT_BF16) return __uint_as_float(e & 1 ? w[j][e / 2] & 0xffff0000u : w[j][e / 2] << 16);
+        else if constexpr (CT == DT_F16) return from_f16(e & 1 ? w[j][e / 2] >> 16 : w[j][e / 2] & 0xffffu);
+        else if constexpr (CT == DT_Q8_0) return __fmul_rn((float)(int8_t)(w[j / 2][j % 2 * 2 + e / 4] >> (8 * (e % 4))), s[j]);
+        else return __fmul_rn((float)((int)(w[j / T::G][j % T::G] << (28 - 8 * (e % 4) - 4 * (e / 4))) >> 28), s[j]);
+    }
+};
+
+// A wave per page and K/V head (two for 256 dims): lane (c, m) has position c of every tile and a quarter of the dims. The
+// bytes of K bound it. grid (pages / 4, heads x parts, rows).
+template <int CT, int HD>
+__global__ __launch_bounds__(kThreads) void paged_bounds_kernel(BoundsArgs g) {
+    using P = Part<CT, HD>;
+    const int lane = threadIdx.x & (kWave - 1), c = lane & 15, m = lane >> 4;
+    const int b = blockIdx.z, hk = blockIdx.y / P::PARTS, part = blockIdx.y % P::PARTS, ps = g.c.page_size;
+    const int n = (int)min((int64_t)max(g.lengths[b], 0), (int64_t)g.table.ld * ps);
+    const int from = g.from ? min(max(g.from[b], 0), n) : 0;
+    if (from >= n) return;
+    const int last = (int)page_of(g.c, (uint32_t)(n - 1) >> 4), first = max((int)page_of(g.c, (uint32_t)from >> 4), last - g.slots + 1);
+    const int i = first + blockIdx.x * kWaves + (threadIdx.x / kWave);
+    if (i > last) return;
+    const int page = g.table.pages[(size_t)b * g.table.ld + i];
+    if (page < 0 || page >= g.c.pages) return;
+    const int here = min(n - i * ps, ps);                      // positions written
+    const uint8_t *tile = g.c.k + ((size_t)page * g.c.nkv + hk) * g.c.tile_bytes;
+    float lo[P::N][P::W], hi[P::N][P::W];
+#pragma unroll
+    for (int j = 0; j < P::N; ++j)
+#pragma unroll
+        for (int e = 0; e < P::W; ++e) {
+            lo[j][e] = INFINITY;
+            hi[j][e] = -INFINITY;
+        }
+    P k;
+    k.load(tile, ps, 0, part, c, m);
+#pragma unroll 1
+    for (int t = 0; t < here; t += 16) {
+        const P x = k;
+        if (t + 16 < here) k.load(tile, ps, t + 16, part, c, m);
+        if (t + 16 <= here) {
+#pragma unroll
+            for (int j = 0; j < P::N; ++j)
+#pragma unroll
+                for (int e = 0; e < P::W; ++e) {
+                    const float v = x.at(j, e);
+                    lo[j][e] = low_of(lo[j][e], v);
+                    hi[j][e] = high_of(hi[j][e], v);
+                }
+        } else if (t + c < here) {                             // positions behind the last one do not count
+#pragma unroll
+            for (int j = 0; j < P::N; ++j)
+#pragma unroll
+                for (int e = 0; e < P::W; ++e) {
+                    const float v = x.at(j, e);
+                    lo[j][e] = low_of(lo[j][e], v);
+                    hi[j][e] = high_of(hi[j][e], v);
+                }
+        }
+    }
+    uint16_t *out = g.bounds + ((size_t)page * g.c.nkv + hk) * 2 * HD + (c & 1) * HD + part * (HD / P::PARTS);
+#pragma unroll
+    for (int j = 0; j < P::N; ++j) {
+        uint32_t w[P::W];
+#pragma unroll
+        for (int e = 0; e < P::W; ++e) {
+            float a = lo[j][e], z = hi[j][e];
+            // (the steps of row16_max)
+            a = low_of(a, lanes::dpp_mov<0xB1>(a)), z = high_of(z, lanes::dpp_mov<0xB1>(z));
+            a = low_of(a, lanes::dpp_mov<0x4E>(a)), z = high_of(z, lanes::dpp_mov<0x4E>(z));
+            a = low_of(a, lanes::dpp_mov<0x141>(a)), z = high_of(z, lanes::dpp_mov<0x141>(z));
+            a = low_of(a, lanes::dpp_mov<0x140>(a)), z = high_of(z, lanes::dpp_mov<0x140>(z));
+            w[e] = c & 1 ? outward<CT>(z, true) : outward<CT>(a, false);
+        }
+        if (c >> 1 == j % 8) {                                 // lanes 2j and 2j + 1 have the low and the high ones to write
+            if constexpr (P::W == 4) *reinterpret_cast<pu2 *>(out + P::dim(j, m)) = pu2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+            else *reinterpret_cast<pu4 *>(out + P::dim(j, m)) = pu4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
+        }
+    }
+}
+
+// ---- the choice ----
+
+constexpr int kHeads = 4;                  // query heads of a wave: their q takes 128 registers in 64 bits
+constexpr u64 kForced = ~0ull;             // above every score's key
+
+struct SelectArgs {
+    PagedCache c;
+    PageTable table;
+    Rows q;
+    const uint16_t *bounds;
+    const int *lengths;
+    int max_length, max_pages, group, k, first, last;
+    u64 *keys;                             // [batch][K/V heads][max_pages]
+    int *selected;
+};
+
+__device__ __forceinline__ int pages_of(const SelectArgs &g, int b) {
+    const int n = min(max(g.lengths[b], 0), g.max_length);
+    return n ? (int)page_of(g.c, (uint32_t)(n - 1) >> 4) + 1 : 0;
+}
+// Larger scores have larger keys, NaN the one of +inf; none is 0.
+__device__ __forceinline__ u64 key_of(double s) {
+    s = s != s ? INFINITY : s + 0.0;
+    const u64 u = (u64)__double_as_longlong(s);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// Eight dims of a page per lane, HD / 8 lanes per page; every page's score, as a key, by four query heads at a time. Pages that
+// are taken anyway have the largest key, ones that do not exist 0. grid (pages, K/V heads, sequences).
+template <int HD, bool F16>
+__global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
+    constexpr int LP = HD / 8, PW = kWave / LP, STEP = kWaves * PW;        // lanes of a page, pages of a wave and of a workgroup
+    const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave, l = lane % LP;
+    const int b = blockIdx.z, hk = blockIdx.y, np = pages_of(g, b);
+    const int i0 = blockIdx.x * STEP + wid * PW + lane / LP;
+    if ((int)blockIdx.x * STEP >= np) return;
+    const int *row = g.table.pages + (size_t)b * g.table.ld;
+    u64 *keys = g.keys + ((size_t)b * g.c.nkv + hk) * g.max_pages;
+    const uint16_t *of_head = g.bounds + (size_t)hk * 2 * HD + l * 8;
+    const size_t stride = (size_t)g.c.nkv * 2 * HD;
+    for (int h0 = 0; h0 < g.group; h0 += kHeads) {
+        double up[kHeads][8], down[kHeads][8];                 // q where it is positive, and where it is negative
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            Raw8 r;
+            float x[8];
+            // (heads behind the last one repeat it)
+            load8(g.q.dtype, false, g.q.p, (int64_t)b * g.q.ts + (int64_t)(hk * g.group + min(h0 + h, g.group - 1)) * g.q.hs + l * 8, r);
+            values8(g.q.dtype, r, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                up[h][e] = x[e] > 0.f ? x[e] : x[e] != x[e] ? x[e] : 0.f;
+                down[h][e] = x[e] < 0.f ? x[e] : 0.f;
+            }
+        }
+        pu4 lo, hi;
+        int page = 0;
+        auto load = [&](int at) {
+            page = at < np ? row[at] : -1;
+            const uint16_t *p = of_head + (page >= 0 && page < g.c.pages ? (size_t)page : 0) * stride;
+            lo = *reinterpret_cast<const pu4 *>(p);
+            hi = *reinterpret_cast<const pu4 *>(p + HD);
+        };
+        load(i0);
+#pragma unroll 1
+        for (int i = i0; i - lane / LP < np; i += gridDim.x * STEP) {
+            const pu4 a = lo, z = hi;
+            const bool there = page >= 0 && page < g.c.pages;
+            load(i + gridDim.x * STEP);
+            double s[kHeads] = {};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t wa = e & 1 ? a[e / 2] >> 16 : a[e / 2] & 0xffffu, wz = e & 1 ? z[e / 2] >> 16 : z[e / 2] & 0xffffu;
+                const double x = F16 ? from_f16(wa) : from_bf16(wa), y = F16 ? from_f16(wz) : from_bf16(wz);
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) s[h] = __builtin_fma(up[h][e], y, __builtin_fma(down[h][e], x, s[h]));
+            }
+            // the lanes' sums
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+                for (int off = 1; off < LP; off *= 2) s[h] += __shfl_xor(s[h], off, kWave);
+            u64 key = 0;
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) {
+                const u64 o = key_of(s[h]);
+                key = o > key ? o : key;
+            }
+            if (l == 0 && i < np) {
+                if (!there) key = 0;
+                else if (i < g.first || i >= np - g.last) key = kForced;
+                else if (h0 > 0) key = keys[i] > key ? keys[i] : key;
+                keys[i] = key;
+            }
+        }
+    }
+}
+
+// The k largest keys of a sequence's K/V head, equal ones from the first page on, in order of the pages. One workgroup; keys of up
+// to 8192 pages stay in its registers. By ten bits at a time from the highest one in which keys differ, until the keys that
+// decide are few enough to be ranked against each other. grid (K/V heads, sequences).
+constexpr int kPick = 1024, kPickWaves = kPick / kWave, kHold = 8, kBins = 1024, kFew = 64;
+__global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
+    __shared__ int bins[kBins], counts[2][kHold][kPickWaves], wave_sums[kPickWaves];
+    __shared__ u64 ors[kPickWaves], ands[kPickWaves], few[kFew], few_key;
+    __shared__ int few_count, found[3], few_ties;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
+    const int hk = blockIdx.x, b = blockIdx.y, np = pages_of(g, b);
+    int *out = g.selected + ((size_t)b * g.c.nkv + hk) * g.k;
+    const u64 *keys = g.keys + ((size_t)b * g.c.nkv + hk) * g.max_pages;
+    const int blocks = (np + kHold * kPick - 1) / (kHold * kPick);
+    u64 key[kHold];
+    auto load = [&](int blk) {
+#pragma unroll
+        for (int e = 0; e < kHold; ++e) {
+            const int i = (blk * kHold + e) * kPick + tid;
+            key[e] = i < np ? keys[i] : 0;
+        }
+    };
+    auto block_sum = [&](int v) {                              // of all threads
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) v += __shfl_xor(v, off, kWave);
+        __syncthreads();
+        if (lane == 0) wave_sums[wid] = v;
+        __syncthreads();
+        int s = 0;
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) s += wave_sums[w];
+        return s;
+    };
+    // pages taken anyway, the others that exist, and the bits in which those differ
+    int forced = 0, others = 0;
+    u64 any = 0, all = ~0ull;
+    for (int blk = 0; blk < blocks; ++blk) {
+        load(blk);
+#pragma unroll
+        for (int e = 0; e < kHold; ++e) {
+            forced += key[e] == kForced;
+            if (key[e] != 0 && key[e] != kForced) {
+                ++others;
+                any |= key[e];
+                all &= key[e];
+            }
+        }
+    }
+    forced = block_sum(forced);
+    others = block_sum(others);
+    int need = min(max(g.k - forced, 0), others), shift = 0;
+    u64 edge = 0;                                              // keys >> shift above it are taken, the first `need` that equal it too
+    if (need == others) {
+        edge = 0;                                              // (no key is 0)
+        need = 0;
+    } else if (need == 0) {
+        edge = kForced - 1;
+    } else {
+        // (need < others, so that there is a key that decides)
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) {
+            any |= __shfl_xor(any, off, kWave);
+            all &= __shfl_xor(all, off, kWave);
+        }
+        if (lane == 0) {
+            ors[wid] = any;
+            ands[wid] = all;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) {
+            any |= ors[w];
+            all &= ands[w];
+        }
+        int top = any == all ? 0 : 64 - __builtin_clzll(any ^ all);        // keys agree from this bit on
+        u64 prefix = top == 64 ? 0 : any >> top;
+        edge = prefix;
+        shift = top;
+        while (top > 0) {
+            shift = max(top - 10, 0);
+            const uint32_t mask = (1u << (top - shift)) - 1;
+            bins[tid] = 0;
+            if (tid == 0) few_count = 0;
+            __syncthreads();
+            for (int blk = 0; blk < blocks; ++blk) {
+                if (blocks > 1) load(blk);
+#pragma unroll
+                for (int e = 0; e < kHold; ++e)
+                    if (key[e] != 0 && key[e] != kForced && (top == 64 ? 0 : key[e] >> top) == prefix)
+                        atomicAdd(&bins[(uint32_t)(key[e] >> shift) & mask], 1);
+            }
+            __syncthreads();
+            // how many keys are above each bin: thread t has bin 1023 - t
+            const int mine = bins[kBins - 1 - tid];
+            int upto = mine;
+#pragma unroll
+            for (int off = 1; off < kWave; off *= 2) {
+                const int o = __shfl_up(upto, off, kWave);
+                upto += lane >= off ? o : 0;
+            }
+            if (lane == kWave - 1) wave_sums[wid] = upto;
+            __syncthreads();
+            for (int w = 0; w < wid; ++w) upto += wave_sums[w];
+            if (upto >= need && upto - mine < need) {
+                found[0] = kBins - 1 - tid;
+                found[1] = need - (upto - mine);
+                found[2] = mine;
+            }
+            __syncthreads();
+            prefix = prefix << (top - shift) | (u64)found[0];
+            edge = prefix;
+            need = found[1];
+            top = shift;
+            const int count = found[2];
+            if (count == need || top == 0) break;
+            if (count <= kFew) {
+                // the keys that decide, each one's place among them
+                for (int blk = 0; blk < blocks; ++blk) {
+                    if (blocks > 1) load(blk);
+#pragma unroll
+                    for (int e = 0; e < kHold; ++e)
+                        if (key[e] != 0 && key[e] != kForced && key[e] >> shift == prefix) few[atomicAdd(&few_count, 1)] = key[e];
+                }
+                __syncthreads();
+                if (tid < count) {
+                    int above = 0, same = 0;
+                    for (int j = 0; j < count; ++j) {
+                        above += few[j] > few[tid];
+                        same += few[j] == few[tid];
+                    }
+                    if (above < need && above + same >= need) {            // (all that equal it write the same)
+                        few_key = few[tid];
+                        few_ties = need - above;
+                    }
+                }
+                __syncthreads();
+                edge = few_key;
+                need = few_ties;
+                shift = 0;
+                break;
+            }
+        }
+    }
+    // in order of the pages: of every thousand the places of each wave's, from the counts of those ahead
+    int taken_before = 0, ties_before = 0;
+    for (int blk = 0; blk < blocks; ++blk) {
+        if (blocks > 1) load(blk);
+        u64 above[kHold], ties[kHold];
+#pragma unroll
+        for (int e = 0; e < kHold; ++e) {
+            const u64 v = key[e] >> shift;
+            const bool on = key[e] != 0, is_forced = key[e] == kForced;
+            above[e] = __ballot(on && (is_forced || v > edge));
+            ties[e] = __ballot(on && !is_forced && v == edge);
+            if (lane == 0) {
+                counts[0][e][wid] = __popcll(above[e]);
+                counts[1][e][wid] = __popcll(ties[e]);
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int e = 0; e < kHold; ++e) {
+            int a = taken_before, t = ties_before, ea = 0, et = 0;
+            for (int w = 0; w < kPickWaves; ++w) {
+                const int ca = counts[0][e][w], ct = counts[1][e][w];
+                if (w < wid) a += ca, t += ct;
+                ea += ca;
+                et += ct;
+            }
+            const u64 below = (1ull << lane) - 1;
+            u64 ma = 0, mt = 0;
+#pragma unroll
+            for (int j = 0; j < kHold; ++j)
+                if (j == e) ma = above[j], mt = ties[j];
+            a += __popcll(ma & below);
+            t += __popcll(mt & below);
+            const bool is_above = ma >> lane & 1, is_tie = (mt >> lane & 1) && t < need;
+            if (is_above || is_tie) out[a + min(t, need)] = (blk * kHold + e) * kPick + tid;
+            taken_before += ea;
+            ties_before += et;
+        }
+        __syncthreads();
+    }
+    const int total = taken_before + min(ties_before, need);
+    for (int i = total + tid; i < g.k; i += kPick) out[i] = -1;
+}
+
+}  // namespace
+
+int launch_paged_bounds(const PagedCache &c, uint16_t *bounds, const PageTable &t, const int *from, const int *lengths, int max_new,
+                        hipStream_t s) {
+    BoundsArgs g;
+    g.c = c;
+    g.table = t;
+    g.from = from;
+    g.lengths = lengths;
+    g.slots = std::min((max_new - 1) / c.page_size + 2, t.ld);
+    g.bounds = bounds;
+    const dim3 grid((g.slots + kWaves - 1) / kWaves, c.nkv * (c.hd > 128 ? 2 : 1), t.rows), block(kThreads);
+#define SPH_BOUNDS(CT, HD) \
+    if (c.dtype == CT && c.hd == HD) hipLaunchKernelGGL((paged_bounds_kernel<CT, HD>), grid, block, 0, s, g);
+#define SPH_BOUNDS_HD(HD) SPH_BOUNDS(DT_F32, HD) SPH_BOUNDS(DT_BF16, HD) SPH_BOUNDS(DT_F16, HD) SPH_BOUNDS(DT_Q8_0, HD) SPH_BOUNDS(DT_Q4_0, HD)
+    SPH_BOUNDS_HD(64) SPH_BOUNDS_HD(128) SPH_BOUNDS_HD(256)
+    return hip_ok(hipGetLastError(), "paged bounds launch") ? 0 : -1;
+}
+
+size_t paged_select_workspace(int nkv, int batch, int max_pages) { return (size_t)batch * nkv * max_pages * sizeof(u64); }
+
+int launch_paged_select(const PagedCache &c, const uint16_t *bounds, const Rows &q, const PageTable &t, const int *lengths, int max_length,
+                        int k, int first, int last, int *selected, void *ws, hipStream_t s) {
+    SelectArgs g;
+    g.c = c;
+    g.table = t;
+    g.q = q;
+    g.bounds = bounds;
+    g.lengths = lengths;
+    g.max_length = max_length;
+    g.max_pages = (max_length + c.page_size - 1) / c.page_size;
+    g.group = q.heads / c.nkv;
+    g.k = k;
+    g.first = first;
+    g.last = last;
+    g.keys = static_cast<u64 *>(ws);
+    g.selected = selected;
+    const int step = kWaves * 512 / c.hd;
+    // q's 64-bit values are loaded once per workgroup: a few steps each where there are many
+    const int64_t pairs = (int64_t)q.tokens * c.nkv, steps = (g.max_pages + step - 1) / step;
+    const int64_t want = std::max<int64_t>(1, 2048 / pairs);
+    const dim3 grid((unsigned)std::min(steps, want), c.nkv, q.tokens);
+#define SPH_SCORES(HD, F16) \
+    if (c.hd == HD && (c.dtype == DT_F16) == F16) hipLaunchKernelGGL((paged_scores_kernel<HD, F16>), grid, dim3(kThreads), 0, s, g);
+    SPH_SCORES(64, false) SPH_SCORES(128, false) SPH_SCORES(256, false) SPH_SCORES(64, true) SPH_SCORES(128, true) SPH_SCORES(256, true)
+    hipLaunchKernelGGL(paged_select_kernel, dim3(c.nkv, q.tokens), dim3(kPick), 0, s, g);
+    return hip_ok(hipGetLastError(), "paged select launch") ? 0 : -1;
+}
+
+}  // namespace sapphire

@@ -276,6 +276,69 @@ int sapphire_paged_reorder_dev(const sapphire_paged_cache_t *c, const sapphire_p
     return launch_paged_reorder(pc, as_table(t), parents, lengths, spare, const_cast<int *>(out->pages), lengths_out, as_stream(stream));
 }
 
+size_t sapphire_paged_bounds_bytes(const sapphire_paged_cache_t *c) {
+    if (!shape_ok(c)) return 0;
+    return (size_t)c->layers * c->pages * c->n_kv_heads * 2 * c->head_dim * sizeof(uint16_t);
+}
+
+// The layer's bounds.
+static bool bounds_ok(const sapphire_paged_cache_t *c, int layer, const void *bounds, uint16_t *&at) {
+    if (!bounds || reinterpret_cast<uintptr_t>(bounds) % 16 != 0) { set_error("paged bounds: must be a 16-byte aligned device buffer"); return false; }
+    at = static_cast<uint16_t *>(const_cast<void *>(bounds)) + (size_t)layer * c->pages * c->n_kv_heads * 2 * c->head_dim;
+    return true;
+}
+
+int sapphire_paged_bounds_dev(const sapphire_paged_cache_t *c, int layer, void *bounds, const sapphire_page_table_t *t, const int *start,
+                              const int *lengths, int max_new, void *stream) {
+    PagedCache pc;
+    uint16_t *at;
+    if (layer < 0) { set_error("paged bounds: layer %d", layer); return -1; }
+    if (!cache_ok(c, layer, pc) || !table_ok(t) || !bounds_ok(c, layer, bounds, at)) return -1;
+    if (!lengths || max_new <= 0 || t->rows > kGridYZ || 2 * c->n_kv_heads > kGridYZ) {
+        set_error("paged bounds: no lengths, max_new %d, %d table rows, %d heads", max_new, t->rows, c->n_kv_heads);
+        return -1;
+    }
+    return launch_paged_bounds(pc, at, as_table(t), start, lengths, max_new, as_stream(stream));
+}
+
+static bool select_shape_ok(const sapphire_paged_cache_t *c, int batch, int max_length) {
+    if (!shape_ok(c)) return false;
+    if (batch <= 0 || batch > kGridYZ || max_length <= 0 || max_length > (1 << 30)) {
+        set_error("paged select: %d sequences of up to %d positions", batch, max_length);
+        return false;
+    }
+    return true;
+}
+
+size_t sapphire_paged_select_workspace_bytes(const sapphire_paged_cache_t *c, int batch, int max_length) {
+    if (!select_shape_ok(c, batch, max_length)) return 0;
+    return paged_select_workspace(c->n_kv_heads, batch, (max_length + c->page_size - 1) / c->page_size);
+}
+
+int sapphire_paged_select_dev(const sapphire_paged_cache_t *c, int layer, const void *bounds, const sapphire_rows_t *q,
+                              const sapphire_page_table_t *t, const int *lengths, int max_length, const sapphire_page_choice_t *choice,
+                              int *selected, void *workspace, void *stream) {
+    PagedCache pc;
+    uint16_t *at;
+    if (layer < 0) { set_error("paged select: layer %d", layer); return -1; }
+    if (!cache_ok(c, layer, pc) || !rows_ok(q, "q", false) || !table_ok(t) || !bounds_ok(c, layer, bounds, at) ||
+        !select_shape_ok(c, q->tokens, max_length))
+        return -1;
+    if (q->heads % c->n_kv_heads != 0) { set_error("paged select: %d heads over %d K/V heads", q->heads, c->n_kv_heads); return -1; }
+    if (q->head_dim != c->head_dim || q->tokens > t->rows || max_length > (int64_t)t->ld * c->page_size) {
+        set_error("paged select: q of %d rows of head_dim %d, max_length %d, for %d table rows of %d pages", q->tokens, q->head_dim, max_length,
+                  t->rows, t->ld);
+        return -1;
+    }
+    if (!lengths || !choice || !selected || !workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("bad paged select arguments"); return -1; }
+    if (choice->pages <= 0 || choice->first < 0 || choice->last < 0 || (int64_t)choice->first + choice->last > choice->pages) {
+        set_error("paged select: %d pages with the first %d and the last %d", choice->pages, choice->first, choice->last);
+        return -1;
+    }
+    return launch_paged_select(pc, at, as_rows(q), as_table(t), lengths, max_length, choice->pages, choice->first, choice->last, selected,
+                               workspace, as_stream(stream));
+}
+
 int sapphire_rope_rows_dev(const sapphire_rows_t *x, const sapphire_rows_t *y, const int *positions,
                            const sapphire_rope_t *rope, void *stream) {
     if (!rows_ok(x, "rope x", false) || !rows_ok(y, "rope y", true)) return -1;

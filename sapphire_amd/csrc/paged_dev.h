@@ -208,6 +208,11 @@ struct PagedAttn {
 };
 size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length);
 int launch_paged_attention(const PagedAttn &a, hipStream_t s);
+int launch_paged_bounds(const PagedCache &c, uint16_t *bounds, const PageTable &t, const int *from, const int *lengths, int max_new,
+                        hipStream_t s);
+size_t paged_select_workspace(int nkv, int batch, int max_pages);
+int launch_paged_select(const PagedCache &c, const uint16_t *bounds, const Rows &q, const PageTable &t, const int *lengths, int max_length,
+                        int k, int first, int last, int *selected, void *ws, hipStream_t s);
 size_t beam_workspace_bytes(int n, int rows, int beams);
 int launch_beam_select(const float *logits, int ld, int n, int requests, int beams, const float *scores, const int *done,
                        int end_token, float *scores_out, int *tokens, int *parents, int *done_out, void *ws,

@@ -6,9 +6,11 @@
 // distribution. Borders of that draw are as close as 1 / n, so everything behind the logits is in 64 bits:
 // weights 2^((l - m) c), c = log2 e / T, and their sums.
 //
-// Three launches: every row's (maximum, sum of weights) by chunks; the decision, made alike by every workgroup of a request
-// from those, and the chunks' sums of max(p - q, 0) of the one row that it ends at; the token, within one chunk.
+// Two launches: every row's (maximum, sum of weights) by units of 2048 logits; then the decision, made alike by every
+// workgroup of a request from those, the units' sums of max(p - q, 0) of the one row that it ends at, and, by the workgroup
+// that is the last to write its sums, the token, within one unit.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "internal.h"
@@ -23,35 +25,40 @@ using lanes::u64_lane;
 typedef unsigned long long u64;
 
 constexpr int kWave = 64, kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kVec = 8;                    // pieces of four logits of a thread
-constexpr int kChunk = kThreads * kVec * 4;
-constexpr int kPickThreads = 1024, kPickEach = kChunk / kPickThreads;
+constexpr int kVec = 8;                    // pieces of four logits of a lane
+constexpr int kUnit = kWave * kVec * 4;    // a wave's logits
+// The second launch: few workgroups, each with a chain of steps, so its waves take a quarter of a unit each.
+constexpr int kThreads2 = 512, kWaves2 = kThreads2 / kWave;
+constexpr int kQuarters = 4, kUnits2 = kWaves2 / kQuarters, kVec2 = kVec / kQuarters;
+constexpr int kEach = kUnit / kThreads2;   // a thread's logits, where a workgroup goes over a unit
 constexpr int kMaxDrafts = 64;
+constexpr int kPerUnit = 2, kFill = 256 * kPerUnit;    // workgroups of the second launch on a compute unit, and at once
 
 struct Part {
-    float m;                               // a chunk's maximum
+    float m;                               // a unit's maximum
     int pad;
     double sum;                            // of weights against it
 };
 struct VerifyArgs {
     const float *logits, *draft;
     int64_t ld, draft_ld;
-    int n, requests, drafts, chunks;
+    int n, requests, drafts, units;
     const int *draft_tokens, *counts;
     const float *draws;
     double c;                              // log2 e / temperature
     int *tokens, *accepted;
-    Part *part;                            // [rows][chunks]: the target's rows, then the draft's
-    double *rest;                          // [requests][chunks]: sums of max(p - q, 0)
-    u64 *key;                              // greedy: [target rows][chunks], in place of part
+    Part *part;                            // [rows][units]: the target's rows, then the draft's
+    double *rest;                          // [requests][units]: sums of max(p - q, 0)
+    unsigned *done;                        // [requests]: workgroups that have written theirs
+    u64 *key;                              // greedy: [target rows][units], in place of the three
 };
 
-// 2^y for y <= 0 (or NaN, which stays one). 2^f, f in [-1/2, 1/2], by the polynomial through the Chebyshev points of degree 8:
-// off by 1.1e-12 relative, far below the 4e-6 between borders of a flat row of 2^18 tokens. (fp64 fused products run at the
-// rate of fp32 ones here.)
+// 2^y for -1000 <= y <= 0. 2^f, f in [-1/2, 1/2], by the polynomial through the Chebyshev points of degree 8: off by 1.1e-12
+// relative, far below the 4e-6 between borders of a flat row of 2^18 tokens. The sum with 1.5 * 2^52 leaves y's nearest
+// whole number in its low word, and the exponent takes it as it is: rounding, conversion and scaling instructions run at a
+// quarter of the fused products' rate.
 __device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -1100.0);                  // 0, as 2^-1074 is the smallest
-    const double n = rint(y), f = y - n;
+    const double t = y + 6755399441055744.0, f = y - (t - 6755399441055744.0);
     double r = 1.3255224887502117e-06;
     r = __builtin_fma(r, f, 1.531007940254368e-05);
     r = __builtin_fma(r, f, 0.0001540345585240991);
@@ -61,9 +68,10 @@ __device__ __forceinline__ double exp2_64(double y) {
     r = __builtin_fma(r, f, 0.2402265069581299);
     r = __builtin_fma(r, f, 0.6931471805459335);
     r = __builtin_fma(r, f, 1.0);
-    return ldexp(r, (int)n);
+    return __hiloint2double(__double2hiint(r) + (__double2loint(t) << 20), __double2loint(r));
 }
-__device__ __forceinline__ float as_logit(float x) { return x != x ? -INFINITY : x; }
+__device__ __forceinline__ double draw_of(float u) { return fmin(fmax((double)u, 0.0), 1.0); }
+__device__ __forceinline__ float as_logit(float x) { return fmaxf(x, -INFINITY); }
 
 // Weights against the maximum m: where that is infinite, the entries that reach it have 1 and the others 0.
 struct Weight {
@@ -71,11 +79,15 @@ struct Weight {
     float m;
     bool finite;
     __device__ __forceinline__ Weight(double c, float m) : c(c), m64(m), m(m), finite(fabsf(m) < INFINITY) {}
-    __device__ __forceinline__ double operator()(float x) const {
-        if (!finite) return x == m ? 1.0 : 0.0;
-        // (one fused product less m c would be off by what m c is rounded by)
-        return exp2_64(((double)x - m64) * c);
+    // (a fused product less m c would be off by what m c is rounded by)
+    __device__ __forceinline__ double log2(float x) const { return ((double)x - m64) * c; }
+    // for sums, in which 2^-1000 is nothing
+    __device__ __forceinline__ double summand(float x) const { return exp2_64(fmax(log2(x), -1000.0)); }
+    __device__ __forceinline__ double of(float x) const {
+        const double y = log2(x), w = exp2_64(fmax(y, -1000.0));
+        return y < -1000.0 ? 0.0 : w;
     }
+    __device__ __forceinline__ double operator()(float x) const { return finite ? of(x) : x == m ? 1.0 : 0.0; }
 };
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -94,13 +106,14 @@ __device__ __forceinline__ double wave_scan64(double v, int lane) {        // in
 
 // Four logits from index i of a row (a multiple of four from 16-byte aligned memory where `i` is inside), -inf outside [0, n).
 __device__ __forceinline__ pf4 load_logits(const float *row, int i, int n) {
-    pf4 x = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    pf4 x;
     if (i >= 0 && i + 4 <= n) {
         x = *reinterpret_cast<const pf4 *>(row + i);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (i + e >= 0 && i + e < n) x[e] = row[i + e];
+        for (int e = 0; e < 4; ++e) x[e] = row[min(max(i + e, 0), n - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = i + e >= 0 && i + e < n ? x[e] : -INFINITY;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = as_logit(x[e]);
@@ -128,108 +141,124 @@ __device__ __forceinline__ u64 key_of(float x, uint32_t i) {
     return (u64)o << 32 | (uint32_t)~i;
 }
 
-// grid (chunks, rows): the chunk's maximum and sum of weights, or its best key (GREEDY).
+// grid (four units, rows): a unit's maximum and sum of weights, or its best key (GREEDY), by one wave.
 template <bool GREEDY>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs g) {
-    __shared__ double part[kWaves];
-    __shared__ float top[kWaves];
-    __shared__ u64 best[kWaves];
+    const int lane = threadIdx.x & (kWave - 1), unit = blockIdx.x * kWaves + threadIdx.x / kWave;
     const float *row = row_of(g, blockIdx.y);
-    if (!row) return;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-    const int i0 = blockIdx.x * kChunk - ahead(row);
+    if (!GREEDY && blockIdx.x == 0 && threadIdx.x == 0 && (int)blockIdx.y < g.requests) g.done[blockIdx.y] = 0;
+    if (!row || unit >= g.units) return;
+    const int i0 = unit * kUnit - ahead(row) + lane * 4;
     pf4 x[kVec];
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) x[v] = load_logits(row, i0 + (v * kThreads + tid) * 4, g.n);
+    for (int v = 0; v < kVec; ++v) x[v] = load_logits(row, i0 + v * kWave * 4, g.n);
     if constexpr (GREEDY) {
         u64 k = 0;
 #pragma unroll
         for (int v = 0; v < kVec; ++v)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = i0 + (v * kThreads + tid) * 4 + e;
+                const int i = i0 + v * kWave * 4 + e;
                 const u64 o = i >= 0 && i < g.n ? key_of(x[v][e], (uint32_t)i) : 0;
                 k = o > k ? o : k;
             }
         k = lanes::u64_wave_max(k);
-        if (lane == 0) best[wid] = k;
-        __syncthreads();
-        if (tid == 0) {
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) k = best[w] > k ? best[w] : k;
-            g.key[(size_t)blockIdx.y * g.chunks + blockIdx.x] = k;
-        }
+        if (lane == 0) g.key[(size_t)blockIdx.y * g.units + unit] = k;
     } else {
         float m = -INFINITY;
 #pragma unroll
         for (int v = 0; v < kVec; ++v) m = fmaxf(m, fmaxf(fmaxf(x[v][0], x[v][1]), fmaxf(x[v][2], x[v][3])));
         m = lanes::wave_max(m);
-        if (lane == 0) top[wid] = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, top[w]);
         const Weight weight(g.c, m);
         double s[4] = {0.0, 0.0, 0.0, 0.0};
+        if (weight.finite) {
 #pragma unroll
-        for (int v = 0; v < kVec; ++v)
+            for (int v = 0; v < kVec; ++v)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = i0 + (v * kThreads + tid) * 4 + e;
-                // (what lies outside is -inf, which counts where a whole chunk is)
-                s[e] += weight.finite || (i >= 0 && i < g.n) ? weight(x[v][e]) : 0.0;
-            }
+                for (int e = 0; e < 4; ++e) s[e] += weight.summand(x[v][e]);
+        } else {                                       // (what lies outside is -inf, which may be the maximum)
+#pragma unroll
+            for (int v = 0; v < kVec; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = i0 + v * kWave * 4 + e;
+                    s[e] += i >= 0 && i < g.n && x[v][e] == m ? 1.0 : 0.0;
+                }
+        }
         const double sum = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
-        if (lane == 0) part[wid] = sum;
-        __syncthreads();
-        if (tid == 0) g.part[(size_t)blockIdx.y * g.chunks + blockIdx.x] = Part{m, 0, (part[0] + part[1]) + (part[2] + part[3])};
+        if (lane == 0) g.part[(size_t)blockIdx.y * g.units + unit] = Part{m, 0, sum};
     }
 }
 
-// A whole row's maximum and sum from its chunks', by one wave; the same in every lane.
+// A whole row's maximum and sum from its units', by sixteen lanes; the same in each. (Ten loads of a lane under way together:
+// one trip for rows of up to 2^18.)
 __device__ __forceinline__ void row_total(const VerifyArgs &g, int y, float &m, double &sum) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const Part *p = g.part + (size_t)y * g.chunks;
+    constexpr int B = 10;
+    const Part *p = g.part + (size_t)y * g.units;
     m = -INFINITY;
-    for (int i = lane; i < g.chunks; i += kWave) m = fmaxf(m, p[i].m);
-    m = lanes::wave_max(m);
-    const Weight weight(g.c, m);
-    double s = 0.0;
-    for (int i = lane; i < g.chunks; i += kWave) s += p[i].sum * weight(p[i].m);
-    sum = wave_sum64(s);
+    sum = 0.0;
+    for (int i0 = threadIdx.x & 15; i0 < g.units; i0 += 16 * B) {
+        Part t[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            t[b] = p[min(i0 + 16 * b, g.units - 1)];
+            if (i0 + 16 * b >= g.units) t[b].sum = 0.0;
+        }
+        float top = m;
+#pragma unroll
+        for (int b = 0; b < B; ++b) top = fmaxf(top, t[b].m);
+        const Weight weight(g.c, top);
+        sum *= weight(m);
+#pragma unroll
+        for (int b = 0; b < B; ++b) sum += t[b].sum * weight(t[b].m);
+        m = top;
+    }
+    const float top = lanes::row16_max(m);
+    sum *= Weight(g.c, top)(m);
+    m = top;
+#pragma unroll
+    for (int off = 1; off < 16; off *= 2) sum += __shfl_xor(sum, off, 16);
 }
 
 struct Row {
     float m;
     double sum;
 };
-// The decision of request r by all waves of a workgroup: how many drafts stay, and the rows that the token behind them comes from.
+// The decision of request r by a workgroup: how many drafts stay, and the rows that the token behind them comes from.
 __device__ __forceinline__ int decide(const VerifyArgs &g, int r, Row &p, Row &q) {
     __shared__ Row rows[2 * kMaxDrafts + 1];   // the target's, then the draft's
-    __shared__ int stays[kMaxDrafts];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave, waves = blockDim.x / kWave;
-    const int count = count_of(g, r), targets = g.requests * (g.drafts + 1);
+    __shared__ u64 refused;
+    const int tid = threadIdx.x, count = count_of(g, r), targets = g.requests * (g.drafts + 1);
+    // (the first wave's lanes: a draft each, its logits under way during the sums)
+    const int x = tid < count ? g.draft_tokens[(size_t)r * g.drafts + tid] : -1;
+    const bool there = x >= 0 && x < g.n;
+    const float u = tid < count ? g.draws[(size_t)r * (g.drafts + 1) + tid] : 0.0f;
+    const float lp = there ? g.logits[((size_t)r * (g.drafts + 1) + tid) * g.ld + x] : 0.0f;
+    const float lq = there && g.draft ? g.draft[((size_t)r * g.drafts + tid) * g.draft_ld + x] : 0.0f;
     const int jobs = count + 1 + (g.draft ? count : 0);
-    for (int j = wid; j < jobs; j += waves) {
+    for (int j = tid / 16; j < jobs; j += kThreads2 / 16) {
         Row t;
         row_total(g, j <= count ? r * (g.drafts + 1) + j : targets + r * g.drafts + j - count - 1, t.m, t.sum);
-        if (lane == 0) rows[j <= count ? j : kMaxDrafts + 1 + j - count - 1] = t;
+        if (tid % 16 == 0) rows[j <= count ? j : kMaxDrafts + j - count] = t;
     }
     __syncthreads();
-    for (int i = tid; i < count; i += blockDim.x) {
-        const int x = g.draft_tokens[(size_t)r * g.drafts + i];
-        bool ok = false;
-        if (x >= 0 && x < g.n) {
-            const Row a = rows[i], b = rows[kMaxDrafts + 1 + i];
-            const double u = fmin(fmax((double)g.draws[(size_t)r * (g.drafts + 1) + i], 0.0), 1.0);
-            const double px = Weight(g.c, a.m)(as_logit(g.logits[((size_t)r * (g.drafts + 1) + i) * g.ld + x]));
-            if (!g.draft) ok = u * a.sum < px;
-            else ok = u * Weight(g.c, b.m)(as_logit(g.draft[((size_t)r * g.drafts + i) * g.draft_ld + x])) * a.sum < px * b.sum;
+    if (tid < kWave) {
+        bool stays = false;
+        if (there) {
+            const Row a = rows[tid];
+            const double px = Weight(g.c, a.m)(as_logit(lp)), d = draw_of(u);
+            if (!g.draft) {
+                stays = d * a.sum < px;
+            } else {
+                const Row b = rows[kMaxDrafts + 1 + tid];
+                stays = d * Weight(g.c, b.m)(as_logit(lq)) * a.sum < px * b.sum;
+            }
         }
-        stays[i] = ok;
+        const u64 mask = __ballot(tid < count && !stays);
+        if (tid == 0) refused = mask;
     }
     __syncthreads();
-    int a = 0;
-    while (a < count && stays[a]) ++a;
+    const int a = refused ? __builtin_ctzll(refused) : count;
     p = rows[a];
     q = rows[kMaxDrafts + 1 + min(a, kMaxDrafts - 1)];
     return a;
@@ -249,110 +278,181 @@ struct Rest {
         if (mode == 1) return fmax(p - wq(lq) * iq, 0.0);
         return mode == 2 && i == drafted ? 0.0 : p;
     }
+    // the same where neither maximum is infinite
+    __device__ __forceinline__ bool plain() const { return wp.finite && (mode != 1 || wq.finite); }
+    __device__ __forceinline__ double of(float lp, float lq, int i) const {
+        const double p = wp.of(lp) * ip;
+        if (mode == 1) return fmax(p - wq.of(lq) * iq, 0.0);
+        return mode == 2 && i == drafted ? 0.0 : p;
+    }
 };
 
-// grid (chunks, requests). Behind the last draft the sums are p's own, which the first launch made.
-__global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs g) {
-    __shared__ double part[kWaves];
+// grid (parts of a row, requests): the decision, the units' sums of what is left of the row that it ends at, and, by the last
+// workgroup of a request, the token. (Behind the last draft the sums are p's own, which the first launch made.)
+__global__ __launch_bounds__(kThreads2, kPerUnit * kWaves2 / 4) void verify_token_kernel(VerifyArgs g) {
+    __shared__ double part[kWaves2], needs[kWaves2];
+    __shared__ int firsts[kWaves2], lasts[kWaves2];
+    __shared__ unsigned arrived;
     const int r = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     Row p, q;
     const int a = decide(g, r, p, q);
-    const Rest rest(g, r, a, p, q);
-    if (rest.mode == 0) return;
-    const float *row = g.logits + ((size_t)r * (g.drafts + 1) + a) * g.ld;
-    const float *other = rest.mode == 1 ? g.draft + ((size_t)r * g.drafts + a) * g.draft_ld : row;
-    const int i0 = blockIdx.x * kChunk - ahead(row);
-    double s = 0.0;
-#pragma unroll 8
-    for (int j = tid; j < kChunk; j += kThreads) {
-        const int i = i0 + j;
-        if (i >= 0 && i < g.n) s += rest(as_logit(row[i]), as_logit(other[i]), i);
-    }
-    s = wave_sum64(s);
-    if (lane == 0) part[wid] = s;
-    __syncthreads();
-    if (tid == 0) g.rest[(size_t)r * g.chunks + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
-}
-
-// grid (requests): the token, and the outputs.
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs g) {
-    constexpr int kW = kPickThreads / kWave;
-    __shared__ double part[kW], left;
-    __shared__ int chunk, token, late, whole;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-    Row p, q;
-    const int a = decide(g, r, p, q);
     Rest rest(g, r, a, p, q);
-    if (wid == 0) {
-        // the chunk in which the running sum passes the draw's share of the whole; past the last one by a rounding: the last
-        // that has any
-        const double *sums = g.rest + (size_t)r * g.chunks;
-        const Part *own = g.part + ((size_t)r * (g.drafts + 1) + a) * g.chunks;
-        bool of_p = rest.mode == 0;
-        auto sum_of = [&](int i) { return i >= g.chunks ? 0.0 : of_p ? own[i].sum * rest.wp(own[i].m) * rest.ip : sums[i]; };
-        double all = 0.0;
-        auto total = [&]() {
-            all = 0.0;
-            for (int i0 = 0; i0 < g.chunks; i0 += kWave) all += wave_sum64(sum_of(i0 + lane));
-        };
-        total();
-        if (all == 0.0) {                              // p and q are the same, or all of p is on the drafted token: p itself
-            of_p = true;
-            total();
-        }
-        const double u = fmin(fmax((double)g.draws[(size_t)r * (g.drafts + 1) + g.drafts], 0.0), 1.0);
-        double run = 0.0;
-        int at = -1, last = 0;
-        double need = 0.0;
-        for (int i0 = 0; i0 < g.chunks && at < 0; i0 += kWave) {
-            const double s = sum_of(i0 + lane), upto = run + wave_scan64(s, lane);
-            const u64 past = __ballot(i0 + lane < g.chunks && upto > u * all), some = __ballot(s > 0.0);
-            if (some) last = i0 + 63 - __builtin_clzll(some);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                at = i0 + l;
-                need = u * all - __shfl(upto - s, l, kWave);
-            }
-            run = __shfl(upto, kWave - 1, kWave);
-        }
-        if (lane == 0) {
-            chunk = at < 0 ? last : at;
-            left = at < 0 ? INFINITY : need;
-            token = 1 << 30;
-            late = -1;
-            whole = of_p;
-        }
-    }
-    __syncthreads();
-    if (whole) rest.mode = 0;
+    const bool plain = rest.plain();
     const float *row = g.logits + ((size_t)r * (g.drafts + 1) + a) * g.ld;
     const float *other = rest.mode == 1 ? g.draft + ((size_t)r * g.drafts + a) * g.draft_ld : row;
-    const int i0 = chunk * kChunk - ahead(row) + tid * kPickEach;
-    double w[kPickEach], sum = 0.0;
+    double *sums = g.rest + (size_t)r * g.units;
+    if (rest.mode == 0) {
+        if (blockIdx.x != 0) return;
+    } else {
+        for (int group = blockIdx.x; group * kUnits2 < g.units; group += gridDim.x) {
+            const int i0 = (group * kWaves2 + wid) * (kUnit / kQuarters) - ahead(row) + lane * 4;
+            pf4 x[kVec2], y[kVec2];
 #pragma unroll
-    for (int j = 0; j < kPickEach; ++j) {
-        w[j] = i0 + j >= 0 && i0 + j < g.n ? rest(as_logit(row[i0 + j]), as_logit(other[i0 + j]), i0 + j) : 0.0;
+            for (int v = 0; v < kVec2; ++v) {
+                const int i = i0 + v * kWave * 4;
+                x[v] = load_logits(row, i, g.n);
+                if (ahead(row) == ahead(other)) {
+                    y[v] = load_logits(other, i, g.n);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[v][e] = as_logit(other[min(max(i + e, 0), g.n - 1)]);
+                }
+            }
+            double s[4] = {0.0, 0.0, 0.0, 0.0};
+            if (plain) {                               // without branches, so that the chains run side by side (outside: 0)
+#pragma unroll
+                for (int v = 0; v < kVec2; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] += rest.of(x[v][e], y[v][e], i0 + v * kWave * 4 + e);
+            } else {
+#pragma unroll
+                for (int v = 0; v < kVec2; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = i0 + v * kWave * 4 + e;
+                        s[e] += i >= 0 && i < g.n ? rest(x[v][e], y[v][e], i) : 0.0;
+                    }
+            }
+            const double sum = wave_sum64((s[0] + s[1]) + (s[2] + s[3]));
+            __syncthreads();                           // the sums before are out of `part`
+            if (lane == 0) part[wid] = sum;
+            __syncthreads();
+            const int mine = group * kUnits2 + tid;
+            if (tid < kUnits2 && mine < g.units) {
+                const double *u = part + tid * kQuarters;
+                __hip_atomic_store(&sums[mine], (u[0] + u[1]) + (u[2] + u[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        // acknowledged before the workgroup counts itself done
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (tid == 0) arrived = __hip_atomic_fetch_add(&g.done[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived != gridDim.x - 1) return;
+    }
+    // The unit in which the running sum passes the draw's share of the whole; past the last one by a rounding: the last one that
+    // has any. A thread takes `each` units.
+    const Part *own = g.part + ((size_t)r * (g.drafts + 1) + a) * g.units;
+    const int each = (g.units + kThreads2 - 1) / kThreads2, u0 = tid * each;
+    const double draw = draw_of(g.draws[(size_t)r * (g.drafts + 1) + g.drafts]);
+    auto sum_of = [&](int i) {
+        if (i >= g.units) return 0.0;
+        if (rest.mode == 0) return own[i].sum * rest.wp(own[i].m) * rest.ip;
+        return __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    double run, all;
+    auto scan = [&](double mine) {                     // run: what the threads ahead have; all: what all have
+        const double upto = wave_scan64(mine, lane);
+        __syncthreads();
+        if (lane == kWave - 1) part[wid] = upto;
+        __syncthreads();
+        run = upto - mine;
+        all = 0.0;
+#pragma unroll
+        for (int w = 0; w < kWaves2; ++w) {
+            run += w < wid ? part[w] : 0.0;
+            all += part[w];
+        }
+    };
+    // the first thread's `found` that is not -1, with its `need`, or the last thread's `some` (0: there is none), and no need
+    auto choose = [&](int found, int some, double &need) {
+        const u64 f = __ballot(found >= 0), l = __ballot(some >= 0);
+        const int ff = __shfl(found, f ? __builtin_ctzll(f) : 0, kWave), ll = __shfl(some, l ? 63 - __builtin_clzll(l) : 0, kWave);
+        const double nn = __shfl(need, f ? __builtin_ctzll(f) : 0, kWave);
+        __syncthreads();
+        if (lane == 0) {
+            firsts[wid] = f ? ff : -1;
+            lasts[wid] = l ? ll : -1;
+            needs[wid] = nn;
+        }
+        __syncthreads();
+        int at = -1, last = 0;
+        need = INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves2; ++w) {
+            if (at < 0 && firsts[w] >= 0) {
+                at = firsts[w];
+                need = needs[w];
+            }
+            last = lasts[w] >= 0 ? lasts[w] : last;
+        }
+        return at >= 0 ? at : last;
+    };
+    auto total = [&]() {
+        double s = 0.0;
+        for (int j = 0; j < each; ++j) s += sum_of(u0 + j);
+        scan(s);
+    };
+    total();
+    if (all == 0.0 && rest.mode != 0) {                // p and q are the same, or all of p is on the drafted token: p itself
+        rest.mode = 0;
+        total();
+    }
+    int found = -1, some = -1;
+    double need = INFINITY;
+    for (int j = 0; j < each; ++j) {
+        const double s = sum_of(u0 + j);
+        if (s > 0.0) {
+            some = u0 + j;
+            if (found < 0 && run + s > draw * all) {
+                found = u0 + j;
+                need = draw * all - run;
+            }
+        }
+        run += s;
+    }
+    const int unit = choose(found, some, need);
+    const double left = need;
+    const int i0 = unit * kUnit - ahead(row) + tid * kEach;
+    float x[kEach], y[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int at = min(max(i0 + j, 0), g.n - 1);
+        x[j] = row[at];
+        y[j] = other[at];
+    }
+    double w[kEach], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const float lx = as_logit(x[j]), ly = as_logit(y[j]);
+        w[j] = rest.plain() ? rest.of(lx, ly, i0 + j) : rest(lx, ly, i0 + j);
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        w[j] = i0 + j >= 0 && i0 + j < g.n ? w[j] : 0.0;
         sum += w[j];
     }
-    const double upto = wave_scan64(sum, lane);
-    if (lane == kWave - 1) part[wid] = upto;
-    __syncthreads();
-    double run = upto - sum;
-    for (int v = 0; v < wid; ++v) run += part[v];
-    int first = 1 << 30, some = -1;
+    scan(sum);
+    found = some = -1;
 #pragma unroll
-    for (int j = 0; j < kPickEach; ++j) {
+    for (int j = 0; j < kEach; ++j) {
         run += w[j];
         if (w[j] > 0.0) {
             some = i0 + j;
-            if (run > left) first = min(first, i0 + j);
+            if (found < 0 && run > left) found = i0 + j;
         }
     }
-    if (first < 1 << 30) atomicMin(&token, first);
-    if (some >= 0) atomicMax(&late, some);
-    __syncthreads();
-    const int pick = token < 1 << 30 ? token : max(late, 0);
-    for (int i = tid; i <= g.drafts; i += kPickThreads)
+    const int pick = choose(found, some, need);
+    for (int i = tid; i <= g.drafts; i += kThreads2)
         g.tokens[(size_t)r * (g.drafts + 1) + i] = i < a ? g.draft_tokens[(size_t)r * g.drafts + i] : i == a ? pick : -1;
     if (tid == 0) g.accepted[r] = a;
 }
@@ -363,8 +463,8 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs g) {
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave, count = count_of(g, r);
     for (int j = wid; j <= count; j += kWaves) {
         u64 k = 0;
-        for (int i = lane; i < g.chunks; i += kWave) {
-            const u64 o = g.key[((size_t)r * (g.drafts + 1) + j) * g.chunks + i];
+        for (int i = lane; i < g.units; i += kWave) {
+            const u64 o = g.key[((size_t)r * (g.drafts + 1) + j) * g.units + i];
             k = o > k ? o : k;
         }
         k = lanes::u64_wave_max(k);
@@ -379,13 +479,13 @@ __global__ __launch_bounds__(kThreads) void verify_greedy_kernel(VerifyArgs g) {
 }
 
 // pieces of four start up to three elements ahead of a row
-int chunks_of(int n) { return (n + 3 + kChunk - 1) / kChunk; }
+int units_of(int n) { return (n + 3 + kUnit - 1) / kUnit; }
 
 }  // namespace
 
 size_t verify_workspace_bytes(int n, int requests, int drafts) {
-    const size_t chunks = (size_t)chunks_of(n), rows = (size_t)requests * (2 * drafts + 1);
-    return chunks * (rows * sizeof(Part) + (size_t)requests * sizeof(double));
+    const size_t units = (size_t)units_of(n), rows = (size_t)requests * (2 * drafts + 1);
+    return units * (rows * sizeof(Part) + (size_t)requests * sizeof(double)) + (size_t)requests * sizeof(unsigned);
 }
 
 int launch_verify(const float *logits, int ld, const float *draft_logits, int draft_ld, int n, int requests, int drafts,
@@ -399,7 +499,7 @@ int launch_verify(const float *logits, int ld, const float *draft_logits, int dr
     g.n = n;
     g.requests = requests;
     g.drafts = drafts;
-    g.chunks = chunks_of(n);
+    g.units = units_of(n);
     g.draft_tokens = draft_tokens;
     g.counts = counts;
     g.draws = draws;
@@ -407,18 +507,22 @@ int launch_verify(const float *logits, int ld, const float *draft_logits, int dr
     g.tokens = tokens;
     g.accepted = accepted;
     const int targets = requests * (drafts + 1);
+    const unsigned groups = (unsigned)((g.units + kWaves - 1) / kWaves);
     if (!(temperature > 0.0f)) {
         g.key = static_cast<u64 *>(ws);
-        hipLaunchKernelGGL(verify_rows_kernel<true>, dim3(g.chunks, targets), dim3(kThreads), 0, s, g);
+        hipLaunchKernelGGL(verify_rows_kernel<true>, dim3(groups, targets), dim3(kThreads), 0, s, g);
         hipLaunchKernelGGL(verify_greedy_kernel, dim3(requests), dim3(kThreads), 0, s, g);
         return hip_ok(hipGetLastError(), "verify launch") ? 0 : -1;
     }
     const int rows = targets + (draft_logits ? requests * drafts : 0);
     g.part = static_cast<Part *>(ws);
-    g.rest = reinterpret_cast<double *>(g.part + (size_t)rows * g.chunks);
-    hipLaunchKernelGGL(verify_rows_kernel<false>, dim3(g.chunks, rows), dim3(kThreads), 0, s, g);
-    hipLaunchKernelGGL(verify_rest_kernel, dim3(g.chunks, requests), dim3(kThreads), 0, s, g);
-    hipLaunchKernelGGL(verify_pick_kernel, dim3(requests), dim3(kPickThreads), 0, s, g);
+    g.rest = reinterpret_cast<double *>(g.part + (size_t)rows * g.units);
+    g.done = reinterpret_cast<unsigned *>(g.rest + (size_t)requests * g.units);
+    hipLaunchKernelGGL(verify_rows_kernel<false>, dim3(groups, rows), dim3(kThreads), 0, s, g);
+    // no more workgroups than run at once (a second round would decide everything again), with even shares of a row
+    const unsigned steps = (unsigned)((g.units + kUnits2 - 1) / kUnits2), most = std::max(1u, (unsigned)(kFill / requests));
+    const unsigned each = (steps + most - 1) / most, parts = (steps + each - 1) / each;
+    hipLaunchKernelGGL(verify_token_kernel, dim3(parts, requests), dim3(kThreads2), 0, s, g);
     return hip_ok(hipGetLastError(), "verify launch") ? 0 : -1;
 }
 

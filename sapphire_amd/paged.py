@@ -9,7 +9,7 @@ from ctypes import byref
 import numpy as np
 
 from . import load
-from ._lib import AttentionC, PageTableC, PagedCacheC, RopeC, RowsC
+from ._lib import AttentionC, PageChoiceC, PageTableC, PagedCacheC, RopeC, RowsC
 from .device import DeviceArray, check
 
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)
@@ -86,6 +86,7 @@ class PagedCache:
         self.v = DeviceArray(self.nbytes) if v is None else v
         self.c.k, self.c.v = _at(self.k), _at(self.v)
         self._write, self._read = lib.sapphire_paged_write_dev, lib.sapphire_paged_read_dev
+        self._bounds, self._select = lib.sapphire_paged_bounds_dev, lib.sapphire_paged_select_dev
         self._attention, self._reorder = lib.sapphire_paged_attention_dev, lib.sapphire_paged_reorder_dev
 
     def write(self, layer, k: RowsC, v: RowsC, table: PageTableC, positions, seqs=None, stream=None) -> None:
@@ -107,6 +108,25 @@ class PagedCache:
         if self._attention(self.ref, layer, byref(q), byref(out), byref(table), _at(lengths), max_length,
                            byref(AttentionC(scale, window, softcap)), _at(lse), _at(workspace), stream):
             check(-1, "paged attention")
+
+    @property
+    def bounds_bytes(self) -> int:
+        return load().sapphire_paged_bounds_bytes(self.ref)
+
+    def bounds(self, layer, bounds, table: PageTableC, lengths, max_new, start=None, stream=None) -> None:
+        """The bounds of K of the pages that hold positions start[b] .. lengths[b] - 1 of each table row."""
+        if self._bounds(self.ref, layer, _at(bounds), byref(table), _at(start), _at(lengths), max_new, stream):
+            check(-1, "paged bounds")
+
+    def select_workspace_bytes(self, batch, max_length) -> int:
+        return load().sapphire_paged_select_workspace_bytes(self.ref, batch, max_length)
+
+    def select(self, layer, bounds, q: RowsC, table: PageTableC, lengths, max_length, selected, pages, first=1, last=1, workspace=None,
+               stream=None) -> None:
+        """selected[b][K/V head] = the `pages` pages of table row b with the largest bounds on q[b] . k."""
+        if self._select(self.ref, layer, _at(bounds), byref(q), byref(table), _at(lengths), max_length,
+                        byref(PageChoiceC(pages, first, last)), _at(selected), _at(workspace), stream):
+            check(-1, "paged select")
 
     def reorder(self, table: PageTableC, parents, lengths, spare, table_out: PageTableC, lengths_out, stream=None) -> None:
         """Row b of table_out continues row parents[b] of table."""
