@@ -143,6 +143,18 @@ int sapphire_paged_select_dev(const sapphire_paged_cache_t *cache, int layer, co
                               const sapphire_page_table_t *table, const int *lengths, int max_length,
                               const sapphire_page_choice_t *choice, int *selected, void *workspace, void *stream);
 
+/* Attention of one new token per sequence over the pages that selected[b][K/V head][0 .. pages) names (as
+ * sapphire_paged_select_dev chooses them): as sapphire_paged_attention_dev, over the positions p of those pages with
+ * max(0, n - window) <= p < n, n = lengths[b] (taken into 0 .. ld * page_size). A place that is negative, at or behind the
+ * sequence's last page, or whose page does not exist, is left out. A list's places are different ones, its first
+ * ceil(n / page_size) count (of a page named twice it is unspecified whether it counts twice), and their order does not matter.
+ * A head without a position gets out = 0 and lse = -inf. workspace:
+ * sapphire_paged_attention_workspace_bytes(cache, tokens, n_heads, pages * page_size). */
+int sapphire_paged_pages_attention_dev(const sapphire_paged_cache_t *cache, int layer, const sapphire_rows_t *q,
+                                       const sapphire_rows_t *out, const sapphire_page_table_t *table, const int *lengths,
+                                       const int *selected, int pages, const sapphire_attention_t *attention, float *lse,
+                                       void *workspace, void *stream);
+
 /* After sapphire_beam_select_dev: row b continues row p = parents[b] of `table`, of which lengths[p]
  * positions are written. Row b of table_out gets p's full pages (shared, not copied); a partly
  * filled last page is copied, in every layer and head, to page spare[b], which takes its place: its

@@ -137,6 +137,7 @@ def load_library(path: str):
     P("sapphire_paged_bounds_dev", i32, [vp, i32, vp, vp, vp, vp, i32, vp])
     P("sapphire_paged_select_workspace_bytes", sz, [vp, i32, i32])
     P("sapphire_paged_select_dev", i32, [vp, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp])
+    P("sapphire_paged_pages_attention_dev", i32, [vp, i32, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp])
     P("sapphire_paged_reorder_dev", i32, [vp, vp, vp, vp, vp, vp, vp, vp])
     P("sapphire_tensor_invalidate", i32, [vp])
     P("sapphire_tensor_device_data", vp, [vp, C.POINTER(i32), vp])

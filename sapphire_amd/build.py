@@ -17,7 +17,8 @@ OUT = os.path.join(HERE, "libsapphire_hip.so")
 SOURCES = ["runtime.cpp", "tensor.cpp", "dispatch.cpp", "decoder.cpp", "gemv.hip", "gemv_mfma.hip", "gemm_mfma.hip", "gemm_wide.hip", "prefill.hip",
            "ops.hip", "sample.hip", "decode.hip",
            "decode_persist.hip", "quantize.hip", "gemm_bf16.hip", "noalloc.cpp", "transformer.cpp", "paged.cpp",
-           "paged_rows.hip", "paged_attention.hip", "rope_rows.hip", "beam.hip", "verify.hip", "page_choice.hip"]
+           "paged_rows.hip", "paged_attention.hip", "rope_rows.hip", "beam.hip", "verify.hip", "page_choice.hip",
+           "paged_pages.hip"]
 ARCH = os.environ.get("SAPPHIRE_OFFLOAD_ARCH", "gfx950")
 
 COMMON = [

@@ -207,53 +207,81 @@ size_t sapphire_paged_attention_workspace_bytes(const sapphire_paged_cache_t *c,
     return paged_attention_workspace(c->dtype, c->n_kv_heads, c->head_dim, batch, n_heads, max_length);
 }
 
+// What the attentions check alike; a's fields but the lengths' bound and the workspace.
+static bool attend_ok(const sapphire_paged_cache_t *c, int layer, const sapphire_rows_t *q, const sapphire_rows_t *out,
+                      const sapphire_page_table_t *t, const int *lengths, const sapphire_attention_t *at, float *lse, PagedAttn &a) {
+    if (layer < 0) { set_error("paged attention: layer %d", layer); return false; }
+    if (!cache_ok(c, layer, a.c) || !rows_ok(q, "q", false) || !rows_ok(out, "out", true) || !table_ok(t)) return false;
+    if (q->dtype != out->dtype || q->tokens != out->tokens || q->heads != out->heads || q->head_dim != c->head_dim ||
+        out->head_dim != c->head_dim) {
+        set_error("paged attention: q and out must have one type and shape, and the cache's head_dim");
+        return false;
+    }
+    if (q->heads % c->n_kv_heads != 0) { set_error("paged attention: %d heads over %d K/V heads", q->heads, c->n_kv_heads); return false; }
+    if (q->dtype != DT_F32 && q->dtype != c->dtype && !is_quant(c->dtype)) {
+        set_error("paged attention: 16-bit rows need a cache of their type or a quantized one (rows %d, cache %d)", q->dtype, c->dtype);
+        return false;
+    }
+    if (!lengths || !at) { set_error("paged attention: no lengths or parameters"); return false; }
+    if (!(std::fabs(at->scale) < INFINITY) || !(at->softcap >= 0.0f) || !(at->softcap < INFINITY)) {
+        set_error("paged attention: scale %g, softcap %g", (double)at->scale, (double)at->softcap);
+        return false;
+    }
+    if (q->tokens > t->rows || q->tokens > kGridYZ || q->heads > kGridYZ) {
+        set_error("paged attention: %d sequences, %d heads, %d table rows", q->tokens, q->heads, t->rows);
+        return false;
+    }
+    if (!identical(q, out) && !apart(q, out)) { set_error("paged attention: out overlaps q without being q"); return false; }
+    a.q = as_rows(q);
+    a.out = as_rows(out);
+    a.table = as_table(t);
+    a.lengths = lengths;
+    a.window = at->window;
+    a.scale = at->scale;
+    a.softcap = at->softcap;
+    a.lse = lse;
+    return true;
+}
+
+static bool workspace_ok(size_t need, void *workspace, PagedAttn &a) {
+    if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) {
+        set_error("paged attention: needs a 16-byte aligned workspace of %zu bytes", need);
+        return false;
+    }
+    a.ws = static_cast<uint8_t *>(workspace);
+    return true;
+}
+
 int sapphire_paged_attention_dev(const sapphire_paged_cache_t *c, int layer, const sapphire_rows_t *q,
                                  const sapphire_rows_t *out, const sapphire_page_table_t *t, const int *lengths,
                                  int max_length, const sapphire_attention_t *at, float *lse, void *workspace,
                                  void *stream) {
     PagedAttn a;
-    if (layer < 0) { set_error("paged attention: layer %d", layer); return -1; }
-    if (!cache_ok(c, layer, a.c) || !rows_ok(q, "q", false) || !rows_ok(out, "out", true) || !table_ok(t)) return -1;
-    if (q->dtype != out->dtype || q->tokens != out->tokens || q->heads != out->heads || q->head_dim != c->head_dim ||
-        out->head_dim != c->head_dim) {
-        set_error("paged attention: q and out must have one type and shape, and the cache's head_dim");
-        return -1;
-    }
-    if (q->heads % c->n_kv_heads != 0) { set_error("paged attention: %d heads over %d K/V heads", q->heads, c->n_kv_heads); return -1; }
-    if (q->dtype != DT_F32 && q->dtype != c->dtype && !is_quant(c->dtype)) {
-        set_error("paged attention: 16-bit rows need a cache of their type or a quantized one (rows %d, cache %d)", q->dtype, c->dtype);
-        return -1;
-    }
-    if (!lengths || !at) { set_error("paged attention: no lengths or parameters"); return -1; }
-    if (!(std::fabs(at->scale) < INFINITY) || !(at->softcap >= 0.0f) || !(at->softcap < INFINITY)) {
-        set_error("paged attention: scale %g, softcap %g", (double)at->scale, (double)at->softcap);
-        return -1;
-    }
-    if (q->tokens > t->rows || q->tokens > kGridYZ || q->heads > kGridYZ) {
-        set_error("paged attention: %d sequences, %d heads, %d table rows", q->tokens, q->heads, t->rows);
-        return -1;
-    }
-    if (!identical(q, out) && !apart(q, out)) { set_error("paged attention: out overlaps q without being q"); return -1; }
+    if (!attend_ok(c, layer, q, out, t, lengths, at, lse, a)) return -1;
     if (max_length <= 0 || max_length > (int64_t)t->ld * c->page_size || max_length > (1 << 30)) {
         set_error("paged attention: max_length %d with %d pages of %d per row", max_length, t->ld, c->page_size);
         return -1;
     }
-    const size_t need = sapphire_paged_attention_workspace_bytes(c, q->tokens, q->heads, max_length);
-    if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) {
-        set_error("paged attention: needs a 16-byte aligned workspace of %zu bytes", need);
+    a.max_length = max_length;
+    if (!workspace_ok(sapphire_paged_attention_workspace_bytes(c, q->tokens, q->heads, max_length), workspace, a)) return -1;
+    return launch_paged_attention(a, as_stream(stream));
+}
+
+int sapphire_paged_pages_attention_dev(const sapphire_paged_cache_t *c, int layer, const sapphire_rows_t *q,
+                                       const sapphire_rows_t *out, const sapphire_page_table_t *t, const int *lengths,
+                                       const int *selected, int pages, const sapphire_attention_t *at, float *lse,
+                                       void *workspace, void *stream) {
+    PagedAttn a;
+    if (!attend_ok(c, layer, q, out, t, lengths, at, lse, a)) return -1;
+    if (!selected || pages <= 0 || (int64_t)pages * c->page_size > (1 << 30)) {
+        set_error("paged attention: lists of %d pages of %d", pages, c->page_size);
         return -1;
     }
-    a.q = as_rows(q);
-    a.out = as_rows(out);
-    a.table = as_table(t);
-    a.lengths = lengths;
-    a.max_length = max_length;
-    a.window = at->window;
-    a.scale = at->scale;
-    a.softcap = at->softcap;
-    a.lse = lse;
-    a.ws = static_cast<uint8_t *>(workspace);
-    return launch_paged_attention(a, as_stream(stream));
+    a.selected = selected;
+    a.listed = pages;
+    a.max_length = (int)std::min<int64_t>((int64_t)t->ld * c->page_size, 1 << 30);
+    if (!workspace_ok(sapphire_paged_attention_workspace_bytes(c, q->tokens, q->heads, pages * c->page_size), workspace, a)) return -1;
+    return launch_paged_pages_attention(a, as_stream(stream));
 }
 
 int sapphire_paged_reorder_dev(const sapphire_paged_cache_t *c, const sapphire_page_table_t *t, const int *parents,

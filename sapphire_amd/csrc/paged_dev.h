@@ -205,9 +205,12 @@ struct PagedAttn {
     float scale = 1.f, softcap = 0.f;
     float *lse = nullptr;
     uint8_t *ws = nullptr;
+    const int *selected = nullptr;         // attention over chosen pages: [batch][K/V heads][listed]
+    int listed = 0;
 };
 size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length);
 int launch_paged_attention(const PagedAttn &a, hipStream_t s);
+int launch_paged_pages_attention(const PagedAttn &a, hipStream_t s);
 int launch_paged_bounds(const PagedCache &c, uint16_t *bounds, const PageTable &t, const int *from, const int *lengths, int max_new,
                         hipStream_t s);
 size_t paged_select_workspace(int nkv, int batch, int max_pages);

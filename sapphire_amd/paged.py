@@ -87,6 +87,7 @@ class PagedCache:
         self.c.k, self.c.v = _at(self.k), _at(self.v)
         self._write, self._read = lib.sapphire_paged_write_dev, lib.sapphire_paged_read_dev
         self._bounds, self._select = lib.sapphire_paged_bounds_dev, lib.sapphire_paged_select_dev
+        self._pages_attention = lib.sapphire_paged_pages_attention_dev
         self._attention, self._reorder = lib.sapphire_paged_attention_dev, lib.sapphire_paged_reorder_dev
 
     def write(self, layer, k: RowsC, v: RowsC, table: PageTableC, positions, seqs=None, stream=None) -> None:
@@ -127,6 +128,13 @@ class PagedCache:
         if self._select(self.ref, layer, _at(bounds), byref(q), byref(table), _at(lengths), max_length,
                         byref(PageChoiceC(pages, first, last)), _at(selected), _at(workspace), stream):
             check(-1, "paged select")
+
+    def pages_attention(self, layer, q: RowsC, out: RowsC, table: PageTableC, lengths, selected, pages, scale, window=0, softcap=0.0,
+                        lse=None, workspace=None, stream=None) -> None:
+        """out[b] = attention of q[b] over the pages of table row b that selected[b][K/V head] names."""
+        if self._pages_attention(self.ref, layer, byref(q), byref(out), byref(table), _at(lengths), _at(selected), pages,
+                                 byref(AttentionC(scale, window, softcap)), _at(lse), _at(workspace), stream):
+            check(-1, "paged attention over pages")
 
     def reorder(self, table: PageTableC, parents, lengths, spare, table_out: PageTableC, lengths_out, stream=None) -> None:
         """Row b of table_out continues row parents[b] of table."""
