@@ -114,6 +114,30 @@ int sapphire_paged_attention_dev(const sapphire_paged_cache_t *cache, int layer,
                                  int max_length, const sapphire_attention_t *attention, float *lse, void *workspace,
                                  void *stream);
 
+/* The same where rows share their first positions: requests behind one prompt, the beams of a request, the drafted tokens of a
+ * sequence (each a row of its own, with the sequence's pages and one position more than the one before). Rows g * rows ..
+ * g * rows + rows - 1 (the last group may have fewer) are group g, and shared[g] (device memory) says that their first shared[g]
+ * positions are the same ones: the same pages, or pages of the same K and V. Those that every row of the group with a length
+ * above 0 has, in whole tiles of 16, are read once for the group, by the table row of its first such row; each row's others by its
+ * own. lengths, softcap, lse, types and rounding as for sapphire_paged_attention_dev, whose results these are but for the order
+ * of sums; a shared[g] of 0 or less shares nothing, one beyond the lengths all. A window is refused: rows that see little share
+ * little. Over the shared positions a NaN or an infinity in V makes its dim (over a quantized cache its block's dims) NaN or
+ * infinite; one in q or K, other than over a cache of the rows' own type, makes its heads' outputs NaN. What is said
+ * there of positions behind the last one and of pages that do not exist holds here too. max_own: about how many
+ * positions a row has behind the shared ones at most; it is for speed only, any value gives the same positions. workspace:
+ * sapphire_paged_shared_attention_workspace_bytes() bytes, 16-byte aligned, which are enough for calls of fewer and shorter rows
+ * too, whatever their groups; calls that share one must be ordered on one stream. */
+typedef struct {
+    const int *shared;
+    int rows, max_own;
+} sapphire_groups_t;
+size_t sapphire_paged_shared_attention_workspace_bytes(const sapphire_paged_cache_t *cache, int batch, int n_heads,
+                                                       int max_length);
+int sapphire_paged_shared_attention_dev(const sapphire_paged_cache_t *cache, int layer, const sapphire_rows_t *q,
+                                        const sapphire_rows_t *out, const sapphire_page_table_t *table, const int *lengths,
+                                        int max_length, const sapphire_groups_t *groups,
+                                        const sapphire_attention_t *attention, float *lse, void *workspace, void *stream);
+
 /* Bounds of K per page, for the choice below: of each dim the lowest and the highest value of the page's written rows, as
  * 16 bits (F16 over an F16 cache, else BF16; values of other types rounded down and up). bounds: a buffer of
  * sapphire_paged_bounds_bytes(), 16-byte aligned, [layers][pages][n_kv_heads][2][head_dim], low ones first. A call makes those

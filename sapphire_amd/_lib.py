@@ -50,6 +50,11 @@ class AttentionC(C.Structure):
     _fields_ = [("scale", C.c_float), ("window", C.c_int), ("softcap", C.c_float)]
 
 
+class GroupsC(C.Structure):
+    """sapphire_groups_t (include/paged.h)."""
+    _fields_ = [("shared", C.c_void_p), ("rows", C.c_int), ("max_own", C.c_int)]
+
+
 class PageChoiceC(C.Structure):
     """sapphire_page_choice_t (include/paged.h)."""
     _fields_ = [("pages", C.c_int), ("first", C.c_int), ("last", C.c_int)]
@@ -138,6 +143,8 @@ def load_library(path: str):
     P("sapphire_paged_select_workspace_bytes", sz, [vp, i32, i32])
     P("sapphire_paged_select_dev", i32, [vp, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp])
     P("sapphire_paged_pages_attention_dev", i32, [vp, i32, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp])
+    P("sapphire_paged_shared_attention_workspace_bytes", sz, [vp, i32, i32, i32])
+    P("sapphire_paged_shared_attention_dev", i32, [vp, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp])
     P("sapphire_paged_reorder_dev", i32, [vp, vp, vp, vp, vp, vp, vp, vp])
     P("sapphire_tensor_invalidate", i32, [vp])
     P("sapphire_tensor_device_data", vp, [vp, C.POINTER(i32), vp])

@@ -284,6 +284,31 @@ int sapphire_paged_pages_attention_dev(const sapphire_paged_cache_t *c, int laye
     return launch_paged_pages_attention(a, as_stream(stream));
 }
 
+size_t sapphire_paged_shared_attention_workspace_bytes(const sapphire_paged_cache_t *c, int batch, int n_heads, int max_length) {
+    if (!shape_ok(c) || batch <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads != 0 || max_length <= 0) return 0;
+    return paged_shared_workspace(c->dtype, c->n_kv_heads, c->head_dim, batch, n_heads, max_length);
+}
+
+int sapphire_paged_shared_attention_dev(const sapphire_paged_cache_t *c, int layer, const sapphire_rows_t *q,
+                                        const sapphire_rows_t *out, const sapphire_page_table_t *t, const int *lengths,
+                                        int max_length, const sapphire_groups_t *groups, const sapphire_attention_t *at,
+                                        float *lse, void *workspace, void *stream) {
+    PagedAttn a;
+    if (!attend_ok(c, layer, q, out, t, lengths, at, lse, a)) return -1;
+    if (max_length <= 0 || max_length > (int64_t)t->ld * c->page_size || max_length > (1 << 30)) {
+        set_error("shared attention: max_length %d with %d pages of %d per row", max_length, t->ld, c->page_size);
+        return -1;
+    }
+    if (!groups || !groups->shared || groups->rows <= 0 || groups->max_own < 0) { set_error("shared attention: bad groups"); return -1; }
+    if (at->window > 0) { set_error("shared attention: a window (%d): its rows share little", at->window); return -1; }
+    a.max_length = max_length;
+    a.shared = groups->shared;
+    a.rows = groups->rows;
+    a.max_own = groups->max_own;
+    if (!workspace_ok(sapphire_paged_shared_attention_workspace_bytes(c, q->tokens, q->heads, max_length), workspace, a)) return -1;
+    return launch_paged_shared_attention(a, as_stream(stream));
+}
+
 int sapphire_paged_reorder_dev(const sapphire_paged_cache_t *c, const sapphire_page_table_t *t, const int *parents,
                                const int *lengths, const int *spare, const sapphire_page_table_t *out, int *lengths_out,
                                void *stream) {

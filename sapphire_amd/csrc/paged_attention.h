@@ -1,6 +1,7 @@
 // paged_attention.h - the kernels of attention of one new token per sequence over the paged cache, by what a sequence's
-// positions are (not installed): all of them (paged_attention.hip), or those of the pages that a list names
-// (paged_pages.hip). The mathematics, the products' forms and what bounds them are in paged_attention.hip.
+// positions are (not installed): all of them (paged_attention.hip), those of the pages that a list names (paged_pages.hip), or
+// those behind what it shares with others (paged_shared.hip). The mathematics, the products' forms and what bounds them are in
+// paged_attention.hip.
 #pragma once
 
 #include <algorithm>
@@ -22,7 +23,8 @@ constexpr int kMaxPieces = 256, kManyPieces = 32;          // of a sequence; tha
 constexpr int kPieceUnit = 64;             // a piece is a multiple of so many positions
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
-enum Mode { WHOLE, LIST };                 // a sequence's positions: all, or those of listed pages, one page after the other
+// A sequence's positions: all; those of listed pages, one page after the other; those behind the ones that its group shares.
+enum Mode { WHOLE, LIST, BEHIND };
 
 struct AttnArgs {
     PagedAttn a;
@@ -31,7 +33,29 @@ struct AttnArgs {
     bool wide;                             // out's data and strides are multiples of 16 bytes
     float *part;                           // [pieces][batch][n_heads][hd], unnormalised O
     float2 *ms;                            // [pieces][batch][n_heads]: maximum (log2 units), sum
+    int first_piece;                       // BEHIND: pieces ahead of these, which the shared positions have
 };
+
+// What the rows of group `i` share: whole tiles of the positions that every row with any has; and the first such row.
+struct Group {
+    int shared, leader;
+};
+__device__ __forceinline__ Group group_of(const PagedAttn &a, int i) {
+    const int lane = threadIdx.x & (kWave - 1), r0 = i * a.rows, r1 = min(r0 + a.rows, a.q.tokens);
+    int least = max(a.shared[i], 0);
+    Group g = {0, -1};
+    for (int r = r0; r < r1; r += kWave) {
+        const int n = r + lane < r1 ? min(max(a.lengths[r + lane], 0), a.max_length) : 0;
+        const unsigned long long live = __ballot(n > 0);
+        if (live && g.leader < 0) g.leader = r + __builtin_ctzll(live);
+        least = n > 0 ? min(least, n) : least;
+    }
+#pragma unroll
+    for (int off = 1; off < kWave; off *= 2) least = min(least, __shfl_xor(least, off, kWave));
+    g.leader = __builtin_amdgcn_readfirstlane(g.leader);
+    g.shared = g.leader < 0 ? 0 : __builtin_amdgcn_readfirstlane(least & ~(kPos - 1));
+    return g;
+}
 
 // A lane's part of 16 positions of K (lane (c, m): position c, chunk m of each load) or V (positions 4m ..
 // 4m + 3, its dims) as raw 16-byte pieces, and their elements as fp32.
@@ -302,20 +326,25 @@ struct Walk {
         ps = a.c.page_size;
         const int n = min(max(a.lengths[b], 0), a.max_length);
         start = a.window > 0 && n > a.window ? n - a.window : 0;
-        lo = walk_from<MODE>(start) + blockIdx.x * g.piece;
-        hi = min(walk_to<MODE>(a, n), lo + g.piece);
+        int piece = g.piece;
+        if constexpr (MODE == BEHIND) {
+            start = min(group_of(a, b / a.rows).shared, n);
+            piece = ((n - start + g.pieces - 1) / g.pieces + kPieceUnit - 1) / kPieceUnit * kPieceUnit;
+        }
+        lo = min((int64_t)walk_from<MODE>(start) + (int64_t)blockIdx.x * piece, (int64_t)INT_MAX - piece);
+        hi = min(walk_to<MODE>(a, n), lo + piece);
         end = MODE == LIST ? n : hi;
         if constexpr (MODE == LIST) list = (const __attribute__((address_space(4))) int *)(a.selected + ((size_t)b * a.c.nkv + hk) * a.listed);
         last = hi > lo ? (hi - 1) & ~(kPos - 1) : 0;           // the piece's last tile
-        slot0 = ((size_t)blockIdx.x * gridDim.z + b) * g.n_heads + h0;
+        slot0 = ((size_t)(MODE == BEHIND ? g.first_piece + blockIdx.x : blockIdx.x) * gridDim.z + b) * g.n_heads + h0;
         head_at = (size_t)hk * a.c.tile_bytes;
         page_bytes = (size_t)a.c.nkv * a.c.tile_bytes;
         row = (const __attribute__((address_space(4))) int *)(a.table.pages + (size_t)b * a.table.ld);
     }
-    // nothing to do: the first piece says so to the join
+    // nothing to do: the first piece says so to the join (BEHIND: all)
     __device__ __forceinline__ bool empty(const AttnArgs &g) const {
-        if (lo < hi || g.pieces == 1) return false;
-        if (blockIdx.x == 0 && (int)threadIdx.x < heads) g.ms[slot0 + threadIdx.x] = make_float2(-INFINITY, 0.f);
+        if (lo < hi || (MODE != BEHIND && g.pieces == 1)) return false;
+        if ((MODE == BEHIND || blockIdx.x == 0) && (int)threadIdx.x < heads) g.ms[slot0 + threadIdx.x] = make_float2(-INFINITY, 0.f);
         return true;
     }
     // tiles t and on; past the end: the last one again
@@ -359,7 +388,7 @@ __device__ __forceinline__ float capped(float x, float cap) { return __fmul_rn(c
 
 // The waves' O ([wave][head][HD + 4], unnormalised) and (maximum, sum) of each head: to out, or to the piece's part. A
 // thread takes four dims.
-template <int HD, int HEADS>
+template <int MODE, int HD, int HEADS>
 __device__ __forceinline__ void finish(const AttnArgs &g, int b, int h0, int heads, size_t slot0, const float *o,
                                        const float (&wm)[kWaves][HEADS], const float (&wsum)[kWaves][HEADS]) {
     constexpr int LD = HD + 4;
@@ -380,7 +409,7 @@ __device__ __forceinline__ void finish(const AttnArgs &g, int b, int h0, int hea
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(ow[e], f, x[e]);
         }
-        if (g.pieces == 1) {
+        if (MODE != BEHIND && g.pieces == 1) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = tot == 0.f ? 0.f : __fdiv_rn(x[e], tot);
             store4(a.out.dtype, g.wide, a.out.p, (int64_t)b * a.out.ts + (int64_t)(h0 + r) * a.out.hs + d, x);
@@ -520,7 +549,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
     for (int x = 0; x < Q; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i) buf[(wid * HEADS + (c & 3)) * LD + R::v_dim(m * Q + x, (c >> 2) * 4 + i)] = o[x][i];
-    finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
+    finish<MODE, HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
 // Rows over a float cache: S^T = K q^T leaves lane (c, m) head c's scores of positions 4m .. 4m + 3, which is the B operand
@@ -746,7 +775,7 @@ __global__ __launch_bounds__(kThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void pa
 #pragma unroll
             for (int r = 0; r < 4; ++r) buf[(wid * kCols + c) * LD + R::v_dim(x, 4 * m + r)] = o[x][r];
     }
-    finish<HD, kCols>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
+    finish<MODE, HD, kCols>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
 // Rows over a quantized cache, 4 NT query heads. K's codes meet q as they are: q is rounded to 2^-31 of its head's
@@ -1021,7 +1050,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 64 || (NT == 1 && C
             for (int x = 0; x < DPL; ++x)
                 buf[(wid * HEADS + 4 * t + (c >> 2)) * LD + R::v_element_dim(x, 4 * m + r)] = __fmul_rn(o[t][x][r], CT == DT_Q4_0 ? 0.0625f : 1.0f);
         }
-    finish<HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
+    finish<MODE, HD, HEADS>(g, at.b, at.h0, at.heads, at.slot0, buf, wm, wsum);
 }
 
 // grid (heads, sequences): the pieces of one head. Every wave has all pieces' weights, one or more per lane, and adds
@@ -1047,7 +1076,8 @@ __global__ __launch_bounds__(W *kWave) void paged_join_kernel(AttnArgs g) {
     load(wid, g.pieces - 1);
     const int n = min(max(a.lengths[b], 0), a.max_length);
     const int start = a.window > 0 && n > a.window ? n - a.window : 0;
-    const int used = max(1, (walk_to<MODE>(a, n) - walk_from<MODE>(start) + g.piece - 1) / g.piece);
+    // (BEHIND: all, those that have nothing with a sum of 0)
+    const int used = MODE == BEHIND ? g.pieces : max(1, (walk_to<MODE>(a, n) - walk_from<MODE>(start) + g.piece - 1) / g.piece);
     float top = lane < used ? ms[0].x : -INFINITY;
 #pragma unroll
     for (int q = 1; q < Q; ++q) {
@@ -1064,7 +1094,7 @@ __global__ __launch_bounds__(W *kWave) void paged_join_kernel(AttnArgs g) {
         mask[q] = 0;
         if (q * kWave >= used) continue;
         // a sum of NaN has a weight of NaN, whatever its maximum; one of 0 the weight 0 (its O may be NaN)
-        const bool on = lane + q * kWave < used && n > 0;
+        const bool on = lane + q * kWave < used && n > 0 && (MODE != BEHIND || ms[q].y != 0.f);
         f[q] = !on || ms[q].y == 0.f ? 0.f : ms[q].y != ms[q].y ? ms[q].y : __builtin_amdgcn_exp2f(ms[q].x - top);
         tot = __builtin_fmaf(on ? ms[q].y : 0.f, f[q], tot);
         mask[q] = __ballot(on);
@@ -1150,22 +1180,10 @@ inline Plan plan_of(int dtype, bool half, int nkv, int hd, int batch, int n_head
 
 inline size_t part_bytes(int hd, int batch, int n_heads, int pieces) { return (size_t)pieces * batch * n_heads * hd * sizeof(float); }
 
+// The kernel that a plan's workgroups run, and the join.
 template <int MODE>
-int launch_attention(const PagedAttn &a, hipStream_t s) {
-    AttnArgs g;
-    g.a = a;
-    g.n_heads = a.q.heads;
-    g.group = g.n_heads / a.c.nkv;
-    const bool half = a.q.dtype != DT_F32;
-    g.longest = MODE == LIST ? (int)std::min<int64_t>(a.max_length, (int64_t)a.listed * a.c.page_size) : a.max_length;
-    const Plan p = plan_of(a.c.dtype, half, a.c.nkv, a.c.hd, a.q.tokens, g.n_heads, g.longest, MODE == LIST ? 0 : a.window);
-    g.col_tiles = p.col_tiles;
-    g.piece = p.piece;
-    g.pieces = p.pieces;
-    g.wide = rows_wide(a.out);
-    g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kLoads.whole;
-    g.part = reinterpret_cast<float *>(a.ws);
-    g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
+bool launch_pieces(const AttnArgs &g, const Plan &p, bool half, hipStream_t s) {
+    const PagedAttn &a = g.a;
     const dim3 grid(p.pieces, a.c.nkv * p.col_tiles, a.q.tokens), block(kThreads);
     const bool short_terms = a.q.dtype == DT_BF16;
 #define SPH_FLOAT(CT, HD, HALF)                                                                    \
@@ -1182,15 +1200,38 @@ int launch_attention(const PagedAttn &a, hipStream_t s) {
     SPH_FLOAT(DT_F32, HD, false) SPH_FLOAT(DT_BF16, HD, false) SPH_FLOAT(DT_BF16, HD, true)       \
     SPH_FLOAT(DT_F16, HD, false) SPH_FLOAT(DT_F16, HD, true) SPH_QUANT(DT_Q8_0, HD) SPH_QUANT(DT_Q4_0, HD)
     SPH_ATTN_HD(64) SPH_ATTN_HD(128) SPH_ATTN_HD(256)
-    if (!hip_ok(hipGetLastError(), "paged attention launch")) return -1;
-    if (p.pieces > 1) {
-        const dim3 jg(g.n_heads, a.q.tokens);
+    return hip_ok(hipGetLastError(), "paged attention launch");
+}
+template <int MODE>
+bool launch_join(const AttnArgs &g, hipStream_t s) {
+    const PagedAttn &a = g.a;
+    const dim3 jg(g.n_heads, a.q.tokens);
 #define SPH_JOIN(HD, W) \
-    if (a.c.hd == HD && (p.pieces > kManyPieces) == (W == 16)) hipLaunchKernelGGL((paged_join_kernel<MODE, HD, W>), jg, dim3(W * kWave), 0, s, g);
+    if (a.c.hd == HD && (g.pieces > kManyPieces) == (W == 16)) hipLaunchKernelGGL((paged_join_kernel<MODE, HD, W>), jg, dim3(W * kWave), 0, s, g);
 #define SPH_JOIN_HD(HD) SPH_JOIN(HD, 4) SPH_JOIN(HD, 16)
-        SPH_JOIN_HD(64) SPH_JOIN_HD(128) SPH_JOIN_HD(256)
-        if (!hip_ok(hipGetLastError(), "paged attention join launch")) return -1;
-    }
+    SPH_JOIN_HD(64) SPH_JOIN_HD(128) SPH_JOIN_HD(256)
+    return hip_ok(hipGetLastError(), "paged attention join launch");
+}
+
+template <int MODE>
+int launch_attention(const PagedAttn &a, hipStream_t s) {
+    AttnArgs g;
+    g.a = a;
+    g.n_heads = a.q.heads;
+    g.group = g.n_heads / a.c.nkv;
+    const bool half = a.q.dtype != DT_F32;
+    static_assert(MODE != BEHIND);
+    g.longest = MODE == LIST ? (int)std::min<int64_t>(a.max_length, (int64_t)a.listed * a.c.page_size) : a.max_length;
+    const Plan p = plan_of(a.c.dtype, half, a.c.nkv, a.c.hd, a.q.tokens, g.n_heads, g.longest, MODE == LIST ? 0 : a.window);
+    g.col_tiles = p.col_tiles;
+    g.piece = p.piece;
+    g.pieces = p.pieces;
+    g.wide = rows_wide(a.out);
+    g.ordered = p.pieces == 1 && a.q.tokens > 1 && a.q.tokens <= kOrdered && p.groups >= kLoads.whole;
+    g.part = reinterpret_cast<float *>(a.ws);
+    g.ms = reinterpret_cast<float2 *>(a.ws + part_bytes(a.c.hd, a.q.tokens, g.n_heads, p.pieces));
+    if (!launch_pieces<MODE>(g, p, half, s)) return -1;
+    if (p.pieces > 1 && !launch_join<MODE>(g, s)) return -1;
     return 0;
 }
 

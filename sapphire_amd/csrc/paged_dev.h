@@ -207,10 +207,14 @@ struct PagedAttn {
     uint8_t *ws = nullptr;
     const int *selected = nullptr;         // attention over chosen pages: [batch][K/V heads][listed]
     int listed = 0;
+    const int *shared = nullptr;           // attention of groups of rows: their first positions that are the same
+    int rows = 1, max_own = 0;             // rows of a group; about how many positions each has behind those
 };
 size_t paged_attention_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length);
 int launch_paged_attention(const PagedAttn &a, hipStream_t s);
 int launch_paged_pages_attention(const PagedAttn &a, hipStream_t s);
+size_t paged_shared_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length);
+int launch_paged_shared_attention(const PagedAttn &a, hipStream_t s);
 int launch_paged_bounds(const PagedCache &c, uint16_t *bounds, const PageTable &t, const int *from, const int *lengths, int max_new,
                         hipStream_t s);
 size_t paged_select_workspace(int nkv, int batch, int max_pages);

@@ -9,7 +9,7 @@ from ctypes import byref
 import numpy as np
 
 from . import load
-from ._lib import AttentionC, PageChoiceC, PageTableC, PagedCacheC, RopeC, RowsC
+from ._lib import AttentionC, GroupsC, PageChoiceC, PageTableC, PagedCacheC, RopeC, RowsC
 from .device import DeviceArray, check
 
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)
@@ -87,6 +87,7 @@ class PagedCache:
         self.c.k, self.c.v = _at(self.k), _at(self.v)
         self._write, self._read = lib.sapphire_paged_write_dev, lib.sapphire_paged_read_dev
         self._bounds, self._select = lib.sapphire_paged_bounds_dev, lib.sapphire_paged_select_dev
+        self._shared_attention = lib.sapphire_paged_shared_attention_dev
         self._pages_attention = lib.sapphire_paged_pages_attention_dev
         self._attention, self._reorder = lib.sapphire_paged_attention_dev, lib.sapphire_paged_reorder_dev
 
@@ -109,6 +110,17 @@ class PagedCache:
         if self._attention(self.ref, layer, byref(q), byref(out), byref(table), _at(lengths), max_length,
                            byref(AttentionC(scale, window, softcap)), _at(lse), _at(workspace), stream):
             check(-1, "paged attention")
+
+    def shared_attention_workspace_bytes(self, batch, n_heads, max_length) -> int:
+        return load().sapphire_paged_shared_attention_workspace_bytes(self.ref, batch, n_heads, max_length)
+
+    def shared_attention(self, layer, q: RowsC, out: RowsC, table: PageTableC, lengths, max_length, rows, shared, scale, max_own=0,
+                         softcap=0.0, lse=None, workspace=None, stream=None) -> None:
+        """As attention(), where every `rows` rows on end share their first shared[group] positions."""
+        if self._shared_attention(self.ref, layer, byref(q), byref(out), byref(table), _at(lengths), max_length,
+                                  byref(GroupsC(_at(shared), rows, max_own)), byref(AttentionC(scale, 0, softcap)), _at(lse),
+                                  _at(workspace), stream):
+            check(-1, "shared attention")
 
     @property
     def bounds_bytes(self) -> int:
