@@ -12,9 +12,9 @@ namespace sapphire {
 
 namespace {
 
-constexpr int kSharedFill = 512;           // workgroups of the shared positions: two per compute unit
+constexpr int kSharedFill = 2048;          // waves of the shared positions: two per SIMD
 constexpr int kSharedUnit = 128;           // positions of a piece at least
-constexpr int kMostCols = 128;             // columns of a workgroup at most
+constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;
     SharedPlan shared;
@@ -25,10 +25,10 @@ Both both_of(int dtype, bool half, int nkv, int hd, int batch, int n_heads, int 
     b.own = plan_of(dtype, half, nkv, hd, batch, n_heads, std::min(max_length, std::max(max_own, 1)), 0);
     b.own.pieces = std::min(b.own.pieces, kMaxPieces / 2);
     b.shared.cols = std::min(rows, batch) * group;
-    const Columns k = columns_of(b.shared.cols, hd);
-    b.shared.col_tiles = (b.shared.cols + 16 * k.cs * k.wc - 1) / (16 * k.cs * k.wc);
+    const Columns k = columns_of(dtype, half, b.shared.cols, hd);
+    b.shared.col_tiles = (b.shared.cols + k.columns() - 1) / k.columns();
     const int64_t wgs = (int64_t)groups * nkv * b.shared.col_tiles;
-    const int64_t want = std::max<int64_t>(1, (kSharedFill + wgs - 1) / wgs);
+    const int64_t want = std::max<int64_t>(1, kSharedFill / (wgs * (k.nw == 8 ? 8 : 4)));
     b.shared.pieces = (int)std::min<int64_t>({want, (max_length + kSharedUnit - 1) / kSharedUnit, kMaxPieces / 2});
     b.shared.total = b.shared.pieces * nkv * groups;
     return b;
@@ -41,7 +41,7 @@ Both both_of(int dtype, bool half, int nkv, int hd, int batch, int n_heads, int 
 size_t paged_shared_workspace(int dtype, int nkv, int hd, int batch, int n_heads, int max_length) {
     const int64_t heads = (int64_t)batch * n_heads, most = std::min<int64_t>(kMaxPieces / 2, ((int64_t)max_length + kSharedUnit - 1) / kSharedUnit);
     const size_t slot = hd * sizeof(float) + sizeof(float2);
-    return (size_t)(heads + std::min<int64_t>(kSharedFill * kMostCols, heads * most)) * slot +
+    return (size_t)(heads + std::min<int64_t>(kSharedFill / 8 * kMostCols, heads * most)) * slot +
            std::max((size_t)heads * slot, paged_attention_workspace(dtype, nkv, hd, batch, n_heads, max_length));
 }
 
