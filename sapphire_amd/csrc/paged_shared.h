@@ -693,24 +693,21 @@ __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArg
                 *reinterpret_cast<pu4 *>(to + (fv + j) * 1024 + lane * 16) = w.on ? *reinterpret_cast<const pu4 *>(w.v + 4 * j) : pu4{0, 0, 0, 0};
         } else {
             uint8_t *at = to + lane * G::VB + (2 * vh + vi) * 4;
+            constexpr float kLess = CT == DT_Q8_0 ? -128.0f : -8.0f;
+            const float s0 = w.on ? w.vs[0] : 0.f, s1 = w.on ? w.vs[1] : 0.f, less0 = __fmul_rn(kLess, s0), less1 = __fmul_rn(kLess, s1);
 #pragma unroll
             for (int e = 0; e < G::VX; e += F::kQuant ? 1 : 2) {
                 const int x = vx * G::VX + e;
                 if constexpr (F::kQuant) {
-                    float x0, x1;
-                    if constexpr (CT == DT_Q8_0) {
-                        const int b0 = e, b1 = G::VX + e;              // bytes of the two positions
-                        x0 = (float)(int8_t)(w.v[b0 / 4] >> (8 * (b0 % 4)));
-                        x1 = (float)(int8_t)(w.v[b1 / 4] >> (8 * (b1 % 4)));
-                    } else {
-                        // (256 dims: a part is the low nibbles of its eight bytes, or the high ones)
-                        constexpr int RB = T::RUN;
-                        const int b0 = HD == 256 ? e : e % RB, b1 = RB + b0, up = HD == 256 ? 4 * vx : 4 * (e / RB);
-                        x0 = (float)((int)(w.v[b0 / 4] >> (8 * (b0 % 4) + up) & 15u) - 8);
-                        x1 = (float)((int)(w.v[b1 / 4] >> (8 * (b1 % 4) + up) & 15u) - 8);
-                    }
-                    x0 = w.on ? __fmul_rn(x0, w.vs[0]) : 0.f;
-                    x1 = w.on ? __fmul_rn(x1, w.vs[1]) : 0.f;
+                    // bytes of the two positions, as they are above -128 (Q4_0: nibbles above -8); times the scale in one
+                    // rounding, as the product of code and scale has
+                    constexpr int RB = CT == DT_Q8_0 ? G::VX : T::RUN;
+                    const int b0 = CT == DT_Q8_0 || HD == 256 ? e : e % RB, b1 = RB + b0;
+                    // (256 dims of Q4_0: a part is the low nibbles of its eight bytes, or the high ones)
+                    const int up = CT == DT_Q8_0 ? 0 : HD == 256 ? 4 * vx : 4 * (e / RB);
+                    const uint32_t w0 = CT == DT_Q8_0 ? w.v[b0 / 4] ^ 0x80808080u : w.v[b0 / 4] >> up & 0x0f0f0f0fu;
+                    const uint32_t w1 = CT == DT_Q8_0 ? w.v[b1 / 4] ^ 0x80808080u : w.v[b1 / 4] >> up & 0x0f0f0f0fu;
+                    float x0 = __builtin_fmaf((float)(w0 >> (8 * (b0 % 4)) & 255u), s0, less0), x1 = __builtin_fmaf((float)(w1 >> (8 * (b1 % 4)) & 255u), s1, less1);
 #pragma unroll
                     for (int t = 0; t < F::TV; ++t) *reinterpret_cast<uint32_t *>(at + (x * F::TV + t) * kWave * G::VB) = take_term<DT_BF16>(x0, x1);
                 } else {

@@ -13,7 +13,7 @@ namespace sapphire {
 namespace {
 
 constexpr int kSharedFill = 2048;          // waves of the shared positions: two per SIMD
-constexpr int kSharedUnit = 128;           // positions of a piece at least
+constexpr int kSharedUnit = 32;            // positions of a piece at least
 constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;
