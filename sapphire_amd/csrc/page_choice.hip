@@ -156,6 +156,7 @@ struct SelectArgs {
     PagedCache c;
     PageTable table;
     Rows q;
+    bool wide;                             // q's data and strides are multiples of 16 bytes
     const uint16_t *bounds;
     const int *lengths;
     int max_length, max_pages, group, k, first, last;
@@ -172,6 +173,60 @@ __device__ __forceinline__ u64 key_of(double s) {
     s = s != s ? INFINITY : s + 0.0;
     const u64 u = (u64)__double_as_longlong(s);
     return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// A double moved by DPP, or between halves of 32 lanes.
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+    const u64 u = (u64)__double_as_longlong(v);
+    return __longlong_as_double((long long)lanes::u64_dpp<CTRL>(u));
+}
+constexpr int kMirror = 0x140, kHalfMirror = 0x141, kXor2 = 0x4E, kXor1 = 0xB1, kOther16 = 0;
+
+// Sums over the LP lanes of a page of four heads' values: each step, which pairs every lane with one of the other half, halves
+// the heads that a lane goes on with, then the sums of what it has left. Lane l of a page ends with head (l / (LP / 4)) % 4.
+template <int CTRL>
+__device__ __forceinline__ double partner(double v) {
+    if constexpr (CTRL == kOther16) return __shfl_xor(v, 16, kWave);
+    else return moved<CTRL>(v);
+}
+template <int A, int B>
+__device__ __forceinline__ double scatter(const double (&s)[4], bool upper_a, bool upper_b) {
+    double t[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) t[i] = (upper_a ? s[2 + i] : s[i]) + partner<A>(upper_a ? s[i] : s[2 + i]);
+    return (upper_b ? t[1] : t[0]) + partner<B>(upper_b ? t[0] : t[1]);
+}
+template <int LP>
+__device__ __forceinline__ double page_sums(const double (&s)[4], int l) {
+    double t;
+    if constexpr (LP == 8) {
+        t = scatter<kHalfMirror, kXor2>(s, l & 4, l & 2);
+        return t + moved<kXor1>(t);
+    } else {
+        if constexpr (LP == 16) t = scatter<kMirror, kHalfMirror>(s, l & 8, l & 4);
+        else {
+            t = scatter<kOther16, kMirror>(s, l & 16, l & 8);
+            t += moved<kHalfMirror>(t);
+        }
+        t += moved<kXor2>(t);
+        return t + moved<kXor1>(t);
+    }
+}
+// The largest of the four heads' keys, in every lane of the page.
+template <int LP>
+__device__ __forceinline__ u64 page_max(u64 k) {
+    auto mx = [](u64 a, u64 b) { return a > b ? a : b; };
+    if constexpr (LP == 8) {
+        k = mx(k, lanes::u64_dpp<kXor2>(k));
+        return mx(k, lanes::u64_dpp<kHalfMirror>(k));
+    } else if constexpr (LP == 16) {
+        k = mx(k, lanes::u64_dpp<kHalfMirror>(k));
+        return mx(k, lanes::u64_dpp<kMirror>(k));
+    } else {
+        k = mx(k, lanes::u64_dpp<kMirror>(k));
+        return mx(k, (u64)__shfl_xor((long long)k, 16, kWave));
+    }
 }
 
 // Eight dims of a page per lane, HD / 8 lanes per page; every page's score, as a key, by four query heads at a time. Pages that
@@ -194,7 +249,7 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
             Raw8 r;
             float x[8];
             // (heads behind the last one repeat it)
-            load8(g.q.dtype, false, g.q.p, (int64_t)b * g.q.ts + (int64_t)(hk * g.group + min(h0 + h, g.group - 1)) * g.q.hs + l * 8, r);
+            load8(g.q.dtype, g.wide, g.q.p, (int64_t)b * g.q.ts + (int64_t)(hk * g.group + min(h0 + h, g.group - 1)) * g.q.hs + l * 8, r);
             values8(g.q.dtype, r, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -202,20 +257,23 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
                 down[h][e] = x[e] < 0.f ? x[e] : 0.f;
             }
         }
+        // a step's bounds are under way during the step before, and its page number during the one before that
+        const int step = gridDim.x * STEP;
         pu4 lo, hi;
-        int page = 0;
-        auto load = [&](int at) {
-            page = at < np ? row[at] : -1;
+        int page, number = i0 < np ? row[i0] : -1;
+        auto load = [&](int next) {
+            page = number;
+            number = next < np ? row[next] : -1;
             const uint16_t *p = of_head + (page >= 0 && page < g.c.pages ? (size_t)page : 0) * stride;
             lo = *reinterpret_cast<const pu4 *>(p);
             hi = *reinterpret_cast<const pu4 *>(p + HD);
         };
-        load(i0);
+        load(i0 + step);
 #pragma unroll 1
-        for (int i = i0; i - lane / LP < np; i += gridDim.x * STEP) {
+        for (int i = i0; i - lane / LP < np; i += step) {
             const pu4 a = lo, z = hi;
             const bool there = page >= 0 && page < g.c.pages;
-            load(i + gridDim.x * STEP);
+            load(i + 2 * step);
             double s[kHeads] = {};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -224,17 +282,8 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) s[h] = __builtin_fma(up[h][e], y, __builtin_fma(down[h][e], x, s[h]));
             }
-            // the lanes' sums
-#pragma unroll
-            for (int h = 0; h < kHeads; ++h)
-#pragma unroll
-                for (int off = 1; off < LP; off *= 2) s[h] += __shfl_xor(s[h], off, kWave);
-            u64 key = 0;
-#pragma unroll
-            for (int h = 0; h < kHeads; ++h) {
-                const u64 o = key_of(s[h]);
-                key = o > key ? o : key;
-            }
+            // (a head behind the last one repeats it)
+            u64 key = page_max<LP>(key_of(page_sums<LP>(s, l)));
             if (l == 0 && i < np) {
                 if (!there) key = 0;
                 else if (i < g.first || i >= np - g.last) key = kForced;
@@ -250,7 +299,8 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
 // decide are few enough to be ranked against each other. grid (K/V heads, sequences).
 constexpr int kPick = 1024, kPickWaves = kPick / kWave, kHold = 8, kBins = 1024, kFew = 64;
 __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
-    __shared__ int bins[kBins], counts[2][kHold][kPickWaves], wave_sums[kPickWaves];
+    __shared__ int bins[kBins], wave_sums[kPickWaves];
+    __shared__ uint32_t counts[kHold * kPickWaves], sums[kHold * kPickWaves / kWave];
     __shared__ u64 ors[kPickWaves], ands[kPickWaves], few[kFew], few_key;
     __shared__ int few_count, found[3], few_ties;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
@@ -266,17 +316,6 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
             key[e] = i < np ? keys[i] : 0;
         }
     };
-    auto block_sum = [&](int v) {                              // of all threads
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) v += __shfl_xor(v, off, kWave);
-        __syncthreads();
-        if (lane == 0) wave_sums[wid] = v;
-        __syncthreads();
-        int s = 0;
-#pragma unroll
-        for (int w = 0; w < kPickWaves; ++w) s += wave_sums[w];
-        return s;
-    };
     // pages taken anyway, the others that exist, and the bits in which those differ
     int forced = 0, others = 0;
     u64 any = 0, all = ~0ull;
@@ -284,16 +323,40 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
         load(blk);
 #pragma unroll
         for (int e = 0; e < kHold; ++e) {
-            forced += key[e] == kForced;
-            if (key[e] != 0 && key[e] != kForced) {
-                ++others;
-                any |= key[e];
-                all &= key[e];
-            }
+            const bool other = key[e] != 0 && key[e] != kForced;
+            forced += __popcll(__ballot(key[e] == kForced));
+            others += __popcll(__ballot(other));
+            any |= other ? key[e] : 0;
+            all &= other ? key[e] : ~0ull;
         }
     }
-    forced = block_sum(forced);
-    others = block_sum(others);
+#pragma unroll
+    for (int off = 1; off < kWave; off *= 2) {
+        any |= __shfl_xor(any, off, kWave);
+        all &= __shfl_xor(all, off, kWave);
+    }
+    if (lane == 0) {
+        ors[wid] = any;
+        ands[wid] = all;
+        bins[wid] = forced;
+        bins[kPickWaves + wid] = others;
+    }
+    __syncthreads();
+    {
+        const int w = lane & (kPickWaves - 1);
+        any = ors[w];
+        all = ands[w];
+        forced = bins[w];
+        others = bins[kPickWaves + w];
+#pragma unroll
+        for (int off = 1; off < kPickWaves; off *= 2) {
+            any |= __shfl_xor(any, off, kWave);
+            all &= __shfl_xor(all, off, kWave);
+            forced += __shfl_xor(forced, off, kWave);
+            others += __shfl_xor(others, off, kWave);
+        }
+    }
+    __syncthreads();
     int need = min(max(g.k - forced, 0), others), shift = 0;
     u64 edge = 0;                                              // keys >> shift above it are taken, the first `need` that equal it too
     if (need == others) {
@@ -303,21 +366,6 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
         edge = kForced - 1;
     } else {
         // (need < others, so that there is a key that decides)
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            any |= __shfl_xor(any, off, kWave);
-            all &= __shfl_xor(all, off, kWave);
-        }
-        if (lane == 0) {
-            ors[wid] = any;
-            ands[wid] = all;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kPickWaves; ++w) {
-            any |= ors[w];
-            all &= ands[w];
-        }
         int top = any == all ? 0 : 64 - __builtin_clzll(any ^ all);        // keys agree from this bit on
         u64 prefix = top == 64 ? 0 : any >> top;
         edge = prefix;
@@ -387,7 +435,8 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
             }
         }
     }
-    // in order of the pages: of every thousand the places of each wave's, from the counts of those ahead
+    // in order of the pages, from how many are taken, and tie, ahead of each wave's of every thousand: both counts of a block
+    // in one word
     int taken_before = 0, ties_before = 0;
     for (int blk = 0; blk < blocks; ++blk) {
         if (blocks > 1) load(blk);
@@ -398,33 +447,37 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
             const bool on = key[e] != 0, is_forced = key[e] == kForced;
             above[e] = __ballot(on && (is_forced || v > edge));
             ties[e] = __ballot(on && !is_forced && v == edge);
-            if (lane == 0) {
-                counts[0][e][wid] = __popcll(above[e]);
-                counts[1][e][wid] = __popcll(ties[e]);
-            }
+            if (lane == 0) counts[e * kPickWaves + wid] = (uint32_t)__popcll(above[e]) | (uint32_t)__popcll(ties[e]) << 16;
         }
         __syncthreads();
-#pragma unroll 1
-        for (int e = 0; e < kHold; ++e) {
-            int a = taken_before, t = ties_before, ea = 0, et = 0;
-            for (int w = 0; w < kPickWaves; ++w) {
-                const int ca = counts[0][e][w], ct = counts[1][e][w];
-                if (w < wid) a += ca, t += ct;
-                ea += ca;
-                et += ct;
-            }
-            const u64 below = (1ull << lane) - 1;
-            u64 ma = 0, mt = 0;
+        if (wid < kHold * kPickWaves / kWave) {
+            const uint32_t mine = counts[tid];
+            uint32_t upto = mine;
 #pragma unroll
-            for (int j = 0; j < kHold; ++j)
-                if (j == e) ma = above[j], mt = ties[j];
-            a += __popcll(ma & below);
-            t += __popcll(mt & below);
-            const bool is_above = ma >> lane & 1, is_tie = (mt >> lane & 1) && t < need;
-            if (is_above || is_tie) out[a + min(t, need)] = (blk * kHold + e) * kPick + tid;
-            taken_before += ea;
-            ties_before += et;
+            for (int off = 1; off < kWave; off *= 2) {
+                const uint32_t o = __shfl_up(upto, off, kWave);
+                upto += lane >= off ? o : 0;
+            }
+            counts[tid] = upto - mine;
+            if (lane == kWave - 1) sums[wid] = upto;
         }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kHold; ++e) {
+            const int at = e * kPickWaves + wid;
+            uint32_t ahead = counts[at];
+#pragma unroll
+            for (int w = 0; w < kHold * kPickWaves / kWave - 1; ++w) ahead += at >= (w + 1) * kWave ? sums[w] : 0;
+            const u64 below = (1ull << lane) - 1;
+            const int a = taken_before + (int)(ahead & 0xffffu) + __popcll(above[e] & below), t = ties_before + (int)(ahead >> 16) + __popcll(ties[e] & below);
+            const bool is_above = above[e] >> lane & 1, is_tie = (ties[e] >> lane & 1) && t < need;
+            if (is_above || is_tie) out[a + min(t, need)] = (blk * kHold + e) * kPick + tid;
+        }
+        uint32_t whole = 0;
+#pragma unroll
+        for (int w = 0; w < kHold * kPickWaves / kWave; ++w) whole += sums[w];
+        taken_before += whole & 0xffffu;
+        ties_before += whole >> 16;
         __syncthreads();
     }
     const int total = taken_before + min(ties_before, need);
@@ -458,6 +511,7 @@ int launch_paged_select(const PagedCache &c, const uint16_t *bounds, const Rows 
     g.c = c;
     g.table = t;
     g.q = q;
+    g.wide = rows_wide(q);
     g.bounds = bounds;
     g.lengths = lengths;
     g.max_length = max_length;
@@ -469,9 +523,10 @@ int launch_paged_select(const PagedCache &c, const uint16_t *bounds, const Rows 
     g.keys = static_cast<u64 *>(ws);
     g.selected = selected;
     const int step = kWaves * 512 / c.hd;
-    // q's 64-bit values are loaded once per workgroup: a few steps each where there are many
+    // q's 64-bit values are loaded once per workgroup, so that a few steps each pay; four documents of up to 131072 positions, 32
+    // heads over 8, in pages of 32: 28.9 us with 1024 workgroups in all (the choice with it), 29.6 with 512, 35.1 with 2048
     const int64_t pairs = (int64_t)q.tokens * c.nkv, steps = (g.max_pages + step - 1) / step;
-    const int64_t want = std::max<int64_t>(1, 2048 / pairs);
+    const int64_t want = std::max<int64_t>(1, 1024 / pairs);
     const dim3 grid((unsigned)std::min(steps, want), c.nkv, q.tokens);
 #define SPH_SCORES(HD, F16) \
     if (c.hd == HD && (c.dtype == DT_F16) == F16) hipLaunchKernelGGL((paged_scores_kernel<HD, F16>), grid, dim3(kThreads), 0, s, g);
