@@ -157,8 +157,8 @@ int sapphire_paged_bounds_dev(const sapphire_paged_cache_t *cache, int layer, vo
  * from bounds or a q that are not finite, counts as +inf. Pages that do not exist are not chosen.
  * selected[b][head][0 .. pages): their places in the sequence (page p / page_size of position p), rising, then -1. q: tokens x
  * n_heads x head_dim as for the attention, of any of the three types. lengths and max_length as there.
- * first + last <= pages. workspace: sapphire_paged_select_workspace_bytes() bytes, 16-byte aligned, which are enough for
- * calls of fewer and shorter sequences too; calls that share one must be ordered. */
+ * first + last <= pages <= 2^30 / page_size. workspace: sapphire_paged_select_workspace_bytes() bytes, 16-byte aligned, which
+ * are enough for calls of fewer and shorter sequences too; calls that share one must be ordered. */
 typedef struct {
     int pages, first, last;
 } sapphire_page_choice_t;

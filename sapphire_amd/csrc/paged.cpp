@@ -303,7 +303,7 @@ int sapphire_paged_shared_attention_dev(const sapphire_paged_cache_t *c, int lay
     if (at->window > 0) { set_error("shared attention: a window (%d): its rows share little", at->window); return -1; }
     a.max_length = max_length;
     a.shared = groups->shared;
-    a.rows = groups->rows;
+    a.rows = std::min(groups->rows, q->tokens);
     a.max_own = groups->max_own;
     if (!workspace_ok(sapphire_paged_shared_attention_workspace_bytes(c, q->tokens, q->heads, max_length), workspace, a)) return -1;
     return launch_paged_shared_attention(a, as_stream(stream));
@@ -384,7 +384,8 @@ int sapphire_paged_select_dev(const sapphire_paged_cache_t *c, int layer, const 
         return -1;
     }
     if (!lengths || !choice || !selected || !workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("bad paged select arguments"); return -1; }
-    if (choice->pages <= 0 || choice->first < 0 || choice->last < 0 || (int64_t)choice->first + choice->last > choice->pages) {
+    if (choice->pages <= 0 || (int64_t)choice->pages * c->page_size > (1 << 30) || choice->first < 0 || choice->last < 0 ||
+        (int64_t)choice->first + choice->last > choice->pages) {
         set_error("paged select: %d pages with the first %d and the last %d", choice->pages, choice->first, choice->last);
         return -1;
     }

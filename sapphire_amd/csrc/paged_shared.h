@@ -105,7 +105,9 @@ struct SharedQuery {
                 top = fmaxf(top, fabsf(x[i][e]));
             }
         }
-        unit = fabsf(sl2);
+        // (never 0: the mask's -inf times it is -inf, and a score of it is as good as 0)
+        constexpr float kLeast = 0x1p-149f;
+        unit = fmaxf(fabsf(sl2), kLeast);
         int sh = 0;
         if constexpr (F::kScaled) {
             top = odd ? INFINITY : top;
@@ -114,7 +116,7 @@ struct SharedQuery {
             int ex;
             (void)frexpf(top, &ex);                    // top < 2^ex
             sh = top > 0.f && top < INFINITY ? 15 - ex : 0;
-            unit = top < INFINITY ? ldexpf(unit, -sh - (CT == DT_Q4_0 ? 4 : 0)) : NAN;
+            unit = top < INFINITY ? fmaxf(ldexpf(unit, -sh - (CT == DT_Q4_0 ? 4 : 0)), kLeast) : NAN;
         }
 #pragma unroll
         for (int i = 0; i < QW; ++i) {
@@ -788,8 +790,11 @@ __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArg
         bool far = false;
 #pragma unroll
         for (int s = 0; s < CS; ++s) {
-            ref[s] = fmaxf(fmaxf(p[s][0][0], p[s][0][1]), fmaxf(p[s][0][2], p[s][0][3]));
-            if constexpr (HALVES == 2) ref[s] = fmaxf(ref[s], fmaxf(fmaxf(p[s][HALVES - 1][0], p[s][HALVES - 1][1]), fmaxf(p[s][HALVES - 1][2], p[s][HALVES - 1][3])));
+            ref[s] = p[s][0][0];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int r = h == 0; r < 4; ++r) ref[s] = __builtin_elementwise_maximum(ref[s], p[s][h][r]);
             ref[s] = cap > 0.f ? ref[s] : __fmul_rn(ref[s], q[s].unit);        // (unit >= 0: the largest score is the largest sum's)
             far |= ref[s] > mx[s] + F::kLift + kLazy;
         }

@@ -33,7 +33,7 @@ def test_bounds_refused(lib, change):
 SELECT = [dict(c=dict(v=None)), dict(layer=-1), dict(layer=2), dict(bounds=None), dict(bounds=P + 2), dict(q=None), dict(q=dict(heads=3)),
           dict(q=dict(hd=128)), dict(q=dict(dtype=Q8_0)), dict(q=dict(tokens=4)), dict(q=dict(ts=-1)), dict(t=dict(rows=2)), dict(t=dict(ld=0)),
           dict(lengths=None), dict(max_length=0), dict(max_length=129), dict(choice=None), dict(choice=(0, 0, 0)), dict(choice=(-1, 0, 0)),
-          dict(choice=(3, 2, 2)), dict(choice=(3, -1, 2)), dict(choice=(3, 1, -1)), dict(choice=(3, 2**31 - 1, 2**31 - 1)), dict(selected=None),
+          dict(choice=(3, 2, 2)), dict(choice=(3, -1, 2)), dict(choice=(3, 1, -1)), dict(choice=(3, 2**31 - 1, 2**31 - 1)), dict(choice=(2**30, 0, 0)), dict(choice=(2**31 - 1, 0, 0)), dict(selected=None),
           dict(ws=None), dict(ws=P + 8)]
 
 

@@ -19,7 +19,7 @@ class Case:
         self.cache, self.io, self.hd, self.nkv, self.heads, self.ps, self.lens = cache, io, hd, nkv, heads, ps, lens
         self.table, pages = tables(rng, lens, ps)
         self.c = Cache(cache, 1, pages, ps, nkv, hd)
-        self.k, self.v = [], []
+        self.k, self.v, self.scale = [], [], hd**-0.5
         for s, n in enumerate(lens):
             k, v = (rng.normal(size=(n, nkv, hd)).astype(np.float32) for _ in range(2))
             self.c.fill(0, self.table, s, k, v)
@@ -38,7 +38,7 @@ class Case:
         k = sel.shape[2]
         self.ws = self.ws or DeviceArray(max(1, self.c.c.attention_workspace_bytes(len(self.lens), self.heads, k * self.ps)))
         self.sel = dev(sel.astype(np.int32))
-        self.c.c.pages_attention(0, self.rq[0], self.ro[0], self.pt, self.dn, self.sel, k, self.hd**-0.5, window=window, softcap=cap, lse=self.lse,
+        self.c.c.pages_attention(0, self.rq[0], self.ro[0], self.pt, self.dn, self.sel, k, self.scale, window=window, softcap=cap, lse=self.lse,
                                  workspace=self.ws, stream=stream)
 
     def check(self, sel, window=0, cap=0.0):
@@ -56,7 +56,7 @@ class Case:
                 keep[:max(0, n - window) if window > 0 else 0] = False
                 keep = keep[:n]
                 q = self.q[s, h * g:(h + 1) * g]
-                out, l, size, mean = ref.attention64(q, self.k[s][keep][:, h:h + 1], self.v[s][keep][:, h:h + 1], self.hd**-0.5, 0, cap)
+                out, l, size, mean = ref.attention64(q, self.k[s][keep][:, h:h + 1], self.v[s][keep][:, h:h + 1], float(np.float32(self.scale)), 0, cap)
                 tol, ltol = ref.attention_bound(self.io, self.io != F32, self.hd, int(keep.sum()), out, l, size, mean, cap)
                 at = slice(h * g, (h + 1) * g)
                 worst = np.max(np.abs(got[s, at] - out) / tol)
@@ -207,3 +207,77 @@ def test_step(hip, cache, io):
         c.check(want)
         c.k, c.v = held
     g.close()
+
+
+def test_pages_past_four_gigabytes(hip):
+    """The same rows in the first pages and in the last ones of pools of more than 2^32 bytes: the same bounds, choice and outputs."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PagedCache, PageTable
+    rng = np.random.default_rng(12)
+    hd, ps, pages, heads, n, chosen_pages = 256, 64, 70000, 4, 700, 4
+    c = PagedCache(F32, 1, pages, ps, 1, hd)
+    assert c.nbytes > 2**32
+    ld = -(-n // ps)
+    k, v = (device_rows(rng.normal(size=(n, 1, hd)).astype(np.float32), F32) for _ in range(2))
+    q = device_rows(rng.normal(size=(1, heads, hd)).astype(np.float32), F32)
+    at, seqs, lens = dev(np.arange(n, dtype=np.int32)), dev(np.zeros(n, np.int32)), dev(np.array([n], np.int32))
+    bounds, got = DeviceArray(c.bounds_bytes), []
+    ws = [DeviceArray(max(1, b)) for b in (c.select_workspace_bytes(1, n), c.attention_workspace_bytes(1, heads, chosen_pages * ps))]
+    for first in (0, pages - ld):
+        t = dev(np.arange(first, first + ld, dtype=np.int32)[None])
+        pt = PageTable(t, 1, ld)
+        o, sel = device_rows(np.zeros((1, heads, hd), np.float32), F32), dev(np.zeros((1, 1, chosen_pages), np.int32))
+        c.write(0, k[0], v[0], pt, at, seqs=seqs)
+        c.bounds(0, bounds, pt, lens, n)
+        c.select(0, bounds, q[0], pt, lens, n, sel, chosen_pages, workspace=ws[0])
+        c.pages_attention(0, q[0], o[0], pt, lens, sel, chosen_pages, hd**-0.5, workspace=ws[1])
+        sync()
+        b = bounds.numpy().view(np.uint16).reshape(pages, 2, hd)[first:first + ld]
+        got.append((b, sel.numpy(), o[1].numpy()))
+    for x, y in zip(*got):
+        np.testing.assert_array_equal(x, y)
+    want = np.stack([page_bounds(F32, k[3][i * ps:(i + 1) * ps])[0] for i in range(ld)])
+    np.testing.assert_array_equal(values(got[0][0], False), values(want, False))
+    for d in (c.k, c.v):
+        d.free()
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+def test_scales(hip, cache, io):
+    """Scales below 0 and of 0; lists that end inside a piece."""
+    rng = np.random.default_rng(13)
+    for scale in (-0.15, 0.0):
+        c = Case(rng, cache, io, 64, 2, 6, 16, [200, 33, 5])
+        c.scale = scale
+        sel = chosen(rng, c.lens, 2, 16, 7)
+        c.run(sel)
+        c.check(sel)
+
+
+def test_calls_at_once(hip):
+    """Choice and attention under way on two streams, each in workspaces of its own: the same as alone."""
+    from tests.test_page_choice_gpu import Select
+    rng = np.random.default_rng(14)
+    cases = [Case(rng, BF16, BF16, 128, 2, 8, 32, [3000, 500]), Case(rng, Q8_0, F32, 64, 1, 4, 16, [900, 100, 5])]
+    chooses = [Select(rng, BF16, BF16, 2, 8, 128, 32, [32 * 9000, 32 * 100]), Select(rng, Q4_0, F32, 1, 3, 64, 16, [16 * 500])]
+    lists = [chosen(rng, c.lens, c.nkv, c.ps, 20) for c in cases]
+    streams = [hip.sapphire_stream_create() for _ in cases]
+    want, keep = [], []
+    for c, sel in zip(cases, lists):
+        c.run(sel)
+        c.check(sel)
+        want.append(c.ro[1].numpy())
+    for _ in range(4):
+        outs = []
+        for _ in range(6):
+            for c, s, sel, stream in zip(cases, chooses, lists, streams):
+                c.run(sel, stream=stream)
+                keep.append(c.sel)                     # (the list is read after the call returns)
+                outs.append((s, s.run(50, 1, 1, stream=stream)))
+        sync()
+        for c, w in zip(cases, want):
+            np.testing.assert_array_equal(c.ro[1].numpy(), w)
+        for s, o in outs[-2:]:
+            np.testing.assert_array_equal(o.numpy(), s.want(50, 1, 1))
+    for s in streams:
+        hip.sapphire_stream_destroy(s)

@@ -25,7 +25,7 @@ class Case:
         order_of = iter(rng.permutation(pages))
         self.table = np.full((len(lens), ld), -1, np.int32)
         self.c = Cache(cache, 1, pages, ps, nkv, hd)
-        self.k, self.v = [], []
+        self.k, self.v, self.scale = [], [], hd**-0.5
         for g in range(groups):
             mine = range(g * rows, min(len(lens), (g + 1) * rows))
             top = max(lens[r] for r in mine) if drafts else -(-common[g] // ps) * ps
@@ -57,7 +57,7 @@ class Case:
         from sapphire_amd.device import DeviceArray
         self.ws = self.ws or DeviceArray(self.c.c.shared_attention_workspace_bytes(len(self.lens), self.heads, self.top))
         self.shared = dev(np.array(shared, np.int32)) if isinstance(shared, list) else shared
-        self.c.c.shared_attention(0, self.rq[0], out or self.ro[0], self.pt, self.dn, self.top, self.rows, self.shared, self.hd**-0.5, max_own=own,
+        self.c.c.shared_attention(0, self.rq[0], out or self.ro[0], self.pt, self.dn, self.top, self.rows, self.shared, self.scale, max_own=own,
                                   softcap=cap, lse=self.lse if lse else None, workspace=self.ws, stream=stream)
 
     def got(self):
@@ -71,8 +71,11 @@ class Case:
         assert (raw[mask] == 7).all(), "elements between the rows were written"
         return got, self.lse.numpy()
 
-    def check(self, cap=0.0):
+    def check(self, cap=0.0, but=None):
+        """but: a (row, head) that is NaN."""
         got, lse = self.got()
+        if but:
+            assert np.isnan(got[but]).all() and np.isnan(lse[but])
         assert (lse[-1] == 5).all()
         for r, n in enumerate(self.lens):
             n = min(max(n, 0), self.top)
@@ -80,8 +83,10 @@ class Case:
             for rr, i in self.broken:
                 if rr == r:
                     keep[i * self.ps:(i + 1) * self.ps] = False
-            out, l, size, mean = ref.attention64(self.q[r], self.k[r][:n][keep], self.v[r][:n][keep], self.hd**-0.5, 0, cap)
+            out, l, size, mean = ref.attention64(self.q[r], self.k[r][:n][keep], self.v[r][:n][keep], float(np.float32(self.scale)), 0, cap)
             tol, ltol = ref.attention_bound(self.io, self.io != F32, self.hd, n, out, l, size, mean, cap)
+            if but and but[0] == r:
+                got[but], lse[but] = out[but[1]], l[but[1]]
             worst = np.max(np.abs(got[r] - out) / tol)
             assert worst <= 1, (r, n, worst)
             dead = np.isneginf(l)
@@ -149,6 +154,123 @@ def test_cap_peaks_and_strides(hip, cache, io):
         c = Case(rng, cache, io, 128, 1, 4, 48, 8, [480], [481 + 9 * r for r in range(8)], order=order, pad=pad, peak=peak)
         c.run([480], 64, cap)
         c.check(cap)
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+@pytest.mark.parametrize("rows", [2, 20], ids=["few", "many"])
+def test_scales_and_sizes_of_q(hip, cache, io, rows):
+    """Scales below 0 and of 0, and rows of q so small that with the scale they leave fp32's range: behind tiles that do not count (a
+    page that does not exist, an odd number of tiles) too."""
+    rng = np.random.default_rng(13)
+    for size, scale in ((1.0, -0.1), (1.0, 0.0), (1e-30, 0.0), (2.0**-149, 0.125), (2.0**-24, 1e-30), (1e30, 1e-31)):
+        c = Case(rng, cache, io, 128, 1, 4, 16, rows, [144], [145 + r for r in range(rows)], broken=[(0, 3)])
+        with np.errstate(over="ignore", under="ignore"):
+            x = ref.to_type(io, np.minimum(np.abs(c.q) * size, 6e4 if io == F16 else 1e38).astype(np.float32) * np.sign(c.q))
+        c.rq[3][...] = x
+        c.rq[1].upload(c.rq[2])
+        c.q, c.scale = ref.from_type(io, x), scale
+        c.run([144], 20)
+        c.check()
+    c = Case(rng, cache, io, 128, 1, 4, 16, rows, [144], [145 + r for r in range(rows)], broken=[(0, 3)])
+    c.scale = -0.2
+    c.run([144], 20, 10.0)
+    c.check(10.0)
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+@pytest.mark.parametrize("rows", [3, 20], ids=["few", "many"])
+def test_not_finite(hip, cache, io, rows):
+    """A NaN and an infinity in V of shared positions: their dim (quantized: the dims of their block) is not finite, the others have
+    the same bits as without; a NaN in q: its head is NaN, the others are not touched."""
+    rng = np.random.default_rng(14)
+    heads, hd = 4, 128
+    c = Case(rng, cache, io, hd, 1, heads, 16, rows, [160], [161 + r for r in range(rows)])
+    c.run([160], 30)
+    want = c.got()[0]
+    q = c.rq[3][1, 2, 7].copy()
+    c.rq[3][1, 2, 7] = ref.to_type(io, np.full(1, np.nan, np.float32))[0]
+    c.rq[1].upload(c.rq[2])
+    c.q[1, 2] = 0.0
+    c.run([160], 30)
+    c.check(but=(1, 2))
+    c.rq[3][1, 2, 7] = q
+    c.rq[1].upload(c.rq[2])
+    k, v = c.k[0][:160], c.v[0][:160].copy()
+    odd = np.zeros((rows, heads, hd), bool)
+    for p, dim, x in ((37, 5, np.nan), (100, 41, np.inf)):
+        v[p, 0, dim] = x
+        if cache in (Q8_0, Q4_0):
+            odd[:, :, dim // 32 * 32:dim // 32 * 32 + 32] = True
+        else:
+            odd[:, :, dim] = True
+    with np.errstate(all="ignore"):
+        c.c.fill(0, c.table, 0, k, v)
+    c.c.upload()
+    c.run([160], 30)
+    got = c.got()[0]
+    assert not np.isfinite(got[odd]).any()
+    if cache not in (Q8_0, Q4_0):                      # (written again, the codes may be others)
+        np.testing.assert_array_equal(got[~odd], want[~odd])
+    assert np.isfinite(got[~odd]).all()
+
+
+def test_rows_of_a_group_beyond_the_call(hip):
+    """A number of rows far above the call's: one group."""
+    rng = np.random.default_rng(15)
+    c = Case(rng, BF16, BF16, 64, 1, 8, 16, 5, [96], [97, 100, 113, 96, 120])
+    for rows in (5, 6, 2**30, 2**31 - 1):
+        c.rows = rows
+        c.run([96], 24)
+        c.check()
+
+
+def test_calls_at_once(hip):
+    """Two calls under way on two streams, each in a workspace of its own, again and again: the same bits as alone."""
+    rng = np.random.default_rng(16)
+    cases = [Case(rng, BF16, BF16, 128, 2, 16, 32, 8, [960], [961 + r for r in range(8)]), Case(rng, Q8_0, F32, 128, 1, 4, 32, 30, [480], [490 + r for r in range(30)])]
+    shared = [dev(np.array([n], np.int32)) for n in (960, 480)]
+    streams = [hip.sapphire_stream_create() for _ in cases]
+    want = []
+    for c, on in zip(cases, shared):
+        c.run(on, 40)
+        want.append(c.got()[0])
+        c.ro[1].upload(c.ro[2] * 0 + 7)
+    for _ in range(5):
+        for _ in range(8):
+            for c, on, s in zip(cases, shared, streams):
+                c.run(on, 40, stream=s)
+        for c, w in zip(cases, want):
+            np.testing.assert_array_equal(c.got()[0], w)
+    for s in streams:
+        hip.sapphire_stream_destroy(s)
+
+
+@pytest.mark.parametrize("rows", [4, 12], ids=["few", "many"])
+def test_pages_past_four_gigabytes(hip, rows):
+    """The same rows in the first pages and in the last ones of pools of more than 2^32 bytes: the same bits."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import PagedCache, PageTable
+    rng = np.random.default_rng(17)
+    hd, ps, pages, heads, n = 256, 64, 140000, 4, 400
+    c = PagedCache(BF16, 1, pages, ps, 1, hd)
+    assert c.nbytes > 2**32
+    ld = -(-n // ps)
+    k, v = (device_rows(rng.normal(size=(n, 1, hd)).astype(np.float32), BF16) for _ in range(2))
+    q = device_rows(rng.normal(size=(rows, heads, hd)).astype(np.float32), BF16)
+    at, lens, shared = dev(np.arange(n, dtype=np.int32)), dev(n - rows + 1 + np.arange(rows, dtype=np.int32)), dev(np.array([n], np.int32))
+    ws, got = DeviceArray(c.shared_attention_workspace_bytes(rows, heads, n)), []
+    for first in (0, pages - ld):
+        table = np.broadcast_to(np.arange(first, first + ld, dtype=np.int32), (rows, ld)).copy()
+        t = dev(table)
+        o = device_rows(np.zeros((rows, heads, hd), np.float32), BF16)
+        c.write(0, k[0], v[0], PageTable(t, rows, ld), at, seqs=dev(np.zeros(n, np.int32)))
+        c.shared_attention(0, q[0], o[0], PageTable(t, rows, ld), lens, n, rows, shared, hd**-0.5, max_own=rows, workspace=ws)
+        sync()
+        got.append(o[1].numpy())
+    np.testing.assert_array_equal(got[0], got[1])
+    assert (got[0] != 0).mean() > 0.9
+    for d in (c.k, c.v):
+        d.free()
 
 
 def test_lengths_are_clamped_and_no_lse(hip):

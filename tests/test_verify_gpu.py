@@ -195,3 +195,45 @@ def test_captured(hip):
         np.testing.assert_array_equal(got[0], want[0])
         np.testing.assert_array_equal(got[1], want[1])
     g.close()
+
+
+def test_rows_past_four_gigabytes(hip):
+    """Rows 2^30 elements apart, of both models: what rows next to each other give."""
+    from sapphire_amd.device import DeviceArray
+    from sapphire_amd.paged import verify, verify_workspace_bytes
+    rng = np.random.default_rng(9)
+    n, ld = 5000, 1 << 30
+    logits, draft, tokens, draws = inputs(rng, 1, 3, n, near=0.1)
+    draws[:, :3] *= 0.5
+    on = [DeviceArray((len(x[0]) - 1) * ld * 4 + n * 4) for x in (logits, draft)]
+    for d, x in zip(on, (logits, draft)):
+        for i, row in enumerate(x[0]):
+            assert hip.sapphire_memcpy_h2d(d.ptr + i * ld * 4, row.ctypes.data, row.nbytes) == 0
+    ws, out, kept = DeviceArray(verify_workspace_bytes(n, 1, 3)), dev(np.zeros((1, 4), np.int32)), dev(np.zeros(1, np.int32))
+    t, d = dev(tokens.astype(np.int32)), dev(draws)
+    for temperature in (1.0, 0.0):
+        verify(on[0], ld, n, 1, 3, t, d, out, kept, ws, draft_logits=on[1], draft_ld=ld, temperature=temperature)
+        assert hip.sapphire_synchronize() == 0
+        want = verify64(logits, draft, tokens, None, draws, temperature)
+        np.testing.assert_array_equal(out.numpy(), want[0])
+        np.testing.assert_array_equal(kept.numpy(), want[1])
+    for x in on:
+        x.free()
+
+
+def test_calls_at_once(hip):
+    """Two calls under way on two streams, each in a workspace of its own: the same as alone."""
+    rng = np.random.default_rng(10)
+    sets = [inputs(rng, 6, 4, 30000), inputs(rng, 2, 7, 5000)]
+    calls = [Call(lo, q, x, None, u) for lo, q, x, u in sets]
+    streams = [hip.sapphire_stream_create() for _ in calls]
+    for _ in range(4):
+        for _ in range(8):
+            for c, s in zip(calls, streams):
+                c.run(stream=s)
+        for c, (lo, q, x, u) in zip(calls, sets):
+            got, want = c.result(), verify64(lo, q, x, None, u, 1.0)
+            np.testing.assert_array_equal(got[0], want[0])
+            np.testing.assert_array_equal(got[1], want[1])
+    for s in streams:
+        hip.sapphire_stream_destroy(s)
