@@ -14,6 +14,7 @@ namespace {
 // group, a tile of them is a workgroup's.
 struct SharedPlan {
     int cols, col_tiles, pieces, total;    // total: (piece, K/V head, group) triples
+    int cs, nw;                            // of Columns
     bool wide;                             // q's data and strides are multiples of 16 bytes
 };
 
@@ -963,37 +964,37 @@ __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArg
 }
 
 // Columns of a workgroup. Up to 32: as few sets as there are, and the waves take different positions. More: all waves side by
-// side, with K and V through LDS; two sets a wave where there are columns for them and they fit the registers of two waves.
+// side, with K and V through LDS.
 constexpr int kFewColumns = 32;
 struct Columns {
     int cs, nw;                            // sets of a wave, waves side by side (0: one, of a workgroup that splits positions)
     int columns() const { return 16 * cs * std::max(nw, 1); }
 };
+// Sets of a wave at most: two where they fit the registers of two waves (Q4_0's do not, for one: 32 rows of 32 bf16 heads over
+// 8 behind 65536 positions 122 us with one, 144 with two).
 constexpr int wide_sets(int dtype, bool half, int hd) {
-    return hd == 64 ? 2 : hd == 128 && half && dtype != DT_Q8_0 ? 2 : hd == 128 && dtype == DT_F16 ? 2 : 1;
+    return hd == 64 ? 2 : hd == 128 && (dtype == DT_F16 || (dtype == DT_BF16 && half)) ? 2 : 1;
 }
-inline Columns columns_of(int dtype, bool half, int cols, int hd) {
+inline Columns columns_of(int sets, int cols, int hd) {
     if (cols <= kFewColumns) return Columns{cols <= 16 || hd == 256 ? 1 : 2, cols > 16 && hd == 256 ? 2 : 0};
-    const int cs = cols <= 64 ? 1 : wide_sets(dtype, half, hd);
+    const int cs = cols <= 64 ? 1 : sets;
     return Columns{cs, cols <= 64 * cs ? 4 : 8};
 }
 
 template <int CT, int HD, bool HALF, bool SHORT>
 void launch_shared_form(const AttnArgs &g, const SharedPlan &sp, hipStream_t s) {
     const dim3 grid((unsigned)((sp.total + 7) / 8 * 8 * sp.col_tiles));
-    const Columns k = columns_of(CT, HALF, sp.cols, HD);
     const bool few = sp.cols <= kFewColumns;
 #define SPH_FEW_COLS(CS, WC) \
-    if (few && k.cs == CS && std::max(k.nw, 1) == WC) hipLaunchKernelGGL((paged_shared_kernel<CT, HD, HALF, SHORT, CS, WC>), grid, dim3(kThreads), 0, s, g, sp);
+    if (few && sp.cs == CS && std::max(sp.nw, 1) == WC) hipLaunchKernelGGL((paged_shared_kernel<CT, HD, HALF, SHORT, CS, WC>), grid, dim3(kThreads), 0, s, g, sp);
     SPH_FEW_COLS(1, 1)
     if constexpr (HD == 256) { SPH_FEW_COLS(1, 2) }
     else { SPH_FEW_COLS(2, 1) }
 #undef SPH_FEW_COLS
 #define SPH_WIDE(CS, NW) \
-    if (!few && k.cs == CS && k.nw == NW) hipLaunchKernelGGL((paged_shared_wide_kernel<CT, HD, HALF, SHORT, CS, NW>), grid, dim3(NW * kWave), 0, s, g, sp);
-    SPH_WIDE(1, 4)
+    if (!few && sp.cs == CS && sp.nw == NW) hipLaunchKernelGGL((paged_shared_wide_kernel<CT, HD, HALF, SHORT, CS, NW>), grid, dim3(NW * kWave), 0, s, g, sp);
+    SPH_WIDE(1, 4) SPH_WIDE(1, 8)
     if constexpr (wide_sets(CT, HALF, HD) == 2) { SPH_WIDE(2, 4) SPH_WIDE(2, 8) }
-    else { SPH_WIDE(1, 8) }
 #undef SPH_WIDE
 }
 

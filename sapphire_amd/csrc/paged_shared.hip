@@ -12,25 +12,50 @@ namespace sapphire {
 
 namespace {
 
-constexpr int kSharedFill = 2048;          // waves of the shared positions: two per SIMD
-constexpr int kSharedUnit = 32;            // positions of a piece at least
+// Pieces: a piece more shortens every workgroup's walk, and adds a slot of each column that is written and joined. As many as
+// fill the chip (two waves per SIMD; of few columns, whose waves have no barriers, one: 8 rows of 32 heads over 8, bf16, behind
+// 16384 positions 28 us, with two 35; behind 131072 109 and 115), of eight steps of a wide workgroup (32 rows behind 4096
+// positions 33 us, of two 40) or one of each wave of few columns; but half of the compute
+// units get a workgroup in any case (six drafted rows of 4 heads behind 1018 positions, fp32: 19.6 us in 32 pieces, 21.8 in 16).
+constexpr int kSharedFill = 2048, kFewFill = 1024;         // waves of the shared positions at once
+constexpr int kSharedUnit = 32, kFewUnit = 128, kWideSteps = 8;
+constexpr int kUnits = 256;               // compute units
+// Positions of a piece from which on two sets a wave pay: they read K and V half as often, but twice as many pieces of half as
+// many workgroups are joined (bf16, 64 rows of 32 heads over 8: behind 16384 positions 69 us with two sets, 62 with one; behind
+// 65536 141 and 162).
+constexpr int kTwoSets = 768;
 constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;
     SharedPlan shared;
 };
+SharedPlan shared_plan(int dtype, int sets, int nkv, int hd, int groups, int cols, int max_length) {
+    SharedPlan p;
+    p.cols = cols;
+    const Columns k = columns_of(sets, cols, hd);
+    p.cs = k.cs;
+    p.nw = k.nw;
+    p.col_tiles = (cols + k.columns() - 1) / k.columns();
+    const bool few = cols <= kFewColumns;
+    const int64_t wgs = (int64_t)groups * nkv * p.col_tiles;
+    const int64_t full = (few ? kFewFill : kSharedFill) / (wgs * (k.nw == 8 ? 8 : 4)), one = kUnits / wgs;
+    const int unit = few ? kFewUnit : kWideSteps * (dtype == DT_F32 || hd == 256 ? 16 : 32);
+    int64_t pieces = std::max(std::min<int64_t>(one / 2, (max_length + kSharedUnit - 1) / kSharedUnit), std::min<int64_t>(full, max_length / unit));
+    // (few compute units with two workgroups would keep the others waiting: 12 rows over 4 K/V heads, fp32, behind 8192 positions
+    // 31 us in 64 pieces, 37.5 in 65)
+    if (pieces > one && 2 * pieces < 3 * one) pieces = one;
+    p.pieces = (int)std::min<int64_t>(std::max<int64_t>(1, pieces), kMaxPieces / 2);
+    p.total = p.pieces * nkv * groups;
+    return p;
+}
 Both both_of(int dtype, bool half, int nkv, int hd, int batch, int n_heads, int max_length, int rows, int max_own) {
     Both b;
-    const int group = n_heads / nkv, groups = (batch + rows - 1) / rows;
+    const int groups = (batch + rows - 1) / rows, cols = std::min(rows, batch) * (n_heads / nkv);
     b.own = plan_of(dtype, half, nkv, hd, batch, n_heads, std::min(max_length, std::max(max_own, 1)), 0);
     b.own.pieces = std::min(b.own.pieces, kMaxPieces / 2);
-    b.shared.cols = std::min(rows, batch) * group;
-    const Columns k = columns_of(dtype, half, b.shared.cols, hd);
-    b.shared.col_tiles = (b.shared.cols + k.columns() - 1) / k.columns();
-    const int64_t wgs = (int64_t)groups * nkv * b.shared.col_tiles;
-    const int64_t want = std::max<int64_t>(1, kSharedFill / (wgs * (k.nw == 8 ? 8 : 4)));
-    b.shared.pieces = (int)std::min<int64_t>({want, (max_length + kSharedUnit - 1) / kSharedUnit, kMaxPieces / 2});
-    b.shared.total = b.shared.pieces * nkv * groups;
+    b.shared = shared_plan(dtype, wide_sets(dtype, half, hd), nkv, hd, groups, cols, max_length);
+    if (b.shared.cs == 2 && cols > kFewColumns && max_length < (int64_t)kTwoSets * b.shared.pieces)
+        b.shared = shared_plan(dtype, 1, nkv, hd, groups, cols, max_length);
     return b;
 }
 
