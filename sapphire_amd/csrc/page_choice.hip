@@ -4,6 +4,7 @@
 // ranked without reading them. Borders between chosen and left pages are as close as scores come, so that sums run in 64 bits
 // and ties go by the page's place in the sequence.
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "lanes.h"
@@ -28,13 +29,33 @@ struct BoundsArgs {
 __device__ __forceinline__ float low_of(float a, float b) { return __builtin_elementwise_minimum(a, b); }      // (NaN stays)
 __device__ __forceinline__ float high_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// fp32 to 16 bits, rounded up or down. The values of a cache of that type stay as they are.
-template <int CT>
+// fp32 to bf16, rounded up or down.
 __device__ __forceinline__ uint32_t outward(float x, bool up) {
-    if constexpr (CT == DT_F16) return to_f16(x);
     if (x != x) return 0x7fc0u;
     const uint32_t u = __float_as_uint(x);
     return ((u >> 31 != 0) == up ? u : u + 0xffffu) >> 16;
+}
+
+// Extremes over a row of 16 lanes: each step, which pairs every lane with one of the other half, halves the values that a lane goes
+// on with. Of N of them, lane c ends with N / 16, from c * N / 16 on; of eight, lanes 2i and 2i + 1 with value i.
+// (Four steps of all N values in every lane are 512 instructions for 32 of them, of both kinds; the elements of a page of 32
+// positions take 192.)
+template <int CTRL, int H, int N, class Op>
+__device__ __forceinline__ void halve(uint32_t (&v)[N], bool upper, Op op) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        const uint32_t keep = upper ? v[H + i] : v[i], give = upper ? v[i] : v[H + i];
+        v[i] = op(keep, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, CTRL, 0xF, 0xF, false));
+    }
+}
+template <int N, class Op>
+__device__ __forceinline__ void row_extremes(uint32_t (&v)[N], int c, Op op) {
+    static_assert(N == 8 || N % 16 == 0);
+    halve<0x140, N / 2>(v, c & 8, op);                 // row_mirror, row_half_mirror, quad_perm [2,3,0,1] and [1,0,3,2]
+    halve<0x141, N / 4>(v, c & 4, op);
+    halve<0x4E, N / 8>(v, c & 2, op);
+    if constexpr (N == 8) v[0] = op(v[0], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[0], 0xB1, 0xF, 0xF, false));
+    else halve<0xB1, N / 16>(v, c & 1, op);
 }
 
 // The dims of a lane (c, m) of 16 positions of K: values e of piece j, and where they are. (The layout is that of the attention's
@@ -68,15 +89,114 @@ struct Part {
     static __device__ __forceinline__ int dim(int j, int m) { return (4 * j + m) * W; }
     __device__ __forceinline__ float at(int j, int e) const {
         if constexpr (CT == DT_F32) return __uint_as_float(w[j][e]);
-        else if constexpr (CT == DT_BF16) return __uint_as_float(e & 1 ? w[j][e / 2] & 0xffff0000u : w[j][e / 2] << 16);
-        else if constexpr (CT == DT_F16) return from_f16(e & 1 ? w[j][e / 2] >> 16 : w[j][e / 2] & 0xffffu);
         else if constexpr (CT == DT_Q8_0) return __fmul_rn((float)(int8_t)(w[j / 2][j % 2 * 2 + e / 4] >> (8 * (e % 4))), s[j]);
         else return __fmul_rn((float)((int)(w[j / T::G][j % T::G] << (28 - 8 * (e % 4) - 4 * (e / 4))) >> 28), s[j]);
     }
 };
 
+// A lane's extremes of its dims over the positions that it has seen, and its part of them over all sixteen lanes as bounds.
+template <int CT, int HD>
+struct Extremes {                          // fp32, Q8_0, Q4_0: as fp32
+    using P = Part<CT, HD>;
+    static constexpr int N = P::N * P::W, EACH = N / 16;
+    uint32_t lo[N], hi[N];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            lo[i] = __float_as_uint(INFINITY);
+            hi[i] = __float_as_uint(-INFINITY);
+        }
+    }
+    __device__ __forceinline__ void add(const P &x) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float v = x.at(i / P::W, i % P::W);
+            lo[i] = __float_as_uint(low_of(__uint_as_float(lo[i]), v));
+            hi[i] = __float_as_uint(high_of(__uint_as_float(hi[i]), v));
+        }
+    }
+    // out: the low ones of the wave's dims; the high ones are HD further on
+    __device__ __forceinline__ void store(uint16_t *out, int c, int m) {
+        row_extremes(lo, c, [](uint32_t a, uint32_t b) { return __float_as_uint(low_of(__uint_as_float(a), __uint_as_float(b))); });
+        row_extremes(hi, c, [](uint32_t a, uint32_t b) { return __float_as_uint(high_of(__uint_as_float(a), __uint_as_float(b))); });
+        uint16_t *at = out + P::dim(c * EACH / P::W, m) + c * EACH % P::W;
+        uint32_t a[EACH], z[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            a[e] = outward(__uint_as_float(lo[e]), false);
+            z[e] = outward(__uint_as_float(hi[e]), true);
+        }
+        if constexpr (EACH == 2) {
+            *reinterpret_cast<uint32_t *>(at) = a[0] | a[1] << 16;
+            *reinterpret_cast<uint32_t *>(at + HD) = z[0] | z[1] << 16;
+        } else {
+            *at = (uint16_t)a[0];
+            at[HD] = (uint16_t)z[0];
+        }
+    }
+};
+// 16-bit floats, two at a time as whole numbers: with sign and magnitude, the highest is the largest signed one or, where none is
+// positive, the smallest unsigned one; the lowest the largest unsigned one if it is negative, or else the smallest. NaN have
+// magnitudes above infinity's.
+template <int CT, int HD>
+struct Extremes16 {
+    using P = Part<CT, HD>;
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    static constexpr int N = P::N * 4;     // words
+    static constexpr uint32_t kInf = CT == DT_F16 ? 0x7c00u : 0x7f80u, kNan = CT == DT_F16 ? 0x7e00u : 0x7fc0u;
+    uint32_t top[N], least[N], most[N];    // largest signed, smallest and largest unsigned
+
+    static __device__ __forceinline__ uint32_t signed_max(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+    }
+    static __device__ __forceinline__ uint32_t unsigned_min(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+    static __device__ __forceinline__ uint32_t unsigned_max(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            top[i] = 0x80008000u;
+            least[i] = 0xffffffffu;
+            most[i] = 0;
+        }
+    }
+    __device__ __forceinline__ void add(const P &x) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t w = x.w[i / 4][i % 4];
+            top[i] = signed_max(top[i], w);
+            least[i] = unsigned_min(least[i], w);
+            most[i] = unsigned_max(most[i], w);
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t *out, int c, int m) {
+        row_extremes(top, c, signed_max);
+        row_extremes(least, c, unsigned_min);
+        row_extremes(most, c, unsigned_max);
+        uint32_t low = 0, high = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t t = top[0] >> (16 * e) & 0xffffu, l = least[0] >> (16 * e) & 0xffffu, u = most[0] >> (16 * e) & 0xffffu;
+            const bool nan = (t < 0x8000u && t > kInf) || u > (0x8000u | kInf);
+            low |= (nan ? kNan : u >= 0x8000u ? u : l) << (16 * e);
+            high |= (nan ? kNan : t < 0x8000u ? t : l) << (16 * e);
+        }
+        const int i = N == 8 ? c >> 1 : c;             // the lane's word
+        uint16_t *at = out + P::dim(i / 4, m) + i % 4 * 2;
+        if (N == 16 || !(c & 1)) *reinterpret_cast<uint32_t *>(at) = low;
+        if (N == 16 || c & 1) *reinterpret_cast<uint32_t *>(at + HD) = high;
+    }
+};
+
 // A wave per page and K/V head (two for 256 dims): lane (c, m) has position c of every tile and a quarter of the dims. The
-// bytes of K bound it. grid (pages / 4, heads x parts, rows).
+// bytes of K bound it: three documents of up to 131072 positions, 8 heads of 128 dims, bf16, pages of 32 (635 MB): 131 us, 4.8 TB/s
+// (with the extremes of 16-bit values as fp32, and of all lanes alike: 151; with waves that go on to further pages: 136). One
+// position of 16 sequences: 5.2 us. grid (pages / 4, heads x parts, rows).
 template <int CT, int HD>
 __global__ __launch_bounds__(kThreads) void paged_bounds_kernel(BoundsArgs g) {
     using P = Part<CT, HD>;
@@ -92,59 +212,21 @@ __global__ __launch_bounds__(kThreads) void paged_bounds_kernel(BoundsArgs g) {
     if (page < 0 || page >= g.c.pages) return;
     const int here = min(n - i * ps, ps);                      // positions written
     const uint8_t *tile = g.c.k + ((size_t)page * g.c.nkv + hk) * g.c.tile_bytes;
-    float lo[P::N][P::W], hi[P::N][P::W];
-#pragma unroll
-    for (int j = 0; j < P::N; ++j)
-#pragma unroll
-        for (int e = 0; e < P::W; ++e) {
-            lo[j][e] = INFINITY;
-            hi[j][e] = -INFINITY;
-        }
-    P k;
-    k.load(tile, ps, 0, part, c, m);
+    typename std::conditional<CT == DT_BF16 || CT == DT_F16, Extremes16<CT, HD>, Extremes<CT, HD>>::type all;
+    all.clear();
+    P k[2];                                                    // two tiles under way
+    k[0].load(tile, ps, 0, part, c, m);
+    if (16 < here) k[1].load(tile, ps, 16, part, c, m);
 #pragma unroll 1
-    for (int t = 0; t < here; t += 16) {
-        const P x = k;
-        if (t + 16 < here) k.load(tile, ps, t + 16, part, c, m);
-        if (t + 16 <= here) {
+    for (int t = 0; t < here; t += 32) {
 #pragma unroll
-            for (int j = 0; j < P::N; ++j)
-#pragma unroll
-                for (int e = 0; e < P::W; ++e) {
-                    const float v = x.at(j, e);
-                    lo[j][e] = low_of(lo[j][e], v);
-                    hi[j][e] = high_of(hi[j][e], v);
-                }
-        } else if (t + c < here) {                             // positions behind the last one do not count
-#pragma unroll
-            for (int j = 0; j < P::N; ++j)
-#pragma unroll
-                for (int e = 0; e < P::W; ++e) {
-                    const float v = x.at(j, e);
-                    lo[j][e] = low_of(lo[j][e], v);
-                    hi[j][e] = high_of(hi[j][e], v);
-                }
+        for (int h = 0; h < 2; ++h) {
+            const int at = t + 16 * h;
+            if (at + c < here) all.add(k[h]);                  // positions behind the last one do not count
+            if (at + 32 < here) k[h].load(tile, ps, at + 32, part, c, m);
         }
     }
-    uint16_t *out = g.bounds + ((size_t)page * g.c.nkv + hk) * 2 * HD + (c & 1) * HD + part * (HD / P::PARTS);
-#pragma unroll
-    for (int j = 0; j < P::N; ++j) {
-        uint32_t w[P::W];
-#pragma unroll
-        for (int e = 0; e < P::W; ++e) {
-            float a = lo[j][e], z = hi[j][e];
-            // (the steps of row16_max)
-            a = low_of(a, lanes::dpp_mov<0xB1>(a)), z = high_of(z, lanes::dpp_mov<0xB1>(z));
-            a = low_of(a, lanes::dpp_mov<0x4E>(a)), z = high_of(z, lanes::dpp_mov<0x4E>(z));
-            a = low_of(a, lanes::dpp_mov<0x141>(a)), z = high_of(z, lanes::dpp_mov<0x141>(z));
-            a = low_of(a, lanes::dpp_mov<0x140>(a)), z = high_of(z, lanes::dpp_mov<0x140>(z));
-            w[e] = c & 1 ? outward<CT>(z, true) : outward<CT>(a, false);
-        }
-        if (c >> 1 == j % 8) {                                 // lanes 2j and 2j + 1 have the low and the high ones to write
-            if constexpr (P::W == 4) *reinterpret_cast<pu2 *>(out + P::dim(j, m)) = pu2{w[0] | w[1] << 16, w[2] | w[3] << 16};
-            else *reinterpret_cast<pu4 *>(out + P::dim(j, m)) = pu4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
-        }
-    }
+    all.store(g.bounds + ((size_t)page * g.c.nkv + hk) * 2 * HD + part * (HD / P::PARTS), c, m);
 }
 
 // ---- the choice ----

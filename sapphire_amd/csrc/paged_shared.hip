@@ -15,7 +15,7 @@ namespace {
 // Pieces: a piece more shortens every workgroup's walk, and adds a slot of each column that is written and joined. As many as
 // fill the chip (two waves per SIMD; of few columns, whose waves have no barriers, one: 8 rows of 32 heads over 8, bf16, behind
 // 16384 positions 28 us, with two 35; behind 131072 109 and 115), of eight steps of a wide workgroup (32 rows behind 4096
-// positions 33 us, of two 40) or one of each wave of few columns; but half of the compute
+// positions 33 us, of four 40) or one of each wave of few columns; but half of the compute
 // units get a workgroup in any case (six drafted rows of 4 heads behind 1018 positions, fp32: 19.6 us in 32 pieces, 21.8 in 16).
 constexpr int kSharedFill = 2048, kFewFill = 1024;         // waves of the shared positions at once
 constexpr int kSharedUnit = 32, kFewUnit = 128, kWideSteps = 8;
