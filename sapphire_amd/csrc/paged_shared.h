@@ -518,6 +518,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(AttnArgs g, S
 // loads and converts a part of them, two steps ahead, and writes it to LDS as the products' operands; a step's operands are
 // read by all while the next one's are written. Four jobs of a step are V's: the DPL dims (of 256: half of them) of a lane at two
 // positions of a tile, a word of every dim's operand; the others copy or convert K, 16 positions of 32 dims each.
+//
+// A step of eight waves with two sets each, bf16, 128 dims: 3500 cycles of two waves per SIMD, of which the matrix cores are busy
+// for 1600. Each wave's are 600 of loads, their addresses and stores, 500 of scores, 400 of the maximum, 700 of weights (an exp2
+// takes 8, two terms of a pair 25), 800 of V's product. Measured and left out: 32x32x16 products, four sets in one wave per
+// SIMD, LDS reads three products ahead (spills: 233 us for 205).
 template <int CT, int HD, bool HALF, bool SHORT>
 struct Stage {
     using F = Form<CT, HALF, SHORT>;
@@ -543,7 +548,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArg
     // K jobs of a wave (where there are eight waves, of the four that have none of V); fp32: KiB of K, and of V
     constexpr int KJ = F::kF32 ? (G::KC < NW ? 1 : G::KC / NW) : G::KC / 4;
     // Where eight waves fill the compute unit, the upper four form a step's weights while the others multiply, and the other way
-    // round: they add V a step later, which needs three steps of V.
+    // round: they add V a step later, which needs three steps of V. (64 rows of 32 heads over 8, bf16, behind 16384 positions: 67 us
+    // for the call, 69.6 without; Q4_0, 32 rows: 63.4 and 66.)
     constexpr bool SPLIT = NW == 8;
     constexpr int VS = SPLIT ? 3 : 2;
     __shared__ __attribute__((aligned(16))) uint8_t klds[2][G::kKBytes], vlds[VS][G::kVBytes];
@@ -964,7 +970,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArg
 }
 
 // Columns of a workgroup. Up to 32: as few sets as there are, and the waves take different positions. More: all waves side by
-// side, with K and V through LDS.
+// side, with K and V through LDS. (48 columns behind 16384 positions, Q4_0: 46 us, as few ones in two tiles 56; bf16 35 and 38. 32
+// columns, bf16: 28 us, as many ones 32.)
 constexpr int kFewColumns = 32;
 struct Columns {
     int cs, nw;                            // sets of a wave, waves side by side (0: one, of a workgroup that splits positions)
