@@ -14,7 +14,10 @@
  * A decode step of a batch: sapphire_rope_rows_dev (sapphire_hip.h) on the q and k heads of the
  * fused projection, sapphire_paged_write_dev of k and v at the sequences' next positions,
  * sapphire_paged_attention_dev; for beam search sapphire_beam_select_dev on the logits and
- * sapphire_paged_reorder_dev.
+ * sapphire_paged_reorder_dev. Where rows share their first positions, or are the drafted tokens that
+ * sapphire_verify_dev decides about, sapphire_paged_shared_attention_dev reads the shared ones once;
+ * of long sequences sapphire_paged_select_dev chooses pages by the bounds that
+ * sapphire_paged_bounds_dev keeps, for sapphire_paged_pages_attention_dev.
  */
 #ifndef SAPPHIRE_HIP_PAGED_H
 #define SAPPHIRE_HIP_PAGED_H

@@ -313,9 +313,9 @@ __device__ __forceinline__ u64 page_max(u64 k) {
 
 // Eight dims of a page per lane, HD / 8 lanes per page; every page's score, as a key, by four query heads at a time. Pages that
 // are taken anyway have the largest key, ones that do not exist 0. Four documents of up to 131072 positions, 32 heads over 8 of
-// 128 dims, pages of 32 (41 MB of bounds): 18.7 us, of which 8 are vector instructions (16 fused products in 64 bits per
-// eight dims and head, and a seventh of that for the sums over lanes), behind the chain page -> bounds of each of the four
-// steps. grid (pages, K/V heads, sequences).
+// 128 dims, pages of 32 (41 MB of bounds): 18.7 us, of which 8 are vector instructions (16 fused products in 64 bits
+// per eight dims and head), the rest the chain lengths -> page -> bounds and the sums over lanes of the steps in turn. grid
+// (pages, K/V heads, sequences).
 template <int HD, bool F16>
 __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
     constexpr int LP = HD / 8, PW = kWave / LP, STEP = kWaves * PW;        // lanes of a page, pages of a wave and of a workgroup
