@@ -18,7 +18,7 @@ SOURCES = ["runtime.cpp", "tensor.cpp", "dispatch.cpp", "decoder.cpp", "gemv.hip
            "ops.hip", "sample.hip", "decode.hip",
            "decode_persist.hip", "quantize.hip", "gemm_bf16.hip", "noalloc.cpp", "transformer.cpp", "paged.cpp",
            "paged_rows.hip", "paged_attention.hip", "rope_rows.hip", "beam.hip", "verify.hip", "page_choice.hip",
-           "paged_pages.hip", "paged_shared.hip", "paged_shared_quant.hip"]
+           "paged_pages.hip", "paged_shared.hip", "paged_shared_quant.hip", "paged_shared_join.hip"]
 ARCH = os.environ.get("SAPPHIRE_OFFLOAD_ARCH", "gfx950")
 
 COMMON = [

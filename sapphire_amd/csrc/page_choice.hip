@@ -379,11 +379,44 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
     }
 }
 
+constexpr int kPick = 1024, kPickWaves = kPick / kWave, kHold = 8, kBins = 1024, kFew = 64;
+constexpr int kRanked = 256;               // pages that are ranked against each other at once
+
+// The choice of few pages, as below: how many keys are ahead of each, a quarter of them counted by each of four threads.
+__device__ __forceinline__ void rank_pages(const u64 *keys, int np, int k, int *out) {
+    constexpr int PARTS = kPick / kRanked, EACH = kRanked / PARTS;
+    __shared__ __attribute__((aligned(16))) u64 all[kRanked];
+    __shared__ int ahead[PARTS][kRanked], taken[kRanked / kWave];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), page = tid % kRanked, part = tid / kRanked;
+    if (tid < kRanked) all[tid] = tid < np ? keys[tid] : 0;
+    __syncthreads();
+    const u64 mine = all[page];
+    int count = 0;
+#pragma unroll 8
+    for (int j = part * EACH; j < (part + 1) * EACH; ++j) count += all[j] > mine || (all[j] == mine && j < page);
+    ahead[part][page] = count;
+    __syncthreads();
+    int rank = 0;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) rank += ahead[p][page];
+    const bool on = mine != 0 && rank < k;
+    const u64 mask = __ballot(on);
+    if (tid < kRanked && lane == 0) taken[tid / kWave] = __popcll(mask);
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kRanked / kWave; ++w) {
+        before += w < page / kWave ? taken[w] : 0;
+        total += taken[w];
+    }
+    if (tid < kRanked && on) out[before + __popcll(mask & ((1ull << lane) - 1))] = page;
+    for (int i = total + tid; i < k; i += kPick) out[i] = -1;
+}
+
 // The k largest keys of a sequence's K/V head, equal ones from the first page on, in order of the pages. One workgroup; keys of up
 // to 8192 pages stay in its registers. By ten bits at a time from the highest one in which keys differ, until the keys that
 // decide are few enough to be ranked against each other. 128 of 4096 pages for 32 lists: 10.7 us, a chain of steps between
 // barriers. grid (K/V heads, sequences).
-constexpr int kPick = 1024, kPickWaves = kPick / kWave, kHold = 8, kBins = 1024, kFew = 64;
 __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
     __shared__ int bins[kBins], wave_sums[kPickWaves];
     __shared__ uint32_t counts[kHold * kPickWaves], sums[kHold * kPickWaves / kWave];
@@ -393,6 +426,10 @@ __global__ __launch_bounds__(kPick) void paged_select_kernel(SelectArgs g) {
     const int hk = blockIdx.x, b = blockIdx.y, np = pages_of(g, b);
     int *out = g.selected + ((size_t)b * g.c.nkv + hk) * g.k;
     const u64 *keys = g.keys + ((size_t)b * g.c.nkv + hk) * g.max_pages;
+    if (np <= kRanked) {
+        rank_pages(keys, np, g.k, out);
+        return;
+    }
     const int blocks = (np + kHold * kPick - 1) / (kHold * kPick);
     u64 key[kHold];
     auto load = [&](int blk) {

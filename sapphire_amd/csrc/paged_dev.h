@@ -179,6 +179,81 @@ __device__ __forceinline__ void store8(int dtype, bool wide, uint8_t *base, int6
     }
 }
 
+// Elements d .. d + 7 of position p of a tile of K or V.
+template <int CT, int HD, bool V>
+__device__ __forceinline__ void load_codes(const uint8_t *tile, uint32_t ps, uint32_t p, uint32_t d, float (&x)[8]) {
+    using T = Tile<CT, HD>;
+    if constexpr (CT == DT_F32) {
+        const uint8_t *a = V ? tile + p * T::ROW + d * 4 : tile + T::k_code(p, d);
+        const uint8_t *b = V ? a + 16 : tile + T::k_code(p, d + 4);
+        const pf4 u = *reinterpret_cast<const pf4 *>(a), w = *reinterpret_cast<const pf4 *>(b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = u[i];
+            x[4 + i] = w[i];
+        }
+    } else if constexpr (!T::kQuant) {
+        pu4 w;
+        if constexpr (V && HD == 64) {
+            const pu2 a = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 4));
+            const pu2 b = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 4 + 1));
+            w = pu4{a.x, a.y, b.x, b.y};
+        } else {
+            w = *reinterpret_cast<const pu4 *>(tile + (V ? p * T::ROW + d * 2 : T::k_code(p, d)));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = from_16(CT, w[i] & 0xffffu);
+            x[2 * i + 1] = from_16(CT, w[i] >> 16);
+        }
+    } else {
+        const float scale = *reinterpret_cast<const float *>(tile + (V ? T::v_scale(ps, p, d / 32) : T::k_scale(ps, p, d / 32)));
+        if constexpr (CT == DT_Q8_0) {
+            uint32_t lo, hi;
+            if constexpr (V && HD == 64) {
+                lo = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 4));
+                hi = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 4 + 1));
+            } else {
+                const pu2 w = *reinterpret_cast<const pu2 *>(tile + (V ? T::v_run(p, d / T::RUN) + d % T::RUN : T::k_code(p, d)));
+                lo = w.x;
+                hi = w.y;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = __fmul_rn((float)(int8_t)(lo >> (8 * i)), scale);
+                x[4 + i] = __fmul_rn((float)(int8_t)(hi >> (8 * i)), scale);
+            }
+        } else {
+            uint32_t lo, hi;                           // codes 0..3 and 4..7, one nibble per byte
+            if constexpr (!V) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + T::k_code(p, d)) ^ 0x88888888u;
+                lo = w & 0x0f0f0f0fu;
+                hi = w >> 4 & 0x0f0f0f0fu;
+            } else if constexpr (HD == 256) {
+                const pu2 w = *reinterpret_cast<const pu2 *>(tile + T::v_run(p, d / 16));
+                const uint32_t sh = d & 8 ? 4 : 0;
+                lo = w.x >> sh & 0x0f0f0f0fu;
+                hi = w.y >> sh & 0x0f0f0f0fu;
+            } else if constexpr (HD == 128) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + T::v_run(p, d / 8));
+                lo = w & 0x0f0f0f0fu;
+                hi = w >> 4 & 0x0f0f0f0fu;
+            } else {
+                const uint32_t a = *reinterpret_cast<const uint16_t *>(tile + T::v_run(p, d / 4));
+                const uint32_t b = *reinterpret_cast<const uint16_t *>(tile + T::v_run(p, d / 4 + 1));
+                lo = (a & 0x0f0fu) | (a >> 4 & 0x0f0fu) << 16;
+                hi = (b & 0x0f0fu) | (b >> 4 & 0x0f0fu) << 16;
+            }
+            asm("" : "+v"(lo), "+v"(hi));              // (the compiler would rather extract nibbles one by one)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = __fmul_rn(__fsub_rn((float)(lo >> (8 * i) & 255u), 8.0f), scale);
+                x[4 + i] = __fmul_rn(__fsub_rn((float)(hi >> (8 * i) & 255u), 8.0f), scale);
+            }
+        }
+    }
+}
+
 inline int elem_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }
 // Data and strides in whole 16-byte pieces.
 inline bool rows_wide(const Rows &r) {

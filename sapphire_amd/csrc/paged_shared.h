@@ -1008,5 +1008,6 @@ void launch_shared_form(const AttnArgs &g, const SharedPlan &sp, hipStream_t s) 
 }  // namespace
 
 bool launch_shared_quant(const void *args, const void *plan, hipStream_t s);
+bool launch_shared_join(const void *args, hipStream_t s);
 
 }  // namespace sapphire

@@ -32,6 +32,7 @@ constexpr int kUnits = 256;               // compute units
 // many workgroups are joined (bf16, 64 rows of 32 heads over 8: behind 16384 positions 69 us with two sets, 62 with one; behind
 // 65536 141 and 162).
 constexpr int kTwoSets = 768;
+constexpr int kOwnJoined = 32;            // positions of a row behind the shared ones that the join takes along
 constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;
@@ -103,6 +104,10 @@ int launch_paged_shared_attention(const PagedAttn &a, hipStream_t s) {
 #define SPH_FORM_HD(HD) SPH_FORM(DT_F32, HD, false) SPH_FORM(DT_BF16, HD, false) SPH_FORM(DT_BF16, HD, true) SPH_FORM(DT_F16, HD, false) SPH_FORM(DT_F16, HD, true)
         SPH_FORM_HD(64) SPH_FORM_HD(128) SPH_FORM_HD(256)
         if (!hip_ok(hipGetLastError(), "shared attention launch")) return -1;
+    }
+    if (a.max_own > 0 && a.max_own <= kOwnJoined) {
+        g.pieces = b.shared.pieces;
+        return launch_shared_join(&g, s) ? 0 : -1;
     }
     if (!launch_pieces<BEHIND>(g, b.own, half, s)) return -1;
     g.pieces = total;

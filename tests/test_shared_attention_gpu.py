@@ -105,8 +105,9 @@ def test_shared(hip, cache, io, hd, nkv, heads, ps):
     common = [ps * 5, ps * 12, ps]
     lens = [common[0] + n for n in (1, 17, 0, 300, 5)] + [0, common[1] + 2, common[1] + 33, 0, common[1] + 1] + [common[2] + 40, common[2] + 1]
     c = Case(rng, cache, io, hd, nkv, heads, ps, 5, common, lens)
-    c.run(common, 300)
-    c.check()
+    for own in (300, 20):                              # the attention's kernels take what is not shared, or the join does
+        c.run(common, own)
+        c.check()
 
 
 SOME = [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F32), (Q8_0, F32), (Q4_0, BF16)]
@@ -119,8 +120,9 @@ def test_columns(hip, cache, io, rows, heads):
     rng = np.random.default_rng(rows * heads)
     for hd, n in ((64, 700), (128, 40), (256, 130)):
         c = Case(rng, cache, io, hd, 1, heads, 32, rows, [n // 32 * 32], [n // 32 * 32 + 1 + r % 7 for r in range(rows)])
-        c.run([n // 32 * 32], 7)
-        c.check()
+        for own in (0, 7):
+            c.run([n // 32 * 32], own)
+            c.check()
 
 
 @pytest.mark.parametrize("cache,io", IO, ids=IDS)
@@ -140,8 +142,9 @@ def test_drafted_tokens(hip, cache, io):
 def test_pages_that_do_not_exist(hip, cache):
     rng = np.random.default_rng(4)
     c = Case(rng, cache, F32, 64, 1, 4, 16, 4, [320, 64], [400, 321, 330, 350, 70, 65, 80, 0], broken=[(0, 0), (0, 7), (0, 8), (0, 19), (0, 20), (1, 0), (1, 1), (1, 2), (1, 3)])
-    c.run([320, 64], 80)
-    c.check()
+    for own in (80, 32):
+        c.run([320, 64], own)
+        c.check()
     c = Case(rng, cache, F32, 128, 1, 2, 16, 2, [64], [64, 64], broken=[(0, i) for i in range(4)])
     c.run([64], 1)
     c.check()
@@ -152,8 +155,9 @@ def test_cap_peaks_and_strides(hip, cache, io):
     rng = np.random.default_rng(5)
     for cap, peak, order, pad in ((30.0, 4.0, "thd", 0), (5.0, 2.0, "htd", 3), (0.0, 100.0, "thd", 192), (0.0, 0.0, "thd", 8)):
         c = Case(rng, cache, io, 128, 1, 4, 48, 8, [480], [481 + 9 * r for r in range(8)], order=order, pad=pad, peak=peak)
-        c.run([480], 64, cap)
-        c.check(cap)
+        for own in (64, 32):
+            c.run([480], own, cap)
+            c.check(cap)
 
 
 @pytest.mark.parametrize("cache,io", IO, ids=IDS)
@@ -169,8 +173,9 @@ def test_scales_and_sizes_of_q(hip, cache, io, rows):
         c.rq[3][...] = x
         c.rq[1].upload(c.rq[2])
         c.q, c.scale = ref.from_type(io, x), scale
-        c.run([144], 20)
-        c.check()
+        for own in (0, 20):
+            c.run([144], own)
+            c.check()
     c = Case(rng, cache, io, 128, 1, 4, 16, rows, [144], [145 + r for r in range(rows)], broken=[(0, 3)])
     c.scale = -0.2
     c.run([144], 20, 10.0)
@@ -191,8 +196,9 @@ def test_not_finite(hip, cache, io, rows):
     c.rq[3][1, 2, 7] = ref.to_type(io, np.full(1, np.nan, np.float32))[0]
     c.rq[1].upload(c.rq[2])
     c.q[1, 2] = 0.0
-    c.run([160], 30)
-    c.check(but=(1, 2))
+    for own in (40, 30):
+        c.run([160], own)
+        c.check(but=(1, 2))
     c.rq[3][1, 2, 7] = q
     c.rq[1].upload(c.rq[2])
     k, v = c.k[0][:160], c.v[0][:160].copy()
@@ -302,22 +308,22 @@ def test_in_place_streams_and_replays(hip):
     """out is q; another stream; a captured call replayed as rows and shared positions grow, in a workspace of the largest call."""
     from sapphire_amd.device import DeviceArray
     rng = np.random.default_rng(8)
-    for cache, io in ((BF16, BF16), (Q8_0, F32)):
+    for cache, io, own in ((BF16, BF16, 80), (Q8_0, F32, 80), (BF16, BF16, 30), (Q4_0, F32, 30)):
         c = Case(rng, cache, io, 64, 1, 8, 32, 4, [320, 320], [400] * 8)
-        c.run([320, 320], 80)
+        c.run([320, 320], own)
         want = c.got()[0]
-        c.run([320, 320], 80, out=c.rq[0])
+        c.run([320, 320], own, out=c.rq[0])
         sync()
         got = ref.from_type(io, c.rq[1].numpy()[:want.size]).reshape(want.shape)
         np.testing.assert_array_equal(got, want)
         c = Case(rng, cache, io, 64, 1, 8, 32, 4, [320, 320], [400] * 8)
         c.ws = DeviceArray(c.c.c.shared_attention_workspace_bytes(50, 16, 100000))
         s = hip.sapphire_stream_create()
-        c.run([320, 320], 80, stream=s)
+        c.run([320, 320], own, stream=s)
         c.check()
         hip.sapphire_stream_destroy(s)
         on = dev(np.array([320, 320], np.int32))
-        g = Graph(lambda stream: c.run(on, 80, stream=stream))
+        g = Graph(lambda stream: c.run(on, own, stream=stream))
         k, v = c.k, c.v
         for lens, shared in (([400] * 8, [320, 320]), ([0] * 4 + [330, 0, 321, 399], [5, 319]), ([7, 400, 330, 1, 0, 0, 0, 0], [320, 320]), ([400] * 8, [320, 0])):
             c.lens = lens
@@ -433,3 +439,27 @@ def test_speculative_decoding(hip, cache, io):
     for r in range(requests):
         n = min(len(want[r]), len(got[r]))
         assert n >= 20 and got[r][:n] == want[r][:n]
+
+
+@pytest.mark.parametrize("cache,io", IO, ids=IDS)
+def test_positions_that_the_join_takes(hip, cache, io):
+    """None to hundreds of positions behind the shared ones, whatever max_own says of them; pieces few and many; a NaN and an
+    infinity in their V: the dim (quantized: its block) of the rows that see them."""
+    rng = np.random.default_rng(18)
+    for hd, n, own in ((64, 64, (0, 1, 15, 16, 63, 64, 65, 300)), (128, 1024, (1, 7, 31, 32, 33, 500)), (256, 4096, (0, 1, 8, 33))):
+        c = Case(rng, cache, io, hd, 2, 6, 16, len(own), [n], [n + i for i in own])
+        c.run([n], 32)
+        c.check()
+    r, hd = 2, 128
+    c = Case(rng, cache, io, hd, 1, 2, 16, 3, [64], [70, 66, 75])
+    k, v = c.k[r], c.v[r].copy()
+    v[68, 0, 5], v[70, 0, 40] = np.nan, np.inf
+    with np.errstate(all="ignore"):
+        c.c.fill(0, c.table, r, k, v)
+    c.c.upload()
+    c.run([64], 16)
+    got = c.got()[0]
+    odd = np.zeros((3, 2, hd), bool)
+    for dim in (5, 40):
+        odd[r, :, slice(dim // 32 * 32, dim // 32 * 32 + 32) if cache in (Q8_0, Q4_0) else dim] = True
+    assert not np.isfinite(got[odd]).any() and np.isfinite(got[~odd]).all()
