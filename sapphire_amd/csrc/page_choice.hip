@@ -380,7 +380,8 @@ __global__ __launch_bounds__(kThreads) void paged_scores_kernel(SelectArgs g) {
 }
 
 constexpr int kPick = 1024, kPickWaves = kPick / kWave, kHold = 8, kBins = 1024, kFew = 64;
-constexpr int kRanked = 256;               // pages that are ranked against each other at once
+// Pages that are ranked against each other at once: 250 pages of one list 10.4 us with their scores, by bits 14.6; of 512, 18.
+constexpr int kRanked = 256;
 
 // The choice of few pages, as below: how many keys are ahead of each, a quarter of them counted by each of four threads.
 __device__ __forceinline__ void rank_pages(const u64 *keys, int np, int k, int *out) {

@@ -3,8 +3,8 @@
 //
 // The query heads of a K/V head of all rows of a group are columns of one product: K and V of the shared positions are read
 // once for all of them, and what would be one row's share of memory becomes work for the matrix cores. The positions are cut
-// into pieces; each row's own positions, behind the shared ones, are the attention's kernels' (paged_attention.h); a last launch
-// joins the pieces of both. Only positions that all rows of a group have count as shared, in whole tiles, so that no score is
+// into pieces; each row's own positions, behind the shared ones, are the attention's kernels' (paged_attention.h), or, where they
+// are few, the last launch's (paged_shared_join.hip); that joins the pieces of both. Only positions that all rows of a group have count as shared, in whole tiles, so that no score is
 // masked for one row and not for another.
 //
 // Few columns are bound by memory and, where positions are few, by the chain page -> K -> scores -> sum: 8 rows of 32 heads over 8
@@ -24,7 +24,7 @@ namespace {
 // fill the chip (two waves per SIMD; of few columns, whose waves have no barriers, one: 8 rows of 32 heads over 8, bf16, behind
 // 16384 positions 28 us, with two 35; behind 131072 109 and 115), of eight steps of a wide workgroup (32 rows behind 4096
 // positions 33 us, of four 40) or one of each wave of few columns; but half of the compute
-// units get a workgroup in any case (six drafted rows of 4 heads behind 1018 positions, fp32: 19.6 us in 32 pieces, 21.8 in 16).
+// units get a workgroup in any case (six drafted rows of 4 heads behind 1018 positions, fp32: 19.6 us in 32 pieces, 21.8 in 16, both with three launches).
 constexpr int kSharedFill = 2048, kFewFill = 1024;         // waves of the shared positions at once
 constexpr int kSharedUnit = 32, kFewUnit = 128, kWideSteps = 8;
 constexpr int kUnits = 256;               // compute units
@@ -32,7 +32,7 @@ constexpr int kUnits = 256;               // compute units
 // many workgroups are joined (bf16, 64 rows of 32 heads over 8: behind 16384 positions 69 us with two sets, 62 with one; behind
 // 65536 141 and 162).
 constexpr int kTwoSets = 768;
-constexpr int kOwnJoined = 32;            // positions of a row behind the shared ones that the join takes along
+constexpr int kOwnJoined = 32;            // positions of a row behind the shared ones that the join takes along (its figures are there)
 constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;

@@ -187,6 +187,25 @@ def test_many_pages(hip, n):
         s.check(k, 0, 1)
 
 
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 255, 256, 257])
+def test_few_pages(hip, n):
+    """Around the number of pages that are ranked at once; some alike, some that do not exist."""
+    rng = np.random.default_rng(n)
+    s = Select(rng, BF16, F32, 2, 6, 128, 16, [16 * n, 16 * n - 15, 5], extra=0)
+    for k in sorted({1, 2, 40, n // 3 + 1, n, n + 3}):
+        s.check(k, 0, 0)
+        s.check(k, 0, 1)
+        if k > 3:
+            s.check(k, 2, 2)
+    s.bits[...] = s.bits[rng.integers(0, min(4, s.pages), s.pages)]
+    s.on.upload(s.bits)
+    s.table[0, rng.integers(0, n, n // 5)] = -1
+    s.dt.upload(s.table)
+    for k in sorted({1, 3, n // 2 + 1, n}):
+        s.check(k, 0, 0)
+        s.check(k, 1, 0)
+
+
 def test_ties(hip):
     """Pages alike: the first ones. All alike, groups of alike ones, and many that differ in the last bits only."""
     rng = np.random.default_rng(3)
