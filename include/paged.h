@@ -127,8 +127,8 @@ int sapphire_paged_attention_dev(const sapphire_paged_cache_t *cache, int layer,
  * little. Over the shared positions a NaN or an infinity in V makes its dim (over a quantized cache its block's dims) NaN or
  * infinite; one in q or K, other than over a cache of the rows' own type, makes its heads' outputs NaN. What is said
  * there of positions behind the last one and of pages that do not exist holds here too. max_own: about how many
- * positions a row has behind the shared ones at most; it is for speed only, any value gives the same positions. workspace:
- * sapphire_paged_shared_attention_workspace_bytes() bytes, 16-byte aligned, which are enough for calls of fewer and shorter rows
+ * positions a row has behind the shared ones at most (0: not known); it is for speed only, any value gives the same positions.
+ * workspace: sapphire_paged_shared_attention_workspace_bytes() bytes, 16-byte aligned, which are enough for calls of fewer and shorter rows
  * too, whatever their groups; calls that share one must be ordered on one stream. */
 typedef struct {
     const int *shared;

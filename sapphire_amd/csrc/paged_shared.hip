@@ -4,8 +4,8 @@
 // The query heads of a K/V head of all rows of a group are columns of one product: K and V of the shared positions are read
 // once for all of them, and what would be one row's share of memory becomes work for the matrix cores. The positions are cut
 // into pieces; each row's own positions, behind the shared ones, are the attention's kernels' (paged_attention.h), or, where they
-// are few, the last launch's (paged_shared_join.hip); that joins the pieces of both. Only positions that all rows of a group have count as shared, in whole tiles, so that no score is
-// masked for one row and not for another.
+// are few, the last launch's (paged_shared_join.hip); that joins the pieces of both. Only positions that all rows of a group
+// have count as shared, in whole tiles, so that no score is masked for one row and not for another.
 //
 // Few columns are bound by memory and, where positions are few, by the chain page -> K -> scores -> sum: 8 rows of 32 heads over 8
 // of 128 dims behind 131072 positions, bf16 (537 MB): 110 us for the call. Many are bound by the issue of vector and matrix
@@ -32,7 +32,7 @@ constexpr int kUnits = 256;               // compute units
 // many workgroups are joined (bf16, 64 rows of 32 heads over 8: behind 16384 positions 69 us with two sets, 62 with one; behind
 // 65536 141 and 162).
 constexpr int kTwoSets = 768;
-constexpr int kOwnJoined = 32;            // positions of a row behind the shared ones that the join takes along (its figures are there)
+constexpr int kOwnJoined = 32;            // positions of a row behind the shared ones that the join takes along
 constexpr int kMostCols = 256;             // columns of a workgroup at most
 struct Both {
     Plan own;
@@ -49,7 +49,8 @@ SharedPlan shared_plan(int dtype, int sets, int nkv, int hd, int groups, int col
     const int64_t wgs = (int64_t)groups * nkv * p.col_tiles;
     const int64_t full = (few ? kFewFill : kSharedFill) / (wgs * (k.nw == 8 ? 8 : 4)), one = kUnits / wgs;
     const int unit = few ? kFewUnit : kWideSteps * (dtype == DT_F32 || hd == 256 ? 16 : 32);
-    int64_t pieces = std::max(std::min<int64_t>(one / 2, (max_length + kSharedUnit - 1) / kSharedUnit), std::min<int64_t>(full, max_length / unit));
+    int64_t pieces = std::max(std::min<int64_t>(one / 2, (max_length + kSharedUnit - 1) / kSharedUnit),
+                              std::min<int64_t>(full, max_length / unit));
     // (few compute units with two workgroups would keep the others waiting: 12 rows over 4 K/V heads, fp32, behind 8192 positions
     // 31 us in 64 pieces, 37.5 in 65)
     if (pieces > one && 2 * pieces < 3 * one) pieces = one;
