@@ -38,13 +38,15 @@ struct Form {
     static __device__ __forceinline__ constexpr bool meets(int v, int p) { return v + p < (TV > TP ? TV : TP); }
 };
 
-// Two values' term of 16 bits in one word, and what it leaves of them.
-template <int T>
+// Two values' term of 16 bits in one word, and what it leaves of them. Rounded to nearest: of a number in [1, 2) two bf16 terms
+// leave 2^-17 (cut off: 2^-15, always of the number's sign), at as many instructions. CUT: for three terms that hold
+// all bits either way, of numbers up to fp32's largest, which rounded up would be an infinity.
+template <int T, bool CUT = false>
 __device__ __forceinline__ uint32_t take_term(float &a, float &b) {
-    if constexpr (T == DT_BF16) {          // cut off: exact, and cheaper than rounding
-        const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-        a = __fsub_rn(a, __uint_as_float(__float_as_uint(a) & 0xffff0000u));
-        b = __fsub_rn(b, __uint_as_float(__float_as_uint(b) & 0xffff0000u));
+    if constexpr (T == DT_BF16) {
+        const uint32_t w = CUT ? __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u) : pack_16(DT_BF16, a, b);
+        a = __fsub_rn(a, __uint_as_float(CUT ? __float_as_uint(a) & 0xffff0000u : w << 16));
+        b = __fsub_rn(b, __uint_as_float((CUT ? __float_as_uint(b) : w) & 0xffff0000u));
         return w;
     } else {
         const uint32_t w = pack_16(DT_F16, a, b);
@@ -131,7 +133,7 @@ struct SharedQuery {
                         w[0][i][e / 2] = pack_16(F::QT, y0, y1);           // (they were of that type: nothing is rounded)
                     } else {
 #pragma unroll
-                        for (int t = 0; t < F::TQ; ++t) w[t][i][e / 2] = take_term<F::QT>(y0, y1);
+                        for (int t = 0; t < F::TQ; ++t) w[t][i][e / 2] = take_term<F::QT, true>(y0, y1);
                     }
                 }
             }
