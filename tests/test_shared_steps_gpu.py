@@ -186,3 +186,16 @@ def test_groups_of_more_rows_than_lanes(hip, cache, io):
         c.dn.upload(c.lens.astype(np.int32).ravel())
         for own in (150, 30):
             c.check((0, 1), own=own)
+
+
+@pytest.mark.parametrize("cache,io", [(F32, F32), (BF16, BF16), (Q4_0, F32)], ids=["f32", "bf16", "q4_0"])
+def test_own_positions_of_unknown_number(hip, cache, io):
+    """max_own = 0, where rows have thousands of positions of their own: cut as with the largest number, to the same bits."""
+    c = Steps(np.random.default_rng(cache + 60), cache, io, 128, 1, 4, 3, [4], 4000)
+    c.lens[0] = 4000, 3000, 64
+    c.seen[...] = np.arange(c.n) < c.lens.reshape(-1, 1)
+    c.dn.upload(c.lens.astype(np.int32).ravel())
+    known = c.run(own=4000)
+    for a, b in zip(known, c.run(own=0)):
+        np.testing.assert_array_equal(a, b)
+    c.check((0,), own=0)
