@@ -979,8 +979,12 @@ struct Columns {
     int cs, nw;                            // sets of a wave, waves side by side (0: one, of a workgroup that splits positions)
     int columns() const { return 16 * cs * std::max(nw, 1); }
 };
-// Sets of a wave at most: two where they fit the registers of two waves (Q4_0's do not, for one: 32 rows of 32 bf16 heads over
-// 8 behind 65536 positions 122 us with one, 144 with two).
+// Sets of a wave at most: two where they are faster over many positions. (32 rows of 32 heads over 8 of 128 dims behind 65536
+// positions, bf16 rows over Q4_0: 122 us with one, 144 with two.) They fit the registers of two waves but for fp32 rows over fp16,
+// of which eight waves spill 33 registers and four 1, and are still ahead from 48 rows on: 128 rows behind 65536 positions 299 us,
+// with one set 323, 64 rows 172 and 176; 24 rows 103 and 97. One set of 256 dims spills too, with fp32 rows: eight waves
+// 16 (fp32, Q8_0), 7 (bf16), 5 (Q4_0), four 11 (Q8_0), 1 (Q4_0); 128 rows behind 8192 positions take 335, 214, 149, 207 us with
+// eight, 335, 238, 157, 223 with four.
 constexpr int wide_sets(int dtype, bool half, int hd) {
     return hd == 64 ? 2 : hd == 128 && (dtype == DT_F16 || (dtype == DT_BF16 && half)) ? 2 : 1;
 }
