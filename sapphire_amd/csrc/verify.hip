@@ -269,13 +269,16 @@ __device__ __forceinline__ int decide(const VerifyArgs &g, int r, Row &p, Row &q
     return a;
 }
 
-// What is left of token i's probability where the drafts end: max(p - q, 0), or p behind the last draft.
+// What is left of token i's probability where the drafts end: max(p - q, 0), or p behind the last draft. p less q is formed of p
+// less 2^-37 of it, 7.3e-12: sums of rows that lie differently in memory differ by up to 4.4e-12 (two factors of 1.1e-12 in each,
+// see exp2_64), and where p and q are the same nothing must be left.
 struct Rest {
     Weight wp, wq;
     double ip, iq;
     int mode, drafted;                     // mode 0: p; 1: p less q; 2: p but for the drafted token
     __device__ __forceinline__ Rest(const VerifyArgs &g, int r, int a, Row p, Row q)
         : wp(g.c, p.m), wq(g.c, q.m), ip(1.0 / p.sum), iq(1.0 / q.sum), mode(a >= count_of(g, r) ? 0 : g.draft ? 1 : 2), drafted(-1) {
+        if (mode == 1) ip *= 1.0 - 0x1p-37;
         if (mode == 2) drafted = g.draft_tokens[(size_t)r * g.drafts + a];
     }
     __device__ __forceinline__ double operator()(float lp, float lq, int i) const {
