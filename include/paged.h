@@ -118,18 +118,23 @@ int sapphire_paged_attention_dev(const sapphire_paged_cache_t *cache, int layer,
                                  void *stream);
 
 /* The same where rows share their first positions: requests behind one prompt, the beams of a request, the drafted tokens of a
- * sequence (each a row of its own, with the sequence's pages and one position more than the one before). Rows g * rows ..
- * g * rows + rows - 1 (the last group may have fewer) are group g, and shared[g] (device memory) says that their first shared[g]
+ * sequence (each a row of its own, with the sequence's pages and one position more than the one before). Group g is the
+ * `rows` rows from g * rows on (the last one may have fewer), and shared[g] (device memory) says that their first shared[g]
  * positions are the same ones: the same pages, or pages of the same K and V. Those that every row of the group with a length
- * above 0 has, in whole tiles of 16, are read once for the group, by the table row of its first such row; each row's others by its
- * own. lengths, softcap, lse, types and rounding as for sapphire_paged_attention_dev, whose results these are but for the order
- * of sums; a shared[g] of 0 or less shares nothing, one beyond the lengths all. A window is refused: rows that see little share
- * little. Over the shared positions a NaN or an infinity in V makes its dim (over a quantized cache its block's dims) NaN or
- * infinite; one in q or K, other than over a cache of the rows' own type, makes its heads' outputs NaN. What is said
- * there of positions behind the last one and of pages that do not exist holds here too. max_own: about how many
- * positions a row has behind the shared ones at most (0: not known); it is for speed only, any value gives the same positions.
- * workspace: sapphire_paged_shared_attention_workspace_bytes() bytes, 16-byte aligned, which are enough for calls of fewer and shorter rows
- * too, whatever their groups; calls that share one must be ordered on one stream. */
+ * above 0 has, in whole tiles of 16, are read once for the group, by the table row of its first such row; each row's others by
+ * its own. lengths, softcap, lse and types as for sapphire_paged_attention_dev, whose results these are but for the order of
+ * sums and what products over the shared positions leave out: over an F16 cache with F32 rows q comes in two fp16 terms (off
+ * by 2^-23 of an element or 2^-39 of its row's largest) and the weights in two (2^-22); over a quantized one q likewise, and V
+ * in bf16 terms as the weights, for BF16 rows two of each (2^-15 of a weight times a value), for others three (2^-24). A
+ * shared[g] of 0 or less shares nothing, one beyond the lengths all. A window is refused: what rows share under one starts
+ * where the last of their windows does, which differs from row to row and is not formed here; layers with one take
+ * sapphire_paged_attention_dev, drafted tokens too, which reads a window's K and V once per row. Over the shared positions a
+ * NaN or an infinity in V makes its dim (over a quantized cache its block's dims) NaN or infinite; one in q or K, other than
+ * over a cache of the rows' own type, makes its heads' outputs NaN. What is said there of positions behind the last one and of
+ * pages that do not exist holds here too. max_own: about how many positions a row has behind the shared ones at most (0: not
+ * known); it is for speed only, any value gives the same positions. workspace:
+ * sapphire_paged_shared_attention_workspace_bytes() bytes, 16-byte aligned, which are enough for calls of fewer and shorter
+ * rows too, whatever their groups; calls that share one must be ordered on one stream. */
 typedef struct {
     const int *shared;
     int rows, max_own;
@@ -155,13 +160,14 @@ int sapphire_paged_bounds_dev(const sapphire_paged_cache_t *cache, int layer, vo
 
 /* The pages of each sequence and K/V head that its new token attends to. With lo and hi the bounds of a page of row b, its
  * score is the largest, over the query heads h of the K/V head, of sum_d max(q_hd lo_d, q_hd hi_d): no q . k of the page is
- * larger (a positive scale is assumed). choice->pages are chosen, all if there are no more: the first `first` and the last `last`
- * of the ceil(lengths[b] / page_size) pages, and the others by score, in 64 bits, of equal ones the first. A score of NaN, as
- * from bounds or a q that are not finite, counts as +inf. Pages that do not exist are not chosen.
- * selected[b][head][0 .. pages): their places in the sequence (page p / page_size of position p), rising, then -1. q: tokens x
- * n_heads x head_dim as for the attention, of any of the three types. lengths and max_length as there.
- * first + last <= pages <= 2^30 / page_size. workspace: sapphire_paged_select_workspace_bytes() bytes, 16-byte aligned, which
- * are enough for calls of fewer and shorter sequences too; calls that share one must be ordered. */
+ * larger (a positive scale is assumed). choice->pages are chosen, all if there are no more: the first `first` and the last
+ * `last` of the ceil(lengths[b] / page_size) pages, and the others by score, in 64 bits, of equal ones the first. The sum is
+ * formed as max(q_hd, 0) hi_d + min(q_hd, 0) lo_d: an infinite bound that q's sign passes over is 0 times an infinity, as a
+ * q_hd of 0 on any, and NaN. A score of NaN, from those or from NaN in q or bounds, counts as +inf. Pages that do not exist
+ * are not chosen. selected[b][head][0 .. pages): their places in the sequence (page p / page_size of position p), rising, then
+ * -1. q: tokens x n_heads x head_dim as for the attention, of any of the three types. lengths and max_length as there. first +
+ * last <= pages <= 2^30 / page_size. workspace: sapphire_paged_select_workspace_bytes() bytes, 16-byte aligned, which are
+ * enough for calls of fewer and shorter sequences too; calls that share one must be ordered. */
 typedef struct {
     int pages, first, last;
 } sapphire_page_choice_t;

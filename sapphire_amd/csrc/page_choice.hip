@@ -195,8 +195,9 @@ struct Extremes16 {
 
 // A wave per page and K/V head (two for 256 dims): lane (c, m) has position c of every tile and a quarter of the dims. The
 // bytes of K bound it: three documents of up to 131072 positions, 8 heads of 128 dims, bf16, pages of 32 (635 MB): 131 us, 4.8 TB/s
-// (with the extremes of 16-bit values as fp32, and of all lanes alike: 151; with waves that go on to further pages: 136). One
-// position of 16 sequences: 5.2 us. grid (pages / 4, heads x parts, rows).
+// (with the extremes of 16-bit values as fp32, and of all lanes alike: 151; with waves that go on to further pages: 136). In
+// Q8_0 108 us and in Q4_0 77, bound by the issue of 6.5e7 and 6.2e7 vector instructions where bf16 has 3.7e7. One position of 16
+// sequences: 5.2 us. grid (pages / 4, heads x parts, rows).
 template <int CT, int HD>
 __global__ __launch_bounds__(kThreads) void paged_bounds_kernel(BoundsArgs g) {
     using P = Part<CT, HD>;

@@ -300,7 +300,7 @@ int sapphire_paged_shared_attention_dev(const sapphire_paged_cache_t *c, int lay
         return -1;
     }
     if (!groups || !groups->shared || groups->rows <= 0 || groups->max_own < 0) { set_error("shared attention: bad groups"); return -1; }
-    if (at->window > 0) { set_error("shared attention: a window (%d): its rows share little", at->window); return -1; }
+    if (at->window > 0) { set_error("shared attention: a window (%d): what rows share under one is not formed", at->window); return -1; }
     a.max_length = max_length;
     a.shared = groups->shared;
     a.rows = std::min(groups->rows, q->tokens);

@@ -10,10 +10,11 @@
 // Few columns are bound by memory and, where positions are few, by the chain page -> K -> scores -> sum: 8 rows of 32 heads over 8
 // of 128 dims behind 131072 positions, bf16 (537 MB): 110 us for the call. Many are bound by the issue of vector and matrix
 // instructions, which take turns: 128 rows behind 32768 positions with up to 1000 of their own, bf16: 183 us, of which the shared
-// positions take 130 (their products 41 us of matrix cores, with the weights in two terms, and 46 of vector instructions at full
-// clock; it falls to 1.9 GHz), the own ones 56, the join 12. 16 rows of each of two documents of 65536 positions, Q4_0, fp32
-// rows: 158 us, of which the shared positions take 150: 73 are vector instructions, most of them V's codes becoming three bf16
-// terms, 46 matrix cores.
+// positions take about 120 (their products 41 us of matrix cores, with the weights in two terms, and 45 of vector instructions at
+// full clock; it falls to 1.9 GHz), the own ones and the join the rest (each kernel alone under a profiler: 137, 56 and 12). 16
+// rows of each of two documents of 65536 positions, Q4_0, fp32 rows: 156 to 161 us, nearly all of it for the shared positions (168
+// alone under a profiler, the others 19): 71 are vector instructions, most of them V's codes becoming three bf16 terms, 46 matrix
+// cores.
 #include "paged_shared.h"
 
 namespace sapphire {

@@ -10,10 +10,11 @@
 // workgroup of a request from those, the units' sums of max(p - q, 0) of the one row that it ends at, and, by the workgroup
 // that is the last to write its sums, the token, within one unit.
 //
-// 16 requests of 5 drafts over 262144 tokens, both models' logits (185 MB): 69 us for a call. The first launch, 39.6 us at 4.7
+// 16 requests of 5 drafts over 262144 tokens, both models' logits (185 MB): 68 us for a call. The first launch, 39.1 us at 4.7
 // TB/s, has as much vector work in 64 bits (16.5 million instructions: 26 us at full clock) as loads, and the two overlap in
-// part. The second, 31.6 us, is a chain: the rows' sums from the units', the decision, three steps of logits in turn, the count of
-// workgroups, and two scans by the last one. One request of 3 drafts over 4096 tokens: 13.6 us, 5.0 and 8.7 on the GPU.
+// part. The second, 31.9 us, is a chain: the rows' sums from the units', the decision, three steps of logits in turn, the count of
+// workgroups, and two scans by the last one. One request of 3 drafts over 4096 tokens: 13.6 us, 4.9 and 8.8 on the GPU.
+// Greedy, the target's 100 MB of the first: 22 us, 18.1 and 4.1.
 #include <algorithm>
 #include <climits>
 #include <cmath>

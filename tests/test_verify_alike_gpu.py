@@ -48,3 +48,22 @@ def test_little_is_left(hip):
     assert (want[0][:, 0] == x).all() and (want[1] == 0).all()
     np.testing.assert_array_equal(got[0], want[0])
     np.testing.assert_array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("n,pad", [((1 << 20) + 5, 3), (1 << 21, 0), ((1 << 21) - 3, 2)])
+def test_the_largest_vocabularies(hip, n, pad):
+    """More units of a row than a workgroup has threads; draws at both ends and between."""
+    rng = np.random.default_rng(n)
+    requests, drafts = 4, 1
+    logits = (rng.normal(size=(requests, drafts + 1, n)) * 2).astype(np.float32)
+    draft = (logits[:, :drafts] + rng.normal(size=(requests, drafts, n))).astype(np.float32)
+    tokens = np.array([[5], [n], [-1], [n - 1]])
+    logits[0, 0, 5] += 5.0
+    draws = np.array([[0.25, 0.999], [0.5, 0.0], [0.1, 1.0], [0.9, 0.625]], np.float32)
+    for q in (draft, None):
+        for t in (1.0, 0.0):
+            c = Call(logits, q, tokens, None, draws, pad)
+            c.run(t)
+            got, want = c.result(), verify64(logits, q, tokens, None, draws, t)
+            np.testing.assert_array_equal(got[1], want[1])
+            np.testing.assert_array_equal(got[0], want[0])
