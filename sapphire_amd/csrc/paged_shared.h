@@ -243,8 +243,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_shared_kernel(AttnArgs g, S
     using F = Form<CT, HALF, SHORT>;
     using K = KeyTile<CT, HD>;
     using V = ValueTile<CT, HD>;
-    using R = Raw<CT, HD>;
-    using T = Tile<CT, HD>;
     constexpr int LD = HD + 4, DPL = HD / 16, WP = kWaves / WC, HALVES = F::kF32 || HD == 256 ? 1 : 2;
     constexpr int QW = F::kF32 ? HD / 16 : HD / 32;            // q: words of 16 bytes of a term
     constexpr int kO = WP > 1 ? kWaves * 16 * LD : 1;
@@ -543,7 +541,6 @@ template <int CT, int HD, bool HALF, bool SHORT, int CS, int NW>
 __global__ __launch_bounds__(NW *kWave, 2) void paged_shared_wide_kernel(AttnArgs g, SharedPlan sp) {
     using F = Form<CT, HALF, SHORT>;
     using G = Stage<CT, HD, HALF, SHORT>;
-    using R = Raw<CT, HD>;
     using T = Tile<CT, HD>;
     constexpr int DPL = G::DPL, HALVES = G::HALVES;
     constexpr int QW = F::kF32 ? HD / 16 : HD / 32;

@@ -154,11 +154,13 @@ bool launch_shared_join(const void *args, hipStream_t s) {
     const AttnArgs &g = *static_cast<const AttnArgs *>(args);
     const PagedAttn &a = g.a;
     const bool wide = rows_wide(a.q);
-#define SPH_JOIN(CT, HD, W)                                                                        \
+#define SPH_SHARED_JOIN(CT, HD, W)                                                                        \
     if (a.c.dtype == CT && a.c.hd == HD && (g.pieces > kManyPieces) == (W == 16))                  \
         hipLaunchKernelGGL((paged_shared_join_kernel<CT, HD, W>), dim3(g.n_heads, a.q.tokens), dim3(W * kWave), 0, s, g, wide);
-#define SPH_JOIN_HD(CT) SPH_JOIN(CT, 64, 4) SPH_JOIN(CT, 64, 16) SPH_JOIN(CT, 128, 4) SPH_JOIN(CT, 128, 16) SPH_JOIN(CT, 256, 4) SPH_JOIN(CT, 256, 16)
-    SPH_JOIN_HD(DT_F32) SPH_JOIN_HD(DT_BF16) SPH_JOIN_HD(DT_F16) SPH_JOIN_HD(DT_Q8_0) SPH_JOIN_HD(DT_Q4_0)
+#define SPH_SHARED_JOIN_HD(CT)                                                                      \
+    SPH_SHARED_JOIN(CT, 64, 4) SPH_SHARED_JOIN(CT, 64, 16) SPH_SHARED_JOIN(CT, 128, 4)             \
+    SPH_SHARED_JOIN(CT, 128, 16) SPH_SHARED_JOIN(CT, 256, 4) SPH_SHARED_JOIN(CT, 256, 16)
+    SPH_SHARED_JOIN_HD(DT_F32) SPH_SHARED_JOIN_HD(DT_BF16) SPH_SHARED_JOIN_HD(DT_F16) SPH_SHARED_JOIN_HD(DT_Q8_0) SPH_SHARED_JOIN_HD(DT_Q4_0)
     return hip_ok(hipGetLastError(), "shared attention join launch");
 }
 
