@@ -242,13 +242,14 @@ int sapphire_beam_select_dev(const float *logits, int ld, int n, int requests, i
  *   the last draft or where that is 0 everywhere (the last t with w(t) > 0 if a rounding leaves none)
  * so that the tokens are distributed as the target's own, whatever the draft model. temperature <= 0: drafts stay
  * while they are the first of the largest logits of their row, which is the next token too; draft_logits and
- * draws are not looked at. In 64 bits, with probabilities right to 5e-12 of themselves: p_a - q_a counts as 0 where it
- * is below 2^-37 p_a, so that nothing is left over of two rows that are the same. draws: [requests][drafts + 1], taken
- * into 0 .. 1 (NaN: 0). A NaN logit counts as -inf; where a row's largest is infinite, the entries equal to it share
- * the probability. A drafted token outside [0, n) does not stay. tokens[r * (drafts + 1) + i]: the drafts that stay,
- * the next token, then -1; accepted[r]: how many stay. Rows of logits behind counts[r] are not read. Outputs overlap
- * neither each other nor inputs. workspace: sapphire_verify_workspace_bytes() bytes of device memory, 16-byte aligned,
- * which are enough for smaller calls too; calls sharing one must be ordered. 1 <= drafts <= 64, 1 <= n <= 2^21, requests * (2 drafts + 1) < 65536. */
+ * draws are not looked at. In 64 bits, with probabilities right to 5e-12 of themselves: in p_a - q_a, p_a is taken
+ * 2^-37 of itself lower, so that nothing is left over of two rows that are the same. draws: [requests][drafts + 1],
+ * taken into 0 .. 1 (NaN: 0). A NaN logit counts as -inf; where a row's largest is infinite, the entries equal to it
+ * share the probability. A drafted token outside [0, n) does not stay. tokens[r * (drafts + 1) + i]: the drafts that
+ * stay, the next token, then -1; accepted[r]: how many stay. Rows of logits behind counts[r] are not read. Outputs
+ * overlap neither each other nor inputs. workspace: sapphire_verify_workspace_bytes() bytes of device memory, 16-byte
+ * aligned, which are enough for smaller calls too; calls sharing one must be ordered. 1 <= drafts <= 64, 1 <= n <=
+ * 2^21, requests * (2 drafts + 1) < 65536. */
 size_t sapphire_verify_workspace_bytes(int n, int requests, int drafts);
 int sapphire_verify_dev(const float *logits, int ld, const float *draft_logits, int draft_ld, int n, int requests,
                         int drafts, const int *draft_tokens, const int *counts, float temperature, const float *draws,
